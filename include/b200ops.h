@@ -45,7 +45,8 @@ typedef enum b200_dtype {
   B200_BF16 = 2,
   B200_I8 = 3,
   B200_I32 = 4,
-  B200_I64 = 5
+  B200_I64 = 5,
+  B200_F8E4M3 = 6 /* 8-bit cache codes only */
 } b200_dtype;
 
 /* ---- launch / tile parameters chosen by the tuner ----------------------
@@ -263,6 +264,96 @@ int b200_paged_attention_noalloc(const void* q, const void* k_cache,
                                  int64_t max_blocks, float scale, int32_t dtype,
                                  int32_t index_dtype,
                                  const b200_launch_cfg* cfg, void* stream);
+
+/* ---- 8-bit paged KV cache ---------------------------------------------------
+ * No counterpart in the reference (its caches are 16-bit).  A cached row (the
+ * D values of one token and one kv head) is D codes of `cache_dtype`
+ * (B200_I8 or B200_F8E4M3) and one fp32 scale:
+ *   scale = max(max|x| / qmax, 1e-12)      qmax: 127 (int8), 448 (e4m3)
+ *   int8: code = clamp(round_half_even(x / scale), -127, 127)
+ *   e4m3: code = the e4m3 value nearest x / scale (half to even)
+ * all in fp32 with every operation rounded on its own; the value read back is
+ * code * scale.  A row that holds an infinity or a NaN gets a NaN scale.
+ * Codes: [num_blocks, block_size, Hkv, D]; scales k_scale, v_scale:
+ * [num_blocks, Hkv, block_size] f32. */
+
+/* Fused RoPE(q, k) + append into the 8-bit cache: b200_rope_kv_append_paged
+ * with the rotated fp32 K row (not rounded to 16 bits first) and the V row
+ * quantised as they are written.  q [T, Hq, D] (NULL with q_out NULL), k, v
+ * [T, Hkv, D] of `dtype` (F16/BF16); positions [T] rows of the cos/sin
+ * tables [cs_rows, D] (`cs_dtype`: dtype or F32); slot_mapping [T].  Tokens
+ * whose slot or position is out of range write no cache row, and their q_out
+ * row is zero when the position is; of several tokens naming one slot the
+ * last that writes wins.  D even.
+ * workspace: b200_rope_kv_append_paged_quant_workspace_size(T) bytes, 16-byte
+ * aligned (0 for T <= 512: NULL may be given); nothing in it is kept between
+ * calls.  cfg: rows_per_cta (rows of a token per thread: 1, 2, 3 or 6;
+ * default 1 up to 512 tokens, else 3). */
+size_t b200_rope_kv_append_paged_quant_workspace_size(int64_t T);
+int b200_rope_kv_append_paged_quant(const void* q, const void* k, const void* v, const int64_t* positions,
+                                    const void* cos, const void* sin, int64_t cs_rows,
+                                    const int64_t* slot_mapping, void* q_out, void* k_cache, void* v_cache,
+                                    float* k_scale, float* v_scale, int64_t T, int64_t Hq, int64_t Hkv, int64_t D,
+                                    int64_t num_blocks, int64_t block_size, int32_t dtype, int32_t cs_dtype,
+                                    int32_t cache_dtype, void* workspace, size_t workspace_bytes,
+                                    const b200_launch_cfg* cfg, void* stream);
+
+/* Reads the contexts of an 8-bit cache back into dense k_out, v_out
+ * [B, Hkv, max_len, D] of `dtype` (F16/BF16), as b200_flash_attn takes K and
+ * V: row s < min(context_len[b], max_len) is code * scale of the sequence's
+ * token s (blocks as in b200_paged_attention: ids outside [0, num_blocks)
+ * are dropped and later blocks move up), rounded once; every other row is
+ * zero.  cfg: none. */
+int b200_paged_kv_dequant(const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
+                          const void* block_table, const void* context_len, void* k_out, void* v_out, int64_t B,
+                          int64_t Hkv, int64_t D, int64_t num_blocks, int64_t block_size, int64_t max_blocks,
+                          int64_t max_len, int32_t dtype, int32_t cache_dtype, int32_t index_dtype,
+                          const b200_launch_cfg* cfg, void* stream);
+
+/* Paged decode attention over an 8-bit cache: b200_paged_attention of the
+ * cache's values code * scale, without writing them out.  Softmax, sums and
+ * accumulation in fp32; the softmax weights enter the second product as f16.  A sequence without
+ * tokens gives a zero row.  workspace: 16-byte aligned, of
+ * b200_paged_attention_quant_workspace_size() bytes (may be 0: NULL); nothing
+ * in it is kept between calls, it needs no clearing.  Streaming kernel for D = 128, block sizes
+ * of 16, 32, ..., 256, 1, 2, 4 or 8 query heads a kv head and 16-byte aligned
+ * tensors; a general kernel for the rest (D <= 256).  cfg: stages (ring depth, default about 132
+ * KB), rows_per_cta (kv heads per CTA, at most 8), flags bit 0: general kernel; bit 3: programmatic
+ * dependent launch (the kernel's prologue overlaps the previous kernel on
+ * the stream; the caller guarantees that kernel writes neither context_len
+ * nor block_table, as the append does not). */
+size_t b200_paged_attention_quant_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t num_blocks,
+                                                 int64_t block_size, int64_t max_blocks, const b200_launch_cfg* cfg);
+int b200_paged_attention_quant(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,
+                               const float* v_scale, const void* block_table, const void* context_len, void* out,
+                               int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t num_blocks,
+                               int64_t block_size, int64_t max_blocks, float scale, int32_t dtype,
+                               int32_t cache_dtype, int32_t index_dtype, void* workspace, size_t workspace_bytes,
+                               const b200_launch_cfg* cfg, void* stream);
+
+/* ---- decode attention of a batch that shares a prefix ------------------------
+ * No counterpart in the reference.  Every sequence attends to the prefix --
+ * the first prefix_len[0] tokens of the blocks prefix_table
+ * [max_prefix_blocks] -- and to its own context_len[b] tokens behind it
+ * (block_table [B, max_blocks], max_blocks may be 0); both by the block rules
+ * of b200_paged_attention, one softmax over both.  The prefix is read once
+ * for the batch: its part is a matrix product of all B * Hq / Hkv query rows
+ * of a kv head.  Caches of `cache_dtype`: dtype itself (scales NULL), or
+ * B200_I8 / B200_F8E4M3 with scales as above.  prefix_len, context_len and
+ * the tables are of `index_dtype` and on the device.  A sequence without any
+ * token gives a zero row.  workspace, cfg and limits as
+ * b200_paged_attention_quant. */
+size_t b200_paged_attention_prefix_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t num_blocks,
+                                                  int64_t block_size, int64_t max_prefix_blocks,
+                                                  int64_t max_blocks, int32_t cache_dtype,
+                                                  const b200_launch_cfg* cfg);
+int b200_paged_attention_prefix(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,
+                                const float* v_scale, const void* prefix_table, const void* prefix_len,
+                                const void* block_table, const void* context_len, void* out, int64_t B, int64_t Hq,
+                                int64_t Hkv, int64_t D, int64_t num_blocks, int64_t block_size,
+                                int64_t max_prefix_blocks, int64_t max_blocks, float scale, int32_t dtype,
+                                int32_t cache_dtype, int32_t index_dtype, void* workspace, size_t workspace_bytes,
+                                const b200_launch_cfg* cfg, void* stream);
 
 /* ---- INT8 GEMM with fused dequant epilogue --------------------------------
  * Restates triton_agent/ops/quant_matmul/reference.py:26-27 for

@@ -28,7 +28,7 @@ ERR_NO_DEVICE = -6
 ERR_INJECTED = -7
 ERR_ALIGNMENT = -8
 
-F32, F16, BF16, I8, I32, I64 = 0, 1, 2, 3, 4, 5
+F32, F16, BF16, I8, I32, I64, F8E4M3 = 0, 1, 2, 3, 4, 5, 6
 
 
 class B200OpsError(RuntimeError):
@@ -105,6 +105,30 @@ SIGNATURES = {
     "b200_paged_attention_noalloc": (
         c_int,
         [P, P, P, P, P, P, I64_, I64_, I64_, I64_, I64_, I64_, I64_, c_float, c_int32, c_int32, PCFG, P],
+    ),
+    "b200_rope_kv_append_paged_quant_workspace_size": (c_size_t, [I64_]),
+    "b200_rope_kv_append_paged_quant": (
+        c_int,
+        [P, P, P, P, P, P, I64_, P, P, P, P, P, P, I64_, I64_, I64_, I64_, I64_, I64_, c_int32, c_int32, c_int32, P,
+         c_size_t, PCFG, P],
+    ),
+    "b200_paged_kv_dequant": (
+        c_int,
+        [P, P, P, P, P, P, P, P, I64_, I64_, I64_, I64_, I64_, I64_, I64_, c_int32, c_int32, c_int32, PCFG, P],
+    ),
+    "b200_paged_attention_quant_workspace_size": (c_size_t, [I64_, I64_, I64_, I64_, I64_, I64_, I64_, PCFG]),
+    "b200_paged_attention_quant": (
+        c_int,
+        [P, P, P, P, P, P, P, P, I64_, I64_, I64_, I64_, I64_, I64_, I64_, c_float, c_int32, c_int32, c_int32, P,
+         c_size_t, PCFG, P],
+    ),
+    "b200_paged_attention_prefix_workspace_size": (
+        c_size_t, [I64_, I64_, I64_, I64_, I64_, I64_, I64_, I64_, c_int32, PCFG],
+    ),
+    "b200_paged_attention_prefix": (
+        c_int,
+        [P, P, P, P, P, P, P, P, P, P, I64_, I64_, I64_, I64_, I64_, I64_, I64_, I64_, c_float, c_int32, c_int32,
+         c_int32, P, c_size_t, PCFG, P],
     ),
     "b200_int8_gemm_workspace_size": (c_size_t, [I64_, I64_, I64_, PCFG]),
     "b200_int8_gemm": (c_int, [P, P, P, P, P, I64_, I64_, I64_, I64_, c_int32, P, P, c_size_t, PCFG, P]),

@@ -20,7 +20,7 @@ import torch
 from . import lib as L
 
 _DT = {torch.float32: L.F32, torch.float16: L.F16, torch.bfloat16: L.BF16, torch.int8: L.I8,
-       torch.int32: L.I32, torch.int64: L.I64}
+       torch.int32: L.I32, torch.int64: L.I64, torch.float8_e4m3fn: L.F8E4M3}
 
 
 def dtype_code(dt: torch.dtype) -> int:
@@ -260,6 +260,204 @@ def paged_attention(q, k_cache, v_cache, block_table, context_len, scale: float 
                                        dtype_code(block_table.dtype), _ptr(ws), ws.numel(), _cfg(cfg),
                                        _stream(dev))
     L.check(st, "paged_attention")
+    return o
+
+
+# --------------------------------------------------------- 8-bit paged KV cache
+_CODE_DTYPES = (torch.int8, torch.float8_e4m3fn)
+
+
+def _scratch(dev: torch.device, nbytes: int) -> torch.Tensor | None:
+    """Workspace of one call, from the current stream's allocator (inside a
+    capture: from the graph's pool), so that calls on other streams and
+    captured graphs share none.  The kernels need no cleared memory and keep
+    nothing in it."""
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+
+
+def _check_cache(op: str, k_cache, v_cache, k_scale, v_scale) -> tuple[int, int, int, int]:
+    """(num_blocks, block_size, Hkv, D) of an 8-bit cache with its scales."""
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype:
+        raise L.B200OpsError(L.ERR_BAD_ARG, op, "caches must be [num_blocks, block_size, Hkv, D] of one shape and dtype")
+    if k_cache.dtype not in _CODE_DTYPES:
+        raise L.B200OpsError(L.ERR_UNSUPPORTED, op, "8-bit caches are int8 or float8_e4m3fn")
+    nb, bs, Hkv, D = k_cache.shape
+    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+        if t is None or tuple(t.shape) != (nb, Hkv, bs) or t.dtype != torch.float32:
+            raise L.B200OpsError(L.ERR_BAD_ARG, op, f"{name} must be float32 [num_blocks, Hkv, block_size]")
+    _contig(op, k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale)
+    return nb, bs, Hkv, D
+
+
+def _check_out(op: str, name: str, t: torch.Tensor, shape: tuple, dtype: torch.dtype):
+    if tuple(t.shape) != tuple(shape) or t.dtype != dtype:
+        raise L.B200OpsError(L.ERR_BAD_ARG, op, f"{name} must be {dtype} {list(shape)}")
+    _contig(op, **{name: t})
+
+
+def _index(op: str, name: str, t: torch.Tensor, like: torch.Tensor, shape: tuple) -> torch.Tensor:
+    if tuple(t.shape) != tuple(shape):
+        raise L.B200OpsError(L.ERR_BAD_ARG, op, f"{name} must be {list(shape)}")
+    if t.dtype not in (torch.int32, torch.int64):
+        raise L.B200OpsError(L.ERR_UNSUPPORTED, op, f"{name} must be int32 or int64")
+    return t.to(like.dtype).contiguous()
+
+
+def rope_kv_append_paged_quant(q, k, v, positions, cos, sin, slot_mapping, k_cache, v_cache, k_scale, v_scale,
+                               q_out: torch.Tensor | None = None, cfg=None):
+    """rope_kv_append_paged into an 8-bit cache: q and k rotated by their
+    positions (fp32), k (rotated, not rounded to 16 bits first) and v written
+    at slot_mapping as codes with one fp32 scale for each (token, kv head).
+
+    q [T,Hq,D] (or None), k/v [T,Hkv,D] fp16 or bf16, positions/slot_mapping
+    [T] int64, cos/sin [P,D] (fp32 or k's dtype), caches [num_blocks,
+    block_size, Hkv, D] int8 or float8_e4m3fn, scales [num_blocks, Hkv,
+    block_size] float32.  scale = max(max|row| / qmax, 1e-12), qmax 127 or 448.
+    Tokens whose slot or position is out of range write nothing (q_out row: zero
+    when the position is); of several tokens naming one slot the last wins.
+    Returns q_out (or None)."""
+    op = "rope_kv_append_paged_quant"
+    dev = _need_cuda(op, q, k, v, positions, cos, sin, slot_mapping, k_cache, v_cache, k_scale, v_scale, q_out)
+    nb, bs, Hkv, D = _check_cache(op, k_cache, v_cache, k_scale, v_scale)
+    _contig(op, q=q, k=k, v=v, cos=cos, sin=sin)
+    if k.dim() != 3 or tuple(k.shape[1:]) != (Hkv, D) or v.shape != k.shape or v.dtype != k.dtype:
+        raise L.B200OpsError(L.ERR_BAD_ARG, op, "k and v must be [T, Hkv, D] of one dtype, as the cache's rows")
+    T = k.shape[0]
+    if q is not None and (q.dim() != 3 or q.shape[0] != T or q.shape[2] != D or q.dtype != k.dtype):
+        raise L.B200OpsError(L.ERR_BAD_ARG, op, "q must be [T, Hq, D] of k's dtype")
+    if cos.dim() != 2 or cos.shape[1] != D or sin.shape != cos.shape or sin.dtype != cos.dtype:
+        raise L.B200OpsError(L.ERR_BAD_ARG, op, "cos and sin must be [positions, D] of one dtype")
+    for name, t in (("positions", positions), ("slot_mapping", slot_mapping)):
+        if t.dtype != torch.int64:
+            raise L.B200OpsError(L.ERR_UNSUPPORTED, op, f"{name} must be int64")
+        if t.numel() != T:
+            raise L.B200OpsError(L.ERR_BAD_ARG, op, f"{name} must have T elements")
+    Hq = q.shape[1] if q is not None else 0
+    if q is None:
+        q_out = None
+    elif q_out is None:
+        q_out = torch.empty_like(q)
+    else:
+        _check_out(op, "q_out", q_out, q.shape, q.dtype)
+    pos, sm = positions.contiguous(), slot_mapping.contiguous()
+    lib = L.load()
+    with torch.cuda.device(dev):
+        ws = _scratch(dev, int(lib.b200_rope_kv_append_paged_quant_workspace_size(T)))
+        st = lib.b200_rope_kv_append_paged_quant(
+            _ptr(q), _ptr(k), _ptr(v), _ptr(pos), _ptr(cos), _ptr(sin), cos.shape[0], _ptr(sm), _ptr(q_out),
+            _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), T, Hq, Hkv, D, nb, bs, dtype_code(k.dtype),
+            dtype_code(cos.dtype), dtype_code(k_cache.dtype), _ptr(ws), ws.numel() if ws is not None else 0,
+            _cfg(cfg), _stream(dev))
+    L.check(st, op)
+    return q_out
+
+
+def paged_kv_dequant(k_cache, v_cache, k_scale, v_scale, block_table, context_len, max_len: int,
+                     dtype: torch.dtype = torch.bfloat16, k_out: torch.Tensor | None = None,
+                     v_out: torch.Tensor | None = None, cfg=None):
+    """Contexts of an 8-bit paged cache read back as dense K and V
+    [B, Hkv, max_len, D] of `dtype`, as flash_attn takes them.  Row s <
+    min(context_len[b], max_len) is code * scale of the sequence's token s
+    (block rules of paged_attention), rounded once; all other rows are zero."""
+    op = "paged_kv_dequant"
+    dev = _need_cuda(op, k_cache, v_cache, k_scale, v_scale, block_table, context_len, k_out, v_out)
+    nb, bs, Hkv, D = _check_cache(op, k_cache, v_cache, k_scale, v_scale)
+    if block_table.dim() != 2 or max_len < 0:
+        raise L.B200OpsError(L.ERR_BAD_ARG, op, "block_table must be [B, max_blocks] and max_len >= 0")
+    B, max_blocks = block_table.shape
+    bt = _index(op, "block_table", block_table, block_table, (B, max_blocks))
+    cl = _index(op, "context_len", context_len, bt, (B,))
+    outs = []
+    for name, t in (("k_out", k_out), ("v_out", v_out)):
+        if t is None:
+            t = torch.empty(B, Hkv, max_len, D, dtype=dtype, device=dev)
+        _check_out(op, name, t, (B, Hkv, max_len, D), dtype)
+        outs.append(t)
+    with torch.cuda.device(dev):
+        st = L.load().b200_paged_kv_dequant(_ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(bt),
+                                            _ptr(cl), _ptr(outs[0]), _ptr(outs[1]), B, Hkv, D, nb, bs, max_blocks,
+                                            max_len, dtype_code(dtype), dtype_code(k_cache.dtype),
+                                            dtype_code(bt.dtype), _cfg(cfg), _stream(dev))
+    L.check(st, op)
+    return outs[0], outs[1]
+
+
+def paged_attention_quant(q, k_cache, v_cache, k_scale, v_scale, block_table, context_len,
+                          scale: float | None = None, out: torch.Tensor | None = None, cfg=None):
+    """paged_attention over an 8-bit cache (values code * scale): q [B,Hq,D]
+    fp16 or bf16; caches [num_blocks, block_size, Hkv, D] int8 or
+    float8_e4m3fn with float32 scales [num_blocks, Hkv, block_size];
+    block_table [B, max_blocks] and context_len [B] int32 or int64.  A
+    sequence without tokens gives zeros.  Returns out [B,Hq,D] in q's dtype."""
+    op = "paged_attention_quant"
+    dev = _need_cuda(op, q, k_cache, v_cache, k_scale, v_scale, block_table, context_len, out)
+    nb, bs, Hkv, D = _check_cache(op, k_cache, v_cache, k_scale, v_scale)
+    if q.dim() != 3 or q.shape[2] != D or block_table.dim() != 2:
+        raise L.B200OpsError(L.ERR_BAD_ARG, op, "q must be [B, Hq, D] and block_table [B, max_blocks]")
+    _contig(op, q=q)
+    B, Hq, _ = q.shape
+    max_blocks = block_table.shape[1]
+    bt = _index(op, "block_table", block_table, block_table, (B, max_blocks))
+    cl = _index(op, "context_len", context_len, bt, (B,))
+    o = torch.empty_like(q) if out is None else out
+    _check_out(op, "out", o, q.shape, q.dtype)
+    sc = float(scale) if scale is not None else 1.0 / math.sqrt(D)
+    lib, c = L.load(), _cfg(cfg)
+    with torch.cuda.device(dev):
+        ws = _scratch(dev, int(lib.b200_paged_attention_quant_workspace_size(B, Hq, Hkv, D, nb, bs, max_blocks, c)))
+        st = lib.b200_paged_attention_quant(_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale),
+                                            _ptr(bt), _ptr(cl), _ptr(o), B, Hq, Hkv, D, nb, bs, max_blocks, sc,
+                                            dtype_code(q.dtype), dtype_code(k_cache.dtype), dtype_code(bt.dtype),
+                                            _ptr(ws), ws.numel() if ws is not None else 0, c, _stream(dev))
+    L.check(st, op)
+    return o
+
+
+def paged_attention_prefix(q, k_cache, v_cache, prefix_table, prefix_len, block_table, context_len, k_scale=None,
+                           v_scale=None, scale: float | None = None, out: torch.Tensor | None = None, cfg=None):
+    """Decode attention of a batch whose sequences share a prefix: sequence b
+    attends to the first prefix_len tokens of the blocks prefix_table [P]
+    (prefix_len: one int32/int64 element on the device) and to its own
+    context_len[b] tokens in block_table [B, max_blocks] behind them, one
+    softmax over both.  The prefix is read once for the whole batch.  q
+    [B,Hq,D]; caches in q's dtype, or int8 / float8_e4m3fn with k_scale and
+    v_scale as in paged_attention_quant.  A sequence without any token gives
+    zeros.  Returns out [B,Hq,D] in q's dtype."""
+    op = "paged_attention_prefix"
+    dev = _need_cuda(op, q, k_cache, v_cache, prefix_table, prefix_len, block_table, context_len, k_scale, v_scale,
+                     out)
+    if k_cache.dtype in _CODE_DTYPES:
+        nb, bs, Hkv, D = _check_cache(op, k_cache, v_cache, k_scale, v_scale)
+    else:
+        if k_scale is not None or v_scale is not None:
+            raise L.B200OpsError(L.ERR_BAD_ARG, op, "scales belong to 8-bit caches")
+        if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or not (k_cache.dtype == v_cache.dtype == q.dtype):
+            raise L.B200OpsError(L.ERR_BAD_ARG, op,
+                                 "caches must be [num_blocks, block_size, Hkv, D] of q's dtype or 8-bit codes")
+        _contig(op, k_cache=k_cache, v_cache=v_cache)
+        nb, bs, Hkv, D = k_cache.shape
+    if q.dim() != 3 or q.shape[2] != D or block_table.dim() != 2 or prefix_table.dim() != 1:
+        raise L.B200OpsError(L.ERR_BAD_ARG, op, "q must be [B, Hq, D], block_table [B, max_blocks], prefix_table [P]")
+    _contig(op, q=q)
+    B, Hq, _ = q.shape
+    max_blocks, max_prefix = block_table.shape[1], prefix_table.shape[0]
+    bt = _index(op, "block_table", block_table, block_table, (B, max_blocks))
+    cl = _index(op, "context_len", context_len, bt, (B,))
+    pt = _index(op, "prefix_table", prefix_table, bt, (max_prefix,))
+    pl = _index(op, "prefix_len", prefix_len.reshape(-1), bt, (1,))
+    o = torch.empty_like(q) if out is None else out
+    _check_out(op, "out", o, q.shape, q.dtype)
+    sc = float(scale) if scale is not None else 1.0 / math.sqrt(D)
+    lib, c, code = L.load(), _cfg(cfg), dtype_code(k_cache.dtype)
+    with torch.cuda.device(dev):
+        ws = _scratch(dev, int(lib.b200_paged_attention_prefix_workspace_size(B, Hq, Hkv, D, nb, bs, max_prefix,
+                                                                              max_blocks, code, c)))
+        st = lib.b200_paged_attention_prefix(_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale),
+                                             _ptr(pt), _ptr(pl), _ptr(bt), _ptr(cl), _ptr(o), B, Hq, Hkv, D, nb, bs,
+                                             max_prefix, max_blocks, sc, dtype_code(q.dtype), code,
+                                             dtype_code(bt.dtype), _ptr(ws), ws.numel() if ws is not None else 0, c,
+                                             _stream(dev))
+    L.check(st, op)
     return o
 
 

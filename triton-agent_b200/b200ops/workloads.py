@@ -69,6 +69,26 @@ def paged_cache(num_blocks=65536, block_size=16, Hkv=8, D=128, dtype=torch.bfloa
     return PagedCache(kc, vc)
 
 
+@dataclass
+class QuantCache:
+    k_cache: torch.Tensor  # codes [num_blocks, block_size, Hkv, D]
+    v_cache: torch.Tensor
+    k_scale: torch.Tensor  # f32 [num_blocks, Hkv, block_size]
+    v_scale: torch.Tensor
+
+
+def quant_cache(num_blocks=4096, block_size=16, Hkv=8, D=128, code_dtype=torch.int8, device="cuda", seed=0):
+    """8-bit paged cache of ~ N(0,1) rows, quantised as the append does."""
+    from .ops.rope_kv_append_paged_quant.reference import quantise_rows
+
+    g = _gen(device, seed + 7000)
+    got = []
+    for _ in range(2):
+        c, s = quantise_rows(torch.randn(num_blocks, block_size, Hkv, D, generator=g, device=device), code_dtype)
+        got.append((c, s.transpose(1, 2).contiguous()))
+    return QuantCache(got[0][0], got[1][0], got[0][1], got[1][1])
+
+
 def decode_append_inputs(cache: PagedCache, n_tok=64, Hq=32, max_pos=4096, theta=1e4, device="cuda", seed=0):
     """Inputs of one decode-step RoPE + paged append."""
     Hkv, D = cache.k_cache.shape[2:]

@@ -1,0 +1,65 @@
+// Codes of the 8-bit KV cache: element types and their exact conversions.
+#pragma once
+
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+namespace b200 {
+
+using e4m3_t = __nv_fp8_e4m3;
+
+// Largest code magnitude.
+template <typename KV>
+__host__ __device__ constexpr float kv8_max() {
+  return std::is_same<KV, int8_t>::value ? 127.0f : 448.0f;
+}
+
+// Four codes (lowest byte first) as fp32.  int8: a byte with its sign bit
+// flipped, placed below the exponent of 2^23, is 2^23 + 128 + code.
+template <typename KV>
+__device__ __forceinline__ void kv8_to_f32x4(uint32_t w, float* f) {
+  if constexpr (std::is_same<KV, int8_t>::value) {
+    const uint32_t u = w ^ 0x80808080u;
+    f[0] = __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7440)) - 8388736.0f;
+    f[1] = __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7441)) - 8388736.0f;
+    f[2] = __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7442)) - 8388736.0f;
+    f[3] = __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7443)) - 8388736.0f;
+  } else {
+    const __half2_raw lo = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3);
+    const __half2_raw hi = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3);
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo));
+    const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+    f[0] = a.x, f[1] = a.y, f[2] = b.x, f[3] = b.y;
+  }
+}
+
+// Bytes (A, B) of w as an f16 pair, exactly (A in the low half).  int8: 1024 +
+// 128 + code has the code's offset in its low mantissa bits; one packed
+// subtraction takes the rest off.  e4m3: the hardware conversion, NaN codes
+// included.
+template <typename KV, int A, int B>
+__device__ __forceinline__ uint32_t kv8_pair(uint32_t w) {
+  if constexpr (std::is_same<KV, int8_t>::value) {
+    const uint32_t u = __byte_perm(w ^ 0x80808080u, 0x64646464u, A | (4 << 4) | (B << 8) | (4 << 12));
+    const uint32_t off = 0x64806480u;
+    const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&u), *reinterpret_cast<const __half2*>(&off));
+    return *reinterpret_cast<const uint32_t*>(&d);
+  } else {
+    const __half2_raw r =
+        __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)__byte_perm(w, 0, A | (B << 4) | 0x4400), __NV_E4M3);
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+}
+
+// The scales of a key and its value as the attention kernels use them: the
+// logit factor ks, log2 vs and 1 / vs.  A value scale below 2^-100 (a slot
+// never written holds 0) counts as 2^-100; NaN stays NaN.
+__device__ __forceinline__ void kv8_value_scale(float vs, float& lvs, float& ivs) {
+  constexpr float kTiny = 7.888609052210118e-31f;  // 2^-100
+  vs = vs < kTiny ? kTiny : vs;
+  lvs = __log2f(vs);
+  ivs = __fdividef(1.0f, vs);
+}
+
+}  // namespace b200

@@ -1,0 +1,297 @@
+// Decode attention over the 8-bit paged cache, and of batches that share a
+// prefix: argument checks, launch geometry, and the kernel that joins pieces.
+// The streaming kernel and its mathematics: kv_attn.cuh.
+#include "common.cuh"
+
+B200_DEVICE_ERROR_WORD()
+
+#include "kv_attn.cuh"
+
+namespace b200 {
+namespace {
+
+constexpr size_t kSmemMost = 227 * 1024;
+
+// ---------------------------------------------------------------------------
+// Join: one warp a query row.  The row's pieces are those of its segment's
+// ranges (sub of them each) and one per prefix split; lanes fold the (m, l) of
+// their pieces, then the warp adds the weighted rows, four dims a lane.  A row
+// that the streaming kernel wrote itself is skipped; a row without any token
+// is zero.
+// ---------------------------------------------------------------------------
+struct JoinParams {
+  int64_t B, Hq;
+  int heads_cta, sub, nseg, grid, always, splits;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+    paged_attn_join_kernel(const int32_t* __restrict__ cum, const float* __restrict__ rows,
+                           const float* __restrict__ prefix, T* __restrict__ out, JoinParams p) {
+  const int64_t row = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (row >= p.B * p.Hq) return;
+  const int64_t b = row / p.Hq;
+  const int h = (int)(row - b * p.Hq), hg = h / p.heads_cta, hh = h - hg * p.heads_cta;
+  const int seg = (int)(hg * p.B + b);
+  const int64_t E = __ldcg(&cum[p.nseg]), s0 = __ldcg(&cum[seg]), s1 = __ldcg(&cum[seg + 1]);
+  const int64_t R = E < p.grid ? E : p.grid;
+  int c1 = 0, own = 0;
+  if (s1 > s0) {
+    c1 = range_of(s0, E, R);
+    const int c2 = range_of(s1 - 1, E, R);
+    if (c1 == c2 && p.sub == 1 && !p.always) return;
+    own = (c2 - c1 + 1) * p.sub;
+  }
+  const int n = own + p.splits;
+  auto piece = [&](int i) -> const float* {
+    return i < own ? rows + ((((int64_t)seg + c1) * p.sub + i) * p.heads_cta + hh) * kPiecePitch
+                   : prefix + ((int64_t)(i - own) * p.B * p.Hq + row) * kPiecePitch;
+  };
+  // weight of a piece before the maximum is taken off: none without tokens
+  // (m = -inf, l = 0); NaN logits only leave m = -inf and l = NaN
+  auto weight = [](float m, float l, float M) { return m == -INFINITY ? (l == 0.f ? 0.f : l) : ex2(m - M); };
+  float M = -INFINITY;
+  for (int i = lane; i < n; i += 32) M = fmaxf(M, __ldcg(piece(i) + kD));
+  M = warp_max(M);
+  float L = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = 0; i0 < n; i0 += 32) {
+    float w = 0.f;
+    if (i0 + lane < n) {
+      const float2 ml = __ldcg(reinterpret_cast<const float2*>(piece(i0 + lane) + kD));
+      w = weight(ml.x, ml.y, M);
+      if (w != 0.f) L += w * ml.y;
+    }
+    const int nb = n - i0 < 32 ? n - i0 : 32;
+    for (int u0 = 0; u0 < nb; u0 += 4) {
+      float4 v[4];
+      float wu[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        wu[u] = __shfl_sync(0xffffffffu, w, (u0 + u) & 31);
+        if (u0 + u >= nb) wu[u] = 0.f;
+        v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (wu[u] != 0.f) v[u] = __ldcg(reinterpret_cast<const float4*>(piece(i0 + u0 + u) + 4 * lane));
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        acc.x = fmaf(wu[u], v[u].x, acc.x);
+        acc.y = fmaf(wu[u], v[u].y, acc.y);
+        acc.z = fmaf(wu[u], v[u].z, acc.z);
+        acc.w = fmaf(wu[u], v[u].w, acc.w);
+      }
+    }
+  }
+  L = warp_sum(L);
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  uint2 pk;
+  pk.x = pack_pair<T>(acc.x * inv, acc.y * inv);
+  pk.y = pack_pair<T>(acc.z * inv, acc.w * inv);
+  *reinterpret_cast<uint2*>(out + row * kD + 4 * lane) = pk;
+}
+
+// ---------------------------------------------------------------------------
+// Geometry.  HG: the largest divisor of Hkv up to 8 whose page leaves room for
+// two stages; sub = 8 / HG pages a stage so that eight consumer warps (or as many
+// as HG divides) have work whatever Hkv is.  The fast path covers head dim 128,
+// blocks of a multiple of 16 tokens up to 256 and 1, 2, 4 or 8 query heads a kv head.
+// ---------------------------------------------------------------------------
+PieceGeom piece_geometry(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t bs, int64_t num_blocks,
+                         int64_t max_blocks, int elem, const b200_launch_cfg* cfg) {
+  PieceGeom g{};
+  const int64_t G = Hq / Hkv;
+  if (D != kD || !(G == 1 || G == 2 || G == 4 || G == 8) || bs % 16 != 0 || bs > 256) return g;
+  // 32-bit token slots (TMA coordinates) and entry counts
+  if (num_blocks * bs >= (1ll << 31) || max_blocks * bs >= (1ll << 31)) return g;
+  g.G = (int)G;
+  const int hg_most = (cfg && cfg->rows_per_cta > 0 && cfg->rows_per_cta <= 8) ? cfg->rows_per_cta : 8;
+  for (int cand = hg_most; cand >= 1 && g.HG == 0; --cand) {
+    if (Hkv % cand) continue;
+    int sub = 8 / cand;
+    const int64_t box = (int64_t)cand * bs * 128;
+    const int64_t page = ((elem == 1 ? 2 * box + 2 * (int64_t)cand * bs * 4 : 4 * box) + 1023) / 1024 * 1024;
+    while (sub > 1 && page * sub > 40 * 1024) sub /= 2;
+    if (2 * page * sub > 176 * 1024) continue;
+    g.HG = cand, g.sub = sub;
+    g.page_bytes = (uint32_t)page;
+    g.stage_bytes = (uint32_t)(page * sub);
+  }
+  if (g.HG == 0) return g;
+  g.n_hg = (int)(Hkv / g.HG);
+  g.seqs = kMaxSeg / g.n_hg < B ? kMaxSeg / g.n_hg : B;
+  if (g.seqs < 1 || g.n_hg * g.seqs * max_blocks >= (1ll << 31)) return g;
+  g.grid = device_sm_count();
+  g.pdl = cfg && (cfg->flags & 8);
+  const size_t fixed = 1024 + (size_t)(g.n_hg * g.seqs + 1) * 4 + (size_t)g.seqs * 4 + 65 * 4;
+  const size_t per = g.stage_bytes + 16 + sizeof(StageMeta);
+  int stages = (cfg && cfg->stages > 0) ? cfg->stages : (int)(132 * 1024 / g.stage_bytes);
+  if (stages < 2) stages = 2;
+  if (stages > 16) stages = 16;
+  while (stages > 2 && stages * per + fixed > kSmemMost) --stages;
+  g.stages = stages;
+  g.smem = stages * per + fixed;
+  g.fast = g.smem <= kSmemMost;
+  return g;
+}
+
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+
+// Bytes of the workspace's parts for one slice.
+struct SpaceBytes {
+  size_t cum, rows, prefix;
+};
+SpaceBytes space_bytes(const PieceGeom& g, int64_t Hq, int prefix_splits) {
+  const int64_t nseg = g.n_hg * g.seqs;
+  SpaceBytes s;
+  s.cum = up256((size_t)(nseg + 1) * 4);
+  s.rows = up256((size_t)(nseg + g.grid) * g.sub * g.HG * g.G * kPiecePitch * 4);
+  s.prefix = up256((size_t)prefix_splits * g.seqs * Hq * kPiecePitch * 4);
+  return s;
+}
+
+template <typename T>
+int launch_join(const AttnCall& a, const PieceGeom& g, const PieceSpace& w, cudaStream_t s) {
+  JoinParams p{a.B, a.Hq, g.HG * g.G, g.sub, (int)(g.n_hg * a.B), g.grid, a.prefix_table != nullptr, w.prefix_splits};
+  cudaLaunchConfig_t lc = {};
+  lc.gridDim = dim3((unsigned)((a.B * a.Hq + 7) / 8));
+  lc.blockDim = dim3(256);
+  lc.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  lc.attrs = attr;
+  lc.numAttrs = 1;
+  return launch_status(cudaLaunchKernelEx(&lc, paged_attn_join_kernel<T>, (const int32_t*)w.cum, (const float*)w.rows,
+                                          (const float*)w.prefix, static_cast<T*>(a.out), p));
+}
+
+int elem_of(const AttnCall& a) { return a.cache_dtype == B200_I8 || a.cache_dtype == B200_F8E4M3 ? 1 : 2; }
+
+// Slice [b0, b0 + n) of a call.
+AttnCall slice_of(const AttnCall& a, int64_t b0, int64_t n) {
+  AttnCall c = a;
+  const size_t isz = a.index_dtype == B200_I64 ? 8 : 4;
+  c.B = n;
+  c.q = static_cast<const char*>(a.q) + (size_t)(b0 * a.Hq * a.D) * 2;
+  c.out = static_cast<char*>(a.out) + (size_t)(b0 * a.Hq * a.D) * 2;
+  c.block_table = static_cast<const char*>(a.block_table) + (size_t)(b0 * a.max_blocks) * isz;
+  c.context_len = static_cast<const char*>(a.context_len) + (size_t)b0 * isz;
+  return c;
+}
+
+int attend(const AttnCall& a, const b200_launch_cfg* cfg, void* workspace, size_t workspace_bytes, cudaStream_t s) {
+  const PieceGeom g = piece_geometry(a.B, a.Hq, a.Hkv, a.D, a.block_size, a.num_blocks, a.max_blocks, elem_of(a), cfg);
+  const bool aligned = aligned16(a.q) && aligned16(a.out) && aligned16(a.k_cache) && aligned16(a.v_cache) &&
+                       aligned16(a.k_scale) && aligned16(a.v_scale);
+  const bool fast = g.fast && aligned && a.prefix_table == nullptr && !(cfg && (cfg->flags & 1));
+  if (!fast) {
+    if (a.D > 256) return B200_ERR_UNSUPPORTED;
+    if (a.cache_dtype == B200_I8) return launch_attn_generic_i8(a, s);
+    if (a.cache_dtype == B200_F8E4M3) return launch_attn_generic_e4m3(a, s);
+    return launch_attn_generic_16(a, s);
+  }
+  const SpaceBytes sb = space_bytes(g, a.Hq, 0);
+  if (workspace == nullptr || workspace_bytes < sb.cum + sb.rows + sb.prefix) return B200_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return B200_ERR_ALIGNMENT;
+  PieceSpace w{};
+  w.cum = static_cast<int32_t*>(workspace);
+  w.rows = reinterpret_cast<float*>(static_cast<char*>(workspace) + sb.cum);
+  w.prefix = reinterpret_cast<float*>(static_cast<char*>(workspace) + sb.cum + sb.rows);
+  for (int64_t b0 = 0; b0 < a.B; b0 += g.seqs) {
+    const AttnCall c = slice_of(a, b0, a.B - b0 < g.seqs ? a.B - b0 : g.seqs);
+    PieceGeom gs = g;
+    if (b0 > 0) gs.pdl = false;  // the kernel before is this call's join, which reads the workspace
+    int st = a.cache_dtype == B200_I8       ? launch_pieces_i8(c, gs, w, false, s)
+             : a.cache_dtype == B200_F8E4M3 ? launch_pieces_e4m3(c, gs, w, false, s)
+                                            : launch_pieces_16(c, gs, w, false, s);
+    if (st) return st;
+    st = B200_DISPATCH_HALF(a.dtype, [&] { return launch_join<scalar_t>(c, gs, w, s); });
+    if (st) return st;
+  }
+  return B200_OK;
+}
+
+// Checks the two entries share.
+int check_call(const AttnCall& a) {
+  if (a.B < 0 || a.Hq <= 0 || a.Hkv <= 0 || a.D <= 0 || a.num_blocks <= 0 || a.block_size <= 0 || a.max_blocks < 0 ||
+      a.Hq % a.Hkv != 0)
+    return B200_ERR_BAD_ARG;
+  if (a.B == 0) return B200_OK;
+  if (!a.q || !a.k_cache || !a.v_cache || !a.out || !a.context_len || (!a.block_table && a.max_blocks > 0))
+    return B200_ERR_BAD_ARG;
+  if (a.index_dtype != B200_I32 && a.index_dtype != B200_I64) return B200_ERR_UNSUPPORTED;
+  if (a.dtype != B200_F16 && a.dtype != B200_BF16) return B200_ERR_UNSUPPORTED;
+  if (a.cache_dtype == B200_I8 || a.cache_dtype == B200_F8E4M3) {
+    if (!a.k_scale || !a.v_scale) return B200_ERR_BAD_ARG;
+  } else if (a.cache_dtype != a.dtype) {
+    return B200_ERR_UNSUPPORTED;
+  }
+  if (a.Hq > 65535 || a.B > (1 << 24)) return B200_ERR_UNSUPPORTED;
+  return B200_OK;
+}
+
+}  // namespace
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" size_t b200_paged_attention_quant_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
+                                                            int64_t num_blocks, int64_t block_size,
+                                                            int64_t max_blocks, const b200_launch_cfg* cfg) {
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || num_blocks <= 0 || block_size <= 0 || max_blocks <= 0 || Hq % Hkv)
+    return 0;
+  const PieceGeom g = piece_geometry(B, Hq, Hkv, D, block_size, num_blocks, max_blocks, 1, cfg);
+  if (!g.fast) return 0;
+  const SpaceBytes sb = space_bytes(g, Hq, 0);
+  return sb.cum + sb.rows + sb.prefix;
+}
+
+extern "C" int b200_paged_attention_quant(const void* q, const void* k_cache, const void* v_cache,
+                                          const float* k_scale, const float* v_scale, const void* block_table,
+                                          const void* context_len, void* out, int64_t B, int64_t Hq, int64_t Hkv,
+                                          int64_t D, int64_t num_blocks, int64_t block_size, int64_t max_blocks,
+                                          float scale, int32_t dtype, int32_t cache_dtype, int32_t index_dtype,
+                                          void* workspace, size_t workspace_bytes, const b200_launch_cfg* cfg,
+                                          void* stream) {
+  if (int e = injected_error("paged_attention_quant")) return e;
+  if (scale <= 0.f && D > 0) scale = 1.0f / sqrtf((float)D);
+  const AttnCall a{q,  k_cache, v_cache, k_scale,    v_scale,    nullptr,    nullptr, block_table, context_len, out,
+                   B,  Hq,      Hkv,     D,          num_blocks, block_size, max_blocks, 0,        scale,       dtype,
+                   cache_dtype, index_dtype};
+  if (cache_dtype != B200_I8 && cache_dtype != B200_F8E4M3) return B200_ERR_UNSUPPORTED;
+  if (max_blocks <= 0) return B200_ERR_BAD_ARG;
+  if (int e = check_call(a)) return e;
+  if (B == 0) return B200_OK;
+  return attend(a, cfg, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" size_t b200_paged_attention_prefix_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
+                                                             int64_t num_blocks, int64_t block_size,
+                                                             int64_t max_prefix_blocks, int64_t max_blocks,
+                                                             int32_t cache_dtype, const b200_launch_cfg* cfg) {
+  (void)B, (void)Hq, (void)Hkv, (void)D, (void)num_blocks, (void)block_size, (void)max_prefix_blocks;
+  (void)max_blocks, (void)cache_dtype, (void)cfg;
+  return 0;
+}
+
+extern "C" int b200_paged_attention_prefix(const void* q, const void* k_cache, const void* v_cache,
+                                           const float* k_scale, const float* v_scale, const void* prefix_table,
+                                           const void* prefix_len, const void* block_table, const void* context_len,
+                                           void* out, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
+                                           int64_t num_blocks, int64_t block_size, int64_t max_prefix_blocks,
+                                           int64_t max_blocks, float scale, int32_t dtype, int32_t cache_dtype,
+                                           int32_t index_dtype, void* workspace, size_t workspace_bytes,
+                                           const b200_launch_cfg* cfg, void* stream) {
+  if (int e = injected_error("paged_attention_prefix")) return e;
+  if (scale <= 0.f && D > 0) scale = 1.0f / sqrtf((float)D);
+  const AttnCall a{q,  k_cache, v_cache, k_scale,    v_scale,    prefix_table, prefix_len, block_table, context_len,
+                   out, B,      Hq,      Hkv,        D,          num_blocks,   block_size, max_blocks,
+                   max_prefix_blocks, scale, dtype, cache_dtype, index_dtype};
+  if (max_prefix_blocks <= 0) return B200_ERR_BAD_ARG;
+  if (int e = check_call(a)) return e;
+  if (B == 0) return B200_OK;
+  if (!prefix_table || !prefix_len) return B200_ERR_BAD_ARG;
+  return attend(a, cfg, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+}

@@ -1,0 +1,745 @@
+// Decode attention over 16-bit or 8-bit paged caches whose result is joined
+// from pieces: the kernel that streams each sequence's own pages, the kernel
+// that joins pieces, and a general kernel for shapes outside the fast path.
+//
+// A piece is what one stretch of the keys of one query row leaves behind:
+// (m, l, o) with o[d] = sum_t 2^(x_t - m) v_t[d], l = sum_t 2^(x_t - m), x_t
+// the logits in log2 units.  Pieces of one row join exactly:
+//   M = max m_i,  out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i.
+//
+// 8-bit caches.  With codes c and scales s (k_t = ks_t ck_t, v_t = vs_t cv_t)
+//   x_t = scale log2(e) ks_t (q . ck_t)
+//   out = sum_t 2^(x_t) vs_t cv_t / sum_t 2^(x_t)
+// so the codes go to the tensor cores as they are (int8 and e4m3 codes are
+// exact in f16) and the scales meet fp32 values only: the kernel keeps
+// y_t = x_t + log2 vs_t, takes the running maximum over y, feeds the weights
+// w_t = 2^(y_t - m) (f16, half a step 2^-12) to the second product with the
+// bare codes, and sums l = sum_t w_t / vs_t in fp32.  Taking the maximum over y
+// rather than x keeps the largest weight at 1 however the value scales of the
+// tokens differ.  bf16 queries become f16 after an exact power-of-two scaling
+// of each head's row (its largest element to 2^13), undone in the logits; only
+// elements below 2^-37 of the row's largest lose bits.
+#pragma once
+
+#include <math.h>
+
+#include "common.cuh"
+#include "decode_mma.cuh"
+#include "kv8.cuh"
+#include "sm100.cuh"
+
+namespace b200 {
+
+constexpr int kPieceDim = 128;
+constexpr int kPiecePitch = kPieceDim + 4;  // floats of a piece row: o[128], m, l, pad
+constexpr int kMaxSeg = 2048;               // (sequence, head group) segments a launch takes
+
+// One attention call, as the C entries take it (host side).
+struct AttnCall {
+  const void *q, *k_cache, *v_cache;
+  const float *k_scale, *v_scale;  // null for 16-bit caches
+  const void *prefix_table, *prefix_len;  // null without a shared prefix
+  const void *block_table, *context_len;
+  void* out;
+  int64_t B, Hq, Hkv, D, num_blocks, block_size, max_blocks, max_prefix_blocks;
+  float scale;  // logits = scale * q . k
+  int32_t dtype, cache_dtype, index_dtype;
+};
+
+// Launch geometry of the fast path.
+struct PieceGeom {
+  bool fast;
+  int G, HG, n_hg, sub;   // query heads a kv head, kv heads a CTA, head groups, warps a kv head
+  int stages, grid;
+  int64_t seqs;           // sequences a launch takes (the batch runs in slices of this many)
+  uint32_t page_bytes, stage_bytes;
+  size_t smem;
+  bool pdl;
+};
+
+// Workspace: [segment prefix sums | pieces of the own pages | pieces of the prefix].
+struct PieceSpace {
+  int32_t* cum;   // nseg + 1
+  float* rows;    // piece (segment + range) * sub + warp, heads_cta rows each
+  float* prefix;  // split-major: [splits][seqs * Hq] rows
+  int prefix_splits;
+};
+
+int launch_pieces_i8(const AttnCall& a, const PieceGeom& g, const PieceSpace& w, bool overlap, cudaStream_t s);
+int launch_pieces_e4m3(const AttnCall& a, const PieceGeom& g, const PieceSpace& w, bool overlap, cudaStream_t s);
+int launch_pieces_16(const AttnCall& a, const PieceGeom& g, const PieceSpace& w, bool overlap, cudaStream_t s);
+int launch_attn_generic_i8(const AttnCall& a, cudaStream_t s);
+int launch_attn_generic_e4m3(const AttnCall& a, cudaStream_t s);
+int launch_attn_generic_16(const AttnCall& a, cudaStream_t s);
+
+// Block ids and lengths are int32 or int64 by a flag (uniform; read by one warp).
+struct IndexPtr {
+  const void* p;
+  int wide;
+  __device__ __forceinline__ int64_t at(int64_t i) const {
+    return wide ? __ldg(static_cast<const long long*>(p) + i) : (int64_t)__ldg(static_cast<const int*>(p) + i);
+  }
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+namespace {
+
+// ---------------------------------------------------------------------------
+// General kernel: any D <= 256, block size, head ratio and alignment.  One
+// CTA of four warps a (sequence, query head); tokens dealt round-robin to the warps, lanes
+// over the head dim; the prefix's pages first, then the sequence's own.
+// ---------------------------------------------------------------------------
+template <typename T, typename KV>
+__global__ void __launch_bounds__(128)
+    paged_attn_pieces_generic_kernel(const T* __restrict__ q, const KV* __restrict__ kc, const KV* __restrict__ vc,
+                                     const float* __restrict__ ks, const float* __restrict__ vs, IndexPtr ptab,
+                                     IndexPtr plen, IndexPtr btab, IndexPtr clen, T* __restrict__ out, int64_t Hq,
+                                     int64_t Hkv, int64_t D, int64_t num_blocks, int64_t bs, int64_t max_blocks,
+                                     int64_t max_prefix, float qscale) {
+  __shared__ float s_m[4], s_l[4], s_o[4][256];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t hq = blockIdx.x, b = blockIdx.y;
+  const int64_t kvh = hq / (Hq / Hkv);
+  const T* qr = q + (b * Hq + hq) * D;
+  float qv[8], ov[8];
+  for (int i = 0; i < 8; ++i) {
+    const int64_t d = lane + 32 * i;
+    qv[i] = d < D ? to_f32(qr[d]) : 0.f;
+    ov[i] = 0.f;
+  }
+  float mrun = -INFINITY, lrun = 0.f;
+  for (int part = ptab.p != nullptr ? 0 : 1; part < 2; ++part) {
+    const IndexPtr tab = part ? btab : ptab;
+    const int64_t at0 = part ? b * max_blocks : 0;
+    const int64_t ctx = part ? clen.at(b) : plen.at(0);
+    const int64_t nvb = ctx > 0 ? min((ctx + bs - 1) / bs, part ? max_blocks : max_prefix) : 0;
+    int64_t rank = 0;
+    for (int64_t j = 0; j < nvb; ++j) {
+      const int64_t id = tab.at(at0 + j);
+      if (id < 0 || id >= num_blocks) continue;
+      int64_t nt = ctx - rank * bs;
+      ++rank;
+      nt = nt < 0 ? 0 : (nt > bs ? bs : nt);
+      for (int64_t t = warp; t < nt; t += 4) {
+        const int64_t row = ((id * bs + t) * Hkv + kvh) * D;
+        float part_sum = 0.f;
+        for (int i = 0; i < 8; ++i) {
+          const int64_t d = lane + 32 * i;
+          if (d < D) part_sum = fmaf(qv[i], (float)kc[row + d], part_sum);
+        }
+        float sc = warp_sum(part_sum) * qscale, vscale = 1.f;
+        if constexpr (sizeof(KV) == 1) {
+          const int64_t sat = (id * Hkv + kvh) * bs + t;
+          sc *= ks[sat];
+          vscale = vs[sat];
+        }
+        const float mn = fmaxf(mrun, sc);
+        const float a = (mrun == -INFINITY) ? 0.f : exp2f(mrun - mn);
+        const float pw = sc == -INFINITY ? 0.f : exp2f(sc - mn);
+        lrun = lrun * a + pw;
+        for (int i = 0; i < 8; ++i) {
+          const int64_t d = lane + 32 * i;
+          ov[i] = ov[i] * a + (d < D ? pw * ((float)vc[row + d] * vscale) : 0.f);
+        }
+        mrun = mn;
+      }
+    }
+  }
+  if (lane == 0) {
+    s_m[warp] = mrun;
+    s_l[warp] = lrun;
+  }
+  for (int i = 0; i < 8; ++i) {
+    const int64_t d = lane + 32 * i;
+    if (d < D) s_o[warp][d] = ov[i];
+  }
+  __syncthreads();
+  float M = -INFINITY;
+  for (int w = 0; w < 4; ++w) M = fmaxf(M, s_m[w]);
+  float L = 0.f, wts[4];
+  for (int w = 0; w < 4; ++w) {
+    wts[w] = (s_m[w] == -INFINITY) ? s_l[w] : exp2f(s_m[w] - M);  // (no tokens: 0; NaN logits only: NaN)
+    L += wts[w] * s_l[w];
+  }
+  for (int64_t d = threadIdx.x; d < D; d += blockDim.x) {
+    float acc = 0.f;
+    for (int w = 0; w < 4; ++w) acc += wts[w] * s_o[w][d];
+    out[(b * Hq + hq) * D + d] = from_f32<T>(L == 0.f ? 0.f : acc / L);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// 8-bit pages on the tensor cores.  As in the 16-bit tiles tokens (S^T = K Q^T)
+// and head dims (O^T = V^T P^T) are the M side of m16n8k16 and the G query
+// heads its N side; what differs is which element an operand register holds, since one
+// 8x8 ldmatrix of 16-bit cells covers 16 codes a row:
+//   K: a cell pair of lane (r, q) holds the codes d = 16j + 4q + {0..3} of
+//      token r; they are k = {2q, 2q+1, 2q+8, 2q+9} of the j-th k-step, and
+//      the query fragments are loaded in that order
+//   V: a transposed cell pair holds d = 16j + 2r + {0, 1} of tokens 2q, 2q+1;
+//      rows r and r + 8 of the j-th m-tile are the dims 16j + 2r and 16j + 2r + 1
+// One 16-token page of a head is 8 ldmatrix.x4, 64 code pairs to f16 and
+// 16 mma.sync.
+// ---------------------------------------------------------------------------
+template <typename T, int G>
+__device__ __forceinline__ void load_q_frags8(const T* __restrict__ qrow0, int lane, float qscale,
+                                              uint32_t (&qb)[8][2], float& slA, float& slB) {
+  const int qh = lane >> 2, qc = (lane & 3) * 4;
+  const T* qr = qrow0 + (qh < G ? qh : 0) * kD;
+  float f[8][4];
+  float amax = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint2 raw = *reinterpret_cast<const uint2*>(qr + 16 * j + qc);
+    const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[j][i] = qh < G ? to_f32(e[i]) : 0.f;
+      amax = fmaxf(amax, fabsf(f[j][i]));
+    }
+  }
+  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+  amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+  // the row's largest element to [2^13, 2^14); zero and non-finite rows stay
+  int e = (int)(__float_as_uint(amax) >> 23) - 127;
+  e = (amax == 0.f || e > 127) ? 13 : (e < -100 ? -100 : e);
+  const float up = __uint_as_float((uint32_t)(13 - e + 127) << 23);
+  const float down = __uint_as_float((uint32_t)(e - 13 + 127) << 23);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    qb[j][0] = pack_pair<__half>(f[j][0] * up, f[j][1] * up);
+    qb[j][1] = pack_pair<__half>(f[j][2] * up, f[j][3] * up);
+  }
+  const float sl = qscale * down;
+  slA = __shfl_sync(0xffffffffu, sl, (lane & 3) * 8);
+  slB = __shfl_sync(0xffffffffu, sl, (lane & 3) * 8 + 4);
+}
+
+// One page (ntok tokens of kv head w: codes at kb / vb as [head][token][128]
+// rows, 128-byte swizzled; scales at ksp / vsp as [head][token]).
+template <typename KV>
+__device__ __forceinline__ void mma_page8(uint32_t kb, uint32_t vb, const float* __restrict__ ksp,
+                                          const float* __restrict__ vsp, int ntok, int w, int bs, int lane, float slA,
+                                          float slB, const uint32_t (&qb)[8][2], float (&o)[8][4], float (&mu)[2],
+                                          float (&lp)[2]) {
+  const int mat = lane >> 3, mrow = lane & 7;
+  const int tr = lane >> 2, tq = (lane & 3) * 2;
+  for (int t0 = 0; t0 < ntok; t0 += 16) {
+    const int row = w * bs + t0 + (mat & 1) * 8 + mrow;
+    const int sw = row & 7;
+    float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+    uint32_t kr[4][4], vr[4][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      ldsm_x4(kb + row * 128 + (((2 * j + (mat >> 1)) ^ sw) << 4), kr[j][0], kr[j][1], kr[j][2], kr[j][3]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      ldsm_x4_t(vb + row * 128 + (((2 * j + (mat >> 1)) ^ sw) << 4), vr[j][0], vr[j][1], vr[j][2], vr[j][3]);
+    const bool ok0 = t0 + tr < ntok, ok1 = t0 + tr + 8 < ntok;
+    const int at = w * bs + t0 + tr;
+    const float k0 = ksp[at], k1 = ksp[at + 8];
+    float lv0, iv0, lv1, iv1;
+    kv8_value_scale(vsp[at], lv0, iv0);
+    kv8_value_scale(vsp[at + 8], lv1, iv1);
+    iv0 = ok0 ? iv0 : 0.f;
+    iv1 = ok1 ? iv1 : 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      mma16816<__half>(s0, kv8_pair<KV, 0, 1>(kr[j][0]), kv8_pair<KV, 0, 1>(kr[j][1]), kv8_pair<KV, 2, 3>(kr[j][0]),
+                       kv8_pair<KV, 2, 3>(kr[j][1]), qb[2 * j][0], qb[2 * j][1]);
+      mma16816<__half>(s1, kv8_pair<KV, 0, 1>(kr[j][2]), kv8_pair<KV, 0, 1>(kr[j][3]), kv8_pair<KV, 2, 3>(kr[j][2]),
+                       kv8_pair<KV, 2, 3>(kr[j][3]), qb[2 * j + 1][0], qb[2 * j + 1][1]);
+    }
+    // y[0]/y[1]: token tr of heads 2(lane%4), +1; y[2]/y[3]: token tr + 8
+    float y[4];
+    y[0] = ok0 ? fmaf(s0[0] + s1[0], k0 * slA, lv0) : -INFINITY;
+    y[1] = ok0 ? fmaf(s0[1] + s1[1], k0 * slB, lv0) : -INFINITY;
+    y[2] = ok1 ? fmaf(s0[2] + s1[2], k1 * slA, lv1) : -INFINITY;
+    y[3] = ok1 ? fmaf(s0[3] + s1[3], k1 * slB, lv1) : -INFINITY;
+    float mA = fmaxf(y[0], y[2]), mB = fmaxf(y[1], y[3]);
+#pragma unroll
+    for (int off = 4; off <= 16; off <<= 1) {
+      mA = fmaxf(mA, __shfl_xor_sync(0xffffffffu, mA, off));
+      mB = fmaxf(mB, __shfl_xor_sync(0xffffffffu, mB, off));
+    }
+    raise_max(mu[0], mA, lp[0], o, 0);
+    raise_max(mu[1], mB, lp[1], o, 1);
+    const float nA = mu[0] == -INFINITY ? 0.f : mu[0], nB = mu[1] == -INFINITY ? 0.f : mu[1];
+    const float p0 = ex2(y[0] - nA), p2 = ex2(y[2] - nA);
+    const float p1 = ex2(y[1] - nB), p3 = ex2(y[3] - nB);
+    lp[0] = fmaf(p0, iv0, fmaf(p2, iv1, lp[0]));
+    lp[1] = fmaf(p1, iv0, fmaf(p3, iv1, lp[1]));
+    const uint32_t b0 = movm_t(pack_pair<__half>(p0, p1));
+    const uint32_t b1 = movm_t(pack_pair<__half>(p2, p3));
+    if (t0 + 16 > ntok) {
+      // tokens past the end may hold any code (e4m3 has a NaN): zero their V.
+      // Each register holds two codes of token tq and two of token tq + 1.
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        vr[j][0] = mask_pair(vr[j][0], t0 + tq, ntok);
+        vr[j][1] = mask_pair(vr[j][1], t0 + 8 + tq, ntok);
+        vr[j][2] = mask_pair(vr[j][2], t0 + tq, ntok);
+        vr[j][3] = mask_pair(vr[j][3], t0 + 8 + tq, ntok);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        mma16816<__half>(o[2 * j + u], kv8_pair<KV, 0, 2>(vr[j][2 * u]), kv8_pair<KV, 1, 3>(vr[j][2 * u]),
+                         kv8_pair<KV, 0, 2>(vr[j][2 * u + 1]), kv8_pair<KV, 1, 3>(vr[j][2 * u + 1]), b0, b1);
+    }
+  }
+}
+
+// Rows of the 8-bit accumulator (dims 16mt + 2r of o[mt][0..1], 16mt + 2r + 1
+// of o[mt][2..3]), normalised, as 8-byte stores of four dims.
+template <typename T, int G>
+__device__ __forceinline__ void store_rows8(T* __restrict__ orow0, const float (&o)[8][4], float lA, float lB,
+                                            int lane) {
+  const float iA = lA == 0.f ? 0.f : 1.f / lA, iB = lB == 0.f ? 0.f : 1.f / lB;
+  const int h = lane >> 2, c = (lane & 3) * 4;
+  T* orow = orow0 + (h < G ? h : 0) * kD;
+#pragma unroll
+  for (int mt = 0; mt < 8; ++mt) {
+    const uint32_t r0 = movm_t(pack_pair<T>(o[mt][0] * iA, o[mt][1] * iB));
+    const uint32_t r1 = movm_t(pack_pair<T>(o[mt][2] * iA, o[mt][3] * iB));
+    if (h < G)
+      *reinterpret_cast<uint2*>(orow + 16 * mt + c) =
+          make_uint2(__byte_perm(r0, r1, 0x5410), __byte_perm(r0, r1, 0x7632));
+  }
+}
+
+template <int G>
+__device__ __forceinline__ void store_piece8(float* __restrict__ row0, const float (&o)[8][4], const float (&mu)[2],
+                                             float lA, float lB, int lane) {
+  const int hA = (lane & 3) * 2, hB = hA + 1, r = lane >> 2;
+#pragma unroll
+  for (int mt = 0; mt < 8; ++mt) {
+    if (hA < G) *reinterpret_cast<float2*>(row0 + hA * kPiecePitch + 16 * mt + 2 * r) = make_float2(o[mt][0], o[mt][2]);
+    if (hB < G) *reinterpret_cast<float2*>(row0 + hB * kPiecePitch + 16 * mt + 2 * r) = make_float2(o[mt][1], o[mt][3]);
+  }
+  if (r == 0) {
+    if (hA < G) *reinterpret_cast<float2*>(row0 + hA * kPiecePitch + kD) = make_float2(mu[0], lA);
+    if (hB < G) *reinterpret_cast<float2*>(row0 + hB * kPiecePitch + kD) = make_float2(mu[1], lB);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Streaming kernel.  All segments' block-table entries (segment s = hg * B + b)
+// laid end to end are cut into one equal contiguous range a CTA, one CTA an
+// SM.  The producer warp walks its range and fills a ring of stages with TMA: a
+// stage is `sub` pages of one segment (K and V boxes of HG heads, and for
+// 8-bit caches the pages' scales by bulk copies), so that every stage
+// feeds HG * sub = up to eight consumer warps: warp w takes head w % HG of page
+// w / HG.  An end marker closes a segment: a segment that one
+// range holds and one warp a head covers is normalised and written; otherwise
+// each warp writes its piece at row (segment + range) * sub + w / HG -- the
+// (segment, range) pairs of a call, taken in order, have distinct sums, so a
+// piece's place needs no counters -- and the join kernel reads them.  No state is
+// kept between calls.
+// ---------------------------------------------------------------------------
+struct PiecesParams {
+  int64_t B, Hq, Hkv, num_blocks, max_blocks;
+  int bs, HG, n_hg, sub, stages, nseg;
+  int always;   // write every segment as pieces (a prefix joins them)
+  int overlap;  // launched beside the previous grid of the call: wait for it at the end
+  uint32_t page_bytes, stage_bytes;
+  float qscale;  // scale * log2(e)
+};
+
+constexpr int kMaxSub = 8;
+struct StageMeta {
+  int kind;  // 0 pages, 1 end of segment, 2 end of stream
+  int seg, piece, direct;
+  int ntok[kMaxSub];
+};
+
+__device__ __forceinline__ int64_t range_lo(int64_t c, int64_t E, int64_t R) { return c * E / R; }
+__device__ __forceinline__ int range_of(int64_t e, int64_t E, int64_t R) { return (int)(((e + 1) * R + E - 1) / E - 1); }
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+      "r"(bytes), "r"(bar)
+      : "memory");
+}
+
+template <typename T, typename KV, int G>
+__global__ void __launch_bounds__(288, 1)
+    paged_attn_pieces_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                             const float* __restrict__ k_scale, const float* __restrict__ v_scale,
+                             const T* __restrict__ q, IndexPtr btab, IndexPtr clen, T* __restrict__ out,
+                             float* __restrict__ ws_rows, int32_t* __restrict__ ws_cum, PiecesParams p) {
+  constexpr bool k8 = sizeof(KV) == 1;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int HG = p.HG, bs = p.bs, consumers = HG * p.sub;
+  const int heads_cta = HG * G;
+  const int64_t B = p.B;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + p.stages * p.stage_bytes);
+  uint64_t* empty_bar = full_bar + p.stages;
+  StageMeta* meta = reinterpret_cast<StageMeta*>(empty_bar + p.stages);
+  int* s_cum = reinterpret_cast<int*>(meta + p.stages);
+  int* s_ctx = s_cum + (p.nseg + 1);
+  int* chunk_id = s_ctx + B;
+  int* chunk_ntok = chunk_id + 32;
+  int* s_abort = chunk_ntok + 32;
+
+  // the join kernel may be scheduled; it waits for this grid
+  asm volatile("griddepcontrol.launch_dependents;");
+  // ---- prologue: contexts, entries before each segment, barriers
+  if (warp == consumers) {
+    const int64_t most = p.max_blocks * bs;
+    for (int64_t b = lane; b < B; b += 32) {
+      const int64_t c = clen.at(b);
+      s_ctx[b] = (int)(c < 0 ? 0 : (c < most ? c : most));
+    }
+    __syncwarp();
+    int run = 0;
+    for (int s0 = 0; s0 < p.nseg; s0 += 32) {
+      const int s = s0 + lane;
+      const int e = s < p.nseg ? (s_ctx[s % (int)B] + bs - 1) / bs : 0;
+      int incl = e;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+      }
+      if (s < p.nseg) s_cum[s + 1] = run + incl;
+      run += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    if (lane == 0) {
+      s_cum[0] = 0;
+      *s_abort = 0;
+      for (int s = 0; s < p.stages; ++s) {
+        sm100::mbar_init(sm100::smem_u32(&full_bar[s]), 1);
+        sm100::mbar_init(sm100::smem_u32(&empty_bar[s]), consumers);
+      }
+      sm100::fence_barrier_init();
+    }
+  }
+  __syncthreads();
+  const int64_t E = s_cum[p.nseg];
+  const int64_t R = E < (int64_t)gridDim.x ? E : (int64_t)gridDim.x;  // ranges
+  const int c = blockIdx.x;
+
+  // Programmatic launch (cfg flags bit 3): what is above and the producer's
+  // walk of the block table up to its first copy overlap the previous kernel,
+  // whose caller guarantees that it writes neither context_len nor block_table.  No
+  // q, page, output or workspace byte is touched before the wait.  A no-op for an
+  // ordinary launch.  `overlap`: the previous kernel is the same call's prefix
+  // grid, which shares nothing with this one; the wait comes at the end.
+  if (warp < consumers && !p.overlap) asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (c == 0 && warp < consumers)
+    for (int s = threadIdx.x; s <= p.nseg; s += consumers * 32) ws_cum[s] = s_cum[s];
+
+  if (c < R && warp == consumers) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0) {
+      sm100::tma_prefetch_desc(&tm_k);
+      sm100::tma_prefetch_desc(&tm_v);
+    }
+    const uint32_t base = sm100::smem_u32(smem);
+    const uint32_t box = (uint32_t)(HG * bs * 128);  // one 128-byte-wide box: all of an 8-bit tile, half of a 16-bit one
+    const uint32_t page_tx = k8 ? 2 * box + (uint32_t)(2 * HG * bs * 4) : 4 * box;
+    const unsigned lt_mask = (1u << lane) - 1u;
+    int it = 0;
+    bool ok = true, waited = p.overlap != 0;
+    // lane 0: the next stage, free to fill; false when the wait gave up
+    auto acquire = [&]() -> bool {
+      if (*(volatile int*)s_abort) return false;
+      return sm100::mbar_wait(sm100::smem_u32(&empty_bar[it % p.stages]), ((it / p.stages) & 1) ^ 1);
+    };
+    auto marker = [&](int kind, int seg, int piece, int direct) -> bool {
+      if (!acquire()) return false;
+      StageMeta& m = meta[it % p.stages];
+      m.kind = kind, m.seg = seg, m.piece = piece, m.direct = direct;
+      sm100::mbar_arrive(sm100::smem_u32(&full_bar[it % p.stages]));
+      ++it;
+      return true;
+    };
+    const int64_t lo = range_lo(c, E, R), hi = range_lo(c + 1, E, R);
+    int s = 0;
+    {
+      int l = 0, r = p.nseg;  // cum[l] <= lo < cum[r]
+      while (r - l > 1) {
+        const int mid = (l + r) >> 1;
+        if (s_cum[mid] <= lo) l = mid;
+        else r = mid;
+      }
+      s = l;
+    }
+    int64_t e = lo;
+    while (e < hi && ok) {
+      while (s_cum[s + 1] == s_cum[s]) ++s;
+      const int64_t b = s % B;
+      const int hg = s / (int)B;
+      const int64_t segs = s_cum[s], sege = s_cum[s + 1];
+      const int j0 = (int)(e - segs), j1 = (int)((hi < sege ? hi : sege) - segs);
+      const int ctx = s_ctx[b];
+      const int64_t bt0 = b * p.max_blocks;
+      // dropped entries before j0 shift the token ranks of this range
+      int inval = 0;
+      for (int jb = 0; jb < j0; jb += 256) {
+        int64_t v[8];
+#pragma unroll
+        for (int rr = 0; rr < 8; ++rr) {
+          const int j = jb + rr * 32 + lane;
+          v[rr] = j < j0 ? btab.at(bt0 + j) : 0;
+        }
+#pragma unroll
+        for (int rr = 0; rr < 8; ++rr) inval += (v[rr] < 0 || v[rr] >= p.num_blocks) ? 1 : 0;
+      }
+      inval = __reduce_add_sync(0xffffffffu, inval);
+      int fill = 0;  // pages already in the open stage (lane 0)
+      for (int jj = j0; jj < j1 && ok; jj += 32) {
+        const int j = jj + lane;
+        const bool in = j < j1;
+        const int64_t id = in ? btab.at(bt0 + j) : -1;
+        const bool valid = in && id >= 0 && id < p.num_blocks;
+        const unsigned ib = __ballot_sync(0xffffffffu, in && !valid);
+        const int rank = j - (inval + __popc(ib & lt_mask));
+        int64_t left = (int64_t)ctx - (int64_t)rank * bs;
+        const int nt = (int)(left < 0 ? 0 : (left > bs ? bs : left));
+        const bool use = valid && nt > 0;
+        const unsigned ub = __ballot_sync(0xffffffffu, use);
+        if (use) {
+          const int k = __popc(ub & lt_mask);
+          chunk_id[k] = (int)id;
+          chunk_ntok[k] = nt;
+        }
+        inval += __popc(ib);
+        __syncwarp();
+        if (lane == 0) {
+          const int n = __popc(ub);
+          for (int u = 0; u < n && ok; ++u) {
+            const int st = it % p.stages;
+            if (fill == 0) {
+              ok = acquire();
+              if (!ok) break;
+              StageMeta& m = meta[st];
+              m.kind = 0, m.seg = s;
+              for (int i = 0; i < p.sub; ++i) m.ntok[i] = 0;
+              if (!waited) {  // programmatic launch: the first copy waits for the previous kernel
+                asm volatile("griddepcontrol.wait;" ::: "memory");
+                waited = true;
+              }
+            }
+            meta[st].ntok[fill] = chunk_ntok[u];
+            const uint32_t fb = sm100::smem_u32(&full_bar[st]);
+            const uint32_t dst = base + st * p.stage_bytes + fill * p.page_bytes;
+            const int id32 = chunk_id[u];
+            const int32_t tok0 = id32 * bs, h0 = hg * HG;
+            ++fill;
+            const bool last = fill == p.sub || (u == n - 1 && jj + 32 >= j1);
+            // the stage's one arrival comes with its last page; earlier pages only add bytes
+            if (last) sm100::mbar_arrive_expect_tx(fb, page_tx);
+            else asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(fb), "r"(page_tx) : "memory");
+            if constexpr (k8) {
+              sm100::tma_load_3d(dst, &tm_k, fb, 0, tok0, h0);
+              sm100::tma_load_3d(dst + box, &tm_v, fb, 0, tok0, h0);
+              const uint32_t sb = (uint32_t)(HG * bs * 4);
+              const int64_t sat = ((int64_t)id32 * p.Hkv + h0) * bs;
+              bulk_load(dst + 2 * box, k_scale + sat, sb, fb);
+              bulk_load(dst + 2 * box + sb, v_scale + sat, sb, fb);
+            } else {
+              sm100::tma_load_3d(dst, &tm_k, fb, 0, tok0, h0);
+              sm100::tma_load_3d(dst + box, &tm_k, fb, 64, tok0, h0);
+              sm100::tma_load_3d(dst + 2 * box, &tm_v, fb, 0, tok0, h0);
+              sm100::tma_load_3d(dst + 3 * box, &tm_v, fb, 64, tok0, h0);
+            }
+            if (last) {
+              ++it;
+              fill = 0;
+            }
+          }
+          if (ok && fill > 0 && jj + 32 >= j1) {
+            // the range's last pages were dropped ids: close the open stage
+            sm100::mbar_arrive(sm100::smem_u32(&full_bar[it % p.stages]));
+            ++it;
+            fill = 0;
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        __syncwarp();
+      }
+      if (lane == 0 && ok) {
+        const bool one = range_of(segs, E, R) == range_of(sege - 1, E, R);
+        ok = marker(1, s, s + c, one && p.sub == 1 && !p.always);
+      }
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      e = segs + j1;
+      if (e == sege) ++s;
+    }
+    if (lane == 0) {
+      if (ok) ok = marker(2, 0, 0, 0);
+      if (!ok) {
+        b200_dev_error(kDevErrTimeoutEmpty);
+        atomicExch(s_abort, 1);
+      }
+      // never leave with copies landing in shared memory
+      for (int i = it - 1; i >= 0 && i >= it - p.stages; --i)
+        if (!sm100::mbar_wait(sm100::smem_u32(&full_bar[i % p.stages]), (i / p.stages) & 1))
+          b200_dev_error(kDevErrTimeoutFull);
+    }
+  } else if (c < R && warp < consumers) {
+    // ------------------------------------------------------------ consumers
+    const int w = warp % HG, slot = warp / HG;
+    const uint32_t base = sm100::smem_u32(smem);
+    const uint32_t box = (uint32_t)(HG * bs * 128);
+    uint32_t qb[8][2];
+    float o[8][4];
+    float mu[2] = {-INFINITY, -INFINITY}, lp[2] = {0.f, 0.f};
+    float slA = p.qscale, slB = p.qscale;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    int cur = -1;
+    for (int it = 0;; ++it) {
+      const int st = it % p.stages;
+      if (!sm100::mbar_wait_warp(sm100::smem_u32(&full_bar[st]), (it / p.stages) & 1)) {
+        b200_dev_error(kDevErrTimeoutFull);
+        atomicExch(s_abort, 1);
+        break;
+      }
+      const int kind = meta[st].kind, seg = meta[st].seg;
+      if (kind == 0) {
+        const int ntok = meta[st].ntok[slot];
+        const int64_t b = seg % B, kvh = (int64_t)(seg / B) * HG + w;
+        const T* qrow = q + (b * p.Hq + kvh * G) * kD;
+        if (seg != cur) {
+          cur = seg;
+          if constexpr (k8) load_q_frags8<T, G>(qrow, lane, p.qscale, qb, slA, slB);
+          else load_q_frags<T, G>(qrow, lane, qb);
+        }
+        const uint32_t pg = base + st * p.stage_bytes + slot * p.page_bytes;
+        if constexpr (k8) {
+          const float* sc = reinterpret_cast<const float*>(smem + st * p.stage_bytes + slot * p.page_bytes + 2 * box);
+          mma_page8<KV>(pg, pg + box, sc, sc + HG * bs, ntok, w, bs, lane, slA, slB, qb, o, mu, lp);
+        } else {
+          mma_page<T>(pg, pg + 2 * box, ntok, w, bs, lane, box, p.qscale, qb, o, mu, lp);
+        }
+      } else if (kind == 1) {
+        const float lA = head_sum(lp[0]), lB = head_sum(lp[1]);
+        const int64_t b = seg % B, hg = seg / B;
+        if (meta[st].direct) {
+          T* orow = out + (b * p.Hq + hg * heads_cta + w * G) * kD;
+          if constexpr (k8) store_rows8<T, G>(orow, o, lA, lB, lane);
+          else store_rows<T, G>(orow, o, lA, lB, lane);
+        } else {
+          float* row0 = ws_rows + (((int64_t)meta[st].piece * p.sub + slot) * heads_cta + w * G) * kPiecePitch;
+          if constexpr (k8) store_piece8<G>(row0, o, mu, lA, lB, lane);
+          else store_partial<G>(row0, kPiecePitch, row0 + kD, kPiecePitch, o, mu, lA, lB, lane);
+        }
+        mu[0] = mu[1] = -INFINITY;
+        lp[0] = lp[1] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+        cur = -1;
+      }
+      __syncwarp();
+      if (lane == 0) sm100::mbar_arrive(sm100::smem_u32(&empty_bar[st]));
+      if (kind == 2) break;
+    }
+  }
+  // this grid counts as done only when the previous one is
+  if (threadIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+// ---------------------------------------------------------------------------
+// Host: tensor maps and launch of one slice of the batch (a.B <= kMaxSeg / n_hg).
+// ---------------------------------------------------------------------------
+template <typename T, typename KV, int G>
+int launch_pieces(const AttnCall& a, const PieceGeom& g, const PieceSpace& w, bool overlap, cudaStream_t stream) {
+  CUtensorMap tk, tv;
+  constexpr bool k8 = sizeof(KV) == 1;
+  constexpr uint64_t el = sizeof(KV);
+  const CUtensorMapDataType dt = k8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                    : (std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                      : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16);
+  // dims (d, token slot, head): a box of 128 bytes of dims x bs tokens x HG heads
+  // lands as rows ordered (head, token) of 128 bytes, swizzled in 8-row atoms
+  const uint64_t dims[3] = {(uint64_t)kD, (uint64_t)(a.num_blocks * a.block_size), (uint64_t)a.Hkv};
+  const uint64_t strides[2] = {(uint64_t)a.Hkv * kD * el, (uint64_t)kD * el};
+  const uint32_t box[3] = {(uint32_t)(128 / el), (uint32_t)a.block_size, (uint32_t)g.HG};
+  int st = encode_tensor_map(&tk, dt, 3, a.k_cache, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (st) return st;
+  st = encode_tensor_map(&tv, dt, 3, a.v_cache, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  if (st) return st;
+  PiecesParams p{};
+  p.B = a.B, p.Hq = a.Hq, p.Hkv = a.Hkv, p.num_blocks = a.num_blocks, p.max_blocks = a.max_blocks;
+  p.bs = (int)a.block_size, p.HG = g.HG, p.n_hg = g.n_hg, p.sub = g.sub, p.stages = g.stages;
+  p.nseg = (int)(g.n_hg * a.B);
+  p.always = a.prefix_table != nullptr;
+  p.overlap = overlap;
+  p.page_bytes = g.page_bytes, p.stage_bytes = g.stage_bytes;
+  p.qscale = a.scale * 1.4426950408889634f;
+  auto kern = paged_attn_pieces_kernel<T, KV, G>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)g.smem);
+  if (e != cudaSuccess) return launch_status(e);
+  cudaLaunchConfig_t lc = {};
+  lc.gridDim = dim3((unsigned)g.grid);
+  lc.blockDim = dim3((unsigned)((g.HG * g.sub + 1) * 32));
+  lc.dynamicSmemBytes = g.smem;
+  lc.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  lc.attrs = attr;
+  lc.numAttrs = (overlap || g.pdl) ? 1 : 0;
+  const int wide = a.index_dtype == B200_I64;
+  e = cudaLaunchKernelEx(&lc, kern, tk, tv, a.k_scale, a.v_scale, static_cast<const T*>(a.q),
+                         IndexPtr{a.block_table, wide}, IndexPtr{a.context_len, wide}, static_cast<T*>(a.out), w.rows,
+                         w.cum, p);
+  return launch_status(e);
+}
+
+template <typename T, typename KV>
+int launch_pieces_by_group(const AttnCall& a, const PieceGeom& g, const PieceSpace& w, bool overlap, cudaStream_t s) {
+  switch (g.G) {
+    case 1: return launch_pieces<T, KV, 1>(a, g, w, overlap, s);
+    case 2: return launch_pieces<T, KV, 2>(a, g, w, overlap, s);
+    case 4: return launch_pieces<T, KV, 4>(a, g, w, overlap, s);
+    default: return launch_pieces<T, KV, 8>(a, g, w, overlap, s);
+  }
+}
+
+template <typename T, typename KV>
+int launch_generic(const AttnCall& a, cudaStream_t s) {
+  const int wide = a.index_dtype == B200_I64;
+  for (int64_t b0 = 0; b0 < a.B; b0 += 65535) {
+    const int64_t n = a.B - b0 < 65535 ? a.B - b0 : 65535;
+    const size_t isz = wide ? 8 : 4;
+    auto at = [&](const void* p, int64_t i) {
+      return static_cast<const void*>(static_cast<const char*>(p) + (size_t)i * isz);
+    };
+    paged_attn_pieces_generic_kernel<T, KV><<<dim3((unsigned)a.Hq, (unsigned)n), 128, 0, s>>>(
+        static_cast<const T*>(a.q) + b0 * a.Hq * a.D, static_cast<const KV*>(a.k_cache),
+        static_cast<const KV*>(a.v_cache), a.k_scale, a.v_scale, IndexPtr{a.prefix_table, wide},
+        IndexPtr{a.prefix_len, wide}, IndexPtr{at(a.block_table, b0 * a.max_blocks), wide},
+        IndexPtr{at(a.context_len, b0), wide}, static_cast<T*>(a.out) + b0 * a.Hq * a.D, a.Hq, a.Hkv, a.D,
+        a.num_blocks, a.block_size, a.max_blocks, a.max_prefix_blocks, a.scale * 1.4426950408889634f);
+    if (cudaError_t e = cudaGetLastError(); e != cudaSuccess) return launch_status(e);
+  }
+  return B200_OK;
+}
+
+}  // namespace
+}  // namespace b200
+
+#define B200_DEFINE_PIECE_LAUNCHERS(NAME, KVT)                                                                  \
+  namespace b200 {                                                                                              \
+  int launch_pieces_##NAME(const AttnCall& a, const PieceGeom& g, const PieceSpace& w, bool overlap,            \
+                           cudaStream_t s) {                                                                    \
+    return B200_DISPATCH_HALF(a.dtype, [&] { return launch_pieces_by_group<scalar_t, KVT>(a, g, w, overlap, s); }); \
+  }                                                                                                             \
+  int launch_attn_generic_##NAME(const AttnCall& a, cudaStream_t s) {                                           \
+    return B200_DISPATCH_HALF(a.dtype, [&] { return launch_generic<scalar_t, KVT>(a, s); });                    \
+  }                                                                                                             \
+  }

@@ -152,6 +152,13 @@ const char* b200_kernel_list(void) {
          "paged_decode_flat_kernel\n"
          "paged_decode_kernel\n"
          "paged_decode_generic_kernel\n"
+         "kv_quant_append_kernel\n"
+         "kv_quant_append_generic_kernel\n"
+         "slot_claim_kernel\n"
+         "kv_dequant_kernel\n"
+         "paged_attn_pieces_kernel\n"
+         "paged_attn_join_kernel\n"
+         "paged_attn_pieces_generic_kernel\n"
          "int8_gemm_pair_kernel\n"
          "int8_gemm_tcgen05_kernel\n"
          "int8_gemm_stream_kernel\n"
@@ -291,6 +298,15 @@ const char* b200_query_config_space(const char* op, int64_t rows) {
     field("tile_m", {0, 2 * (int64_t)sms}, "CTAs of the persistent grid (0: one per SM)");
     field("tile_k", {0, 10, 25, 50}, "percent of the block-table entries handed out as claimed chunks (0: none)");
     field("tile_n", {0, 1, 2, 8}, "pages per claimed chunk (0: 4)");
+  } else if (o == "rope_kv_append_paged_quant") {
+    kernel = "kv_quant_append_kernel";
+    field("rows_per_cta", {0, 1, 2, 3, 6}, "rows of a token per thread (0: 1 up to 512 tokens, else 3)");
+  } else if (o == "paged_kv_dequant") {
+    kernel = "kv_dequant_kernel";
+  } else if (o == "paged_attention_quant" || o == "paged_attention_prefix") {
+    kernel = "paged_attn_pieces_kernel";
+    field("stages", {0, 2, 3, 4, 6}, "page ring depth (0: about 132 KB of pages in flight)");
+    field("rows_per_cta", {0, 1, 2, 4, 8}, "kv heads per CTA, a divisor of H_kv (0: the largest <= 8 that fits)");
   } else if (o == "quant_matmul") {
     if (rows > 0 && rows <= 64) {
       kernel = "int8_gemm_stream_kernel";
