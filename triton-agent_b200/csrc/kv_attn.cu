@@ -5,7 +5,7 @@
 
 B200_DEVICE_ERROR_WORD()
 
-#include "kv_attn.cuh"
+#include "prefix_attn.cuh"
 
 namespace b200 {
 namespace {
@@ -124,7 +124,7 @@ PieceGeom piece_geometry(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t 
   if (g.seqs < 1 || g.n_hg * g.seqs * max_blocks >= (1ll << 31)) return g;
   g.grid = device_sm_count();
   g.pdl = cfg && (cfg->flags & 8);
-  const size_t fixed = 1024 + (size_t)(g.n_hg * g.seqs + 1) * 4 + (size_t)g.seqs * 4 + 65 * 4;
+  const size_t fixed = 1024 + (size_t)(g.n_hg * g.seqs + 1) * 4 + (size_t)g.seqs * 4 + 66 * 4;
   const size_t per = g.stage_bytes + 16 + sizeof(StageMeta);
   int stages = (cfg && cfg->stages > 0) ? cfg->stages : (int)(132 * 1024 / g.stage_bytes);
   if (stages < 2) stages = 2;
@@ -134,6 +134,22 @@ PieceGeom piece_geometry(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t 
   g.smem = stages * per + fixed;
   g.fast = g.smem <= kSmemMost;
   return g;
+}
+
+// Splits of the prefix.  A CTA of the prefix kernel is one (split, pair of
+// 128-row tiles, kv head) and holds its SM alone, so the time is about
+// waves * (key tiles a split + the CTA's start and end, about three tiles' time); the
+// fewest splits within the minimum, since each leaves a piece a row to join.
+// The length lives on the device; the table's size bounds it.
+int prefix_splits(const PieceGeom& g, int64_t B, int64_t Hkv, int64_t bs, int64_t max_prefix_blocks) {
+  const int64_t ppt = 128 / bs, tiles = (max_prefix_blocks + ppt - 1) / ppt;
+  const int64_t units = (B * g.G + 255) / 256 * Hkv;
+  int64_t best = 1, best_cost = INT64_MAX;
+  for (int64_t s = 1; s <= tiles && s <= g.grid; ++s) {
+    const int64_t cost = (units * s + g.grid - 1) / g.grid * ((tiles + s - 1) / s + 3);
+    if (cost < best_cost) best = s, best_cost = cost;
+  }
+  return (int)best;
 }
 
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
@@ -181,18 +197,26 @@ AttnCall slice_of(const AttnCall& a, int64_t b0, int64_t n) {
   return c;
 }
 
+// The prefix kernel's tiles: whole pages within 128 keys.
+bool prefix_fits(const PieceGeom& g, int64_t Hkv, int64_t bs, int64_t max_prefix_blocks) {
+  return g.fast && bs <= 128 && Hkv <= 65535 && max_prefix_blocks * bs < (1ll << 31);
+}
+
 int attend(const AttnCall& a, const b200_launch_cfg* cfg, void* workspace, size_t workspace_bytes, cudaStream_t s) {
   const PieceGeom g = piece_geometry(a.B, a.Hq, a.Hkv, a.D, a.block_size, a.num_blocks, a.max_blocks, elem_of(a), cfg);
   const bool aligned = aligned16(a.q) && aligned16(a.out) && aligned16(a.k_cache) && aligned16(a.v_cache) &&
                        aligned16(a.k_scale) && aligned16(a.v_scale);
-  const bool fast = g.fast && aligned && a.prefix_table == nullptr && !(cfg && (cfg->flags & 1));
+  const bool prefix = a.prefix_table != nullptr;
+  const bool fast = g.fast && aligned && (!prefix || prefix_fits(g, a.Hkv, a.block_size, a.max_prefix_blocks)) &&
+                    !(cfg && (cfg->flags & 1));
   if (!fast) {
     if (a.D > 256) return B200_ERR_UNSUPPORTED;
     if (a.cache_dtype == B200_I8) return launch_attn_generic_i8(a, s);
     if (a.cache_dtype == B200_F8E4M3) return launch_attn_generic_e4m3(a, s);
     return launch_attn_generic_16(a, s);
   }
-  const SpaceBytes sb = space_bytes(g, a.Hq, 0);
+  const int splits = prefix ? prefix_splits(g, g.seqs, a.Hkv, a.block_size, a.max_prefix_blocks) : 0;
+  const SpaceBytes sb = space_bytes(g, a.Hq, splits);
   if (workspace == nullptr || workspace_bytes < sb.cum + sb.rows + sb.prefix) return B200_ERR_WORKSPACE;
   if (!aligned16(workspace)) return B200_ERR_ALIGNMENT;
   PieceSpace w{};
@@ -203,9 +227,17 @@ int attend(const AttnCall& a, const b200_launch_cfg* cfg, void* workspace, size_
     const AttnCall c = slice_of(a, b0, a.B - b0 < g.seqs ? a.B - b0 : g.seqs);
     PieceGeom gs = g;
     if (b0 > 0) gs.pdl = false;  // the kernel before is this call's join, which reads the workspace
-    int st = a.cache_dtype == B200_I8       ? launch_pieces_i8(c, gs, w, false, s)
-             : a.cache_dtype == B200_F8E4M3 ? launch_pieces_e4m3(c, gs, w, false, s)
-                                            : launch_pieces_16(c, gs, w, false, s);
+    w.prefix_splits = splits;
+    int st = B200_OK;
+    if (prefix) {
+      st = a.cache_dtype == B200_I8       ? launch_prefix_i8(c, gs, w, s)
+           : a.cache_dtype == B200_F8E4M3 ? launch_prefix_e4m3(c, gs, w, s)
+                                          : launch_prefix_16(c, gs, w, s);
+      if (st) return st;
+    }
+    st = a.cache_dtype == B200_I8       ? launch_pieces_i8(c, gs, w, prefix, s)
+             : a.cache_dtype == B200_F8E4M3 ? launch_pieces_e4m3(c, gs, w, prefix, s)
+                                            : launch_pieces_16(c, gs, w, prefix, s);
     if (st) return st;
     st = B200_DISPATCH_HALF(a.dtype, [&] { return launch_join<scalar_t>(c, gs, w, s); });
     if (st) return st;
@@ -271,9 +303,14 @@ extern "C" size_t b200_paged_attention_prefix_workspace_size(int64_t B, int64_t 
                                                              int64_t num_blocks, int64_t block_size,
                                                              int64_t max_prefix_blocks, int64_t max_blocks,
                                                              int32_t cache_dtype, const b200_launch_cfg* cfg) {
-  (void)B, (void)Hq, (void)Hkv, (void)D, (void)num_blocks, (void)block_size, (void)max_prefix_blocks;
-  (void)max_blocks, (void)cache_dtype, (void)cfg;
-  return 0;
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || num_blocks <= 0 || block_size <= 0 || max_prefix_blocks <= 0 ||
+      max_blocks < 0 || Hq % Hkv)
+    return 0;
+  const int elem = cache_dtype == B200_I8 || cache_dtype == B200_F8E4M3 ? 1 : 2;
+  const PieceGeom g = piece_geometry(B, Hq, Hkv, D, block_size, num_blocks, max_blocks, elem, cfg);
+  if (!prefix_fits(g, Hkv, block_size, max_prefix_blocks)) return 0;
+  const SpaceBytes sb = space_bytes(g, Hq, prefix_splits(g, g.seqs, Hkv, block_size, max_prefix_blocks));
+  return sb.cum + sb.rows + sb.prefix;
 }
 
 extern "C" int b200_paged_attention_prefix(const void* q, const void* k_cache, const void* v_cache,

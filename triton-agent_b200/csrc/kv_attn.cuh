@@ -186,6 +186,15 @@ __global__ void __launch_bounds__(128)
 // One 16-token page of a head is 8 ldmatrix.x4, 64 code pairs to f16 and
 // 16 mma.sync.
 // ---------------------------------------------------------------------------
+// Power-of-two factors that take a row with this largest magnitude to [2^13,
+// 2^14) and back; zero and non-finite rows stay.
+__device__ __forceinline__ void pow2_scale(float amax, float& up, float& down) {
+  int e = (int)(__float_as_uint(amax) >> 23) - 127;
+  e = (amax == 0.f || e > 127) ? 13 : (e < -100 ? -100 : e);
+  up = __uint_as_float((uint32_t)(13 - e + 127) << 23);
+  down = __uint_as_float((uint32_t)(e - 13 + 127) << 23);
+}
+
 template <typename T, int G>
 __device__ __forceinline__ void load_q_frags8(const T* __restrict__ qrow0, int lane, float qscale,
                                               uint32_t (&qb)[8][2], float& slA, float& slB) {
@@ -205,11 +214,8 @@ __device__ __forceinline__ void load_q_frags8(const T* __restrict__ qrow0, int l
   }
   amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
   amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-  // the row's largest element to [2^13, 2^14); zero and non-finite rows stay
-  int e = (int)(__float_as_uint(amax) >> 23) - 127;
-  e = (amax == 0.f || e > 127) ? 13 : (e < -100 ? -100 : e);
-  const float up = __uint_as_float((uint32_t)(13 - e + 127) << 23);
-  const float down = __uint_as_float((uint32_t)(e - 13 + 127) << 23);
+  float up, down;
+  pow2_scale(amax, up, down);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     qb[j][0] = pack_pair<__half>(f[j][0] * up, f[j][1] * up);
@@ -391,6 +397,7 @@ __global__ void __launch_bounds__(288, 1)
   int* chunk_id = s_ctx + B;
   int* chunk_ntok = chunk_id + 32;
   int* s_abort = chunk_ntok + 32;
+  int* s_drop = s_abort + 1;  // dropped entries of the first segment before this range
 
   // the join kernel may be scheduled; it waits for this grid
   asm volatile("griddepcontrol.launch_dependents;");
@@ -418,6 +425,7 @@ __global__ void __launch_bounds__(288, 1)
     if (lane == 0) {
       s_cum[0] = 0;
       *s_abort = 0;
+      *s_drop = 0;
       for (int s = 0; s < p.stages; ++s) {
         sm100::mbar_init(sm100::smem_u32(&full_bar[s]), 1);
         sm100::mbar_init(sm100::smem_u32(&empty_bar[s]), consumers);
@@ -429,6 +437,28 @@ __global__ void __launch_bounds__(288, 1)
   const int64_t E = s_cum[p.nseg];
   const int64_t R = E < (int64_t)gridDim.x ? E : (int64_t)gridDim.x;  // ranges
   const int c = blockIdx.x;
+  const int64_t lo = c < R ? range_lo(c, E, R) : 0, hi = c < R ? range_lo(c + 1, E, R) : 0;
+  int seg0 = 0;  // segment of the range's first entry
+  if (c < R) {
+    int r = p.nseg;  // cum[seg0] <= lo < cum[r]
+    while (r - seg0 > 1) {
+      const int mid = (seg0 + r) >> 1;
+      if (s_cum[mid] <= lo) seg0 = mid;
+      else r = mid;
+    }
+    // Dropped entries before the range shift the token ranks of its pages:
+    // counted by the whole CTA (a warp alone takes 20 us over 8192 entries).
+    const int j0 = (int)(lo - s_cum[seg0]);
+    int drop = 0;
+#pragma unroll 8
+    for (int j = threadIdx.x; j < j0; j += blockDim.x) {
+      const int64_t id = btab.at((seg0 % B) * p.max_blocks + j);
+      drop += id < 0 || id >= p.num_blocks;
+    }
+    drop = __reduce_add_sync(0xffffffffu, drop);
+    if (lane == 0 && drop) atomicAdd(s_drop, drop);
+  }
+  __syncthreads();
 
   // Programmatic launch (cfg flags bit 3): what is above and the producer's
   // walk of the block table up to its first copy overlap the previous kernel,
@@ -465,17 +495,7 @@ __global__ void __launch_bounds__(288, 1)
       ++it;
       return true;
     };
-    const int64_t lo = range_lo(c, E, R), hi = range_lo(c + 1, E, R);
-    int s = 0;
-    {
-      int l = 0, r = p.nseg;  // cum[l] <= lo < cum[r]
-      while (r - l > 1) {
-        const int mid = (l + r) >> 1;
-        if (s_cum[mid] <= lo) l = mid;
-        else r = mid;
-      }
-      s = l;
-    }
+    int s = seg0;
     int64_t e = lo;
     while (e < hi && ok) {
       while (s_cum[s + 1] == s_cum[s]) ++s;
@@ -485,19 +505,7 @@ __global__ void __launch_bounds__(288, 1)
       const int j0 = (int)(e - segs), j1 = (int)((hi < sege ? hi : sege) - segs);
       const int ctx = s_ctx[b];
       const int64_t bt0 = b * p.max_blocks;
-      // dropped entries before j0 shift the token ranks of this range
-      int inval = 0;
-      for (int jb = 0; jb < j0; jb += 256) {
-        int64_t v[8];
-#pragma unroll
-        for (int rr = 0; rr < 8; ++rr) {
-          const int j = jb + rr * 32 + lane;
-          v[rr] = j < j0 ? btab.at(bt0 + j) : 0;
-        }
-#pragma unroll
-        for (int rr = 0; rr < 8; ++rr) inval += (v[rr] < 0 || v[rr] >= p.num_blocks) ? 1 : 0;
-      }
-      inval = __reduce_add_sync(0xffffffffu, inval);
+      int inval = e == lo ? *s_drop : 0;
       int fill = 0;  // pages already in the open stage (lane 0)
       for (int jj = j0; jj < j1 && ok; jj += 32) {
         const int j = jj + lane;

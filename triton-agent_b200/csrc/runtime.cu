@@ -157,6 +157,7 @@ const char* b200_kernel_list(void) {
          "slot_claim_kernel\n"
          "kv_dequant_kernel\n"
          "paged_attn_pieces_kernel\n"
+         "prefix_attn_kernel\n"
          "paged_attn_join_kernel\n"
          "paged_attn_pieces_generic_kernel\n"
          "int8_gemm_pair_kernel\n"
