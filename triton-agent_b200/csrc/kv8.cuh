@@ -58,8 +58,8 @@ __device__ __forceinline__ uint32_t kv8_pair(uint32_t w) {
 __device__ __forceinline__ void kv8_value_scale(float vs, float& lvs, float& ivs) {
   constexpr float kTiny = 7.888609052210118e-31f;  // 2^-100
   vs = vs < kTiny ? kTiny : vs;
-  lvs = __log2f(vs);
-  ivs = __fdividef(1.0f, vs);
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(lvs) : "f"(vs));
+  asm("rcp.approx.f32 %0, %1;" : "=f"(ivs) : "f"(vs));
 }
 
 }  // namespace b200

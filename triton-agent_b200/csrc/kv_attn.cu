@@ -13,58 +13,66 @@ namespace {
 constexpr size_t kSmemMost = 227 * 1024;
 
 // ---------------------------------------------------------------------------
-// Join: one warp a query row.  The row's pieces are those of its segment's
-// ranges (sub of them each) and one per prefix split; lanes fold the (m, l) of
-// their pieces, then the warp adds the weighted rows, four dims a lane.  A row
-// that the streaming kernel wrote itself is skipped; a row without any token
-// is zero.
+// Join: W warps a query row (1, 2, 4 or 8: as many as keep a GPU's worth of
+// warps busy when rows are few and their pieces many).  The row's pieces are those
+// of its segment's ranges and those of the prefix's splits; every warp folds the (m) of
+// all of them, then adds the weighted rows of its share, four dims a lane,
+// and the first warp adds up the shares.  A row that the streaming kernel
+// wrote itself is skipped; a row without any token is zero.
 // ---------------------------------------------------------------------------
 struct JoinParams {
   int64_t B, Hq;
-  int heads_cta, sub, nseg, grid, always, splits;
+  int heads_cta, nseg, grid, always, splits, W;
 };
 
 template <typename T>
 __global__ void __launch_bounds__(256)
     paged_attn_join_kernel(const int32_t* __restrict__ cum, const float* __restrict__ rows,
                            const float* __restrict__ prefix, T* __restrict__ out, JoinParams p) {
-  const int64_t row = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (row >= p.B * p.Hq) return;
-  const int64_t b = row / p.Hq;
+  __shared__ float s_part[8][kPiecePitch];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int W = p.W, share = warp % W;
+  const int64_t row = (int64_t)blockIdx.x * (8 / W) + warp / W;
+  const bool live = row < p.B * p.Hq;
+  const int64_t b = live ? row / p.Hq : 0;
   const int h = (int)(row - b * p.Hq), hg = h / p.heads_cta, hh = h - hg * p.heads_cta;
   const int seg = (int)(hg * p.B + b);
-  const int64_t E = __ldcg(&cum[p.nseg]), s0 = __ldcg(&cum[seg]), s1 = __ldcg(&cum[seg + 1]);
-  const int64_t R = E < p.grid ? E : p.grid;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   int c1 = 0, own = 0;
-  if (s1 > s0) {
-    c1 = range_of(s0, E, R);
-    const int c2 = range_of(s1 - 1, E, R);
-    if (c1 == c2 && p.sub == 1 && !p.always) return;
-    own = (c2 - c1 + 1) * p.sub;
+  bool done = !live;
+  if (live) {
+    const int64_t E = __ldcg(&cum[p.nseg]), s0 = __ldcg(&cum[seg]), s1 = __ldcg(&cum[seg + 1]);
+    const int64_t R = E < p.grid ? E : p.grid;
+    if (s1 > s0) {
+      c1 = range_of(s0, E, R);
+      const int c2 = range_of(s1 - 1, E, R);
+      done = c1 == c2 && !p.always;
+      own = c2 - c1 + 1;
+    }
   }
-  const int n = own + p.splits;
+  const int n = done ? 0 : own + p.splits;
   auto piece = [&](int i) -> const float* {
-    return i < own ? rows + ((((int64_t)seg + c1) * p.sub + i) * p.heads_cta + hh) * kPiecePitch
+    return i < own ? rows + (((int64_t)seg + c1 + i) * p.heads_cta + hh) * kPiecePitch
                    : prefix + ((int64_t)(i - own) * p.B * p.Hq + row) * kPiecePitch;
   };
-  // weight of a piece before the maximum is taken off: none without tokens
-  // (m = -inf, l = 0); NaN logits only leave m = -inf and l = NaN
+  // weight of a piece: none without tokens (m = -inf, l = 0); NaN logits
+  // only leave m = -inf and l = NaN
   auto weight = [](float m, float l, float M) { return m == -INFINITY ? (l == 0.f ? 0.f : l) : ex2(m - M); };
   float M = -INFINITY;
   for (int i = lane; i < n; i += 32) M = fmaxf(M, __ldcg(piece(i) + kD));
   M = warp_max(M);
   float L = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i0 = 0; i0 < n; i0 += 32) {
+  // this warp's share: pieces share, share + W, ...; 32 of them at a time
+  const int mine = n > share ? (n - share + W - 1) / W : 0;
+  for (int i0 = 0; i0 < mine; i0 += 32) {
     float w = 0.f;
-    if (i0 + lane < n) {
-      const float2 ml = __ldcg(reinterpret_cast<const float2*>(piece(i0 + lane) + kD));
+    if (i0 + lane < mine) {
+      const float2 ml = __ldcg(reinterpret_cast<const float2*>(piece(share + (i0 + lane) * W) + kD));
       w = weight(ml.x, ml.y, M);
       if (w != 0.f) L += w * ml.y;
     }
-    const int nb = n - i0 < 32 ? n - i0 : 32;
+    const int nb = mine - i0 < 32 ? mine - i0 : 32;
     for (int u0 = 0; u0 < nb; u0 += 4) {
       float4 v[4];
       float wu[4];
@@ -73,7 +81,8 @@ __global__ void __launch_bounds__(256)
         wu[u] = __shfl_sync(0xffffffffu, w, (u0 + u) & 31);
         if (u0 + u >= nb) wu[u] = 0.f;
         v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (wu[u] != 0.f) v[u] = __ldcg(reinterpret_cast<const float4*>(piece(i0 + u0 + u) + 4 * lane));
+        if (wu[u] != 0.f)
+          v[u] = __ldcg(reinterpret_cast<const float4*>(piece(share + (i0 + u0 + u) * W) + 4 * lane));
       }
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
@@ -85,6 +94,19 @@ __global__ void __launch_bounds__(256)
     }
   }
   L = warp_sum(L);
+  if (W > 1) {
+    *reinterpret_cast<float4*>(&s_part[warp][4 * lane]) = acc;
+    if (lane == 0) s_part[warp][kD] = L;
+    __syncthreads();
+    if (share == 0) {
+      for (int u = 1; u < W; ++u) {
+        const float4 v = *reinterpret_cast<const float4*>(&s_part[warp + u][4 * lane]);
+        acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+        L += s_part[warp + u][kD];
+      }
+    }
+  }
+  if (done || share != 0) return;
   const float inv = L == 0.f ? 0.f : 1.f / L;
   uint2 pk;
   pk.x = pack_pair<T>(acc.x * inv, acc.y * inv);
@@ -94,8 +116,7 @@ __global__ void __launch_bounds__(256)
 
 // ---------------------------------------------------------------------------
 // Geometry.  HG: the largest divisor of Hkv up to 8 whose page leaves room for
-// two stages; sub = 8 / HG pages a stage so that eight consumer warps (or as many
-// as HG divides) have work whatever Hkv is.  The fast path covers head dim 128,
+// two ring entries; sub warps share a head.  The fast path covers head dim 128,
 // blocks of a multiple of 16 tokens up to 256 and 1, 2, 4 or 8 query heads a kv head.
 // ---------------------------------------------------------------------------
 PieceGeom piece_geometry(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t bs, int64_t num_blocks,
@@ -109,14 +130,11 @@ PieceGeom piece_geometry(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t 
   const int hg_most = (cfg && cfg->rows_per_cta > 0 && cfg->rows_per_cta <= 8) ? cfg->rows_per_cta : 8;
   for (int cand = hg_most; cand >= 1 && g.HG == 0; --cand) {
     if (Hkv % cand) continue;
-    int sub = 8 / cand;
     const int64_t box = (int64_t)cand * bs * 128;
     const int64_t page = ((elem == 1 ? 2 * box + 2 * (int64_t)cand * bs * 4 : 4 * box) + 1023) / 1024 * 1024;
-    while (sub > 1 && page * sub > 40 * 1024) sub /= 2;
-    if (2 * page * sub > 176 * 1024) continue;
-    g.HG = cand, g.sub = sub;
+    if (2 * page > 176 * 1024) continue;
+    g.HG = cand, g.sub = (elem == 1 ? kConsumers : kConsumers / 2) / cand;
     g.page_bytes = (uint32_t)page;
-    g.stage_bytes = (uint32_t)(page * sub);
   }
   if (g.HG == 0) return g;
   g.n_hg = (int)(Hkv / g.HG);
@@ -124,12 +142,23 @@ PieceGeom piece_geometry(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t 
   if (g.seqs < 1 || g.n_hg * g.seqs * max_blocks >= (1ll << 31)) return g;
   g.grid = device_sm_count();
   g.pdl = cfg && (cfg->flags & 8);
-  const size_t fixed = 1024 + (size_t)(g.n_hg * g.seqs + 1) * 4 + (size_t)g.seqs * 4 + 66 * 4;
-  const size_t per = g.stage_bytes + 16 + sizeof(StageMeta);
-  int stages = (cfg && cfg->stages > 0) ? cfg->stages : (int)(132 * 1024 / g.stage_bytes);
+  const size_t per = g.page_bytes + 16 + sizeof(PageMeta);
+  size_t fixed = 1024 + 16 * 8 + (size_t)(g.n_hg * g.seqs + 1) * 4 + (size_t)g.seqs * 4 + 66 * 4;
+  auto xch = [&] { return (size_t)(g.sub - 1) * g.HG * kXchPitch * 4; };
+  // The ring holds a multiple of sub entries, so that an entry belongs to one
+  // slot: its warps have then seen each earlier filling of the entry they wait
+  // for (copies complete out of order, and a wait tells only two fillings apart).
+  // Large pages leave room for fewer slots.
+  while (g.sub > 2 && g.sub * per + fixed + xch() > kSmemMost) g.sub /= 2;
+  if (g.sub > 1 && 2 * per + fixed + xch() > kSmemMost) g.sub = 1;
+  fixed += xch();
+  const int unit = g.sub > 1 ? g.sub : 1;
+  int stages = (cfg && cfg->stages > 0) ? cfg->stages : (int)((elem == 1 ? 132 : 196) * 1024 / g.page_bytes);
+  if (stages > 64) stages = 64;
+  stages = stages / unit * unit;
+  while (stages > unit && stages * per + fixed > kSmemMost) stages -= unit;
+  if (stages < unit) stages = unit;
   if (stages < 2) stages = 2;
-  if (stages > 16) stages = 16;
-  while (stages > 2 && stages * per + fixed > kSmemMost) --stages;
   g.stages = stages;
   g.smem = stages * per + fixed;
   g.fast = g.smem <= kSmemMost;
@@ -162,16 +191,20 @@ SpaceBytes space_bytes(const PieceGeom& g, int64_t Hq, int prefix_splits) {
   const int64_t nseg = g.n_hg * g.seqs;
   SpaceBytes s;
   s.cum = up256((size_t)(nseg + 1) * 4);
-  s.rows = up256((size_t)(nseg + g.grid) * g.sub * g.HG * g.G * kPiecePitch * 4);
+  s.rows = up256((size_t)(nseg + g.grid) * g.HG * g.G * kPiecePitch * 4);
   s.prefix = up256((size_t)prefix_splits * g.seqs * Hq * kPiecePitch * 4);
   return s;
 }
 
 template <typename T>
 int launch_join(const AttnCall& a, const PieceGeom& g, const PieceSpace& w, cudaStream_t s) {
-  JoinParams p{a.B, a.Hq, g.HG * g.G, g.sub, (int)(g.n_hg * a.B), g.grid, a.prefix_table != nullptr, w.prefix_splits};
+  JoinParams p{a.B, a.Hq, g.HG * g.G, (int)(g.n_hg * a.B), g.grid, a.prefix_table != nullptr, w.prefix_splits, 1};
+  // pieces a row, about: the grid's ranges over the segments, and the splits;
+  // two or three a warp while the rows alone would not fill the SMs
+  const int64_t rows = a.B * a.Hq, pieces = g.grid / p.nseg + 1 + w.prefix_splits;
+  while (p.W < 8 && p.W * 3 <= pieces && rows * p.W < 16 * (int64_t)g.grid) p.W *= 2;
   cudaLaunchConfig_t lc = {};
-  lc.gridDim = dim3((unsigned)((a.B * a.Hq + 7) / 8));
+  lc.gridDim = dim3((unsigned)((rows * p.W + 7) / 8));
   lc.blockDim = dim3(256);
   lc.stream = s;
   cudaLaunchAttribute attr[1];

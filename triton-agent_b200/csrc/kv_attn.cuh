@@ -52,7 +52,7 @@ struct PieceGeom {
   int G, HG, n_hg, sub;   // query heads a kv head, kv heads a CTA, head groups, warps a kv head
   int stages, grid;
   int64_t seqs;           // sequences a launch takes (the batch runs in slices of this many)
-  uint32_t page_bytes, stage_bytes;
+  uint32_t page_bytes;
   size_t smem;
   bool pdl;
 };
@@ -60,7 +60,7 @@ struct PieceGeom {
 // Workspace: [segment prefix sums | pieces of the own pages | pieces of the prefix].
 struct PieceSpace {
   int32_t* cum;   // nseg + 1
-  float* rows;    // piece (segment + range) * sub + warp, heads_cta rows each
+  float* rows;    // piece segment + range, heads_cta rows each
   float* prefix;  // split-major: [splits][seqs * Hq] rows
   int prefix_splits;
 };
@@ -226,34 +226,49 @@ __device__ __forceinline__ void load_q_frags8(const T* __restrict__ qrow0, int l
   slB = __shfl_sync(0xffffffffu, sl, (lane & 3) * 8 + 4);
 }
 
-// One page (ntok tokens of kv head w: codes at kb / vb as [head][token][128]
-// rows, 128-byte swizzled; scales at ksp / vsp as [head][token]).
+// Raises the running maxima of this thread's two heads to the maxima of four
+// logits (tokens tr, tr + 8), when one in the warp exceeds its maximum by more than
+// 2^8 (exact: O and l share the offset).  Most pages need one vote here and no exchange.
+__device__ __forceinline__ void raise_max_lazy(const float (&y)[4], float (&mu)[2], float (&lp)[2],
+                                               float (&o)[8][4]) {
+  const bool up = fmaxf(y[0], y[2]) > mu[0] + 8.0f || fmaxf(y[1], y[3]) > mu[1] + 8.0f;
+  if (!__any_sync(0xffffffffu, up)) return;
+  float m[2] = {fmaxf(y[0], y[2]), fmaxf(y[1], y[3])};
+#pragma unroll
+  for (int off = 4; off <= 16; off <<= 1) {
+    m[0] = fmaxf(m[0], __shfl_xor_sync(0xffffffffu, m[0], off));
+    m[1] = fmaxf(m[1], __shfl_xor_sync(0xffffffffu, m[1], off));
+  }
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    if (!(m[c] > mu[c])) continue;
+    const float alpha = mu[c] == -INFINITY ? 0.f : ex2(mu[c] - m[c]);
+    mu[c] = m[c];
+    lp[c] = lp[c] == 0.f ? 0.f : lp[c] * alpha;
+#pragma unroll
+    for (int mt = 0; mt < 8; ++mt) {
+      o[mt][c] *= alpha;
+      o[mt][c + 2] *= alpha;
+    }
+  }
+}
+
+// Tokens [t0, t0 + 16) of kv head w's rows of a page (codes at kb / vb as
+// [head][token][128] rows, 128-byte swizzled; scales at ksp / vsp as [head][token]).
 template <typename KV>
-__device__ __forceinline__ void mma_page8(uint32_t kb, uint32_t vb, const float* __restrict__ ksp,
-                                          const float* __restrict__ vsp, int ntok, int w, int bs, int lane, float slA,
-                                          float slB, const uint32_t (&qb)[8][2], float (&o)[8][4], float (&mu)[2],
-                                          float (&lp)[2]) {
+__device__ __forceinline__ void mma_chunk8(uint32_t kb, uint32_t vb, const float* __restrict__ ksp,
+                                           const float* __restrict__ vsp, int t0, int ntok, int row0, int lane,
+                                           float slA, float slB, const uint32_t (&qb)[8][2], float (&o)[8][4],
+                                           float (&mu)[2], float (&lp)[2]) {
   const int mat = lane >> 3, mrow = lane & 7;
   const int tr = lane >> 2, tq = (lane & 3) * 2;
-  for (int t0 = 0; t0 < ntok; t0 += 16) {
-    const int row = w * bs + t0 + (mat & 1) * 8 + mrow;
-    const int sw = row & 7;
-    float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
-    uint32_t kr[4][4], vr[4][4];
+  const int row = row0 + t0 + (mat & 1) * 8 + mrow;
+  const uint32_t at = row * 128, sw = ((mat >> 1) ^ (row & 7)) << 4;  // chunk 2j + (mat >> 1), swizzled: sw ^ (j << 5)
+  float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+  {
+    uint32_t kr[4][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      ldsm_x4(kb + row * 128 + (((2 * j + (mat >> 1)) ^ sw) << 4), kr[j][0], kr[j][1], kr[j][2], kr[j][3]);
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      ldsm_x4_t(vb + row * 128 + (((2 * j + (mat >> 1)) ^ sw) << 4), vr[j][0], vr[j][1], vr[j][2], vr[j][3]);
-    const bool ok0 = t0 + tr < ntok, ok1 = t0 + tr + 8 < ntok;
-    const int at = w * bs + t0 + tr;
-    const float k0 = ksp[at], k1 = ksp[at + 8];
-    float lv0, iv0, lv1, iv1;
-    kv8_value_scale(vsp[at], lv0, iv0);
-    kv8_value_scale(vsp[at + 8], lv1, iv1);
-    iv0 = ok0 ? iv0 : 0.f;
-    iv1 = ok1 ? iv1 : 0.f;
+    for (int j = 0; j < 4; ++j) ldsm_x4(kb + at + (sw ^ (j << 5)), kr[j][0], kr[j][1], kr[j][2], kr[j][3]);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       mma16816<__half>(s0, kv8_pair<KV, 0, 1>(kr[j][0]), kv8_pair<KV, 0, 1>(kr[j][1]), kv8_pair<KV, 2, 3>(kr[j][0]),
@@ -261,46 +276,103 @@ __device__ __forceinline__ void mma_page8(uint32_t kb, uint32_t vb, const float*
       mma16816<__half>(s1, kv8_pair<KV, 0, 1>(kr[j][2]), kv8_pair<KV, 0, 1>(kr[j][3]), kv8_pair<KV, 2, 3>(kr[j][2]),
                        kv8_pair<KV, 2, 3>(kr[j][3]), qb[2 * j + 1][0], qb[2 * j + 1][1]);
     }
-    // y[0]/y[1]: token tr of heads 2(lane%4), +1; y[2]/y[3]: token tr + 8
-    float y[4];
-    y[0] = ok0 ? fmaf(s0[0] + s1[0], k0 * slA, lv0) : -INFINITY;
-    y[1] = ok0 ? fmaf(s0[1] + s1[1], k0 * slB, lv0) : -INFINITY;
-    y[2] = ok1 ? fmaf(s0[2] + s1[2], k1 * slA, lv1) : -INFINITY;
-    y[3] = ok1 ? fmaf(s0[3] + s1[3], k1 * slB, lv1) : -INFINITY;
-    float mA = fmaxf(y[0], y[2]), mB = fmaxf(y[1], y[3]);
+  }
+  uint32_t vr[4][4];
 #pragma unroll
-    for (int off = 4; off <= 16; off <<= 1) {
-      mA = fmaxf(mA, __shfl_xor_sync(0xffffffffu, mA, off));
-      mB = fmaxf(mB, __shfl_xor_sync(0xffffffffu, mB, off));
-    }
-    raise_max(mu[0], mA, lp[0], o, 0);
-    raise_max(mu[1], mB, lp[1], o, 1);
-    const float nA = mu[0] == -INFINITY ? 0.f : mu[0], nB = mu[1] == -INFINITY ? 0.f : mu[1];
-    const float p0 = ex2(y[0] - nA), p2 = ex2(y[2] - nA);
-    const float p1 = ex2(y[1] - nB), p3 = ex2(y[3] - nB);
-    lp[0] = fmaf(p0, iv0, fmaf(p2, iv1, lp[0]));
-    lp[1] = fmaf(p1, iv0, fmaf(p3, iv1, lp[1]));
-    const uint32_t b0 = movm_t(pack_pair<__half>(p0, p1));
-    const uint32_t b1 = movm_t(pack_pair<__half>(p2, p3));
-    if (t0 + 16 > ntok) {
-      // tokens past the end may hold any code (e4m3 has a NaN): zero their V.
-      // Each register holds two codes of token tq and two of token tq + 1.
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        vr[j][0] = mask_pair(vr[j][0], t0 + tq, ntok);
-        vr[j][1] = mask_pair(vr[j][1], t0 + 8 + tq, ntok);
-        vr[j][2] = mask_pair(vr[j][2], t0 + tq, ntok);
-        vr[j][3] = mask_pair(vr[j][3], t0 + 8 + tq, ntok);
-      }
-    }
+  for (int j = 0; j < 4; ++j) ldsm_x4_t(vb + at + (sw ^ (j << 5)), vr[j][0], vr[j][1], vr[j][2], vr[j][3]);
+  const int tok = row0 + t0 + tr;
+  const float k0 = ksp[tok], k1 = ksp[tok + 8];
+  float lv0, iv0, lv1, iv1;
+  kv8_value_scale(vsp[tok], lv0, iv0);
+  kv8_value_scale(vsp[tok + 8], lv1, iv1);
+  // y[0]/y[1]: token tr of heads 2(lane%4), +1; y[2]/y[3]: token tr + 8
+  float y[4];
+  y[0] = fmaf(s0[0] + s1[0], k0 * slA, lv0);
+  y[1] = fmaf(s0[1] + s1[1], k0 * slB, lv0);
+  y[2] = fmaf(s0[2] + s1[2], k1 * slA, lv1);
+  y[3] = fmaf(s0[3] + s1[3], k1 * slB, lv1);
+  if (t0 + 16 > ntok) {
+    // tokens past the end may hold any code (e4m3 has a NaN) and any scale: no
+    // weight, and V zero.  A V register holds two codes of token tq and two of tq + 1.
+    if (t0 + tr >= ntok) y[0] = y[1] = -INFINITY, iv0 = 0.f;
+    if (t0 + tr + 8 >= ntok) y[2] = y[3] = -INFINITY, iv1 = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-        mma16816<__half>(o[2 * j + u], kv8_pair<KV, 0, 2>(vr[j][2 * u]), kv8_pair<KV, 1, 3>(vr[j][2 * u]),
-                         kv8_pair<KV, 0, 2>(vr[j][2 * u + 1]), kv8_pair<KV, 1, 3>(vr[j][2 * u + 1]), b0, b1);
+      vr[j][0] = mask_pair(vr[j][0], t0 + tq, ntok);
+      vr[j][1] = mask_pair(vr[j][1], t0 + 8 + tq, ntok);
+      vr[j][2] = mask_pair(vr[j][2], t0 + tq, ntok);
+      vr[j][3] = mask_pair(vr[j][3], t0 + 8 + tq, ntok);
     }
   }
+  raise_max_lazy(y, mu, lp, o);
+  const float nA = mu[0] == -INFINITY ? 0.f : mu[0], nB = mu[1] == -INFINITY ? 0.f : mu[1];
+  const float p0 = ex2(y[0] - nA), p2 = ex2(y[2] - nA);
+  const float p1 = ex2(y[1] - nB), p3 = ex2(y[3] - nB);
+  lp[0] = fmaf(p0, iv0, fmaf(p2, iv1, lp[0]));
+  lp[1] = fmaf(p1, iv0, fmaf(p3, iv1, lp[1]));
+  const uint32_t b0 = movm_t(pack_pair<__half>(p0, p1));
+  const uint32_t b1 = movm_t(pack_pair<__half>(p2, p3));
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      mma16816<__half>(o[2 * j + u], kv8_pair<KV, 0, 2>(vr[j][2 * u]), kv8_pair<KV, 1, 3>(vr[j][2 * u]),
+                       kv8_pair<KV, 0, 2>(vr[j][2 * u + 1]), kv8_pair<KV, 1, 3>(vr[j][2 * u + 1]), b0, b1);
+  }
+}
+
+// The same for 16-bit caches: K and V as two boxes of 64 dims each, `box` bytes apart.
+template <typename T>
+__device__ __forceinline__ void mma_chunk16(uint32_t kb, uint32_t vb, uint32_t box, int t0, int ntok, int row0,
+                                            int lane, float sl, const uint32_t (&qb)[8][2], float (&o)[8][4],
+                                            float (&mu)[2], float (&lp)[2]) {
+  const int mat = lane >> 3, mrow = lane & 7;
+  const int tr = lane >> 2, tq = (lane & 3) * 2;
+  float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+  {
+    // A = K rows: matrix `mat` = (token half mat&1, dim-chunk parity mat>>1)
+    const int row = row0 + t0 + (mat & 1) * 8 + mrow;
+    const uint32_t at = kb + row * 128, sw = ((mat >> 1) ^ (row & 7)) << 4;
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks) {
+      uint32_t a0, a1, a2, a3;
+      ldsm_x4(at + (ks >> 2) * box + (sw ^ ((ks & 3) << 5)), a0, a1, a2, a3);
+      mma16816<T>((ks & 1) ? s1 : s0, a0, a1, a2, a3, qb[ks][0], qb[ks][1]);
+    }
+  }
+  // A = V^T by ldmatrix.trans: matrix `mat` = (token half mat>>1, dim-chunk parity mat&1)
+  uint32_t va[8][4];
+  {
+    const int row = row0 + t0 + (mat >> 1) * 8 + mrow;
+    const uint32_t at = vb + row * 128, sw = ((mat & 1) ^ (row & 7)) << 4;
+#pragma unroll
+    for (int mt = 0; mt < 8; ++mt)
+      ldsm_x4_t(at + (mt >> 2) * box + (sw ^ ((mt & 3) << 5)), va[mt][0], va[mt][1], va[mt][2], va[mt][3]);
+  }
+  float y[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] = (s0[i] + s1[i]) * sl;
+  if (t0 + 16 > ntok) {
+    if (t0 + tr >= ntok) y[0] = y[1] = -INFINITY;
+    if (t0 + tr + 8 >= ntok) y[2] = y[3] = -INFINITY;
+#pragma unroll
+    for (int mt = 0; mt < 8; ++mt) {
+      va[mt][0] = mask_pair(va[mt][0], t0 + tq, ntok);
+      va[mt][1] = mask_pair(va[mt][1], t0 + tq, ntok);
+      va[mt][2] = mask_pair(va[mt][2], t0 + 8 + tq, ntok);
+      va[mt][3] = mask_pair(va[mt][3], t0 + 8 + tq, ntok);
+    }
+  }
+  raise_max_lazy(y, mu, lp, o);
+  const float nA = mu[0] == -INFINITY ? 0.f : mu[0], nB = mu[1] == -INFINITY ? 0.f : mu[1];
+  const float p0 = ex2(y[0] - nA), p2 = ex2(y[2] - nA);
+  const float p1 = ex2(y[1] - nB), p3 = ex2(y[3] - nB);
+  lp[0] += p0 + p2;
+  lp[1] += p1 + p3;
+  const uint32_t b0 = movm_t(pack_pair<T>(p0, p1));
+  const uint32_t b1 = movm_t(pack_pair<T>(p2, p3));
+#pragma unroll
+  for (int mt = 0; mt < 8; ++mt) mma16816<T>(o[mt], va[mt][0], va[mt][1], va[mt][2], va[mt][3], b0, b1);
 }
 
 // Rows of the 8-bit accumulator (dims 16mt + 2r of o[mt][0..1], 16mt + 2r + 1
@@ -339,32 +411,37 @@ __device__ __forceinline__ void store_piece8(float* __restrict__ row0, const flo
 // ---------------------------------------------------------------------------
 // Streaming kernel.  All segments' block-table entries (segment s = hg * B + b)
 // laid end to end are cut into one equal contiguous range a CTA, one CTA an
-// SM.  The producer warp walks its range and fills a ring of stages with TMA: a
-// stage is `sub` pages of one segment (K and V boxes of HG heads, and for
-// 8-bit caches the pages' scales by bulk copies), so that every stage
-// feeds HG * sub = up to eight consumer warps: warp w takes head w % HG of page
-// w / HG.  An end marker closes a segment: a segment that one
-// range holds and one warp a head covers is normalised and written; otherwise
-// each warp writes its piece at row (segment + range) * sub + w / HG -- the
-// (segment, range) pairs of a call, taken in order, have distinct sums, so a
-// piece's place needs no counters -- and the join kernel reads them.  No state is
-// kept between calls.
+// SM.  The producer warp walks its range and fills a ring of pages with TMA (K
+// and V boxes of HG heads, and for 8-bit caches the page's scales by bulk
+// copies).  sub consumer warps share a kv head: page i of the ring goes to the
+// HG warps of slot i % sub, so that sixteen warps (eight for 16-bit pages, which need
+// no widening and fill the ring by themselves) have work whatever Hkv is: a
+// page's chain from ldmatrix over exp2 to the second product is long, and with
+// two warps a scheduler the kernel waits on it (64 sequences, int8: 164 us
+// with eight consumer warps, 118 with sixteen).  End
+// markers, one for each slot, close a segment: the warps of a head add up their (m,
+// l, o) in shared memory, and the first writes the normalised row when the
+// range holds the whole segment, else the range's piece at row segment +
+// range -- the (segment, range) pairs of a call, taken in order, have distinct sums, so
+// a piece's place needs no counters.  No state is kept between calls.
 // ---------------------------------------------------------------------------
 struct PiecesParams {
   int64_t B, Hq, Hkv, num_blocks, max_blocks;
   int bs, HG, n_hg, sub, stages, nseg;
   int always;   // write every segment as pieces (a prefix joins them)
   int overlap;  // launched beside the previous grid of the call: wait for it at the end
-  uint32_t page_bytes, stage_bytes;
+  uint32_t page_bytes;
   float qscale;  // scale * log2(e)
 };
 
-constexpr int kMaxSub = 8;
-struct StageMeta {
-  int kind;  // 0 pages, 1 end of segment, 2 end of stream
-  int seg, piece, direct;
-  int ntok[kMaxSub];
+constexpr int kConsumers = 16;  // consumer warps, at most
+struct PageMeta {
+  int kind;  // 0 page, 1 end of segment, 2 end of stream
+  int seg;
+  int ntok;   // page: tokens
+  int piece;  // end of segment: row of the piece, -1: the segment's only one
 };
+constexpr int kXchPitch = 36 * 32;  // floats a warp hands over: 32 o, 2 m, 2 l a lane
 
 __device__ __forceinline__ int64_t range_lo(int64_t c, int64_t E, int64_t R) { return c * E / R; }
 __device__ __forceinline__ int range_of(int64_t e, int64_t E, int64_t R) { return (int)(((e + 1) * R + E - 1) / E - 1); }
@@ -377,7 +454,7 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 }
 
 template <typename T, typename KV, int G>
-__global__ void __launch_bounds__(288, 1)
+__global__ void __launch_bounds__((kConsumers + 1) * 32, 1)
     paged_attn_pieces_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                              const float* __restrict__ k_scale, const float* __restrict__ v_scale,
                              const T* __restrict__ q, IndexPtr btab, IndexPtr clen, T* __restrict__ out,
@@ -386,12 +463,15 @@ __global__ void __launch_bounds__(288, 1)
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int HG = p.HG, bs = p.bs, consumers = HG * p.sub;
+  const int HG = p.HG, bs = p.bs, sub = p.sub, consumers = HG * sub;
   const int heads_cta = HG * G;
   const int64_t B = p.B;
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + p.stages * p.stage_bytes);
+  float* xch = reinterpret_cast<float*>(smem + p.stages * p.page_bytes);  // [sub - 1][HG][kXchPitch]
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(xch + (sub - 1) * HG * kXchPitch);
   uint64_t* empty_bar = full_bar + p.stages;
-  StageMeta* meta = reinterpret_cast<StageMeta*>(empty_bar + p.stages);
+  uint64_t* xch_full = empty_bar + p.stages;  // [8]
+  uint64_t* xch_empty = xch_full + 8;         // [8]
+  PageMeta* meta = reinterpret_cast<PageMeta*>(xch_empty + 8);
   int* s_cum = reinterpret_cast<int*>(meta + p.stages);
   int* s_ctx = s_cum + (p.nseg + 1);
   int* chunk_id = s_ctx + B;
@@ -426,12 +506,17 @@ __global__ void __launch_bounds__(288, 1)
       s_cum[0] = 0;
       *s_abort = 0;
       *s_drop = 0;
-      for (int s = 0; s < p.stages; ++s) {
-        sm100::mbar_init(sm100::smem_u32(&full_bar[s]), 1);
-        sm100::mbar_init(sm100::smem_u32(&empty_bar[s]), consumers);
-      }
-      sm100::fence_barrier_init();
     }
+  } else if (warp == 0 && lane == 0) {
+    for (int s = 0; s < p.stages; ++s) {
+      sm100::mbar_init(sm100::smem_u32(&full_bar[s]), 1);
+      sm100::mbar_init(sm100::smem_u32(&empty_bar[s]), HG);
+    }
+    for (int w = 0; w < HG; ++w) {
+      sm100::mbar_init(sm100::smem_u32(&xch_full[w]), sub > 1 ? sub - 1 : 1);
+      sm100::mbar_init(sm100::smem_u32(&xch_empty[w]), 1);
+    }
+    sm100::fence_barrier_init();
   }
   __syncthreads();
   const int64_t E = s_cum[p.nseg];
@@ -449,16 +534,18 @@ __global__ void __launch_bounds__(288, 1)
     // Dropped entries before the range shift the token ranks of its pages:
     // counted by the whole CTA (a warp alone takes 20 us over 8192 entries).
     const int j0 = (int)(lo - s_cum[seg0]);
-    int drop = 0;
+    if (j0 > 0) {
+      int drop = 0;
 #pragma unroll 8
-    for (int j = threadIdx.x; j < j0; j += blockDim.x) {
-      const int64_t id = btab.at((seg0 % B) * p.max_blocks + j);
-      drop += id < 0 || id >= p.num_blocks;
+      for (int j = threadIdx.x; j < j0; j += blockDim.x) {
+        const int64_t id = btab.at((seg0 % B) * p.max_blocks + j);
+        drop += id < 0 || id >= p.num_blocks;
+      }
+      drop = __reduce_add_sync(0xffffffffu, drop);
+      if (lane == 0 && drop) atomicAdd(s_drop, drop);
+      __syncthreads();
     }
-    drop = __reduce_add_sync(0xffffffffu, drop);
-    if (lane == 0 && drop) atomicAdd(s_drop, drop);
   }
-  __syncthreads();
 
   // Programmatic launch (cfg flags bit 3): what is above and the producer's
   // walk of the block table up to its first copy overlap the previous kernel,
@@ -480,19 +567,28 @@ __global__ void __launch_bounds__(288, 1)
     const uint32_t box = (uint32_t)(HG * bs * 128);  // one 128-byte-wide box: all of an 8-bit tile, half of a 16-bit one
     const uint32_t page_tx = k8 ? 2 * box + (uint32_t)(2 * HG * bs * 4) : 4 * box;
     const unsigned lt_mask = (1u << lane) - 1u;
-    int it = 0;
+    int it = 0, st = 0;
+    uint32_t ph = 1;  // parity of the empty barriers in this round
     bool ok = true, waited = p.overlap != 0;
-    // lane 0: the next stage, free to fill; false when the wait gave up
+    // lane 0: the next ring entry, free to fill; false when the wait gave up
     auto acquire = [&]() -> bool {
       if (*(volatile int*)s_abort) return false;
-      return sm100::mbar_wait(sm100::smem_u32(&empty_bar[it % p.stages]), ((it / p.stages) & 1) ^ 1);
+      return sm100::mbar_wait(sm100::smem_u32(&empty_bar[st]), ph);
     };
-    auto marker = [&](int kind, int seg, int piece, int direct) -> bool {
-      if (!acquire()) return false;
-      StageMeta& m = meta[it % p.stages];
-      m.kind = kind, m.seg = seg, m.piece = piece, m.direct = direct;
-      sm100::mbar_arrive(sm100::smem_u32(&full_bar[it % p.stages]));
+    auto advance = [&]() {
       ++it;
+      if (++st == p.stages) {
+        st = 0;
+        ph ^= 1u;
+      }
+    };
+    auto markers = [&](int kind, int seg, int piece) -> bool {  // one for each slot
+      for (int i = 0; i < sub; ++i) {
+        if (!acquire()) return false;
+        meta[st] = PageMeta{kind, seg, 0, piece};
+        sm100::mbar_arrive(sm100::smem_u32(&full_bar[st]));
+        advance();
+      }
       return true;
     };
     int s = seg0;
@@ -506,7 +602,6 @@ __global__ void __launch_bounds__(288, 1)
       const int ctx = s_ctx[b];
       const int64_t bt0 = b * p.max_blocks;
       int inval = e == lo ? *s_drop : 0;
-      int fill = 0;  // pages already in the open stage (lane 0)
       for (int jj = j0; jj < j1 && ok; jj += 32) {
         const int j = jj + lane;
         const bool in = j < j1;
@@ -527,34 +622,22 @@ __global__ void __launch_bounds__(288, 1)
         __syncwarp();
         if (lane == 0) {
           const int n = __popc(ub);
-          for (int u = 0; u < n && ok; ++u) {
-            const int st = it % p.stages;
-            if (fill == 0) {
-              ok = acquire();
-              if (!ok) break;
-              StageMeta& m = meta[st];
-              m.kind = 0, m.seg = s;
-              for (int i = 0; i < p.sub; ++i) m.ntok[i] = 0;
-              if (!waited) {  // programmatic launch: the first copy waits for the previous kernel
-                asm volatile("griddepcontrol.wait;" ::: "memory");
-                waited = true;
-              }
+          for (int u = 0; u < n; ++u) {
+            ok = acquire();
+            if (!ok) break;
+            if (!waited) {  // programmatic launch: the first copy waits for the previous kernel
+              asm volatile("griddepcontrol.wait;" ::: "memory");
+              waited = true;
             }
-            meta[st].ntok[fill] = chunk_ntok[u];
-            const uint32_t fb = sm100::smem_u32(&full_bar[st]);
-            const uint32_t dst = base + st * p.stage_bytes + fill * p.page_bytes;
-            const int id32 = chunk_id[u];
-            const int32_t tok0 = id32 * bs, h0 = hg * HG;
-            ++fill;
-            const bool last = fill == p.sub || (u == n - 1 && jj + 32 >= j1);
-            // the stage's one arrival comes with its last page; earlier pages only add bytes
-            if (last) sm100::mbar_arrive_expect_tx(fb, page_tx);
-            else asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(fb), "r"(page_tx) : "memory");
+            meta[st] = PageMeta{0, s, chunk_ntok[u], 0};
+            const uint32_t fb = sm100::smem_u32(&full_bar[st]), dst = base + st * p.page_bytes;
+            const int32_t tok0 = chunk_id[u] * bs, h0 = hg * HG;
+            sm100::mbar_arrive_expect_tx(fb, page_tx);
             if constexpr (k8) {
               sm100::tma_load_3d(dst, &tm_k, fb, 0, tok0, h0);
               sm100::tma_load_3d(dst + box, &tm_v, fb, 0, tok0, h0);
               const uint32_t sb = (uint32_t)(HG * bs * 4);
-              const int64_t sat = ((int64_t)id32 * p.Hkv + h0) * bs;
+              const int64_t sat = ((int64_t)chunk_id[u] * p.Hkv + h0) * bs;
               bulk_load(dst + 2 * box, k_scale + sat, sb, fb);
               bulk_load(dst + 2 * box + sb, v_scale + sat, sb, fb);
             } else {
@@ -563,16 +646,7 @@ __global__ void __launch_bounds__(288, 1)
               sm100::tma_load_3d(dst + 2 * box, &tm_v, fb, 0, tok0, h0);
               sm100::tma_load_3d(dst + 3 * box, &tm_v, fb, 64, tok0, h0);
             }
-            if (last) {
-              ++it;
-              fill = 0;
-            }
-          }
-          if (ok && fill > 0 && jj + 32 >= j1) {
-            // the range's last pages were dropped ids: close the open stage
-            sm100::mbar_arrive(sm100::smem_u32(&full_bar[it % p.stages]));
-            ++it;
-            fill = 0;
+            advance();
           }
         }
         ok = __shfl_sync(0xffffffffu, ok, 0);
@@ -580,14 +654,14 @@ __global__ void __launch_bounds__(288, 1)
       }
       if (lane == 0 && ok) {
         const bool one = range_of(segs, E, R) == range_of(sege - 1, E, R);
-        ok = marker(1, s, s + c, one && p.sub == 1 && !p.always);
+        ok = markers(1, s, one && !p.always ? -1 : s + c);
       }
       ok = __shfl_sync(0xffffffffu, ok, 0);
       e = segs + j1;
       if (e == sege) ++s;
     }
     if (lane == 0) {
-      if (ok) ok = marker(2, 0, 0, 0);
+      if (ok) ok = markers(2, 0, 0);
       if (!ok) {
         b200_dev_error(kDevErrTimeoutEmpty);
         atomicExch(s_abort, 1);
@@ -609,41 +683,98 @@ __global__ void __launch_bounds__(288, 1)
 #pragma unroll
     for (int i = 0; i < 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     int cur = -1;
-    for (int it = 0;; ++it) {
-      const int st = it % p.stages;
-      if (!sm100::mbar_wait_warp(sm100::smem_u32(&full_bar[st]), (it / p.stages) & 1)) {
-        b200_dev_error(kDevErrTimeoutFull);
-        atomicExch(s_abort, 1);
+    uint32_t xph = 0;
+    int st = slot % p.stages;
+    uint32_t ph = (slot / p.stages) & 1;
+    for (;;) {
+      if (!sm100::mbar_wait_warp(sm100::smem_u32(&full_bar[st]), ph)) {
+        if (lane == 0) {
+          b200_dev_error(kDevErrTimeoutFull);
+          atomicExch(s_abort, 1);
+        }
         break;
       }
-      const int kind = meta[st].kind, seg = meta[st].seg;
-      if (kind == 0) {
-        const int ntok = meta[st].ntok[slot];
-        const int64_t b = seg % B, kvh = (int64_t)(seg / B) * HG + w;
-        const T* qrow = q + (b * p.Hq + kvh * G) * kD;
-        if (seg != cur) {
-          cur = seg;
+      const PageMeta m = meta[st];
+      if (m.kind == 0) {
+        if (m.seg != cur) {
+          cur = m.seg;
+          const int64_t b = m.seg % B, kvh = (int64_t)(m.seg / B) * HG + w;
+          const T* qrow = q + (b * p.Hq + kvh * G) * kD;
           if constexpr (k8) load_q_frags8<T, G>(qrow, lane, p.qscale, qb, slA, slB);
           else load_q_frags<T, G>(qrow, lane, qb);
         }
-        const uint32_t pg = base + st * p.stage_bytes + slot * p.page_bytes;
-        if constexpr (k8) {
-          const float* sc = reinterpret_cast<const float*>(smem + st * p.stage_bytes + slot * p.page_bytes + 2 * box);
-          mma_page8<KV>(pg, pg + box, sc, sc + HG * bs, ntok, w, bs, lane, slA, slB, qb, o, mu, lp);
-        } else {
-          mma_page<T>(pg, pg + 2 * box, ntok, w, bs, lane, box, p.qscale, qb, o, mu, lp);
+        const uint32_t pg = base + st * p.page_bytes;
+        const float* sc = reinterpret_cast<const float*>(smem + st * p.page_bytes + 2 * box);
+        for (int t0 = 0; t0 < m.ntok; t0 += 16) {
+          if constexpr (k8)
+            mma_chunk8<KV>(pg, pg + box, sc, sc + HG * bs, t0, m.ntok, w * bs, lane, slA, slB, qb, o, mu, lp);
+          else
+            mma_chunk16<T>(pg, pg + 2 * box, box, t0, m.ntok, w * bs, lane, p.qscale, qb, o, mu, lp);
         }
-      } else if (kind == 1) {
-        const float lA = head_sum(lp[0]), lB = head_sum(lp[1]);
-        const int64_t b = seg % B, hg = seg / B;
-        if (meta[st].direct) {
-          T* orow = out + (b * p.Hq + hg * heads_cta + w * G) * kD;
-          if constexpr (k8) store_rows8<T, G>(orow, o, lA, lB, lane);
-          else store_rows<T, G>(orow, o, lA, lB, lane);
-        } else {
-          float* row0 = ws_rows + (((int64_t)meta[st].piece * p.sub + slot) * heads_cta + w * G) * kPiecePitch;
-          if constexpr (k8) store_piece8<G>(row0, o, mu, lA, lB, lane);
-          else store_partial<G>(row0, kPiecePitch, row0 + kD, kPiecePitch, o, mu, lA, lB, lane);
+      } else if (m.kind == 1) {
+        bool write = true;
+        if (sub > 1) {
+          // the head's other warps hand over their state; slot 0 adds it up
+          float* x = xch + ((slot - 1) * HG + w) * kXchPitch + lane;
+          if (slot > 0) {
+            write = false;
+            if (!sm100::mbar_wait_warp(sm100::smem_u32(&xch_empty[w]), xph ^ 1u)) {
+              if (lane == 0) {
+                b200_dev_error(kDevErrTimeoutCombine);
+                atomicExch(s_abort, 1);
+              }
+              break;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+              for (int k = 0; k < 4; ++k) x[(4 * i + k) * 32] = o[i][k];
+            x[32 * 32] = mu[0], x[33 * 32] = mu[1], x[34 * 32] = lp[0], x[35 * 32] = lp[1];
+            __syncwarp();
+            if (lane == 0) sm100::mbar_arrive(sm100::smem_u32(&xch_full[w]));
+          } else {
+            if (!sm100::mbar_wait_warp(sm100::smem_u32(&xch_full[w]), xph)) {
+              if (lane == 0) {
+                b200_dev_error(kDevErrTimeoutCombine);
+                atomicExch(s_abort, 1);
+              }
+              break;
+            }
+            for (int v = 1; v < sub; ++v) {
+              const float* y = xch + ((v - 1) * HG + w) * kXchPitch + lane;
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                // piece factors: 1 and 2^(difference); no tokens (m = -inf) adds nothing
+                const float mo = y[(32 + k) * 32], lo2 = y[(34 + k) * 32];
+                const float mn = fmaxf(mu[k], mo);
+                const float fa = mu[k] == mn || mu[k] == -INFINITY ? 1.f : ex2(mu[k] - mn);
+                const float fb = mo == mn || mo == -INFINITY ? 1.f : ex2(mo - mn);
+                mu[k] = mn;
+                lp[k] = lp[k] * fa + lo2 * fb;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                  o[i][k] = o[i][k] * fa + y[(4 * i + k) * 32] * fb;
+                  o[i][k + 2] = o[i][k + 2] * fa + y[(4 * i + k + 2) * 32] * fb;
+                }
+              }
+            }
+            __syncwarp();
+            if (lane == 0) sm100::mbar_arrive(sm100::smem_u32(&xch_empty[w]));
+          }
+          xph ^= 1u;
+        }
+        if (write) {
+          const float lA = head_sum(lp[0]), lB = head_sum(lp[1]);
+          const int64_t b = m.seg % B, hg = m.seg / B;
+          if (m.piece < 0) {
+            T* orow = out + (b * p.Hq + hg * heads_cta + w * G) * kD;
+            if constexpr (k8) store_rows8<T, G>(orow, o, lA, lB, lane);
+            else store_rows<T, G>(orow, o, lA, lB, lane);
+          } else {
+            float* row0 = ws_rows + ((int64_t)m.piece * heads_cta + w * G) * kPiecePitch;
+            if constexpr (k8) store_piece8<G>(row0, o, mu, lA, lB, lane);
+            else store_partial<G>(row0, kPiecePitch, row0 + kD, kPiecePitch, o, mu, lA, lB, lane);
+          }
         }
         mu[0] = mu[1] = -INFINITY;
         lp[0] = lp[1] = 0.f;
@@ -653,7 +784,12 @@ __global__ void __launch_bounds__(288, 1)
       }
       __syncwarp();
       if (lane == 0) sm100::mbar_arrive(sm100::smem_u32(&empty_bar[st]));
-      if (kind == 2) break;
+      if (m.kind == 2) break;
+      st += sub;
+      while (st >= p.stages) {
+        st -= p.stages;
+        ph ^= 1u;
+      }
     }
   }
   // this grid counts as done only when the previous one is
@@ -686,7 +822,7 @@ int launch_pieces(const AttnCall& a, const PieceGeom& g, const PieceSpace& w, bo
   p.nseg = (int)(g.n_hg * a.B);
   p.always = a.prefix_table != nullptr;
   p.overlap = overlap;
-  p.page_bytes = g.page_bytes, p.stage_bytes = g.stage_bytes;
+  p.page_bytes = g.page_bytes;
   p.qscale = a.scale * 1.4426950408889634f;
   auto kern = paged_attn_pieces_kernel<T, KV, G>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)g.smem);

@@ -10,6 +10,10 @@
 //                then weights), so that a thread needs few registers; O rescaled only when the
 //                maximum grew by more than 2^8
 //   O += P V     P (16-bit) over S's columns in tensor memory, V MN-major
+// With one row tile the two softmax warpgroups take its even and its odd key
+// tiles, each with an O of its own, joined in shared memory at the end: the
+// chain S -> softmax -> P V of one tile then runs beside the other's as with two row tiles.
+//
 // Reading the prefix costs its bytes once a CTA column instead of once a
 // sequence: at 64 sequences of an 8192-token prefix 33.5 MB instead of 2.1 GB.
 //
@@ -109,6 +113,7 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
   const int split = blockIdx.x, h = blockIdx.z;
   const int64_t R = p.B * p.G, row0 = (int64_t)blockIdx.y * 2 * kPM;
   const int tiles = R - row0 > kPM ? 2 : 1;
+  const int both = tiles == 2;  // else: streams 0 and 1 are the even and odd key tiles of one row tile
   const int bs = p.bs, tile_tok = p.ppt * bs;
 
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::oCodes + (k8 ? p.codes * kPCodes : 0));
@@ -171,7 +176,7 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
       sm100::mbar_init(sm100::smem_u32(&p_full[i]), 4);
       sm100::mbar_init(sm100::smem_u32(&o_done[i]), 1);
       sm100::mbar_init(sm100::smem_u32(&sc_full[i]), 4);
-      sm100::mbar_init(sm100::smem_u32(&sc_empty[i]), 4 * tiles);
+      sm100::mbar_init(sm100::smem_u32(&sc_empty[i]), 4 * tiles);  // one stream's warps, or both's
     }
     sm100::mbar_init(sm100::smem_u32(v_fixed), 1);
     for (int i = 0; i < kPMaxCodes; ++i) {
@@ -285,10 +290,11 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
       return sm100::mbar_wait_warp(sm100::smem_u32(&ring_full[it % kRing]), (it / kRing) & 1);
     };
     auto release = [&](int it) { sm100::tc_commit(sm100::smem_u32(&ring_empty[it % kRing]), leader); };
+    // stream t's n-th key tile: j = n with two row tiles, 2n + t with one
     auto issue_s = [&](int t, int j) -> bool {
       if (!full(2 * j)) return false;
       sm100::tc_fence_after();
-      const uint64_t ad = dq + (uint64_t)((t * kPTile) >> 4);
+      const uint64_t ad = dq + (uint64_t)((both * t * kPTile) >> 4);
       const uint64_t bd = dk + (uint64_t)((((2 * j) % kRing) * kPTile) >> 4);
 #pragma unroll
       for (int kk = 0; kk < kPieceDim / 16; ++kk) {
@@ -298,35 +304,52 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
       sm100::tc_commit(sm100::smem_u32(&s_full[t]), leader);
       return true;
     };
-    auto issue_pv = [&](int t, int j) -> bool {
-      if (!sm100::mbar_wait_warp(sm100::smem_u32(&p_full[t]), j & 1) || !full(2 * j + 1)) return false;
+    auto issue_pv = [&](int t, int n, int j) -> bool {
+      if (!sm100::mbar_wait_warp(sm100::smem_u32(&p_full[t]), n & 1) || !full(2 * j + 1)) return false;
       if (fix_v && j == nkt - 1 && !sm100::mbar_wait_warp(sm100::smem_u32(v_fixed), 0)) return false;
       sm100::tc_fence_after();
       const uint64_t bd = dv + (uint64_t)((((2 * j + 1) % kRing) * kPTile) >> 4);
 #pragma unroll
       for (int kk = 0; kk < kPM / 16; ++kk)
         sm100::mma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, bd + (uint64_t)((kk * 2048) >> 4), idesc_o,
-                          (j > 0 || kk > 0) ? 1u : 0u, leader);
+                          (n > 0 || kk > 0) ? 1u : 0u, leader);
       return true;
     };
-    for (int t = 0; t < tiles && ok; ++t) ok = issue_s(t, 0);
-    if (ok) release(0);
-    for (int j = 0; ok && j < nkt; ++j) {
-      if (*(volatile int*)s_abort) ok = false;
-      for (int t = 0; t < tiles && ok; ++t) {
-        ok = issue_pv(t, j);
-        if (ok && t == tiles - 1) release(2 * j + 1);
-        if (ok && j + 1 < nkt) ok = issue_s(t, j + 1);
-        if (ok && j + 1 == nkt) sm100::tc_commit(sm100::smem_u32(&o_done[t]), leader);
+    if (both) {
+      for (int t = 0; t < 2 && ok; ++t) ok = issue_s(t, 0);
+      if (ok) release(0);
+      for (int j = 0; ok && j < nkt; ++j) {
+        if (*(volatile int*)s_abort) ok = false;
+        for (int t = 0; t < 2 && ok; ++t) {
+          ok = issue_pv(t, j, j);
+          if (ok && t == 1) release(2 * j + 1);
+          if (ok && j + 1 < nkt) ok = issue_s(t, j + 1);
+          if (ok && j + 1 == nkt) sm100::tc_commit(sm100::smem_u32(&o_done[t]), leader);
+        }
+        if (ok && j + 1 < nkt) release(2 * (j + 1));
       }
-      if (ok && j + 1 < nkt) release(2 * (j + 1));
+    } else {
+      // S of tile j + 1 is issued before P V of tile j, which it runs beside
+      if (ok) ok = issue_s(0, 0);
+      if (ok) release(0);
+      for (int j = 0; ok && j < nkt; ++j) {
+        if (*(volatile int*)s_abort) ok = false;
+        if (ok && j + 1 < nkt) {
+          // (the stream's last P was read by its last P V, issued before)
+          ok = issue_s((j + 1) & 1, j + 1);
+          if (ok) release(2 * (j + 1));
+        }
+        if (ok) ok = issue_pv(j & 1, j >> 1, j);
+        if (ok) release(2 * j + 1);
+        if (ok && j + 2 >= nkt) sm100::tc_commit(sm100::smem_u32(&o_done[j & 1]), leader);
+      }
     }
     if (!ok && nkt > 0) {
       if (leader) {
         b200_dev_error(kDevErrTimeoutFull);
         atomicExch(s_abort, 1);
       }
-      for (int t = 0; t < tiles; ++t) sm100::tc_commit(sm100::smem_u32(&o_done[t]), leader);
+      for (int t = 0; t < 2; ++t) sm100::tc_commit(sm100::smem_u32(&o_done[t]), leader);
     }
   } else if (warp == 2) {
     // ---------------------------------- V rows behind the last token are zero
@@ -404,25 +427,28 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
         atomicExch(s_abort, 1);
       }
     }
-  } else if (warp >= 4 && warp < 12 && (warp >> 2) - 1 < tiles) {
+  } else if (warp >= 4 && warp < 12) {
     // --------------------------------------------------------------- softmax
     const int t = (warp >> 2) - 1, quarter = warp & 3;
     const int r = quarter * 32 + lane;
-    const int64_t qr = row0 + t * kPM + r;  // row of Q_h
+    const int64_t qr = row0 + both * t * kPM + r;  // row of Q_h
     const bool live = qr < R;
     const int64_t b = live ? qr / p.G : 0;
     const int64_t qrow = b * p.Hq + (int64_t)h * p.G + (live ? qr - b * p.G : 0);
+    // (with one row tile the second stream stages it too, into the unused tile, for the row's factor)
     const float sl = stage_q_row<T, k8>(q + qrow * kPieceDim, live, smem + L::oQ + t * kPTile, r, p.qscale);
     sm100::fence_proxy_async_smem();
     __syncwarp();
-    if (lane == 0) sm100::mbar_arrive(sm100::smem_u32(q_full));
+    if (lane == 0 && (both || t == 0)) sm100::mbar_arrive(sm100::smem_u32(q_full));
 
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
     const uint32_t tS = tmem + t * 128 + lane_off, tO = tmem + 256 + t * 128 + lane_off;
     float m_used = -INFINITY, l = 0.f;
     bool ok = true;
-    for (int j = 0; j < nkt; ++j) {
-      ok = sm100::mbar_wait_warp(sm100::smem_u32(&s_full[t]), j & 1);
+    const int n_tiles = both ? nkt : (nkt - t + 1) / 2;  // key tiles of this stream
+    for (int n = 0; n < n_tiles; ++n) {
+      const int j = both ? n : 2 * n + t;
+      ok = sm100::mbar_wait_warp(sm100::smem_u32(&s_full[t]), n & 1);
       if (k8 && ok) ok = sm100::mbar_wait_warp(sm100::smem_u32(&sc_full[j & 1]), (j >> 1) & 1);
       if (!ok) break;
       sm100::tc_fence_after();
@@ -509,24 +535,61 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
       }
     }
     // ---- the row's piece
-    if (ok && nkt > 0) ok = sm100::mbar_wait_warp(sm100::smem_u32(&o_done[t]), 0);
+    if (ok && n_tiles > 0) ok = sm100::mbar_wait_warp(sm100::smem_u32(&o_done[t]), 0);
     if (!ok) {
       b200_dev_error(kDevErrTimeoutMma);
       atomicExch(s_abort, 1);
     }
     sm100::tc_fence_after();
-    float* dst = pieces + ((int64_t)split * p.B * p.Hq + qrow) * kPiecePitch;
-    if (live) *reinterpret_cast<float2*>(dst + kPieceDim) = make_float2(m_used, l);
-    if (nkt > 0) {
+    // With one row tile stream 1 hands its state to stream 0 through the K/V
+    // ring, which nothing reads any more once both streams' products are done.
+    // (Every path leads both warpgroups to the barrier.)
+    float* hand = reinterpret_cast<float*>(smem + L::oRing);  // [130][128]
+    const bool join = !both && nkt > 1;
+    float f0 = 1.f, f1 = 0.f;
+    if (join) {
+      if (t == 1) {
+        if (ok && !sm100::mbar_wait_warp(sm100::smem_u32(&o_done[0]), 0)) ok = false;
+        sm100::tc_fence_after();
 #pragma unroll 1
-      for (int c = 0; c < kPieceDim; c += 32) {
-        uint32_t o[32];
-        sm100::tmem_ld_32x32b_x32(tO + c, o);
-        sm100::tmem_wait_ld_regs(o);
-        if (live) {
+        for (int c = 0; c < kPieceDim; c += 32) {
+          uint32_t o[32];
+          sm100::tmem_ld_32x32b_x32(tO + c, o);
+          sm100::tmem_wait_ld_regs(o);
 #pragma unroll
-          for (int i = 0; i < 32; i += 4)
-            *reinterpret_cast<uint4*>(dst + c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          for (int i = 0; i < 32; ++i) hand[(c + i) * kPM + r] = __uint_as_float(o[i]);
+        }
+        hand[128 * kPM + r] = m_used;
+        hand[129 * kPM + r] = l;
+      }
+      named_bar_sync(1, 256);
+      if (t == 0) {
+        const float m1 = hand[128 * kPM + r], mn = fmaxf(m_used, m1);
+        f0 = m_used == mn || m_used == -INFINITY ? 1.f : ex2(m_used - mn);
+        f1 = m1 == mn || m1 == -INFINITY ? 1.f : ex2(m1 - mn);
+        m_used = mn;
+        l = l * f0 + hand[129 * kPM + r] * f1;
+      }
+    }
+    if (both || t == 0) {
+      float* dst = pieces + ((int64_t)split * p.B * p.Hq + qrow) * kPiecePitch;
+      if (live) *reinterpret_cast<float2*>(dst + kPieceDim) = make_float2(m_used, l);
+      if (n_tiles > 0) {
+#pragma unroll 1
+        for (int c = 0; c < kPieceDim; c += 32) {
+          uint32_t o[32];
+          sm100::tmem_ld_32x32b_x32(tO + c, o);
+          sm100::tmem_wait_ld_regs(o);
+          if (join) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              o[i] = __float_as_uint(__uint_as_float(o[i]) * f0 + hand[(c + i) * kPM + r] * f1);
+          }
+          if (live) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              *reinterpret_cast<uint4*>(dst + c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          }
         }
       }
     }
