@@ -31,7 +31,7 @@
 namespace b200 {
 
 constexpr int kPieceDim = 128;
-constexpr int kPiecePitch = kPieceDim + 4;  // floats of a piece row: o[128], m, l, pad
+constexpr int kPiecePitch = kPieceDim + 8;  // floats of a piece row: o[128], m, l, pad to whole 32-byte sectors
 constexpr int kMaxSeg = 2048;               // (sequence, head group) segments a launch takes
 
 // One attention call, as the C entries take it (host side).
@@ -85,6 +85,30 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Shared memory by 32-bit address (the kernels' base is aligned at run time,
+// which hides its address space from the compiler: plain accesses would be generic).
+__device__ __forceinline__ float lds_f32(uint32_t a) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 lds_f32x4(uint32_t a) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ int lds_s32(uint32_t a) {
+  int v;
+  asm volatile("ld.shared.s32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts_f32(uint32_t a, float v) {
+  asm volatile("st.shared.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory");
+}
+__device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
 namespace {
@@ -256,8 +280,7 @@ __device__ __forceinline__ void raise_max_lazy(const float (&y)[4], float (&mu)[
 // Tokens [t0, t0 + 16) of kv head w's rows of a page (codes at kb / vb as
 // [head][token][128] rows, 128-byte swizzled; scales at ksp / vsp as [head][token]).
 template <typename KV>
-__device__ __forceinline__ void mma_chunk8(uint32_t kb, uint32_t vb, const float* __restrict__ ksp,
-                                           const float* __restrict__ vsp, int t0, int ntok, int row0, int lane,
+__device__ __forceinline__ void mma_chunk8(uint32_t kb, uint32_t vb, uint32_t ksp, uint32_t vsp, int t0, int ntok, int row0, int lane,
                                            float slA, float slB, const uint32_t (&qb)[8][2], float (&o)[8][4],
                                            float (&mu)[2], float (&lp)[2]) {
   const int mat = lane >> 3, mrow = lane & 7;
@@ -280,11 +303,11 @@ __device__ __forceinline__ void mma_chunk8(uint32_t kb, uint32_t vb, const float
   uint32_t vr[4][4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) ldsm_x4_t(vb + at + (sw ^ (j << 5)), vr[j][0], vr[j][1], vr[j][2], vr[j][3]);
-  const int tok = row0 + t0 + tr;
-  const float k0 = ksp[tok], k1 = ksp[tok + 8];
+  const uint32_t tok = (uint32_t)(row0 + t0 + tr) * 4;
+  const float k0 = lds_f32(ksp + tok), k1 = lds_f32(ksp + tok + 32);
   float lv0, iv0, lv1, iv1;
-  kv8_value_scale(vsp[tok], lv0, iv0);
-  kv8_value_scale(vsp[tok + 8], lv1, iv1);
+  kv8_value_scale(lds_f32(vsp + tok), lv0, iv0);
+  kv8_value_scale(lds_f32(vsp + tok + 32), lv1, iv1);
   // y[0]/y[1]: token tr of heads 2(lane%4), +1; y[2]/y[3]: token tr + 8
   float y[4];
   y[0] = fmaf(s0[0] + s1[0], k0 * slA, lv0);
@@ -471,6 +494,7 @@ __global__ void __launch_bounds__((kConsumers + 1) * 32, 1)
   uint64_t* empty_bar = full_bar + p.stages;
   uint64_t* xch_full = empty_bar + p.stages;  // [8]
   uint64_t* xch_empty = xch_full + 8;         // [8]
+  static_assert(sizeof(PageMeta) == 16, "read as one vector");
   PageMeta* meta = reinterpret_cast<PageMeta*>(xch_empty + 8);
   int* s_cum = reinterpret_cast<int*>(meta + p.stages);
   int* s_ctx = s_cum + (p.nseg + 1);
@@ -674,7 +698,8 @@ __global__ void __launch_bounds__((kConsumers + 1) * 32, 1)
   } else if (c < R && warp < consumers) {
     // ------------------------------------------------------------ consumers
     const int w = warp % HG, slot = warp / HG;
-    const uint32_t base = sm100::smem_u32(smem);
+    const uint32_t base = sm100::smem_u32(smem), meta_at = sm100::smem_u32(meta);
+    const uint32_t xch_at = sm100::smem_u32(xch) + (uint32_t)(w * kXchPitch + lane) * 4;
     const uint32_t box = (uint32_t)(HG * bs * 128);
     uint32_t qb[8][2];
     float o[8][4];
@@ -694,7 +719,8 @@ __global__ void __launch_bounds__((kConsumers + 1) * 32, 1)
         }
         break;
       }
-      const PageMeta m = meta[st];
+      const uint4 mw = lds128(meta_at + st * (int)sizeof(PageMeta));
+      const PageMeta m{(int)mw.x, (int)mw.y, (int)mw.z, (int)mw.w};
       if (m.kind == 0) {
         if (m.seg != cur) {
           cur = m.seg;
@@ -704,10 +730,10 @@ __global__ void __launch_bounds__((kConsumers + 1) * 32, 1)
           else load_q_frags<T, G>(qrow, lane, qb);
         }
         const uint32_t pg = base + st * p.page_bytes;
-        const float* sc = reinterpret_cast<const float*>(smem + st * p.page_bytes + 2 * box);
+        const uint32_t sc = pg + 2 * box;
         for (int t0 = 0; t0 < m.ntok; t0 += 16) {
           if constexpr (k8)
-            mma_chunk8<KV>(pg, pg + box, sc, sc + HG * bs, t0, m.ntok, w * bs, lane, slA, slB, qb, o, mu, lp);
+            mma_chunk8<KV>(pg, pg + box, sc, sc + HG * bs * 4, t0, m.ntok, w * bs, lane, slA, slB, qb, o, mu, lp);
           else
             mma_chunk16<T>(pg, pg + 2 * box, box, t0, m.ntok, w * bs, lane, p.qscale, qb, o, mu, lp);
         }
@@ -715,7 +741,7 @@ __global__ void __launch_bounds__((kConsumers + 1) * 32, 1)
         bool write = true;
         if (sub > 1) {
           // the head's other warps hand over their state; slot 0 adds it up
-          float* x = xch + ((slot - 1) * HG + w) * kXchPitch + lane;
+          const uint32_t x = xch_at + (uint32_t)((slot - 1) * HG * kXchPitch) * 4;
           if (slot > 0) {
             write = false;
             if (!sm100::mbar_wait_warp(sm100::smem_u32(&xch_empty[w]), xph ^ 1u)) {
@@ -728,8 +754,11 @@ __global__ void __launch_bounds__((kConsumers + 1) * 32, 1)
 #pragma unroll
             for (int i = 0; i < 8; ++i)
 #pragma unroll
-              for (int k = 0; k < 4; ++k) x[(4 * i + k) * 32] = o[i][k];
-            x[32 * 32] = mu[0], x[33 * 32] = mu[1], x[34 * 32] = lp[0], x[35 * 32] = lp[1];
+              for (int k = 0; k < 4; ++k) sts_f32(x + (4 * i + k) * 128, o[i][k]);
+            sts_f32(x + 32 * 128, mu[0]);
+            sts_f32(x + 33 * 128, mu[1]);
+            sts_f32(x + 34 * 128, lp[0]);
+            sts_f32(x + 35 * 128, lp[1]);
             __syncwarp();
             if (lane == 0) sm100::mbar_arrive(sm100::smem_u32(&xch_full[w]));
           } else {
@@ -741,11 +770,11 @@ __global__ void __launch_bounds__((kConsumers + 1) * 32, 1)
               break;
             }
             for (int v = 1; v < sub; ++v) {
-              const float* y = xch + ((v - 1) * HG + w) * kXchPitch + lane;
+              const uint32_t y = xch_at + (uint32_t)((v - 1) * HG * kXchPitch) * 4;
 #pragma unroll
               for (int k = 0; k < 2; ++k) {
                 // piece factors: 1 and 2^(difference); no tokens (m = -inf) adds nothing
-                const float mo = y[(32 + k) * 32], lo2 = y[(34 + k) * 32];
+                const float mo = lds_f32(y + (32 + k) * 128), lo2 = lds_f32(y + (34 + k) * 128);
                 const float mn = fmaxf(mu[k], mo);
                 const float fa = mu[k] == mn || mu[k] == -INFINITY ? 1.f : ex2(mu[k] - mn);
                 const float fb = mo == mn || mo == -INFINITY ? 1.f : ex2(mo - mn);
@@ -753,8 +782,8 @@ __global__ void __launch_bounds__((kConsumers + 1) * 32, 1)
                 lp[k] = lp[k] * fa + lo2 * fb;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                  o[i][k] = o[i][k] * fa + y[(4 * i + k) * 32] * fb;
-                  o[i][k + 2] = o[i][k + 2] * fa + y[(4 * i + k + 2) * 32] * fb;
+                  o[i][k] = o[i][k] * fa + lds_f32(y + (4 * i + k) * 128) * fb;
+                  o[i][k + 2] = o[i][k + 2] * fa + lds_f32(y + (4 * i + k + 2) * 128) * fb;
                 }
               }
             }

@@ -6,9 +6,8 @@
 // stretch of the prefix's block table, and leaves one piece (m, l, o) a row --
 // the pieces the streaming kernel leaves for the own tokens, joined with them:
 //   S = Q K^T    tcgen05.mma 128 x 128 x 16 (Q, K K-major in shared memory), fp32 in tensor memory
-//   softmax      one thread a row: the row's 128 logits read twice from tensor memory (maximum,
-//                then weights), so that a thread needs few registers; O rescaled only when the
-//                maximum grew by more than 2^8
+//   softmax      one thread a row, the row's 128 logits in registers; O rescaled only
+//                when the maximum grew by more than 2^8
 //   O += P V     P (16-bit) over S's columns in tensor memory, V MN-major
 // With one row tile the two softmax warpgroups take its even and its odd key
 // tiles, each with an O of its own, joined in shared memory at the end: the
@@ -17,9 +16,9 @@
 // Reading the prefix costs its bytes once a CTA column instead of once a
 // sequence: at 64 sequences of an 8192-token prefix 33.5 MB instead of 2.1 GB.
 //
-// Roles: warp 0 walks the block table and copies pages (TMA boxes of bs
+// Roles: warps 0, 2 and 3 walk the block table and copy pages (TMA boxes of bs
 // tokens; a tile is as many pages as fit 128 tokens), warp 1 issues the MMAs,
-// warps 4-11 are the two tiles' softmax warpgroups.  16-bit caches: pages land
+// warps 4-11 are the two streams' softmax warpgroups.  16-bit caches: pages land
 // in the K/V ring as the MMA reads them; warp 2 zeroes V rows behind the last
 // token (a weight of 0 times a NaN left in the cache is NaN).  8-bit caches:
 // pages land in a ring of code tiles, and warps 12-15 widen them to f16 tiles
@@ -47,7 +46,7 @@ constexpr int kPMaxPages = 8;              // pages of a tile (block size 16)
 
 struct PrefixParams {
   int64_t B, Hq, Hkv, num_blocks, max_prefix;
-  int G, bs, ppt;  // pages a key tile
+  int lgG, bs, ppt;  // log2 of the query heads a kv head, block size, pages a key tile
   int codes;       // ring depth of the code tiles (8-bit)
   int splits;
   float qscale;  // scale * log2(e)
@@ -60,42 +59,59 @@ struct PrefixSmem {
   static constexpr uint32_t oCodes = oRing + (k8 ? kPRing8 : kPRing16) * kPTile;
 };
 
-// One row of Q into the swizzled tile: 16-byte chunk c of row r sits at chunk
-// c ^ (r & 7) of its 128-byte row, dims 64.. in the second half.  8-bit caches: f16, the
-// row scaled to [2^13, 2^14) by a power of two; returns its logit factor.
+// A warp's 32 rows of Q (row r of the batch's matrix: sequence r / G, head h G +
+// r % G) into the swizzled tile at `tile`: 16-byte chunk c of row r sits at
+// chunk c ^ (r & 7) of its 128-byte row, dims 64.. in the second half.  Sixteen
+// lanes a row, so that the loads are whole rows.  8-bit caches: f16, each row scaled
+// to [2^13, 2^14) by a power of two.  Returns the logit factor of row `lane`.
 template <typename T, bool k8>
-__device__ __forceinline__ float stage_q_row(const T* __restrict__ src, bool live, uint8_t* tile, int r, float qscale) {
+__device__ __forceinline__ float stage_q_rows(const T* __restrict__ q, int r0, int R, int64_t Hq, int h, int lgG,
+                                              uint32_t tile, int r_tile, int lane, float qscale) {
+  const int c = lane & 15, odd = lane >> 4;
   uint4 raw[16];
 #pragma unroll
-  for (int c = 0; c < 16; ++c)
-    raw[c] = live ? __ldg(reinterpret_cast<const uint4*>(src) + c) : make_uint4(0, 0, 0, 0);
-  float factor = qscale;
-  if constexpr (k8) {
-    float amax = 0.f;
-#pragma unroll
-    for (int c = 0; c < 16; ++c) {
-      float f[8];
-      unpack16<T>(raw[c], f);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(f[i]));
-    }
-    float up, down;
-    pow2_scale(amax, up, down);
-    factor *= down;
-#pragma unroll
-    for (int c = 0; c < 16; ++c) {
-      float f[8];
-      unpack16<T>(raw[c], f);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] *= up;
-      raw[c] = pack16<__half>(f);
+  for (int i = 0; i < 16; ++i) {
+    const int r = r0 + 2 * i + odd;
+    raw[i] = make_uint4(0, 0, 0, 0);
+    if (r < R) {
+      const int64_t row = (int64_t)(r >> lgG) * Hq + (h << lgG) + (r & ((1 << lgG) - 1));
+      raw[i] = __ldg(reinterpret_cast<const uint4*>(q + row * kPieceDim) + c);
     }
   }
+  float factor = qscale;
 #pragma unroll
-  for (int c = 0; c < 16; ++c)
-    *reinterpret_cast<uint4*>(tile + (c >> 3) * kPHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = raw[c];
+  for (int i = 0; i < 16; ++i) {
+    if constexpr (k8) {
+      float f[8], amax = 0.f, up, down;
+      unpack16<T>(raw[i], f);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) amax = fmaxf(amax, fabsf(f[k]));
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      pow2_scale(amax, up, down);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) f[k] *= up;
+      raw[i] = pack16<__half>(f);
+      const float d = __shfl_sync(0xffffffffu, down, (lane & 1) * 16);
+      if (i == lane >> 1) factor = qscale * d;
+    }
+    const int r = r_tile + 2 * i + odd;
+    sts128(tile + (c >> 3) * kPHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4), raw[i]);
+  }
   return factor;
 }
+
+// 32 bytes of one lane as one store (whole sectors).
+__device__ __forceinline__ void stg256(float* dst, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
+// Producer warps share a tile's boxes: issuing one costs a thread about a
+// hundred cycles, and a tile of 16-token pages is 16 or 32 of them.
+constexpr int kPProducers = 3;
+constexpr int kPRegsLow = 72, kPRegsHigh = 184;  // 8-bit kernel: 8 warps each way, 128 a thread at launch
 
 template <typename T, typename KV>
 __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
@@ -111,14 +127,13 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
   const uint32_t sbase = sm100::smem_u32(smem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int split = blockIdx.x, h = blockIdx.z;
-  const int64_t R = p.B * p.G, row0 = (int64_t)blockIdx.y * 2 * kPM;
+  const int R = (int)p.B << p.lgG, row0 = (int)blockIdx.y * 2 * kPM;
   const int tiles = R - row0 > kPM ? 2 : 1;
   const int both = tiles == 2;  // else: streams 0 and 1 are the even and odd key tiles of one row tile
   const int bs = p.bs, tile_tok = p.ppt * bs;
 
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::oCodes + (k8 ? p.codes * kPCodes : 0));
-  uint64_t* q_full = bars;
-  uint64_t* ring_full = bars + 1;               // [kRing]
+  uint64_t* ring_full = bars;                   // [kRing]
   uint64_t* ring_empty = ring_full + kPRing16;  // [kRing]
   uint64_t* s_full = ring_empty + kPRing16;     // [2]
   uint64_t* p_full = s_full + 2;                // [2]
@@ -129,8 +144,9 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
   uint64_t* code_full = sc_empty + 2;           // [kPMaxCodes]
   uint64_t* code_empty = code_full + kPMaxCodes;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(code_empty + kPMaxCodes);
-  int* s_misc = reinterpret_cast<int*>(tmem_slot + 1);  // [0] abort, [1] valid entries before the split, [2] in it
-  int* s_ids = s_misc + 3;                              // [kPMaxCodes][kPMaxPages] page ids of a code tile
+  int* s_abort = reinterpret_cast<int*>(tmem_slot + 1);
+  int* s_count = s_abort + 5;  // (16-byte aligned from here) [2][4] valid entries before the split and in it, by warp
+  int* s_ids = s_count + 8;    // [kPMaxCodes][kPMaxPages] page ids of a code tile
   float* s_sc = reinterpret_cast<float*>(s_ids + kPMaxCodes * kPMaxPages);  // [2][3][kPM]: ks, log2 vs, 1 / vs
 
   // the own-token kernel may run beside this one
@@ -148,27 +164,28 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
     const int64_t a = (int64_t)split * per, b = a + per;
     e0 = (int)(a < E ? a : E);
     e1 = (int)(b < E ? b : E);
-    if (threadIdx.x < 3) s_misc[threadIdx.x] = 0;
-    __syncthreads();
-    // valid entries before the split and in it, counted by the whole CTA
-    int before = 0, in = 0;
-    for (int j = threadIdx.x; j < e1; j += blockDim.x) {
-      const int64_t id = ptab.at(j);
-      const int ok = id >= 0 && id < p.num_blocks;
-      if (j < e0) before += ok;
-      else in += ok;
-    }
-    before = __reduce_add_sync(0xffffffffu, before);
-    in = __reduce_add_sync(0xffffffffu, in);
-    if (lane == 0) {
-      atomicAdd(&s_misc[1], before);
-      atomicAdd(&s_misc[2], in);
+    if (warp < 4) {
+      // valid entries before the split and in it, counted by the first four warps
+      int before = 0, in = 0;
+#pragma unroll 4
+      for (int j = threadIdx.x; j < e1; j += 128) {
+        const int64_t id = ptab.at(j);
+        const int ok = id >= 0 && id < p.num_blocks;
+        if (j < e0) before += ok;
+        else in += ok;
+      }
+      before = __reduce_add_sync(0xffffffffu, before);
+      in = __reduce_add_sync(0xffffffffu, in);
+      if (lane == 0) {
+        s_count[warp] = before;
+        s_count[4 + warp] = in;
+      }
     }
   }
   if (threadIdx.x == 32) {
-    sm100::mbar_init(sm100::smem_u32(q_full), 4 * tiles);
+    *s_abort = 0;
     for (int i = 0; i < kRing; ++i) {
-      sm100::mbar_init(sm100::smem_u32(&ring_full[i]), k8 ? 4 : 1);
+      sm100::mbar_init(sm100::smem_u32(&ring_full[i]), k8 ? 4 : kPProducers);
       sm100::mbar_init(sm100::smem_u32(&ring_empty[i]), 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -180,7 +197,7 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
     }
     sm100::mbar_init(sm100::smem_u32(v_fixed), 1);
     for (int i = 0; i < kPMaxCodes; ++i) {
-      sm100::mbar_init(sm100::smem_u32(&code_full[i]), 1);
+      sm100::mbar_init(sm100::smem_u32(&code_full[i]), kPProducers);
       sm100::mbar_init(sm100::smem_u32(&code_empty[i]), 4);
     }
     sm100::fence_barrier_init();
@@ -197,51 +214,66 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
     sm100::tmem_alloc(sm100::smem_u32(tmem_slot), 512);
     sm100::tmem_relinquish();
   }
+  // the softmax warps stage Q meanwhile (with one row tile the second stream
+  // stages it too, into the unused tile, for its rows' factors)
+  float sl = p.qscale;
+  if (warp >= 4 && warp < 12) {
+    const int t = (warp >> 2) - 1, rw = (warp & 3) * 32;
+    sl = stage_q_rows<T, k8>(q, row0 + both * t * kPM + rw, R, p.Hq, h, p.lgG, sbase + L::oQ + t * kPTile, rw, lane,
+                             p.qscale);
+    sm100::fence_proxy_async_smem();
+  }
   sm100::tc_fence_before();
   __syncthreads();
   sm100::tc_fence_after();
   const uint32_t tmem = *tmem_slot;  // columns: S_t at 128 t, O_t at 256 + 128 t
-  int* s_abort = &s_misc[0];
   int ntok;
   {
-    const int64_t left = plen_tokens - (int64_t)s_misc[1] * bs, have = (int64_t)s_misc[2] * bs;
+    const int before = s_count[0] + s_count[1] + s_count[2] + s_count[3];
+    const int in = s_count[4] + s_count[5] + s_count[6] + s_count[7];
+    const int64_t left = plen_tokens - (int64_t)before * bs, have = (int64_t)in * bs;
     ntok = (int)(left < 0 ? 0 : (left < have ? left : have));
   }
   const int nkt = (ntok + tile_tok - 1) / tile_tok;
   const int last_valid = ntok - (nkt - 1) * tile_tok;  // tokens of the last tile
   const bool fix_v = !k8 && nkt > 0 && last_valid < tile_tok;
 
-  if (warp == 0) {
-    // -------------------------------------------------------------- producer
+  if (k8 && warp < 4) sm100::setmaxnreg_dec<kPRegsLow>();
+  if (warp == 0 || warp == 2 || warp == 3) {
+    // ------------------------------------------------------------- producers
+    const int mine = warp == 0 ? 0 : warp - 1;  // of kPProducers
     if (lane == 0) {
       sm100::tma_prefetch_desc(&tm_k);
       sm100::tma_prefetch_desc(&tm_v);
     }
+    constexpr int kHalves = k8 ? 1 : 2;  // boxes of a page
+    const int depth = k8 ? p.codes : kRing;
+    uint64_t* fulls = k8 ? code_full : ring_full;
+    uint64_t* empties = k8 ? code_empty : ring_empty;
     int left = (ntok + bs - 1) / bs;  // pages still to copy
-    int issued = 0, np = 0;           // (lane 0) copies of tiles issued, pages of the open tile
+    int issued = 0, np = 0;           // tiles issued, pages of the open tile
     int ids[kPMaxPages];
     bool ok = true;
+    // lane 0: this warp's boxes of a tile (box x = page and half)
     auto copy_tile = [&](int which) -> bool {
-      const int depth = k8 ? p.codes : kRing;
       const int slot = issued % depth;
-      uint64_t* empty = k8 ? code_empty : ring_empty;
       if (*(volatile int*)s_abort) return false;
-      if (!sm100::mbar_wait(sm100::smem_u32(&empty[slot]), ((issued / depth) & 1) ^ 1)) return false;
-      const uint32_t fb = sm100::smem_u32(&(k8 ? code_full : ring_full)[slot]);
+      if (!sm100::mbar_wait(sm100::smem_u32(&empties[slot]), ((issued / depth) & 1) ^ 1)) return false;
+      const uint32_t fb = sm100::smem_u32(&fulls[slot]);
       const CUtensorMap* map = which ? &tm_v : &tm_k;
-      if constexpr (k8) {
+      const uint32_t dst = sbase + (k8 ? L::oCodes + slot * kPCodes : L::oRing + slot * kPTile);
+      if (k8 && mine == 0) {
 #pragma unroll
         for (int i = 0; i < kPMaxPages; ++i)
           if (i < np) s_ids[slot * kPMaxPages + i] = ids[i];
       }
-      sm100::mbar_arrive_expect_tx(fb, (uint32_t)(np * bs * (k8 ? 128 : 256)));
-      const uint32_t dst = sbase + (k8 ? L::oCodes + slot * kPCodes : L::oRing + slot * kPTile);
+      const int n = np * kHalves;
+      sm100::mbar_arrive_expect_tx(fb, (uint32_t)((n - mine + kPProducers - 1) / kPProducers * bs * 128));
 #pragma unroll
-      for (int i = 0; i < kPMaxPages; ++i) {
-        if (i < np) {
-          sm100::tma_load_3d(dst + i * bs * 128, map, fb, 0, ids[i] * bs, h);
-          if constexpr (!k8) sm100::tma_load_3d(dst + kPHalf + i * bs * 128, map, fb, 64, ids[i] * bs, h);
-        }
+      for (int x = 0; x < kPMaxPages * kHalves; ++x) {
+        if (x % kPProducers == mine && x < n)
+          sm100::tma_load_3d(dst + (x % kHalves) * kPHalf + (x / kHalves) * bs * 128, map, fb, (x % kHalves) * 64,
+                             ids[x / kHalves] * bs, h);
       }
       ++issued;
       return true;
@@ -271,10 +303,26 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
         atomicExch(s_abort, 1);
       }
       // no copy may still be writing shared memory when the CTA exits
-      const int depth = k8 ? p.codes : kRing;
       for (int i = issued - 1; i >= 0 && i >= issued - depth; --i)
-        if (!sm100::mbar_wait(sm100::smem_u32(&(k8 ? code_full : ring_full)[i % depth]), (i / depth) & 1))
-          b200_dev_error(kDevErrTimeoutFull);
+        if (!sm100::mbar_wait(sm100::smem_u32(&fulls[i % depth]), (i / depth) & 1)) b200_dev_error(kDevErrTimeoutFull);
+    }
+    __syncwarp();
+    if (warp == 2 && fix_v) {
+      // V rows behind the last token are zero
+      const int it = 2 * nkt - 1, slot = it % kRing;
+      if (sm100::mbar_wait_warp(sm100::smem_u32(&ring_full[slot]), (it / kRing) & 1)) {
+        for (int i = lane; i < 2 * (tile_tok - last_valid) * 8; i += 32) {
+          const int c = i & 7, r = (i >> 3) % (tile_tok - last_valid), half = (i >> 3) / (tile_tok - last_valid);
+          sts128(sbase + L::oRing + slot * kPTile + half * kPHalf + (last_valid + r) * 128 + c * 16,
+                 make_uint4(0, 0, 0, 0));
+        }
+        sm100::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) sm100::mbar_arrive(sm100::smem_u32(v_fixed));
+      } else if (lane == 0) {
+        b200_dev_error(kDevErrTimeoutFull);
+        atomicExch(s_abort, 1);
+      }
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------- MMA issue
@@ -285,7 +333,7 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
     const uint64_t dq = sm100::make_smem_desc(sbase + L::oQ, 16, 1024, sm100::kSwizzle128B);
     const uint64_t dk = sm100::make_smem_desc(sbase + L::oRing, 16, 1024, sm100::kSwizzle128B);
     const uint64_t dv = sm100::make_smem_desc(sbase + L::oRing, kPHalf, 1024, sm100::kSwizzle128B);
-    bool ok = nkt > 0 && sm100::mbar_wait_warp(sm100::smem_u32(q_full), 0);
+    bool ok = nkt > 0;
     auto full = [&](int it) -> bool {
       return sm100::mbar_wait_warp(sm100::smem_u32(&ring_full[it % kRing]), (it / kRing) & 1);
     };
@@ -351,27 +399,10 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
       }
       for (int t = 0; t < 2; ++t) sm100::tc_commit(sm100::smem_u32(&o_done[t]), leader);
     }
-  } else if (warp == 2) {
-    // ---------------------------------- V rows behind the last token are zero
-    if (fix_v) {
-      const int it = 2 * nkt - 1, slot = it % kRing;
-      if (sm100::mbar_wait_warp(sm100::smem_u32(&ring_full[slot]), (it / kRing) & 1)) {
-        for (int i = lane; i < 2 * (tile_tok - last_valid) * 8; i += 32) {
-          const int c = i & 7, r = (i >> 3) % (tile_tok - last_valid), half = (i >> 3) / (tile_tok - last_valid);
-          *reinterpret_cast<uint4*>(smem + L::oRing + slot * kPTile + half * kPHalf + (last_valid + r) * 128 + c * 16) =
-              make_uint4(0, 0, 0, 0);
-        }
-        sm100::fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) sm100::mbar_arrive(sm100::smem_u32(v_fixed));
-      } else if (lane == 0) {
-        b200_dev_error(kDevErrTimeoutFull);
-        atomicExch(s_abort, 1);
-      }
-    }
   } else if (k8 && warp >= 12) {
     // ------------------------------------------------- code tiles to f16 tiles
     if constexpr (k8) {
+      sm100::setmaxnreg_dec<kPRegsLow>();
       const int r = threadIdx.x - 384;  // this thread's key of every tile
       const int page = r / bs, off = r - page * bs;
       bool ok = true;
@@ -382,27 +413,30 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
         ok = sm100::mbar_wait_warp(sm100::smem_u32(&code_full[cs]), (it / p.codes) & 1);
         float ks = 0.f, vs = 1.f;
         if (ok && which == 0 && live) {
-          const int64_t at = ((int64_t)s_ids[cs * kPMaxPages + page] * p.Hkv + h) * bs + off;
+          const int64_t at = ((int64_t)lds_s32(sm100::smem_u32(s_ids + cs * kPMaxPages + page)) * p.Hkv + h) * bs + off;
           ks = __ldg(&k_scale[at]);
           vs = __ldg(&v_scale[at]);
         }
         ok = ok && sm100::mbar_wait_warp(sm100::smem_u32(&ring_empty[slot]), ((it / kRing) & 1) ^ 1);
         if (!ok) break;
-        const uint8_t* src = smem + L::oCodes + cs * kPCodes + r * 128;
-        uint8_t* dst = smem + L::oRing + slot * kPTile + r * 128;
+        const uint32_t src = sbase + L::oCodes + cs * kPCodes + r * 128;
+        const uint32_t dst = sbase + L::oRing + slot * kPTile + r * 128;
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          uint4 w = make_uint4(0, 0, 0, 0), a = w, b = w;
-          if (live) {
-            w = *reinterpret_cast<const uint4*>(src + ((c ^ (r & 7)) << 4));
-            a = make_uint4(kv8_pair<KV, 0, 1>(w.x), kv8_pair<KV, 2, 3>(w.x), kv8_pair<KV, 0, 1>(w.y),
-                           kv8_pair<KV, 2, 3>(w.y));
-            b = make_uint4(kv8_pair<KV, 0, 1>(w.z), kv8_pair<KV, 2, 3>(w.z), kv8_pair<KV, 0, 1>(w.w),
-                           kv8_pair<KV, 2, 3>(w.w));
+        for (int c0 = 0; c0 < 8; c0 += 4) {
+          uint4 w[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) w[c] = lds128(src + (((c0 + c) ^ (r & 7)) << 4));
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint4 a = make_uint4(kv8_pair<KV, 0, 1>(w[c].x), kv8_pair<KV, 2, 3>(w[c].x), kv8_pair<KV, 0, 1>(w[c].y),
+                                 kv8_pair<KV, 2, 3>(w[c].y));
+            uint4 b = make_uint4(kv8_pair<KV, 0, 1>(w[c].z), kv8_pair<KV, 2, 3>(w[c].z), kv8_pair<KV, 0, 1>(w[c].w),
+                                 kv8_pair<KV, 2, 3>(w[c].w));
+            if (!live) a = b = make_uint4(0, 0, 0, 0);
+            const uint32_t d = dst + (c0 >> 2) * kPHalf;
+            sts128(d + (((2 * c) ^ (r & 7)) << 4), a);
+            sts128(d + (((2 * c + 1) ^ (r & 7)) << 4), b);
           }
-          uint8_t* d = dst + (c >> 2) * kPHalf;
-          *reinterpret_cast<uint4*>(d + ((((2 * c) & 7) ^ (r & 7)) << 4)) = a;
-          *reinterpret_cast<uint4*>(d + ((((2 * c + 1) & 7) ^ (r & 7)) << 4)) = b;
         }
         sm100::fence_proxy_async_smem();
         if (which == 0) {
@@ -410,10 +444,10 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
           ok = sm100::mbar_wait_warp(sm100::smem_u32(&sc_empty[j & 1]), ((j >> 1) & 1) ^ 1);
           float lv = -INFINITY, iv = 0.f;
           if (live) kv8_value_scale(vs, lv, iv);
-          float* sc = s_sc + (j & 1) * 3 * kPM;
-          sc[r] = ks;
-          sc[kPM + r] = lv;
-          sc[2 * kPM + r] = iv;
+          const uint32_t sc = sm100::smem_u32(s_sc) + (uint32_t)((j & 1) * 3 * kPM + r) * 4;
+          sts_f32(sc, ks);
+          sts_f32(sc + kPM * 4, lv);
+          sts_f32(sc + 2 * kPM * 4, iv);
         }
         __syncwarp();
         if (lane == 0) {
@@ -429,18 +463,12 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
     }
   } else if (warp >= 4 && warp < 12) {
     // --------------------------------------------------------------- softmax
+    if constexpr (k8) sm100::setmaxnreg_inc<kPRegsHigh>();
     const int t = (warp >> 2) - 1, quarter = warp & 3;
     const int r = quarter * 32 + lane;
-    const int64_t qr = row0 + both * t * kPM + r;  // row of Q_h
+    const int qr = row0 + both * t * kPM + r;  // row of Q_h
     const bool live = qr < R;
-    const int64_t b = live ? qr / p.G : 0;
-    const int64_t qrow = b * p.Hq + (int64_t)h * p.G + (live ? qr - b * p.G : 0);
-    // (with one row tile the second stream stages it too, into the unused tile, for the row's factor)
-    const float sl = stage_q_row<T, k8>(q + qrow * kPieceDim, live, smem + L::oQ + t * kPTile, r, p.qscale);
-    sm100::fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0 && (both || t == 0)) sm100::mbar_arrive(sm100::smem_u32(q_full));
-
+    const int64_t qrow = live ? (int64_t)(qr >> p.lgG) * p.Hq + (h << p.lgG) + (qr & ((1 << p.lgG) - 1)) : 0;
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
     const uint32_t tS = tmem + t * 128 + lane_off, tO = tmem + 256 + t * 128 + lane_off;
     float m_used = -INFINITY, l = 0.f;
@@ -452,36 +480,45 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
       if (k8 && ok) ok = sm100::mbar_wait_warp(sm100::smem_u32(&sc_full[j & 1]), (j >> 1) & 1);
       if (!ok) break;
       sm100::tc_fence_after();
-      const int valid = j == nkt - 1 ? last_valid : tile_tok;
-      const float* sc = s_sc + (j & 1) * 3 * kPM;
-      // logits (log2 units; 8-bit: plus log2 of the value's scale) of 32 keys
-      auto logits = [&](int c, float* y) {
-        uint32_t v[32];
-        sm100::tmem_ld_32x32b_x32(tS + c * 32, v);
-        sm100::tmem_wait_ld_regs(v);
-        if constexpr (k8) {
+      uint32_t v[kPM];
+      sm100::tmem_ld_32x32b_x64(tS, v);
+      sm100::tmem_ld_32x32b_x64(tS + 64, v + 64);
+      sm100::tmem_wait_ld_regs(v);
+      sm100::tmem_wait_ld_regs(v + 32);
+      sm100::tmem_wait_ld_regs(v + 64);
+      sm100::tmem_wait_ld_regs(v + 96);
+      const uint32_t sc = sm100::smem_u32(s_sc) + (uint32_t)((j & 1) * 3 * kPM) * 4;
+      float f = sl;  // logits in log2 units: f times v (16-bit), or v itself
+      if constexpr (k8) {
+        // y = (S sl) ks + log2 vs; a key behind the last token has log2 vs = -inf
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            const float4 k4 = *reinterpret_cast<const float4*>(sc + c * 32 + i);
-            const float4 l4 = *reinterpret_cast<const float4*>(sc + kPM + c * 32 + i);
-            y[i] = fmaf(__uint_as_float(v[i]) * sl, k4.x, l4.x);
-            y[i + 1] = fmaf(__uint_as_float(v[i + 1]) * sl, k4.y, l4.y);
-            y[i + 2] = fmaf(__uint_as_float(v[i + 2]) * sl, k4.z, l4.z);
-            y[i + 3] = fmaf(__uint_as_float(v[i + 3]) * sl, k4.w, l4.w);
-          }
-        } else {
+        for (int i = 0; i < kPM; i += 4) {
+          const float4 k4 = lds_f32x4(sc + i * 4), l4 = lds_f32x4(sc + (kPM + i) * 4);
+          float y[4];
+          sm100::fmul2_bcast(y[0], y[1], __uint_as_float(v[i]), __uint_as_float(v[i + 1]), sl);
+          sm100::fmul2_bcast(y[2], y[3], __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]), sl);
+          sm100::ffma2(y[0], y[1], y[0], y[1], k4.x, k4.y, l4.x, l4.y);
+          sm100::ffma2(y[2], y[3], y[2], y[3], k4.z, k4.w, l4.z, l4.w);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) y[i] = c * 32 + i < valid ? __uint_as_float(v[i]) * sl : -INFINITY;
+          for (int u = 0; u < 4; ++u) v[i + u] = __float_as_uint(y[u]);
         }
-      };
-      float mx = -INFINITY;
-#pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
-        float y[32];
-        logits(c, y);
+        f = 1.f;
+      } else {
+        const int valid = j == nkt - 1 ? last_valid : tile_tok;
+        if (valid < kPM) {
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) mx = sm100::fmax3(mx, y[i], y[i + 1]);
+          for (int i = 0; i < kPM; ++i)
+            if (i >= valid) v[i] = 0xff800000u;
+        }
       }
+      float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int i = 0; i < kPM; i += 8) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          mx4[u] = sm100::fmax3(mx4[u], __uint_as_float(v[i + 2 * u]), __uint_as_float(v[i + 2 * u + 1]));
+      }
+      const float mx = sm100::fmax3(mx4[0], mx4[1], fmaxf(mx4[2], mx4[3])) * f;
       float alpha = 1.f;
       bool rescale = false;
       if (m_used == -INFINITY) {
@@ -491,7 +528,29 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
         m_used = mx;
         rescale = true;
       }
-      const float m0 = m_used == -INFINITY ? 0.f : m_used;
+      const float neg = m_used == -INFINITY ? 0.f : -m_used;
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < kPM; i += 4) {
+        float w[4];
+        if constexpr (k8) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u) w[u] = ex2(__uint_as_float(v[i + u]) + neg);
+          const float4 i4 = lds_f32x4(sc + (2 * kPM + i) * 4);
+          sm100::ffma2(sum[0], sum[1], w[0], w[1], i4.x, i4.y, sum[0], sum[1]);
+          sm100::ffma2(sum[2], sum[3], w[2], w[3], i4.z, i4.w, sum[2], sum[3]);
+        } else {
+          sm100::ffma2_bcast(w[0], w[1], __uint_as_float(v[i]), __uint_as_float(v[i + 1]), f, neg);
+          sm100::ffma2_bcast(w[2], w[3], __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]), f, neg);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) w[u] = ex2(w[u]);
+          sm100::fadd2_acc(sum[0], sum[1], w[0], w[1]);
+          sm100::fadd2_acc(sum[2], sum[3], w[2], w[3]);
+        }
+        v[i / 2] = pack_pair<M>(w[0], w[1]);
+        v[i / 2 + 1] = pack_pair<M>(w[2], w[3]);
+      }
+      sm100::tmem_st_32x32b_x64(tS, v);  // P over the logits' columns
       // O holds the products of the tiles before this one (complete: S of this tile is)
       if (__any_sync(0xffffffffu, rescale)) {
 #pragma unroll 1
@@ -504,28 +563,7 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
           sm100::tmem_st_32x32b_x32(tO + c, o);
         }
       }
-      float sum = 0.f;
-#pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
-        float y[32];
-        logits(c, y);
-        uint32_t pk[16];
-#pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-          float w0 = ex2(y[i] - m0), w1 = ex2(y[i + 1] - m0), w2 = ex2(y[i + 2] - m0), w3 = ex2(y[i + 3] - m0);
-          pk[i / 2] = pack_pair<M>(w0, w1);
-          pk[i / 2 + 1] = pack_pair<M>(w2, w3);
-          if constexpr (k8) {
-            const float4 i4 = *reinterpret_cast<const float4*>(sc + 2 * kPM + c * 32 + i);
-            sum = fmaf(w0, i4.x, fmaf(w1, i4.y, fmaf(w2, i4.z, fmaf(w3, i4.w, sum))));
-          } else {
-            sum += (w0 + w1) + (w2 + w3);
-          }
-        }
-        // P's 16 columns overwrite logits this thread has read already
-        sm100::tmem_st_32x32b_x16(tS + c * 16, pk);
-      }
-      l = l * alpha + sum;
+      l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
       sm100::tmem_wait_st();
       sm100::tc_fence_before();
       __syncwarp();
@@ -544,7 +582,7 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
     // With one row tile stream 1 hands its state to stream 0 through the K/V
     // ring, which nothing reads any more once both streams' products are done.
     // (Every path leads both warpgroups to the barrier.)
-    float* hand = reinterpret_cast<float*>(smem + L::oRing);  // [130][128]
+    const uint32_t hand = sbase + L::oRing + r * 4;  // [130][128] floats
     const bool join = !both && nkt > 1;
     float f0 = 1.f, f1 = 0.f;
     if (join) {
@@ -557,18 +595,18 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
           sm100::tmem_ld_32x32b_x32(tO + c, o);
           sm100::tmem_wait_ld_regs(o);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) hand[(c + i) * kPM + r] = __uint_as_float(o[i]);
+          for (int i = 0; i < 32; ++i) sts_f32(hand + (c + i) * kPM * 4, __uint_as_float(o[i]));
         }
-        hand[128 * kPM + r] = m_used;
-        hand[129 * kPM + r] = l;
+        sts_f32(hand + 128 * kPM * 4, m_used);
+        sts_f32(hand + 129 * kPM * 4, l);
       }
       named_bar_sync(1, 256);
       if (t == 0) {
-        const float m1 = hand[128 * kPM + r], mn = fmaxf(m_used, m1);
+        const float m1 = lds_f32(hand + 128 * kPM * 4), mn = fmaxf(m_used, m1);
         f0 = m_used == mn || m_used == -INFINITY ? 1.f : ex2(m_used - mn);
         f1 = m1 == mn || m1 == -INFINITY ? 1.f : ex2(m1 - mn);
         m_used = mn;
-        l = l * f0 + hand[129 * kPM + r] * f1;
+        l = l * f0 + lds_f32(hand + 129 * kPM * 4) * f1;
       }
     }
     if (both || t == 0) {
@@ -583,12 +621,11 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
           if (join) {
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              o[i] = __float_as_uint(__uint_as_float(o[i]) * f0 + hand[(c + i) * kPM + r] * f1);
+              o[i] = __float_as_uint(__uint_as_float(o[i]) * f0 + lds_f32(hand + (c + i) * kPM * 4) * f1);
           }
           if (live) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 4)
-              *reinterpret_cast<uint4*>(dst + c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+            for (int i = 0; i < 32; i += 8) stg256(dst + c + i, o + i);
           }
         }
       }
@@ -620,14 +657,26 @@ int launch_prefix(const AttnCall& a, const PieceGeom& g, const PieceSpace& w, cu
   if (st) return st;
   PrefixParams p{};
   p.B = a.B, p.Hq = a.Hq, p.Hkv = a.Hkv, p.num_blocks = a.num_blocks, p.max_prefix = a.max_prefix_blocks;
-  p.G = g.G, p.bs = (int)a.block_size, p.ppt = kPM / (int)a.block_size;
+  while ((1 << p.lgG) < g.G) ++p.lgG;
+  p.bs = (int)a.block_size, p.ppt = kPM / (int)a.block_size;
   p.codes = 3;
   p.splits = w.prefix_splits;
   p.qscale = a.scale * 1.4426950408889634f;
   const size_t smem = 1024 + PrefixSmem<k8>::oCodes + (k8 ? p.codes * kPCodes : 0) +
-                      8 * (1 + 2 * kPRing16 + 6 + 1 + 4 + 2 * kPMaxCodes) + 16 + 4 * kPMaxCodes * kPMaxPages +
+                      8 * (2 * kPRing16 + 6 + 1 + 4 + 2 * kPMaxCodes) + 24 + 32 + 4 * kPMaxCodes * kPMaxPages +
                       (k8 ? 2 * 3 * kPM * 4 : 0);
   auto kern = prefix_attn_kernel<T, KV>;
+  if (k8) {
+    // the register split (setmaxnreg) needs what it hands out at launch
+    static const int regs = [&] {
+      cudaFuncAttributes at{};
+      return cudaFuncGetAttributes(&at, kern) == cudaSuccess ? at.numRegs : 0;
+    }();
+    if (regs * 512 < 256 * (kPRegsLow + kPRegsHigh)) {
+      set_last_error_detail("prefix_attn_kernel: too few registers at launch for its split");
+      return B200_ERR_LAUNCH;
+    }
+  }
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return launch_status(e);
   const int64_t pairs = (a.B * g.G + 2 * kPM - 1) / (2 * kPM);
