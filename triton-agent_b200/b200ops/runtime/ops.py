@@ -12,6 +12,7 @@ inside the reference project).
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 import threading
 
@@ -264,43 +265,104 @@ def paged_attention(q, k_cache, v_cache, block_table, context_len, scale: float 
 
 
 # --------------------------------------------------------- 8-bit paged KV cache
+# A decode step calls these once a layer, so the checks are kept to attribute
+# reads: a call costs the host 10-15 us, launches included.
 _CODE_DTYPES = (torch.int8, torch.float8_e4m3fn)
 
 
-def _scratch(dev: torch.device, nbytes: int) -> torch.Tensor | None:
+def _on_one_device(op: str, *ts: torch.Tensor | None) -> int:
+    """Index of the CUDA device all the given tensors are on."""
+    i = ts[0].get_device()
+    for t in ts:
+        if t is not None and t.get_device() != i:
+            break
+    else:
+        if i >= 0:
+            return i
+    _need_cuda(op, *ts)  # names what is wrong
+    raise L.B200OpsError(L.ERR_BAD_ARG, op, "tensors on different devices")
+
+
+class _Device:
+    """Makes a device current for a call when it is not."""
+
+    __slots__ = ("index", "old")
+
+    def __init__(self, index: int):
+        self.index = index
+
+    def __enter__(self):
+        self.old = torch.cuda.current_device()
+        if self.old != self.index:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.old != self.index:
+            torch.cuda.set_device(self.old)
+
+
+def _raw_stream(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+if hasattr(torch._C, "_cuda_getCurrentRawStream"):
+    _raw_stream = torch._C._cuda_getCurrentRawStream  # noqa: F811  (the same handle without a Stream object)
+
+
+def _p(t: torch.Tensor | None):
+    return t.data_ptr() if t is not None else None
+
+
+def _scratch(like: torch.Tensor, nbytes: int) -> torch.Tensor | None:
     """Workspace of one call, from the current stream's allocator (inside a
     capture: from the graph's pool), so that calls on other streams and
     captured graphs share none.  The kernels need no cleared memory and keep
     nothing in it."""
-    return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    return like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+
+
+@functools.lru_cache(maxsize=256)
+def _scratch_bytes(fn: str, *sizes) -> int:
+    """A workspace size query of the library at the default launch parameters."""
+    return int(getattr(L.load(), fn)(*sizes))
+
+
+def _scratch_size(fn: str, cfg, *sizes) -> int:
+    if cfg is None:
+        return _scratch_bytes(fn, *sizes, None)
+    return int(getattr(L.load(), fn)(*sizes, cfg))
 
 
 def _check_cache(op: str, k_cache, v_cache, k_scale, v_scale) -> tuple[int, int, int, int]:
     """(num_blocks, block_size, Hkv, D) of an 8-bit cache with its scales."""
-    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype:
+    shape = k_cache.shape
+    if len(shape) != 4 or v_cache.shape != shape or v_cache.dtype != k_cache.dtype:
         raise L.B200OpsError(L.ERR_BAD_ARG, op, "caches must be [num_blocks, block_size, Hkv, D] of one shape and dtype")
     if k_cache.dtype not in _CODE_DTYPES:
         raise L.B200OpsError(L.ERR_UNSUPPORTED, op, "8-bit caches are int8 or float8_e4m3fn")
-    nb, bs, Hkv, D = k_cache.shape
-    for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-        if t is None or tuple(t.shape) != (nb, Hkv, bs) or t.dtype != torch.float32:
-            raise L.B200OpsError(L.ERR_BAD_ARG, op, f"{name} must be float32 [num_blocks, Hkv, block_size]")
+    nb, bs, Hkv, D = shape
+    want = (nb, Hkv, bs)
+    if k_scale is None or v_scale is None or k_scale.shape != want or v_scale.shape != want or \
+            k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
+        raise L.B200OpsError(L.ERR_BAD_ARG, op, "scales must be float32 [num_blocks, Hkv, block_size]")
     _contig(op, k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale)
     return nb, bs, Hkv, D
 
 
 def _check_out(op: str, name: str, t: torch.Tensor, shape: tuple, dtype: torch.dtype):
-    if tuple(t.shape) != tuple(shape) or t.dtype != dtype:
+    if t.shape != shape or t.dtype != dtype:
         raise L.B200OpsError(L.ERR_BAD_ARG, op, f"{name} must be {dtype} {list(shape)}")
     _contig(op, **{name: t})
 
 
-def _index(op: str, name: str, t: torch.Tensor, like: torch.Tensor, shape: tuple) -> torch.Tensor:
-    if tuple(t.shape) != tuple(shape):
+def _index(op: str, name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple) -> torch.Tensor:
+    if t.shape != shape:
         raise L.B200OpsError(L.ERR_BAD_ARG, op, f"{name} must be {list(shape)}")
     if t.dtype not in (torch.int32, torch.int64):
         raise L.B200OpsError(L.ERR_UNSUPPORTED, op, f"{name} must be int32 or int64")
-    return t.to(like.dtype).contiguous()
+    if t.dtype != dtype:
+        t = t.to(dtype)
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def rope_kv_append_paged_quant(q, k, v, positions, cos, sin, slot_mapping, k_cache, v_cache, k_scale, v_scale,
@@ -317,38 +379,40 @@ def rope_kv_append_paged_quant(q, k, v, positions, cos, sin, slot_mapping, k_cac
     when the position is); of several tokens naming one slot the last wins.
     Returns q_out (or None)."""
     op = "rope_kv_append_paged_quant"
-    dev = _need_cuda(op, q, k, v, positions, cos, sin, slot_mapping, k_cache, v_cache, k_scale, v_scale, q_out)
+    dev = _on_one_device(op, k, q, v, positions, cos, sin, slot_mapping, k_cache, v_cache, k_scale, v_scale, q_out)
     nb, bs, Hkv, D = _check_cache(op, k_cache, v_cache, k_scale, v_scale)
     _contig(op, q=q, k=k, v=v, cos=cos, sin=sin)
-    if k.dim() != 3 or tuple(k.shape[1:]) != (Hkv, D) or v.shape != k.shape or v.dtype != k.dtype:
+    T = k.shape[0] if k.dim() == 3 else -1
+    dt = k.dtype
+    if k.shape != (T, Hkv, D) or v.shape != (T, Hkv, D) or v.dtype != dt:
         raise L.B200OpsError(L.ERR_BAD_ARG, op, "k and v must be [T, Hkv, D] of one dtype, as the cache's rows")
-    T = k.shape[0]
-    if q is not None and (q.dim() != 3 or q.shape[0] != T or q.shape[2] != D or q.dtype != k.dtype):
-        raise L.B200OpsError(L.ERR_BAD_ARG, op, "q must be [T, Hq, D] of k's dtype")
+    Hq = 0
+    if q is not None:
+        Hq = q.shape[1] if q.dim() == 3 else -1
+        if q.shape != (T, Hq, D) or q.dtype != dt:
+            raise L.B200OpsError(L.ERR_BAD_ARG, op, "q must be [T, Hq, D] of k's dtype")
     if cos.dim() != 2 or cos.shape[1] != D or sin.shape != cos.shape or sin.dtype != cos.dtype:
         raise L.B200OpsError(L.ERR_BAD_ARG, op, "cos and sin must be [positions, D] of one dtype")
-    for name, t in (("positions", positions), ("slot_mapping", slot_mapping)):
-        if t.dtype != torch.int64:
-            raise L.B200OpsError(L.ERR_UNSUPPORTED, op, f"{name} must be int64")
-        if t.numel() != T:
-            raise L.B200OpsError(L.ERR_BAD_ARG, op, f"{name} must have T elements")
-    Hq = q.shape[1] if q is not None else 0
+    if positions.dtype != torch.int64 or slot_mapping.dtype != torch.int64:
+        raise L.B200OpsError(L.ERR_UNSUPPORTED, op, "positions and slot_mapping must be int64")
+    if positions.numel() != T or slot_mapping.numel() != T:
+        raise L.B200OpsError(L.ERR_BAD_ARG, op, "positions and slot_mapping must have T elements")
     if q is None:
         q_out = None
     elif q_out is None:
         q_out = torch.empty_like(q)
     else:
-        _check_out(op, "q_out", q_out, q.shape, q.dtype)
-    pos, sm = positions.contiguous(), slot_mapping.contiguous()
-    lib = L.load()
-    with torch.cuda.device(dev):
-        ws = _scratch(dev, int(lib.b200_rope_kv_append_paged_quant_workspace_size(T)))
-        st = lib.b200_rope_kv_append_paged_quant(
-            _ptr(q), _ptr(k), _ptr(v), _ptr(pos), _ptr(cos), _ptr(sin), cos.shape[0], _ptr(sm), _ptr(q_out),
-            _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), T, Hq, Hkv, D, nb, bs, dtype_code(k.dtype),
-            dtype_code(cos.dtype), dtype_code(k_cache.dtype), _ptr(ws), ws.numel() if ws is not None else 0,
-            _cfg(cfg), _stream(dev))
-    L.check(st, op)
+        _check_out(op, "q_out", q_out, q.shape, dt)
+    pos, sm, c = positions.contiguous(), slot_mapping.contiguous(), _cfg(cfg)
+    with _Device(dev):
+        ws = _scratch(k, _scratch_bytes("b200_rope_kv_append_paged_quant_workspace_size", T)) if T > 512 else None
+        st = L.load().b200_rope_kv_append_paged_quant(
+            _p(q), k.data_ptr(), v.data_ptr(), pos.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0],
+            sm.data_ptr(), _p(q_out), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+            T, Hq, Hkv, D, nb, bs, dtype_code(dt), dtype_code(cos.dtype), dtype_code(k_cache.dtype), _p(ws),
+            ws.numel() if ws is not None else 0, c, _raw_stream(dev))
+    if st:
+        L.check(st, op)
     return q_out
 
 
@@ -360,26 +424,33 @@ def paged_kv_dequant(k_cache, v_cache, k_scale, v_scale, block_table, context_le
     min(context_len[b], max_len) is code * scale of the sequence's token s
     (block rules of paged_attention), rounded once; all other rows are zero."""
     op = "paged_kv_dequant"
-    dev = _need_cuda(op, k_cache, v_cache, k_scale, v_scale, block_table, context_len, k_out, v_out)
+    dev = _on_one_device(op, k_cache, v_cache, k_scale, v_scale, block_table, context_len, k_out, v_out)
     nb, bs, Hkv, D = _check_cache(op, k_cache, v_cache, k_scale, v_scale)
     if block_table.dim() != 2 or max_len < 0:
         raise L.B200OpsError(L.ERR_BAD_ARG, op, "block_table must be [B, max_blocks] and max_len >= 0")
     B, max_blocks = block_table.shape
-    bt = _index(op, "block_table", block_table, block_table, (B, max_blocks))
-    cl = _index(op, "context_len", context_len, bt, (B,))
-    outs = []
-    for name, t in (("k_out", k_out), ("v_out", v_out)):
-        if t is None:
-            t = torch.empty(B, Hkv, max_len, D, dtype=dtype, device=dev)
-        _check_out(op, name, t, (B, Hkv, max_len, D), dtype)
-        outs.append(t)
-    with torch.cuda.device(dev):
-        st = L.load().b200_paged_kv_dequant(_ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(bt),
-                                            _ptr(cl), _ptr(outs[0]), _ptr(outs[1]), B, Hkv, D, nb, bs, max_blocks,
-                                            max_len, dtype_code(dtype), dtype_code(k_cache.dtype),
-                                            dtype_code(bt.dtype), _cfg(cfg), _stream(dev))
-    L.check(st, op)
-    return outs[0], outs[1]
+    ix = block_table.dtype
+    bt = _index(op, "block_table", block_table, ix, (B, max_blocks))
+    cl = _index(op, "context_len", context_len, ix, (B,))
+    shape = (B, Hkv, max_len, D)
+    if k_out is None:
+        k_out = k_cache.new_empty(shape, dtype=dtype)
+    else:
+        _check_out(op, "k_out", k_out, shape, dtype)
+    if v_out is None:
+        v_out = v_cache.new_empty(shape, dtype=dtype)
+    else:
+        _check_out(op, "v_out", v_out, shape, dtype)
+    c = _cfg(cfg)
+    with _Device(dev):
+        st = L.load().b200_paged_kv_dequant(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+                                            v_scale.data_ptr(), bt.data_ptr(), cl.data_ptr(), k_out.data_ptr(),
+                                            v_out.data_ptr(), B, Hkv, D, nb, bs, max_blocks, max_len,
+                                            dtype_code(dtype), dtype_code(k_cache.dtype), dtype_code(ix), c,
+                                            _raw_stream(dev))
+    if st:
+        L.check(st, op)
+    return k_out, v_out
 
 
 def paged_attention_quant(q, k_cache, v_cache, k_scale, v_scale, block_table, context_len,
@@ -390,27 +461,32 @@ def paged_attention_quant(q, k_cache, v_cache, k_scale, v_scale, block_table, co
     block_table [B, max_blocks] and context_len [B] int32 or int64.  A
     sequence without tokens gives zeros.  Returns out [B,Hq,D] in q's dtype."""
     op = "paged_attention_quant"
-    dev = _need_cuda(op, q, k_cache, v_cache, k_scale, v_scale, block_table, context_len, out)
+    dev = _on_one_device(op, q, k_cache, v_cache, k_scale, v_scale, block_table, context_len, out)
     nb, bs, Hkv, D = _check_cache(op, k_cache, v_cache, k_scale, v_scale)
     if q.dim() != 3 or q.shape[2] != D or block_table.dim() != 2:
         raise L.B200OpsError(L.ERR_BAD_ARG, op, "q must be [B, Hq, D] and block_table [B, max_blocks]")
     _contig(op, q=q)
     B, Hq, _ = q.shape
-    max_blocks = block_table.shape[1]
-    bt = _index(op, "block_table", block_table, block_table, (B, max_blocks))
-    cl = _index(op, "context_len", context_len, bt, (B,))
-    o = torch.empty_like(q) if out is None else out
-    _check_out(op, "out", o, q.shape, q.dtype)
+    max_blocks, ix = block_table.shape[1], block_table.dtype
+    bt = _index(op, "block_table", block_table, ix, (B, max_blocks))
+    cl = _index(op, "context_len", context_len, ix, (B,))
+    if out is None:
+        out = torch.empty_like(q)
+    else:
+        _check_out(op, "out", out, q.shape, q.dtype)
     sc = float(scale) if scale is not None else 1.0 / math.sqrt(D)
-    lib, c = L.load(), _cfg(cfg)
-    with torch.cuda.device(dev):
-        ws = _scratch(dev, int(lib.b200_paged_attention_quant_workspace_size(B, Hq, Hkv, D, nb, bs, max_blocks, c)))
-        st = lib.b200_paged_attention_quant(_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale),
-                                            _ptr(bt), _ptr(cl), _ptr(o), B, Hq, Hkv, D, nb, bs, max_blocks, sc,
-                                            dtype_code(q.dtype), dtype_code(k_cache.dtype), dtype_code(bt.dtype),
-                                            _ptr(ws), ws.numel() if ws is not None else 0, c, _stream(dev))
-    L.check(st, op)
-    return o
+    c = _cfg(cfg)
+    with _Device(dev):
+        ws = _scratch(q, _scratch_size("b200_paged_attention_quant_workspace_size", c, B, Hq, Hkv, D, nb, bs,
+                                       max_blocks))
+        st = L.load().b200_paged_attention_quant(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                                                 k_scale.data_ptr(), v_scale.data_ptr(), bt.data_ptr(), cl.data_ptr(),
+                                                 out.data_ptr(), B, Hq, Hkv, D, nb, bs, max_blocks, sc,
+                                                 dtype_code(q.dtype), dtype_code(k_cache.dtype), dtype_code(ix),
+                                                 _p(ws), ws.numel() if ws is not None else 0, c, _raw_stream(dev))
+    if st:
+        L.check(st, op)
+    return out
 
 
 def paged_attention_prefix(q, k_cache, v_cache, prefix_table, prefix_len, block_table, context_len, k_scale=None,
@@ -424,8 +500,8 @@ def paged_attention_prefix(q, k_cache, v_cache, prefix_table, prefix_len, block_
     v_scale as in paged_attention_quant.  A sequence without any token gives
     zeros.  Returns out [B,Hq,D] in q's dtype."""
     op = "paged_attention_prefix"
-    dev = _need_cuda(op, q, k_cache, v_cache, prefix_table, prefix_len, block_table, context_len, k_scale, v_scale,
-                     out)
+    dev = _on_one_device(op, q, k_cache, v_cache, prefix_table, prefix_len, block_table, context_len, k_scale,
+                         v_scale, out)
     if k_cache.dtype in _CODE_DTYPES:
         nb, bs, Hkv, D = _check_cache(op, k_cache, v_cache, k_scale, v_scale)
     else:
@@ -438,27 +514,32 @@ def paged_attention_prefix(q, k_cache, v_cache, prefix_table, prefix_len, block_
         nb, bs, Hkv, D = k_cache.shape
     if q.dim() != 3 or q.shape[2] != D or block_table.dim() != 2 or prefix_table.dim() != 1:
         raise L.B200OpsError(L.ERR_BAD_ARG, op, "q must be [B, Hq, D], block_table [B, max_blocks], prefix_table [P]")
+    if prefix_len.numel() != 1:
+        raise L.B200OpsError(L.ERR_BAD_ARG, op, "prefix_len must be one element")
     _contig(op, q=q)
     B, Hq, _ = q.shape
-    max_blocks, max_prefix = block_table.shape[1], prefix_table.shape[0]
-    bt = _index(op, "block_table", block_table, block_table, (B, max_blocks))
-    cl = _index(op, "context_len", context_len, bt, (B,))
-    pt = _index(op, "prefix_table", prefix_table, bt, (max_prefix,))
-    pl = _index(op, "prefix_len", prefix_len.reshape(-1), bt, (1,))
-    o = torch.empty_like(q) if out is None else out
-    _check_out(op, "out", o, q.shape, q.dtype)
+    max_blocks, max_prefix, ix = block_table.shape[1], prefix_table.shape[0], block_table.dtype
+    bt = _index(op, "block_table", block_table, ix, (B, max_blocks))
+    cl = _index(op, "context_len", context_len, ix, (B,))
+    pt = _index(op, "prefix_table", prefix_table, ix, (max_prefix,))
+    pl = _index(op, "prefix_len", prefix_len, ix, prefix_len.shape)
+    if out is None:
+        out = torch.empty_like(q)
+    else:
+        _check_out(op, "out", out, q.shape, q.dtype)
     sc = float(scale) if scale is not None else 1.0 / math.sqrt(D)
-    lib, c, code = L.load(), _cfg(cfg), dtype_code(k_cache.dtype)
-    with torch.cuda.device(dev):
-        ws = _scratch(dev, int(lib.b200_paged_attention_prefix_workspace_size(B, Hq, Hkv, D, nb, bs, max_prefix,
-                                                                              max_blocks, code, c)))
-        st = lib.b200_paged_attention_prefix(_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale),
-                                             _ptr(pt), _ptr(pl), _ptr(bt), _ptr(cl), _ptr(o), B, Hq, Hkv, D, nb, bs,
-                                             max_prefix, max_blocks, sc, dtype_code(q.dtype), code,
-                                             dtype_code(bt.dtype), _ptr(ws), ws.numel() if ws is not None else 0, c,
-                                             _stream(dev))
-    L.check(st, op)
-    return o
+    c, code = _cfg(cfg), dtype_code(k_cache.dtype)
+    with _Device(dev):
+        ws = _scratch(q, _scratch_size("b200_paged_attention_prefix_workspace_size", c, B, Hq, Hkv, D, nb, bs,
+                                       max_prefix, max_blocks, code))
+        st = L.load().b200_paged_attention_prefix(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _p(k_scale),
+                                                  _p(v_scale), pt.data_ptr(), pl.data_ptr(), bt.data_ptr(),
+                                                  cl.data_ptr(), out.data_ptr(), B, Hq, Hkv, D, nb, bs, max_prefix,
+                                                  max_blocks, sc, dtype_code(q.dtype), code, dtype_code(ix), _p(ws),
+                                                  ws.numel() if ws is not None else 0, c, _raw_stream(dev))
+    if st:
+        L.check(st, op)
+    return out
 
 
 # ----------------------------------------------------------------- INT8 GEMM

@@ -10,6 +10,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/b200ops.h"
 
 namespace b200 {
@@ -47,6 +49,28 @@ inline int device_sm_count() {
   if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
   return n;
 }
+
+// Shared memory beyond the default for a kernel, requested once for each device
+// and size (a request costs about a microsecond a launch otherwise).  One
+// SmemGrant per kernel, static at its launch site.
+struct SmemGrant {
+  std::atomic<int> most[64] = {};
+  template <typename K>
+  cudaError_t operator()(K kern, size_t bytes) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const bool known = dev >= 0 && dev < 64;
+    if (known && most[dev].load(std::memory_order_relaxed) >= (int)bytes) return cudaSuccess;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess && known) {
+      int old = most[dev].load(std::memory_order_relaxed);
+      while (old < (int)bytes && !most[dev].compare_exchange_weak(old, (int)bytes)) {
+      }
+    }
+    return e;
+  }
+};
 
 // Registry of per-translation-unit device error readers (see
 // B200_DEVICE_ERROR_WORD).  Each reader copies its word to the host, clears

@@ -854,7 +854,8 @@ int launch_pieces(const AttnCall& a, const PieceGeom& g, const PieceSpace& w, bo
   p.page_bytes = g.page_bytes;
   p.qscale = a.scale * 1.4426950408889634f;
   auto kern = paged_attn_pieces_kernel<T, KV, G>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)g.smem);
+  static SmemGrant grant;
+  cudaError_t e = grant(kern, g.smem);
   if (e != cudaSuccess) return launch_status(e);
   cudaLaunchConfig_t lc = {};
   lc.gridDim = dim3((unsigned)g.grid);

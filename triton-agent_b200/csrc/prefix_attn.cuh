@@ -677,7 +677,8 @@ int launch_prefix(const AttnCall& a, const PieceGeom& g, const PieceSpace& w, cu
       return B200_ERR_LAUNCH;
     }
   }
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static SmemGrant grant;
+  cudaError_t e = grant(kern, smem);
   if (e != cudaSuccess) return launch_status(e);
   const int64_t pairs = (a.B * g.G + 2 * kPM - 1) / (2 * kPM);
   kern<<<dim3((unsigned)p.splits, (unsigned)pairs, (unsigned)a.Hkv), k8 ? 512 : 384, smem, stream>>>(
