@@ -287,8 +287,8 @@ int b200_paged_attention_noalloc(const void* q, const void* k_cache,
  * last that writes wins.  D even.
  * workspace: b200_rope_kv_append_paged_quant_workspace_size(T) bytes, 16-byte
  * aligned (0 for T <= 512: NULL may be given); nothing in it is kept between
- * calls.  cfg: rows_per_cta (rows of a token per thread: 1, 2, 3 or 6;
- * default 1 up to 512 tokens, else 3). */
+ * calls.  cfg: rows_per_cta (T > 512: rows of a token per thread, 1 to 8;
+ * default 2). */
 size_t b200_rope_kv_append_paged_quant_workspace_size(int64_t T);
 int b200_rope_kv_append_paged_quant(const void* q, const void* k, const void* v, const int64_t* positions,
                                     const void* cos, const void* sin, int64_t cs_rows,

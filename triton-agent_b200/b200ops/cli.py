@@ -236,7 +236,7 @@ def space_rows(op: str, parsed: dict[str, int], gen_fn=None) -> int:
     get = lambda k, d=0: int(parsed.get(k, dflt.get(k, d)))  # noqa: E731
     if op in ("quant_matmul", "matmul_epilogue"):
         return get("B", 1) * get("M", 0)
-    if op == "rope_kv_append_paged":
+    if op in ("rope_kv_append_paged", "rope_kv_append_paged_quant"):
         return get("T", 0)
     if op == "paged_attention":
         return get("B", 0)

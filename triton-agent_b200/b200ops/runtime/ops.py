@@ -283,30 +283,17 @@ def _on_one_device(op: str, *ts: torch.Tensor | None) -> int:
     raise L.B200OpsError(L.ERR_BAD_ARG, op, "tensors on different devices")
 
 
-class _Device:
-    """Makes a device current for a call when it is not."""
-
-    __slots__ = ("index", "old")
-
-    def __init__(self, index: int):
-        self.index = index
-
-    def __enter__(self):
-        self.old = torch.cuda.current_device()
-        if self.old != self.index:
-            torch.cuda.set_device(self.index)
-
-    def __exit__(self, *exc):
-        if self.old != self.index:
-            torch.cuda.set_device(self.old)
-
-
 def _raw_stream(index: int) -> int:
     return torch.cuda.current_stream(index).cuda_stream
 
 
 if hasattr(torch._C, "_cuda_getCurrentRawStream"):
     _raw_stream = torch._C._cuda_getCurrentRawStream  # noqa: F811  (the same handle without a Stream object)
+
+
+def _elsewhere(dev: int) -> bool:
+    """Whether another device than the tensors' is current."""
+    return torch.cuda.current_device() != dev
 
 
 def _p(t: torch.Tensor | None):
@@ -345,7 +332,9 @@ def _check_cache(op: str, k_cache, v_cache, k_scale, v_scale) -> tuple[int, int,
     if k_scale is None or v_scale is None or k_scale.shape != want or v_scale.shape != want or \
             k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
         raise L.B200OpsError(L.ERR_BAD_ARG, op, "scales must be float32 [num_blocks, Hkv, block_size]")
-    _contig(op, k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale)
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous() and k_scale.is_contiguous() and
+            v_scale.is_contiguous()):
+        _contig(op, k_cache=k_cache, v_cache=v_cache, k_scale=k_scale, v_scale=v_scale)
     return nb, bs, Hkv, D
 
 
@@ -380,8 +369,14 @@ def rope_kv_append_paged_quant(q, k, v, positions, cos, sin, slot_mapping, k_cac
     Returns q_out (or None)."""
     op = "rope_kv_append_paged_quant"
     dev = _on_one_device(op, k, q, v, positions, cos, sin, slot_mapping, k_cache, v_cache, k_scale, v_scale, q_out)
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return rope_kv_append_paged_quant(q, k, v, positions, cos, sin, slot_mapping, k_cache, v_cache, k_scale, v_scale,
+                                              q_out, cfg)
     nb, bs, Hkv, D = _check_cache(op, k_cache, v_cache, k_scale, v_scale)
-    _contig(op, q=q, k=k, v=v, cos=cos, sin=sin)
+    if not (k.is_contiguous() and v.is_contiguous() and cos.is_contiguous() and sin.is_contiguous() and
+            (q is None or q.is_contiguous())):
+        _contig(op, q=q, k=k, v=v, cos=cos, sin=sin)
     T = k.shape[0] if k.dim() == 3 else -1
     dt = k.dtype
     if k.shape != (T, Hkv, D) or v.shape != (T, Hkv, D) or v.dtype != dt:
@@ -404,13 +399,12 @@ def rope_kv_append_paged_quant(q, k, v, positions, cos, sin, slot_mapping, k_cac
     else:
         _check_out(op, "q_out", q_out, q.shape, dt)
     pos, sm, c = positions.contiguous(), slot_mapping.contiguous(), _cfg(cfg)
-    with _Device(dev):
-        ws = _scratch(k, _scratch_bytes("b200_rope_kv_append_paged_quant_workspace_size", T)) if T > 512 else None
-        st = L.load().b200_rope_kv_append_paged_quant(
-            _p(q), k.data_ptr(), v.data_ptr(), pos.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0],
-            sm.data_ptr(), _p(q_out), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-            T, Hq, Hkv, D, nb, bs, dtype_code(dt), dtype_code(cos.dtype), dtype_code(k_cache.dtype), _p(ws),
-            ws.numel() if ws is not None else 0, c, _raw_stream(dev))
+    ws = _scratch(k, _scratch_bytes("b200_rope_kv_append_paged_quant_workspace_size", T)) if T > 512 else None
+    st = L.load().b200_rope_kv_append_paged_quant(
+        _p(q), k.data_ptr(), v.data_ptr(), pos.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0],
+        sm.data_ptr(), _p(q_out), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+        T, Hq, Hkv, D, nb, bs, dtype_code(dt), dtype_code(cos.dtype), dtype_code(k_cache.dtype), _p(ws),
+        ws.numel() if ws is not None else 0, c, _raw_stream(dev))
     if st:
         L.check(st, op)
     return q_out
@@ -425,6 +419,10 @@ def paged_kv_dequant(k_cache, v_cache, k_scale, v_scale, block_table, context_le
     (block rules of paged_attention), rounded once; all other rows are zero."""
     op = "paged_kv_dequant"
     dev = _on_one_device(op, k_cache, v_cache, k_scale, v_scale, block_table, context_len, k_out, v_out)
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return paged_kv_dequant(k_cache, v_cache, k_scale, v_scale, block_table, context_len, max_len, dtype, k_out,
+                                    v_out, cfg)
     nb, bs, Hkv, D = _check_cache(op, k_cache, v_cache, k_scale, v_scale)
     if block_table.dim() != 2 or max_len < 0:
         raise L.B200OpsError(L.ERR_BAD_ARG, op, "block_table must be [B, max_blocks] and max_len >= 0")
@@ -442,12 +440,11 @@ def paged_kv_dequant(k_cache, v_cache, k_scale, v_scale, block_table, context_le
     else:
         _check_out(op, "v_out", v_out, shape, dtype)
     c = _cfg(cfg)
-    with _Device(dev):
-        st = L.load().b200_paged_kv_dequant(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
-                                            v_scale.data_ptr(), bt.data_ptr(), cl.data_ptr(), k_out.data_ptr(),
-                                            v_out.data_ptr(), B, Hkv, D, nb, bs, max_blocks, max_len,
-                                            dtype_code(dtype), dtype_code(k_cache.dtype), dtype_code(ix), c,
-                                            _raw_stream(dev))
+    st = L.load().b200_paged_kv_dequant(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(),
+                                        v_scale.data_ptr(), bt.data_ptr(), cl.data_ptr(), k_out.data_ptr(),
+                                        v_out.data_ptr(), B, Hkv, D, nb, bs, max_blocks, max_len,
+                                        dtype_code(dtype), dtype_code(k_cache.dtype), dtype_code(ix), c,
+                                        _raw_stream(dev))
     if st:
         L.check(st, op)
     return k_out, v_out
@@ -462,10 +459,14 @@ def paged_attention_quant(q, k_cache, v_cache, k_scale, v_scale, block_table, co
     sequence without tokens gives zeros.  Returns out [B,Hq,D] in q's dtype."""
     op = "paged_attention_quant"
     dev = _on_one_device(op, q, k_cache, v_cache, k_scale, v_scale, block_table, context_len, out)
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return paged_attention_quant(q, k_cache, v_cache, k_scale, v_scale, block_table, context_len, scale, out, cfg)
     nb, bs, Hkv, D = _check_cache(op, k_cache, v_cache, k_scale, v_scale)
     if q.dim() != 3 or q.shape[2] != D or block_table.dim() != 2:
         raise L.B200OpsError(L.ERR_BAD_ARG, op, "q must be [B, Hq, D] and block_table [B, max_blocks]")
-    _contig(op, q=q)
+    if not q.is_contiguous():
+        _contig(op, q=q)
     B, Hq, _ = q.shape
     max_blocks, ix = block_table.shape[1], block_table.dtype
     bt = _index(op, "block_table", block_table, ix, (B, max_blocks))
@@ -476,14 +477,13 @@ def paged_attention_quant(q, k_cache, v_cache, k_scale, v_scale, block_table, co
         _check_out(op, "out", out, q.shape, q.dtype)
     sc = float(scale) if scale is not None else 1.0 / math.sqrt(D)
     c = _cfg(cfg)
-    with _Device(dev):
-        ws = _scratch(q, _scratch_size("b200_paged_attention_quant_workspace_size", c, B, Hq, Hkv, D, nb, bs,
-                                       max_blocks))
-        st = L.load().b200_paged_attention_quant(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
-                                                 k_scale.data_ptr(), v_scale.data_ptr(), bt.data_ptr(), cl.data_ptr(),
-                                                 out.data_ptr(), B, Hq, Hkv, D, nb, bs, max_blocks, sc,
-                                                 dtype_code(q.dtype), dtype_code(k_cache.dtype), dtype_code(ix),
-                                                 _p(ws), ws.numel() if ws is not None else 0, c, _raw_stream(dev))
+    ws = _scratch(q, _scratch_size("b200_paged_attention_quant_workspace_size", c, B, Hq, Hkv, D, nb, bs,
+                                   max_blocks))
+    st = L.load().b200_paged_attention_quant(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                                             k_scale.data_ptr(), v_scale.data_ptr(), bt.data_ptr(), cl.data_ptr(),
+                                             out.data_ptr(), B, Hq, Hkv, D, nb, bs, max_blocks, sc,
+                                             dtype_code(q.dtype), dtype_code(k_cache.dtype), dtype_code(ix),
+                                             _p(ws), ws.numel() if ws is not None else 0, c, _raw_stream(dev))
     if st:
         L.check(st, op)
     return out
@@ -502,6 +502,10 @@ def paged_attention_prefix(q, k_cache, v_cache, prefix_table, prefix_len, block_
     op = "paged_attention_prefix"
     dev = _on_one_device(op, q, k_cache, v_cache, prefix_table, prefix_len, block_table, context_len, k_scale,
                          v_scale, out)
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return paged_attention_prefix(q, k_cache, v_cache, prefix_table, prefix_len, block_table, context_len,
+                                          k_scale, v_scale, scale, out, cfg)
     if k_cache.dtype in _CODE_DTYPES:
         nb, bs, Hkv, D = _check_cache(op, k_cache, v_cache, k_scale, v_scale)
     else:
@@ -516,7 +520,8 @@ def paged_attention_prefix(q, k_cache, v_cache, prefix_table, prefix_len, block_
         raise L.B200OpsError(L.ERR_BAD_ARG, op, "q must be [B, Hq, D], block_table [B, max_blocks], prefix_table [P]")
     if prefix_len.numel() != 1:
         raise L.B200OpsError(L.ERR_BAD_ARG, op, "prefix_len must be one element")
-    _contig(op, q=q)
+    if not q.is_contiguous():
+        _contig(op, q=q)
     B, Hq, _ = q.shape
     max_blocks, max_prefix, ix = block_table.shape[1], prefix_table.shape[0], block_table.dtype
     bt = _index(op, "block_table", block_table, ix, (B, max_blocks))
@@ -529,14 +534,13 @@ def paged_attention_prefix(q, k_cache, v_cache, prefix_table, prefix_len, block_
         _check_out(op, "out", out, q.shape, q.dtype)
     sc = float(scale) if scale is not None else 1.0 / math.sqrt(D)
     c, code = _cfg(cfg), dtype_code(k_cache.dtype)
-    with _Device(dev):
-        ws = _scratch(q, _scratch_size("b200_paged_attention_prefix_workspace_size", c, B, Hq, Hkv, D, nb, bs,
-                                       max_prefix, max_blocks, code))
-        st = L.load().b200_paged_attention_prefix(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _p(k_scale),
-                                                  _p(v_scale), pt.data_ptr(), pl.data_ptr(), bt.data_ptr(),
-                                                  cl.data_ptr(), out.data_ptr(), B, Hq, Hkv, D, nb, bs, max_prefix,
-                                                  max_blocks, sc, dtype_code(q.dtype), code, dtype_code(ix), _p(ws),
-                                                  ws.numel() if ws is not None else 0, c, _raw_stream(dev))
+    ws = _scratch(q, _scratch_size("b200_paged_attention_prefix_workspace_size", c, B, Hq, Hkv, D, nb, bs,
+                                   max_prefix, max_blocks, code))
+    st = L.load().b200_paged_attention_prefix(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _p(k_scale),
+                                              _p(v_scale), pt.data_ptr(), pl.data_ptr(), bt.data_ptr(),
+                                              cl.data_ptr(), out.data_ptr(), B, Hq, Hkv, D, nb, bs, max_prefix,
+                                              max_blocks, sc, dtype_code(q.dtype), code, dtype_code(ix), _p(ws),
+                                              ws.numel() if ws is not None else 0, c, _raw_stream(dev))
     if st:
         L.check(st, op)
     return out

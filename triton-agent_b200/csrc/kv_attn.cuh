@@ -821,8 +821,9 @@ __global__ void __launch_bounds__((kConsumers + 1) * 32, 1)
       }
     }
   }
-  // this grid counts as done only when the previous one is
-  if (threadIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
+  // this grid counts as done only when the previous one is (the other CTAs
+  // may leave their SMs)
+  if (blockIdx.x == 0 && threadIdx.x == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // ---------------------------------------------------------------------------

@@ -153,6 +153,8 @@ const char* b200_kernel_list(void) {
          "paged_decode_kernel\n"
          "paged_decode_generic_kernel\n"
          "kv_quant_append_kernel\n"
+         "kv_quant_append_stream_kernel\n"
+         "kv_quant_repair_kernel\n"
          "kv_quant_append_generic_kernel\n"
          "slot_claim_kernel\n"
          "kv_dequant_kernel\n"
@@ -300,8 +302,9 @@ const char* b200_query_config_space(const char* op, int64_t rows) {
     field("tile_k", {0, 10, 25, 50}, "percent of the block-table entries handed out as claimed chunks (0: none)");
     field("tile_n", {0, 1, 2, 8}, "pages per claimed chunk (0: 4)");
   } else if (o == "rope_kv_append_paged_quant") {
-    kernel = "kv_quant_append_kernel";
-    field("rows_per_cta", {0, 1, 2, 3, 6}, "rows of a token per thread (0: 1 up to 512 tokens, else 3)");
+    // (its rows_per_cta choice belongs to the prefill kernel)
+    kernel = rows > 512 ? "kv_quant_append_stream_kernel" : "kv_quant_append_kernel";
+    if (rows > 512) field("rows_per_cta", {0, 1, 2, 3, 4, 6, 8}, "rows of a token per thread (0: 2)");
   } else if (o == "paged_kv_dequant") {
     kernel = "kv_dequant_kernel";
   } else if (o == "paged_attention_quant" || o == "paged_attention_prefix") {
