@@ -317,7 +317,7 @@ int b200_paged_kv_dequant(const void* k_cache, const void* v_cache, const float*
  * b200_paged_attention_quant_workspace_size() bytes (may be 0: NULL); nothing
  * in it is kept between calls, it needs no clearing.  Streaming kernel for D = 128, block sizes
  * of 16, 32, ..., 256, 1, 2, 4 or 8 query heads a kv head and 16-byte aligned
- * tensors; a general kernel for the rest (D <= 256).  cfg: stages (ring depth, default about 132
+ * tensors; a general kernel for the rest (D <= 256).  cfg: stages (ring depth in entries of 32 tokens, default about 204
  * KB), rows_per_cta (kv heads per CTA, at most 8), flags bit 0: general kernel; bit 3: programmatic
  * dependent launch (the kernel's prologue overlaps the previous kernel on
  * the stream; the caller guarantees that kernel writes neither context_len

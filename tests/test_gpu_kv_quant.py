@@ -341,7 +341,8 @@ def test_prefix_attention(Hq, Hkv, D, bs, B, dtype, code, cuda_device):
     n_prefix = (1000 + bs - 1) // bs
     q, cache, bt, cl = attention_case(cuda_device, B, Hq, Hkv, D, bs, dtype, code, ctx, seed=B,
                                       nb=B * 16 + n_prefix + 40, index=torch.int32)
-    pt = torch.randperm(cache[0].shape[0], device=cuda_device)[:n_prefix].to(torch.int32)
+    pt = torch.randperm(cache[0].shape[0], generator=torch.Generator().manual_seed(B))[:n_prefix].to(
+        cuda_device, torch.int32)
     for n in (0, 1, bs, 130, 1000):
         pl = torch.tensor([n], dtype=torch.int32, device=cuda_device)
         out = K.paged_attention_prefix(q, cache[0], cache[1], pt, pl, bt, cl, cache[2], cache[3])
@@ -357,7 +358,10 @@ def test_prefix_attention(Hq, Hkv, D, bs, B, dtype, code, cuda_device):
 def test_prefix_dropped_ids_garbage_and_no_own_tokens(bs, code, cuda_device):
     B, n = 20, 515
     q, cache, bt, cl = attention_case(cuda_device, B, 16, 4, 128, bs, torch.bfloat16, code, [7] * B, nb=400, index=torch.int64)
-    pt = torch.randperm(300, device=cuda_device)[: (n + bs - 1) // bs + 3]
+    # blocks of the prefix alone (garbage behind its last token must not be a sequence's live token)
+    free = torch.ones(400, dtype=torch.bool, device=cuda_device)
+    free[bt.flatten()] = False
+    pt = torch.nonzero(free).flatten().flip(0)[: (n + bs - 1) // bs + 3].clone()
     last, off = int(pt[(n - 1) // bs]), (n - 1) % bs + 1
     for c in cache[:2]:
         if code is None:

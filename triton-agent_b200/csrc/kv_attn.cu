@@ -55,9 +55,9 @@ __global__ void __launch_bounds__(256)
     return i < own ? rows + (((int64_t)seg + c1 + i) * p.heads_cta + hh) * kPiecePitch
                    : prefix + ((int64_t)(i - own) * p.B * p.Hq + row) * kPiecePitch;
   };
-  // weight of a piece: none without tokens (m = -inf, l = 0); NaN logits
-  // only leave m = -inf and l = NaN
-  auto weight = [](float m, float l, float M) { return m == -INFINITY ? (l == 0.f ? 0.f : l) : ex2(m - M); };
+  // weight of a piece: none without tokens (l = 0); NaN logits only leave m
+  // without a value and l = NaN
+  auto weight = [](float m, float l, float M) { return l == 0.f ? 0.f : (m > -1e29f ? ex2(m - M) : l); };
   float M = -INFINITY;
   for (int i = lane; i < n; i += 32) M = fmaxf(M, __ldcg(piece(i) + kD));
   M = warp_max(M);
@@ -115,45 +115,36 @@ __global__ void __launch_bounds__(256)
 }
 
 // ---------------------------------------------------------------------------
-// Geometry.  HG: the largest divisor of Hkv up to 8 whose page leaves room for
-// two ring entries; sub warps share a head.  The fast path covers head dim 128,
-// blocks of a multiple of 16 tokens up to 256 and 1, 2, 4 or 8 query heads a kv head.
+// Geometry.  HG: the largest divisor of Hkv up to 8; sub warps share a head.
+// The fast path covers head dim 128, blocks of a multiple of 16 tokens up to 256 and
+// 1, 2, 4 or 8 query heads a kv head.
 // ---------------------------------------------------------------------------
 PieceGeom piece_geometry(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t bs, int64_t num_blocks,
                          int64_t max_blocks, int elem, const b200_launch_cfg* cfg) {
   PieceGeom g{};
   const int64_t G = Hq / Hkv;
   if (D != kD || !(G == 1 || G == 2 || G == 4 || G == 8) || bs % 16 != 0 || bs > 256) return g;
-  // 32-bit token slots (TMA coordinates) and entry counts
-  if (num_blocks * bs >= (1ll << 31) || max_blocks * bs >= (1ll << 31)) return g;
+  // 32-bit token slots and scale rows (TMA coordinates) and entry counts
+  if (num_blocks * bs >= (1ll << 31) || num_blocks * Hkv >= (1ll << 31) || max_blocks * bs >= (1ll << 31)) return g;
   g.G = (int)G;
-  const int hg_most = (cfg && cfg->rows_per_cta > 0 && cfg->rows_per_cta <= 8) ? cfg->rows_per_cta : 8;
-  for (int cand = hg_most; cand >= 1 && g.HG == 0; --cand) {
-    if (Hkv % cand) continue;
-    const int64_t box = (int64_t)cand * bs * 128;
-    const int64_t page = ((elem == 1 ? 2 * box + 2 * (int64_t)cand * bs * 4 : 4 * box) + 1023) / 1024 * 1024;
-    if (2 * page > 176 * 1024) continue;
-    g.HG = cand, g.sub = (elem == 1 ? kConsumers : kConsumers / 2) / cand;
-    g.page_bytes = (uint32_t)page;
-  }
-  if (g.HG == 0) return g;
+  g.HG = (cfg && cfg->rows_per_cta > 0 && cfg->rows_per_cta <= 8) ? cfg->rows_per_cta : 8;
+  while (Hkv % g.HG) --g.HG;
+  g.sub = kConsumers / g.HG;
+  const int box = g.HG * kChunk * 128;
+  g.entry_bytes = (uint32_t)(elem == 1 ? 2 * (2 * box + 1024) : 4 * box);
   g.n_hg = (int)(Hkv / g.HG);
   g.seqs = kMaxSeg / g.n_hg < B ? kMaxSeg / g.n_hg : B;
   if (g.seqs < 1 || g.n_hg * g.seqs * max_blocks >= (1ll << 31)) return g;
   g.grid = device_sm_count();
   g.pdl = cfg && (cfg->flags & 8);
-  const size_t per = g.page_bytes + 16 + sizeof(PageMeta);
-  size_t fixed = 1024 + 16 * 8 + (size_t)(g.n_hg * g.seqs + 1) * 4 + (size_t)g.seqs * 4 + 66 * 4;
-  auto xch = [&] { return (size_t)(g.sub - 1) * g.HG * kXchPitch * 4; };
+  const size_t per = g.entry_bytes + 16 + sizeof(EntryMeta);
+  const size_t fixed = 1024 + 16 * 8 + (size_t)(g.n_hg * g.seqs + 1) * 4 + (size_t)g.seqs * 4 + 66 * 4 +
+                       (size_t)(g.sub - 1) * g.HG * kXchPitch * 4;
   // The ring holds a multiple of sub entries, so that an entry belongs to one
   // slot: its warps have then seen each earlier filling of the entry they wait
   // for (copies complete out of order, and a wait tells only two fillings apart).
-  // Large pages leave room for fewer slots.
-  while (g.sub > 2 && g.sub * per + fixed + xch() > kSmemMost) g.sub /= 2;
-  if (g.sub > 1 && 2 * per + fixed + xch() > kSmemMost) g.sub = 1;
-  fixed += xch();
-  const int unit = g.sub > 1 ? g.sub : 1;
-  int stages = (cfg && cfg->stages > 0) ? cfg->stages : (int)((elem == 1 ? 132 : 196) * 1024 / g.page_bytes);
+  const int unit = g.sub;
+  int stages = (cfg && cfg->stages > 0) ? cfg->stages : (int)(204 * 1024 / g.entry_bytes);
   if (stages > 64) stages = 64;
   stages = stages / unit * unit;
   while (stages > unit && stages * per + fixed > kSmemMost) stages -= unit;

@@ -4,7 +4,7 @@
 //
 // A piece is what one stretch of the keys of one query row leaves behind:
 // (m, l, o) with o[d] = sum_t 2^(x_t - m) v_t[d], l = sum_t 2^(x_t - m), x_t
-// the logits in log2 units.  Pieces of one row join exactly:
+// the logits in log2 units (no tokens: m = -1e30 or -inf, l = 0).  Pieces of one row join exactly:
 //   M = max m_i,  out = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i.
 //
 // 8-bit caches.  With codes c and scales s (k_t = ks_t ck_t, v_t = vs_t cv_t)
@@ -52,7 +52,7 @@ struct PieceGeom {
   int G, HG, n_hg, sub;   // query heads a kv head, kv heads a CTA, head groups, warps a kv head
   int stages, grid;
   int64_t seqs;           // sequences a launch takes (the batch runs in slices of this many)
-  uint32_t page_bytes;
+  uint32_t entry_bytes;
   size_t smem;
   bool pdl;
 };
@@ -203,8 +203,8 @@ __global__ void __launch_bounds__(128)
 // heads its N side; what differs is which element an operand register holds, since one
 // 8x8 ldmatrix of 16-bit cells covers 16 codes a row:
 //   K: a cell pair of lane (r, q) holds the codes d = 16j + 4q + {0..3} of
-//      token r; they are k = {2q, 2q+1, 2q+8, 2q+9} of the j-th k-step, and
-//      the query fragments are loaded in that order
+//      token r; in the order 0, 2, 1, 3 they are k = {2q, 2q+1, 2q+8, 2q+9} of
+//      the j-th k-step, and the query fragments are loaded in that order
 //   V: a transposed cell pair holds d = 16j + 2r + {0, 1} of tokens 2q, 2q+1;
 //      rows r and r + 8 of the j-th m-tile are the dims 16j + 2r and 16j + 2r + 1
 // One 16-token page of a head is 8 ldmatrix.x4, 64 code pairs to f16 and
@@ -242,22 +242,25 @@ __device__ __forceinline__ void load_q_frags8(const T* __restrict__ qrow0, int l
   pow2_scale(amax, up, down);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    qb[j][0] = pack_pair<__half>(f[j][0] * up, f[j][1] * up);
-    qb[j][1] = pack_pair<__half>(f[j][2] * up, f[j][3] * up);
+    qb[j][0] = pack_pair<__half>(f[j][0] * up, f[j][2] * up);
+    qb[j][1] = pack_pair<__half>(f[j][1] * up, f[j][3] * up);
   }
   const float sl = qscale * down;
   slA = __shfl_sync(0xffffffffu, sl, (lane & 3) * 8);
   slB = __shfl_sync(0xffffffffu, sl, (lane & 3) * 8 + 4);
 }
 
-// Raises the running maxima of this thread's two heads to the maxima of four
-// logits (tokens tr, tr + 8), when one in the warp exceeds its maximum by more than
-// 2^8 (exact: O and l share the offset).  Most pages need one vote here and no exchange.
-__device__ __forceinline__ void raise_max_lazy(const float (&y)[4], float (&mu)[2], float (&lp)[2],
+// Running maximum of a head without tokens: so low that any logit raises it
+// and nothing scaled by it survives, and finite, so that differences are.
+constexpr float kNoMax = -1e30f;
+
+// Raises the running maxima of this thread's two heads to the largest logits
+// in the warp (of this thread: top), when one exceeds its maximum by more than
+// 2^8 (exact: O and l share the offset).  Most entries need one vote here and no exchange.
+__device__ __forceinline__ void raise_max_lazy(const float (&top)[2], float (&mu)[2], float (&lp)[2],
                                                float (&o)[8][4]) {
-  const bool up = fmaxf(y[0], y[2]) > mu[0] + 8.0f || fmaxf(y[1], y[3]) > mu[1] + 8.0f;
-  if (!__any_sync(0xffffffffu, up)) return;
-  float m[2] = {fmaxf(y[0], y[2]), fmaxf(y[1], y[3])};
+  float m[2] = {top[0], top[1]};
+  if (!__any_sync(0xffffffffu, m[0] - mu[0] > 8.0f || m[1] - mu[1] > 8.0f)) return;
 #pragma unroll
   for (int off = 4; off <= 16; off <<= 1) {
     m[0] = fmaxf(m[0], __shfl_xor_sync(0xffffffffu, m[0], off));
@@ -266,9 +269,9 @@ __device__ __forceinline__ void raise_max_lazy(const float (&y)[4], float (&mu)[
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     if (!(m[c] > mu[c])) continue;
-    const float alpha = mu[c] == -INFINITY ? 0.f : ex2(mu[c] - m[c]);
+    const float alpha = ex2(mu[c] - m[c]);
     mu[c] = m[c];
-    lp[c] = lp[c] == 0.f ? 0.f : lp[c] * alpha;
+    lp[c] *= alpha;
 #pragma unroll
     for (int mt = 0; mt < 8; ++mt) {
       o[mt][c] *= alpha;
@@ -277,76 +280,94 @@ __device__ __forceinline__ void raise_max_lazy(const float (&y)[4], float (&mu)[
   }
 }
 
-// Tokens [t0, t0 + 16) of kv head w's rows of a page (codes at kb / vb as
-// [head][token][128] rows, 128-byte swizzled; scales at ksp / vsp as [head][token]).
+// Two chunks of sixteen tokens (nt[c] of them live) of one kv head: codes as
+// [head][token][128] rows, 128-byte swizzled, scales as [head][token], chunk c
+// at at + c * chunk_bytes.  Two at once, so that one's chain of ldmatrix,
+// products, exp2 and products runs under the other's.
+// row_at: the lane's ldmatrix row with its first 16 bytes (16 bytes 2j + k of the
+// row are 32 j on, in the swizzle an exclusive or); scale_at: its token's key scale.
 template <typename KV>
-__device__ __forceinline__ void mma_chunk8(uint32_t kb, uint32_t vb, uint32_t ksp, uint32_t vsp, int t0, int ntok, int row0, int lane,
-                                           float slA, float slB, const uint32_t (&qb)[8][2], float (&o)[8][4],
-                                           float (&mu)[2], float (&lp)[2]) {
-  const int mat = lane >> 3, mrow = lane & 7;
+__device__ __forceinline__ void mma_chunks8(uint32_t at, uint32_t chunk_bytes, uint32_t box, uint32_t row_at,
+                                            uint32_t scale_at, const int (&nt)[2], int lane, float slA, float slB,
+                                            const uint32_t (&qb)[8][2], float (&o)[8][4], float (&mu)[2],
+                                            float (&lp)[2]) {
   const int tr = lane >> 2, tq = (lane & 3) * 2;
-  const int row = row0 + t0 + (mat & 1) * 8 + mrow;
-  const uint32_t at = row * 128, sw = ((mat >> 1) ^ (row & 7)) << 4;  // chunk 2j + (mat >> 1), swizzled: sw ^ (j << 5)
-  float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
-  {
+  float y[2][4], iv[2][2];
+  uint32_t vr[2][4][4];
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const uint32_t ka = at + c * chunk_bytes + row_at, sa = at + c * chunk_bytes + scale_at;
+    float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
     uint32_t kr[4][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) ldsm_x4(kb + at + (sw ^ (j << 5)), kr[j][0], kr[j][1], kr[j][2], kr[j][3]);
+    for (int j = 0; j < 4; ++j) ldsm_x4(ka ^ (j << 5), kr[j][0], kr[j][1], kr[j][2], kr[j][3]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      ldsm_x4_t((ka + box) ^ (j << 5), vr[c][j][0], vr[c][j][1], vr[c][j][2], vr[c][j][3]);
+    const float k0 = lds_f32(sa), k1 = lds_f32(sa + 32);
+    float lv0, lv1;
+    kv8_value_scale(lds_f32(sa + 512), lv0, iv[c][0]);
+    kv8_value_scale(lds_f32(sa + 544), lv1, iv[c][1]);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      mma16816<__half>(s0, kv8_pair<KV, 0, 1>(kr[j][0]), kv8_pair<KV, 0, 1>(kr[j][1]), kv8_pair<KV, 2, 3>(kr[j][0]),
-                       kv8_pair<KV, 2, 3>(kr[j][1]), qb[2 * j][0], qb[2 * j][1]);
-      mma16816<__half>(s1, kv8_pair<KV, 0, 1>(kr[j][2]), kv8_pair<KV, 0, 1>(kr[j][3]), kv8_pair<KV, 2, 3>(kr[j][2]),
-                       kv8_pair<KV, 2, 3>(kr[j][3]), qb[2 * j + 1][0], qb[2 * j + 1][1]);
+      uint32_t a[4], b[4];
+      kv8_pairs<KV>(kr[j][0], a[0], a[2]);
+      kv8_pairs<KV>(kr[j][1], a[1], a[3]);
+      kv8_pairs<KV>(kr[j][2], b[0], b[2]);
+      kv8_pairs<KV>(kr[j][3], b[1], b[3]);
+      mma16816<__half>(s0, a[0], a[1], a[2], a[3], qb[2 * j][0], qb[2 * j][1]);
+      mma16816<__half>(s1, b[0], b[1], b[2], b[3], qb[2 * j + 1][0], qb[2 * j + 1][1]);
+    }
+    // y[0]/y[1]: token tr of heads 2(lane%4), +1; y[2]/y[3]: token tr + 8
+    y[c][0] = fmaf(s0[0] + s1[0], k0 * slA, lv0);
+    y[c][1] = fmaf(s0[1] + s1[1], k0 * slB, lv0);
+    y[c][2] = fmaf(s0[2] + s1[2], k1 * slA, lv1);
+    y[c][3] = fmaf(s0[3] + s1[3], k1 * slB, lv1);
+    if (nt[c] < 16) {
+      // tokens past the end may hold any code (e4m3 has a NaN) and any scale: no
+      // weight, and V zero.  A V register holds two codes of token tq and two of tq + 1.
+      if (tr >= nt[c]) y[c][0] = y[c][1] = -INFINITY, iv[c][0] = 0.f;
+      if (tr + 8 >= nt[c]) y[c][2] = y[c][3] = -INFINITY, iv[c][1] = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        vr[c][j][0] = mask_pair(vr[c][j][0], tq, nt[c]);
+        vr[c][j][1] = mask_pair(vr[c][j][1], 8 + tq, nt[c]);
+        vr[c][j][2] = mask_pair(vr[c][j][2], tq, nt[c]);
+        vr[c][j][3] = mask_pair(vr[c][j][3], 8 + tq, nt[c]);
+      }
     }
   }
-  uint32_t vr[4][4];
+  const float top[2] = {fmaxf(sm100::fmax3(y[0][0], y[0][2], y[1][0]), y[1][2]),
+                        fmaxf(sm100::fmax3(y[0][1], y[0][3], y[1][1]), y[1][3])};
+  raise_max_lazy(top, mu, lp, o);
+  uint32_t pb[2][2];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) ldsm_x4_t(vb + at + (sw ^ (j << 5)), vr[j][0], vr[j][1], vr[j][2], vr[j][3]);
-  const uint32_t tok = (uint32_t)(row0 + t0 + tr) * 4;
-  const float k0 = lds_f32(ksp + tok), k1 = lds_f32(ksp + tok + 32);
-  float lv0, iv0, lv1, iv1;
-  kv8_value_scale(lds_f32(vsp + tok), lv0, iv0);
-  kv8_value_scale(lds_f32(vsp + tok + 32), lv1, iv1);
-  // y[0]/y[1]: token tr of heads 2(lane%4), +1; y[2]/y[3]: token tr + 8
-  float y[4];
-  y[0] = fmaf(s0[0] + s1[0], k0 * slA, lv0);
-  y[1] = fmaf(s0[1] + s1[1], k0 * slB, lv0);
-  y[2] = fmaf(s0[2] + s1[2], k1 * slA, lv1);
-  y[3] = fmaf(s0[3] + s1[3], k1 * slB, lv1);
-  if (t0 + 16 > ntok) {
-    // tokens past the end may hold any code (e4m3 has a NaN) and any scale: no
-    // weight, and V zero.  A V register holds two codes of token tq and two of tq + 1.
-    if (t0 + tr >= ntok) y[0] = y[1] = -INFINITY, iv0 = 0.f;
-    if (t0 + tr + 8 >= ntok) y[2] = y[3] = -INFINITY, iv1 = 0.f;
+  for (int c = 0; c < 2; ++c) {
+    const float p0 = ex2(y[c][0] - mu[0]), p2 = ex2(y[c][2] - mu[0]);
+    const float p1 = ex2(y[c][1] - mu[1]), p3 = ex2(y[c][3] - mu[1]);
+    lp[0] = fmaf(p0, iv[c][0], fmaf(p2, iv[c][1], lp[0]));
+    lp[1] = fmaf(p1, iv[c][0], fmaf(p3, iv[c][1], lp[1]));
+    pb[c][0] = movm_t(pack_pair<__half>(p0, p1));
+    pb[c][1] = movm_t(pack_pair<__half>(p2, p3));
+  }
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      vr[j][0] = mask_pair(vr[j][0], t0 + tq, ntok);
-      vr[j][1] = mask_pair(vr[j][1], t0 + 8 + tq, ntok);
-      vr[j][2] = mask_pair(vr[j][2], t0 + tq, ntok);
-      vr[j][3] = mask_pair(vr[j][3], t0 + 8 + tq, ntok);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        uint32_t a[4];
+        kv8_pairs<KV>(vr[c][j][2 * u], a[0], a[1]);
+        kv8_pairs<KV>(vr[c][j][2 * u + 1], a[2], a[3]);
+        mma16816<__half>(o[2 * j + u], a[0], a[1], a[2], a[3], pb[c][0], pb[c][1]);
+      }
     }
-  }
-  raise_max_lazy(y, mu, lp, o);
-  const float nA = mu[0] == -INFINITY ? 0.f : mu[0], nB = mu[1] == -INFINITY ? 0.f : mu[1];
-  const float p0 = ex2(y[0] - nA), p2 = ex2(y[2] - nA);
-  const float p1 = ex2(y[1] - nB), p3 = ex2(y[3] - nB);
-  lp[0] = fmaf(p0, iv0, fmaf(p2, iv1, lp[0]));
-  lp[1] = fmaf(p1, iv0, fmaf(p3, iv1, lp[1]));
-  const uint32_t b0 = movm_t(pack_pair<__half>(p0, p1));
-  const uint32_t b1 = movm_t(pack_pair<__half>(p2, p3));
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-      mma16816<__half>(o[2 * j + u], kv8_pair<KV, 0, 2>(vr[j][2 * u]), kv8_pair<KV, 1, 3>(vr[j][2 * u]),
-                       kv8_pair<KV, 0, 2>(vr[j][2 * u + 1]), kv8_pair<KV, 1, 3>(vr[j][2 * u + 1]), b0, b1);
   }
 }
 
 // The same for 16-bit caches: K and V as two boxes of 64 dims each, `box` bytes apart.
 template <typename T>
-__device__ __forceinline__ void mma_chunk16(uint32_t kb, uint32_t vb, uint32_t box, int t0, int ntok, int row0,
+__device__ __forceinline__ void mma_chunk16(uint32_t kb, uint32_t vb, uint32_t box, int ntok, int row0,
                                             int lane, float sl, const uint32_t (&qb)[8][2], float (&o)[8][4],
                                             float (&mu)[2], float (&lp)[2]) {
   const int mat = lane >> 3, mrow = lane & 7;
@@ -354,7 +375,7 @@ __device__ __forceinline__ void mma_chunk16(uint32_t kb, uint32_t vb, uint32_t b
   float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
   {
     // A = K rows: matrix `mat` = (token half mat&1, dim-chunk parity mat>>1)
-    const int row = row0 + t0 + (mat & 1) * 8 + mrow;
+    const int row = row0 + (mat & 1) * 8 + mrow;
     const uint32_t at = kb + row * 128, sw = ((mat >> 1) ^ (row & 7)) << 4;
 #pragma unroll
     for (int ks = 0; ks < 8; ++ks) {
@@ -366,7 +387,7 @@ __device__ __forceinline__ void mma_chunk16(uint32_t kb, uint32_t vb, uint32_t b
   // A = V^T by ldmatrix.trans: matrix `mat` = (token half mat>>1, dim-chunk parity mat&1)
   uint32_t va[8][4];
   {
-    const int row = row0 + t0 + (mat >> 1) * 8 + mrow;
+    const int row = row0 + (mat >> 1) * 8 + mrow;
     const uint32_t at = vb + row * 128, sw = ((mat & 1) ^ (row & 7)) << 4;
 #pragma unroll
     for (int mt = 0; mt < 8; ++mt)
@@ -375,21 +396,21 @@ __device__ __forceinline__ void mma_chunk16(uint32_t kb, uint32_t vb, uint32_t b
   float y[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) y[i] = (s0[i] + s1[i]) * sl;
-  if (t0 + 16 > ntok) {
-    if (t0 + tr >= ntok) y[0] = y[1] = -INFINITY;
-    if (t0 + tr + 8 >= ntok) y[2] = y[3] = -INFINITY;
+  if (ntok < 16) {
+    if (tr >= ntok) y[0] = y[1] = -INFINITY;
+    if (tr + 8 >= ntok) y[2] = y[3] = -INFINITY;
 #pragma unroll
     for (int mt = 0; mt < 8; ++mt) {
-      va[mt][0] = mask_pair(va[mt][0], t0 + tq, ntok);
-      va[mt][1] = mask_pair(va[mt][1], t0 + tq, ntok);
-      va[mt][2] = mask_pair(va[mt][2], t0 + 8 + tq, ntok);
-      va[mt][3] = mask_pair(va[mt][3], t0 + 8 + tq, ntok);
+      va[mt][0] = mask_pair(va[mt][0], tq, ntok);
+      va[mt][1] = mask_pair(va[mt][1], tq, ntok);
+      va[mt][2] = mask_pair(va[mt][2], 8 + tq, ntok);
+      va[mt][3] = mask_pair(va[mt][3], 8 + tq, ntok);
     }
   }
-  raise_max_lazy(y, mu, lp, o);
-  const float nA = mu[0] == -INFINITY ? 0.f : mu[0], nB = mu[1] == -INFINITY ? 0.f : mu[1];
-  const float p0 = ex2(y[0] - nA), p2 = ex2(y[2] - nA);
-  const float p1 = ex2(y[1] - nB), p3 = ex2(y[3] - nB);
+  const float top[2] = {fmaxf(y[0], y[2]), fmaxf(y[1], y[3])};
+  raise_max_lazy(top, mu, lp, o);
+  const float p0 = ex2(y[0] - mu[0]), p2 = ex2(y[2] - mu[0]);
+  const float p1 = ex2(y[1] - mu[1]), p3 = ex2(y[3] - mu[1]);
   lp[0] += p0 + p2;
   lp[1] += p1 + p3;
   const uint32_t b0 = movm_t(pack_pair<T>(p0, p1));
@@ -434,14 +455,14 @@ __device__ __forceinline__ void store_piece8(float* __restrict__ row0, const flo
 // ---------------------------------------------------------------------------
 // Streaming kernel.  All segments' block-table entries (segment s = hg * B + b)
 // laid end to end are cut into one equal contiguous range a CTA, one CTA an
-// SM.  The producer warp walks its range and fills a ring of pages with TMA (K
-// and V boxes of HG heads, and for 8-bit caches the page's scales by bulk
-// copies).  sub consumer warps share a kv head: page i of the ring goes to the
-// HG warps of slot i % sub, so that sixteen warps (eight for 16-bit pages, which need
-// no widening and fill the ring by themselves) have work whatever Hkv is: a
-// page's chain from ldmatrix over exp2 to the second product is long, and with
-// two warps a scheduler the kernel waits on it (64 sequences, int8: 164 us
-// with eight consumer warps, 118 with sixteen).  End
+// SM.  The producer warp walks its range and fills a ring with TMA; an entry is
+// one chunk of sixteen tokens of a page (16-bit caches) or two (8-bit): K and V boxes of
+// HG heads, and for 8-bit caches the tokens' scales.  sub consumer warps share
+// a kv head: entry i goes to the HG warps of slot i % sub, so that eight
+// warps have work whatever Hkv is.  A chunk's chain from ldmatrix over exp2 to the
+// second product is long: 8-bit chunks go through it in pairs (64 sequences,
+// int8: 164 us with one chunk at a time and eight warps, 118 us with sixteen
+// warps of 96 registers, which spill).  End
 // markers, one for each slot, close a segment: the warps of a head add up their (m,
 // l, o) in shared memory, and the first writes the normalised row when the
 // range holds the whole segment, else the range's piece at row segment +
@@ -451,18 +472,20 @@ __device__ __forceinline__ void store_piece8(float* __restrict__ row0, const flo
 struct PiecesParams {
   int64_t B, Hq, Hkv, num_blocks, max_blocks;
   int bs, HG, n_hg, sub, stages, nseg;
+  int scale_maps;  // scales by tensor maps (pages of more than 16 tokens), else one copy a page
   int always;   // write every segment as pieces (a prefix joins them)
   int overlap;  // launched beside the previous grid of the call: wait for it at the end
-  uint32_t page_bytes;
+  uint32_t entry_bytes;
   float qscale;  // scale * log2(e)
 };
 
-constexpr int kConsumers = 16;  // consumer warps, at most
-struct PageMeta {
-  int kind;  // 0 page, 1 end of segment, 2 end of stream
+constexpr int kChunk = 16;     // tokens of a chunk
+constexpr int kConsumers = 8;  // consumer warps, at most
+struct EntryMeta {
+  int kind;  // 0 tokens, 1 end of segment, 2 end of stream
   int seg;
-  int ntok;   // page: tokens
-  int piece;  // end of segment: row of the piece, -1: the segment's only one
+  int ntok;   // live tokens of the first chunk
+  int piece;  // live tokens of the second; end of segment: row of the piece, -1: the segment's only one
 };
 constexpr int kXchPitch = 36 * 32;  // floats a warp hands over: 32 o, 2 m, 2 l a lane
 
@@ -479,6 +502,7 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 template <typename T, typename KV, int G>
 __global__ void __launch_bounds__((kConsumers + 1) * 32, 1)
     paged_attn_pieces_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                             const __grid_constant__ CUtensorMap tm_ks, const __grid_constant__ CUtensorMap tm_vs,
                              const float* __restrict__ k_scale, const float* __restrict__ v_scale,
                              const T* __restrict__ q, IndexPtr btab, IndexPtr clen, T* __restrict__ out,
                              float* __restrict__ ws_rows, int32_t* __restrict__ ws_cum, PiecesParams p) {
@@ -489,13 +513,13 @@ __global__ void __launch_bounds__((kConsumers + 1) * 32, 1)
   const int HG = p.HG, bs = p.bs, sub = p.sub, consumers = HG * sub;
   const int heads_cta = HG * G;
   const int64_t B = p.B;
-  float* xch = reinterpret_cast<float*>(smem + p.stages * p.page_bytes);  // [sub - 1][HG][kXchPitch]
+  float* xch = reinterpret_cast<float*>(smem + p.stages * p.entry_bytes);  // [sub - 1][HG][kXchPitch]
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(xch + (sub - 1) * HG * kXchPitch);
   uint64_t* empty_bar = full_bar + p.stages;
   uint64_t* xch_full = empty_bar + p.stages;  // [8]
   uint64_t* xch_empty = xch_full + 8;         // [8]
-  static_assert(sizeof(PageMeta) == 16, "read as one vector");
-  PageMeta* meta = reinterpret_cast<PageMeta*>(xch_empty + 8);
+  static_assert(sizeof(EntryMeta) == 16, "read as one vector");
+  EntryMeta* meta = reinterpret_cast<EntryMeta*>(xch_empty + 8);
   int* s_cum = reinterpret_cast<int*>(meta + p.stages);
   int* s_ctx = s_cum + (p.nseg + 1);
   int* chunk_id = s_ctx + B;
@@ -588,8 +612,11 @@ __global__ void __launch_bounds__((kConsumers + 1) * 32, 1)
       sm100::tma_prefetch_desc(&tm_v);
     }
     const uint32_t base = sm100::smem_u32(smem);
-    const uint32_t box = (uint32_t)(HG * bs * 128);  // one 128-byte-wide box: all of an 8-bit tile, half of a 16-bit one
-    const uint32_t page_tx = k8 ? 2 * box + (uint32_t)(2 * HG * bs * 4) : 4 * box;
+    const uint32_t box = (uint32_t)(HG * kChunk * 128);  // 128 bytes wide: all of an 8-bit tile, half of a 16-bit one
+    const uint32_t sbox = (uint32_t)(HG * kChunk * 4);
+    const uint32_t chunk_tx = k8 ? 2 * box + 2 * sbox : 4 * box;
+    const uint32_t chunk_bytes = k8 ? 2 * box + 1024 : 4 * box;
+    int fill = 0;  // (lane 0) chunks in the open entry
     const unsigned lt_mask = (1u << lane) - 1u;
     int it = 0, st = 0;
     uint32_t ph = 1;  // parity of the empty barriers in this round
@@ -609,7 +636,7 @@ __global__ void __launch_bounds__((kConsumers + 1) * 32, 1)
     auto markers = [&](int kind, int seg, int piece) -> bool {  // one for each slot
       for (int i = 0; i < sub; ++i) {
         if (!acquire()) return false;
-        meta[st] = PageMeta{kind, seg, 0, piece};
+        meta[st] = EntryMeta{kind, seg, 0, piece};
         sm100::mbar_arrive(sm100::smem_u32(&full_bar[st]));
         advance();
       }
@@ -646,37 +673,64 @@ __global__ void __launch_bounds__((kConsumers + 1) * 32, 1)
         __syncwarp();
         if (lane == 0) {
           const int n = __popc(ub);
-          for (int u = 0; u < n; ++u) {
-            ok = acquire();
-            if (!ok) break;
-            if (!waited) {  // programmatic launch: the first copy waits for the previous kernel
-              asm volatile("griddepcontrol.wait;" ::: "memory");
-              waited = true;
+          for (int u = 0; u < n && ok; ++u) {
+            const int32_t id = chunk_id[u], h0 = hg * HG;
+            const int nt_page = chunk_ntok[u];
+            for (int t0 = 0; t0 < nt_page; t0 += kChunk) {
+              if (fill == 0) {
+                ok = acquire();
+                if (!ok) break;
+                if (!waited) {  // programmatic launch: the first copy waits for the previous kernel
+                  asm volatile("griddepcontrol.wait;" ::: "memory");
+                  waited = true;
+                }
+              }
+              const int live = nt_page - t0 < kChunk ? nt_page - t0 : kChunk;
+              const uint32_t fb = sm100::smem_u32(&full_bar[st]);
+              const uint32_t dst = base + st * p.entry_bytes + fill * chunk_bytes;
+              const int32_t tok0 = id * bs + t0;
+              if (fill == 0) meta[st] = EntryMeta{0, s, live, 0};
+              else meta[st].piece = live;
+              ++fill;
+              const bool full = !k8 || fill == 2;
+              // an entry's one arrival comes with its last chunk; the first only adds bytes
+              if (full) sm100::mbar_arrive_expect_tx(fb, chunk_tx);
+              else
+                asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(fb), "r"(chunk_tx)
+                             : "memory");
+              if constexpr (k8) {
+                sm100::tma_load_3d(dst, &tm_k, fb, 0, tok0, h0);
+                sm100::tma_load_3d(dst + box, &tm_v, fb, 0, tok0, h0);
+                if (p.scale_maps) {
+                  sm100::tma_load_2d(dst + 2 * box, &tm_ks, fb, t0, id * (int32_t)p.Hkv + h0);
+                  sm100::tma_load_2d(dst + 2 * box + 512, &tm_vs, fb, t0, id * (int32_t)p.Hkv + h0);
+                } else {
+                  const int64_t sat = ((int64_t)id * p.Hkv + h0) * kChunk;
+                  bulk_load(dst + 2 * box, k_scale + sat, sbox, fb);
+                  bulk_load(dst + 2 * box + 512, v_scale + sat, sbox, fb);
+                }
+              } else {
+                sm100::tma_load_3d(dst, &tm_k, fb, 0, tok0, h0);
+                sm100::tma_load_3d(dst + box, &tm_k, fb, 64, tok0, h0);
+                sm100::tma_load_3d(dst + 2 * box, &tm_v, fb, 0, tok0, h0);
+                sm100::tma_load_3d(dst + 3 * box, &tm_v, fb, 64, tok0, h0);
+              }
+              if (full) {
+                advance();
+                fill = 0;
+              }
             }
-            meta[st] = PageMeta{0, s, chunk_ntok[u], 0};
-            const uint32_t fb = sm100::smem_u32(&full_bar[st]), dst = base + st * p.page_bytes;
-            const int32_t tok0 = chunk_id[u] * bs, h0 = hg * HG;
-            sm100::mbar_arrive_expect_tx(fb, page_tx);
-            if constexpr (k8) {
-              sm100::tma_load_3d(dst, &tm_k, fb, 0, tok0, h0);
-              sm100::tma_load_3d(dst + box, &tm_v, fb, 0, tok0, h0);
-              const uint32_t sb = (uint32_t)(HG * bs * 4);
-              const int64_t sat = ((int64_t)chunk_id[u] * p.Hkv + h0) * bs;
-              bulk_load(dst + 2 * box, k_scale + sat, sb, fb);
-              bulk_load(dst + 2 * box + sb, v_scale + sat, sb, fb);
-            } else {
-              sm100::tma_load_3d(dst, &tm_k, fb, 0, tok0, h0);
-              sm100::tma_load_3d(dst + box, &tm_k, fb, 64, tok0, h0);
-              sm100::tma_load_3d(dst + 2 * box, &tm_v, fb, 0, tok0, h0);
-              sm100::tma_load_3d(dst + 3 * box, &tm_v, fb, 64, tok0, h0);
-            }
-            advance();
           }
         }
         ok = __shfl_sync(0xffffffffu, ok, 0);
         __syncwarp();
       }
       if (lane == 0 && ok) {
+        if (fill > 0) {  // the segment ends in the first chunk of an entry
+          sm100::mbar_arrive(sm100::smem_u32(&full_bar[st]));
+          advance();
+          fill = 0;
+        }
         const bool one = range_of(segs, E, R) == range_of(sege - 1, E, R);
         ok = markers(1, s, one && !p.always ? -1 : s + c);
       }
@@ -700,10 +754,13 @@ __global__ void __launch_bounds__((kConsumers + 1) * 32, 1)
     const int w = warp % HG, slot = warp / HG;
     const uint32_t base = sm100::smem_u32(smem), meta_at = sm100::smem_u32(meta);
     const uint32_t xch_at = sm100::smem_u32(xch) + (uint32_t)(w * kXchPitch + lane) * 4;
-    const uint32_t box = (uint32_t)(HG * bs * 128);
+    const uint32_t box = (uint32_t)(HG * kChunk * 128);
+    const int mat = lane >> 3, lrow = w * kChunk + (mat & 1) * 8 + (lane & 7);
+    const uint32_t row_at = lrow * 128 + (((mat >> 1) ^ (lrow & 7)) << 4);
+    const uint32_t scale_at = 2 * box + (uint32_t)(w * kChunk + (lane >> 2)) * 4;
     uint32_t qb[8][2];
     float o[8][4];
-    float mu[2] = {-INFINITY, -INFINITY}, lp[2] = {0.f, 0.f};
+    float mu[2] = {kNoMax, kNoMax}, lp[2] = {0.f, 0.f};
     float slA = p.qscale, slB = p.qscale;
 #pragma unroll
     for (int i = 0; i < 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
@@ -719,8 +776,8 @@ __global__ void __launch_bounds__((kConsumers + 1) * 32, 1)
         }
         break;
       }
-      const uint4 mw = lds128(meta_at + st * (int)sizeof(PageMeta));
-      const PageMeta m{(int)mw.x, (int)mw.y, (int)mw.z, (int)mw.w};
+      const uint4 mw = lds128(meta_at + st * (int)sizeof(EntryMeta));
+      const EntryMeta m{(int)mw.x, (int)mw.y, (int)mw.z, (int)mw.w};
       if (m.kind == 0) {
         if (m.seg != cur) {
           cur = m.seg;
@@ -729,13 +786,12 @@ __global__ void __launch_bounds__((kConsumers + 1) * 32, 1)
           if constexpr (k8) load_q_frags8<T, G>(qrow, lane, p.qscale, qb, slA, slB);
           else load_q_frags<T, G>(qrow, lane, qb);
         }
-        const uint32_t pg = base + st * p.page_bytes;
-        const uint32_t sc = pg + 2 * box;
-        for (int t0 = 0; t0 < m.ntok; t0 += 16) {
-          if constexpr (k8)
-            mma_chunk8<KV>(pg, pg + box, sc, sc + HG * bs * 4, t0, m.ntok, w * bs, lane, slA, slB, qb, o, mu, lp);
-          else
-            mma_chunk16<T>(pg, pg + 2 * box, box, t0, m.ntok, w * bs, lane, p.qscale, qb, o, mu, lp);
+        const uint32_t pg = base + st * p.entry_bytes;
+        if constexpr (k8) {
+          const int nt[2] = {m.ntok, m.piece};
+          mma_chunks8<KV>(pg, 2 * box + 1024, box, row_at, scale_at, nt, lane, slA, slB, qb, o, mu, lp);
+        } else {
+          mma_chunk16<T>(pg, pg + 2 * box, box, m.ntok, w * kChunk, lane, p.qscale, qb, o, mu, lp);
         }
       } else if (m.kind == 1) {
         bool write = true;
@@ -773,11 +829,10 @@ __global__ void __launch_bounds__((kConsumers + 1) * 32, 1)
               const uint32_t y = xch_at + (uint32_t)((v - 1) * HG * kXchPitch) * 4;
 #pragma unroll
               for (int k = 0; k < 2; ++k) {
-                // piece factors: 1 and 2^(difference); no tokens (m = -inf) adds nothing
+                // (no tokens: m = kNoMax with l and o zero)
                 const float mo = lds_f32(y + (32 + k) * 128), lo2 = lds_f32(y + (34 + k) * 128);
                 const float mn = fmaxf(mu[k], mo);
-                const float fa = mu[k] == mn || mu[k] == -INFINITY ? 1.f : ex2(mu[k] - mn);
-                const float fb = mo == mn || mo == -INFINITY ? 1.f : ex2(mo - mn);
+                const float fa = ex2(mu[k] - mn), fb = ex2(mo - mn);
                 mu[k] = mn;
                 lp[k] = lp[k] * fa + lo2 * fb;
 #pragma unroll
@@ -805,7 +860,7 @@ __global__ void __launch_bounds__((kConsumers + 1) * 32, 1)
             else store_partial<G>(row0, kPiecePitch, row0 + kD, kPiecePitch, o, mu, lA, lB, lane);
           }
         }
-        mu[0] = mu[1] = -INFINITY;
+        mu[0] = mu[1] = kNoMax;
         lp[0] = lp[1] = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
@@ -831,28 +886,42 @@ __global__ void __launch_bounds__((kConsumers + 1) * 32, 1)
 // ---------------------------------------------------------------------------
 template <typename T, typename KV, int G>
 int launch_pieces(const AttnCall& a, const PieceGeom& g, const PieceSpace& w, bool overlap, cudaStream_t stream) {
-  CUtensorMap tk, tv;
+  CUtensorMap tk, tv, tks{}, tvs{};
   constexpr bool k8 = sizeof(KV) == 1;
   constexpr uint64_t el = sizeof(KV);
   const CUtensorMapDataType dt = k8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                     : (std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                                       : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16);
-  // dims (d, token slot, head): a box of 128 bytes of dims x bs tokens x HG heads
+  // dims (d, token slot, head): a box of 128 bytes of dims x 16 tokens x HG heads
   // lands as rows ordered (head, token) of 128 bytes, swizzled in 8-row atoms
   const uint64_t dims[3] = {(uint64_t)kD, (uint64_t)(a.num_blocks * a.block_size), (uint64_t)a.Hkv};
   const uint64_t strides[2] = {(uint64_t)a.Hkv * kD * el, (uint64_t)kD * el};
-  const uint32_t box[3] = {(uint32_t)(128 / el), (uint32_t)a.block_size, (uint32_t)g.HG};
+  const uint32_t box[3] = {(uint32_t)(128 / el), (uint32_t)kChunk, (uint32_t)g.HG};
   int st = encode_tensor_map(&tk, dt, 3, a.k_cache, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
   if (st) return st;
   st = encode_tensor_map(&tv, dt, 3, a.v_cache, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
   if (st) return st;
+  const bool scale_maps = k8 && a.block_size != kChunk;
+  if (scale_maps) {
+    // scales [num_blocks * Hkv rows][block_size]: a box of 16 tokens x HG heads
+    const uint64_t sdims[2] = {(uint64_t)a.block_size, (uint64_t)(a.num_blocks * a.Hkv)};
+    const uint64_t sstride[1] = {(uint64_t)a.block_size * 4};
+    const uint32_t sbox[2] = {(uint32_t)kChunk, (uint32_t)g.HG};
+    st = encode_tensor_map(&tks, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, a.k_scale, sdims, sstride, sbox,
+                           CU_TENSOR_MAP_SWIZZLE_NONE);
+    if (st) return st;
+    st = encode_tensor_map(&tvs, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, a.v_scale, sdims, sstride, sbox,
+                           CU_TENSOR_MAP_SWIZZLE_NONE);
+    if (st) return st;
+  }
   PiecesParams p{};
+  p.scale_maps = scale_maps;
   p.B = a.B, p.Hq = a.Hq, p.Hkv = a.Hkv, p.num_blocks = a.num_blocks, p.max_blocks = a.max_blocks;
   p.bs = (int)a.block_size, p.HG = g.HG, p.n_hg = g.n_hg, p.sub = g.sub, p.stages = g.stages;
   p.nseg = (int)(g.n_hg * a.B);
   p.always = a.prefix_table != nullptr;
   p.overlap = overlap;
-  p.page_bytes = g.page_bytes;
+  p.entry_bytes = g.entry_bytes;
   p.qscale = a.scale * 1.4426950408889634f;
   auto kern = paged_attn_pieces_kernel<T, KV, G>;
   static SmemGrant grant;
@@ -869,7 +938,7 @@ int launch_pieces(const AttnCall& a, const PieceGeom& g, const PieceSpace& w, bo
   lc.attrs = attr;
   lc.numAttrs = (overlap || g.pdl) ? 1 : 0;
   const int wide = a.index_dtype == B200_I64;
-  e = cudaLaunchKernelEx(&lc, kern, tk, tv, a.k_scale, a.v_scale, static_cast<const T*>(a.q),
+  e = cudaLaunchKernelEx(&lc, kern, tk, tv, tks, tvs, a.k_scale, a.v_scale, static_cast<const T*>(a.q),
                          IndexPtr{a.block_table, wide}, IndexPtr{a.context_len, wide}, static_cast<T*>(a.out), w.rows,
                          w.cum, p);
   return launch_status(e);

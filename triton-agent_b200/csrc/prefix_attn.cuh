@@ -428,10 +428,11 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
           for (int c = 0; c < 4; ++c) w[c] = lds128(src + (((c0 + c) ^ (r & 7)) << 4));
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            uint4 a = make_uint4(kv8_pair<KV, 0, 1>(w[c].x), kv8_pair<KV, 2, 3>(w[c].x), kv8_pair<KV, 0, 1>(w[c].y),
-                                 kv8_pair<KV, 2, 3>(w[c].y));
-            uint4 b = make_uint4(kv8_pair<KV, 0, 1>(w[c].z), kv8_pair<KV, 2, 3>(w[c].z), kv8_pair<KV, 0, 1>(w[c].w),
-                                 kv8_pair<KV, 2, 3>(w[c].w));
+            uint4 a, b;
+            kv8_in_order<KV>(w[c].x, a.x, a.y);
+            kv8_in_order<KV>(w[c].y, a.z, a.w);
+            kv8_in_order<KV>(w[c].z, b.x, b.y);
+            kv8_in_order<KV>(w[c].w, b.z, b.w);
             if (!live) a = b = make_uint4(0, 0, 0, 0);
             const uint32_t d = dst + (c0 >> 2) * kPHalf;
             sts128(d + (((2 * c) ^ (r & 7)) << 4), a);

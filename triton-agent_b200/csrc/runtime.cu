@@ -309,7 +309,7 @@ const char* b200_query_config_space(const char* op, int64_t rows) {
     kernel = "kv_dequant_kernel";
   } else if (o == "paged_attention_quant" || o == "paged_attention_prefix") {
     kernel = "paged_attn_pieces_kernel";
-    field("stages", {0, 2, 3, 4, 6}, "page ring depth (0: about 132 KB of pages in flight)");
+    field("stages", {0, 2, 3, 4, 6}, "ring depth in entries of 32 tokens (16-bit caches: 16; 0: about 204 KB)");
     field("rows_per_cta", {0, 1, 2, 4, 8}, "kv heads per CTA, a divisor of H_kv (0: the largest <= 8 that fits)");
   } else if (o == "quant_matmul") {
     if (rows > 0 && rows <= 64) {
