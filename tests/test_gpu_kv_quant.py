@@ -407,7 +407,7 @@ def test_prefix_equals_attention_over_the_joined_tables(code, cuda_device):
     for b in range(B):
         _, bound = attend64(q[b], rows64(cache[0], cache[2], joined[b], both[b]),
                             rows64(cache[1], cache[3], joined[b], both[b]), q.dtype,
-                            torch.bfloat16 if code is None else torch.float16)
+                            torch.bfloat16 if code is None else torch.float16, code=code is not None)
         assert ((out[b].double() - one[b].double()).abs() <= 2 * bound).all()
 
 

@@ -4,6 +4,7 @@
 #include <cuda_fp8.h>
 
 #include "common.cuh"
+#include "sm100.cuh"
 
 namespace b200 {
 
@@ -72,6 +73,67 @@ __device__ __forceinline__ void kv8_in_order(uint32_t w, uint32_t& lo, uint32_t&
     lo = *reinterpret_cast<const uint32_t*>(&a);
     hi = *reinterpret_cast<const uint32_t*>(&b);
   }
+}
+
+// D = A B + C on 16 x 8 x 32 tiles of 8-bit operands: A codes, B a term of the
+// other operand (e4m3; int8 as signed bytes, or unsigned ones).  Accumulators are
+// 32-bit words: fp32 for e4m3, int32 for int8.  The first form starts all of D at
+// one word (no register has to be set first).
+#define B200_MMA8(SHAPE, TYPES, CT, CLIST, ...)                                                               \
+  asm volatile("mma.sync.aligned." SHAPE ".row.col." TYPES " {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, " CLIST ";" \
+               : "=" CT(d[0]), "=" CT(d[1]), "=" CT(d[2]), "=" CT(d[3])                                       \
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), __VA_ARGS__)
+template <bool UB>
+__device__ __forceinline__ void mma8_start(int32_t (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, int32_t c) {
+  if constexpr (UB) B200_MMA8("m16n8k32", "s32.s8.u8.s32", "r", "{%10,%10,%10,%10}", "r"(c));
+  else B200_MMA8("m16n8k32", "s32.s8.s8.s32", "r", "{%10,%10,%10,%10}", "r"(c));
+}
+template <bool UB>
+__device__ __forceinline__ void mma8_add(int32_t (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  const int32_t c0 = d[0], c1 = d[1], c2 = d[2], c3 = d[3];
+  if constexpr (UB)
+    B200_MMA8("m16n8k32", "s32.s8.u8.s32", "r", "{%10,%11,%12,%13}", "r"(c0), "r"(c1), "r"(c2), "r"(c3));
+  else
+    B200_MMA8("m16n8k32", "s32.s8.s8.s32", "r", "{%10,%11,%12,%13}", "r"(c0), "r"(c1), "r"(c2), "r"(c3));
+}
+template <bool UB>
+__device__ __forceinline__ void mma8_start(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c) {
+  B200_MMA8("m16n8k32", "f32.e4m3.e4m3.f32", "f", "{%10,%10,%10,%10}", "f"(c));
+}
+template <bool UB>
+__device__ __forceinline__ void mma8_add(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  const float c0 = d[0], c1 = d[1], c2 = d[2], c3 = d[3];
+  B200_MMA8("m16n8k32", "f32.e4m3.e4m3.f32", "f", "{%10,%11,%12,%13}", "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+}
+#undef B200_MMA8
+
+// Accumulators of the codes' products.  int32 sums below 2^22 start at the bit
+// pattern of 1.5 * 2^23, whose low bits they then count: a value is one exact
+// subtraction, without the conversion pipe.
+template <typename KV>
+struct Acc8 {
+  using word = typename std::conditional<std::is_same<KV, int8_t>::value, int32_t, float>::type;
+  static __device__ __forceinline__ word start() {
+    if constexpr (std::is_same<KV, int8_t>::value) return 0x4B400000;
+    else return 0.0f;
+  }
+  // Values of two accumulators.
+  static __device__ __forceinline__ void values(word a, word b, float& x, float& y) {
+    if constexpr (std::is_same<KV, int8_t>::value) {
+      x = -12582912.0f, y = -12582912.0f;
+      sm100::fadd2_acc(x, y, __int_as_float(a), __int_as_float(b));
+    } else {
+      x = a, y = b;
+    }
+  }
+};
+
+// Two 16 x 16 byte matrices, transposed: lane (r, q) gets rows 4q..4q+3 of
+// columns r and r + 8 of the first (lanes 0-15 give its row addresses) and of the second.
+__device__ __forceinline__ void ldsm_x2_t8(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
 }
 
 // The scales of a key and its value as the attention kernels use them: the

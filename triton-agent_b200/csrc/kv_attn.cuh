@@ -10,15 +10,15 @@
 // 8-bit caches.  With codes c and scales s (k_t = ks_t ck_t, v_t = vs_t cv_t)
 //   x_t = scale log2(e) ks_t (q . ck_t)
 //   out = sum_t 2^(x_t) vs_t cv_t / sum_t 2^(x_t)
-// so the codes go to the tensor cores as they are (int8 and e4m3 codes are
-// exact in f16) and the scales meet fp32 values only: the kernel keeps
-// y_t = x_t + log2 vs_t, takes the running maximum over y, feeds the weights
-// w_t = 2^(y_t - m) (f16, half a step 2^-12) to the second product with the
-// bare codes, and sums l = sum_t w_t / vs_t in fp32.  Taking the maximum over y
-// rather than x keeps the largest weight at 1 however the value scales of the
-// tokens differ.  bf16 queries become f16 after an exact power-of-two scaling
-// of each head's row (its largest element to 2^13), undone in the logits; only
-// elements below 2^-37 of the row's largest lose bits.
+// so the codes go to the tensor cores as they are and the scales meet fp32
+// values only: the kernels keep y_t = x_t + log2 vs_t, take maxima over y,
+// feed weights w_t = 2^(y_t - m) to the second product with the bare codes, and sum
+// l = sum_t w_t / vs_t in fp32.  Taking maxima over y rather than x keeps the largest
+// weight at 1 however the value scales of the tokens differ.
+// The streaming kernel multiplies 8-bit by 8-bit: q and the weights are sums
+// of 8-bit terms, each its own product, added in fp32 (below).  The prefix kernel
+// widens the codes to f16 (exact), q to f16 after an exact power-of-two scaling of
+// each row, and rounds the weights to f16 (half a step 2^-12).
 #pragma once
 
 #include <math.h>
@@ -199,29 +199,44 @@ __global__ void __launch_bounds__(128)
 
 // ---------------------------------------------------------------------------
 // 8-bit pages on the tensor cores.  As in the 16-bit tiles tokens (S^T = K Q^T)
-// and head dims (O^T = V^T P^T) are the M side of m16n8k16 and the G query
-// heads its N side; what differs is which element an operand register holds, since one
-// 8x8 ldmatrix of 16-bit cells covers 16 codes a row:
-//   K: a cell pair of lane (r, q) holds the codes d = 16j + 4q + {0..3} of
-//      token r; in the order 0, 2, 1, 3 they are k = {2q, 2q+1, 2q+8, 2q+9} of
-//      the j-th k-step, and the query fragments are loaded in that order
-//   V: a transposed cell pair holds d = 16j + 2r + {0, 1} of tokens 2q, 2q+1;
-//      rows r and r + 8 of the j-th m-tile are the dims 16j + 2r and 16j + 2r + 1
-// One 16-token page of a head is 8 ldmatrix.x4, 64 code pairs to f16 and
-// 16 mma.sync.
+// and head dims (O^T = V^T P^T) are the M side and the G query heads the N side,
+// but the tiles are m16n8k32 of 8-bit operands, so that codes need no widening
+// (which was two thirds of the instructions: 64 sequences int8 121 us with codes
+// widened to f16).  The other operand is split into 8-bit terms:
+//   q   int8: the row scaled by a power of two to [2^22, 2^23), rounded to an
+//       integer, its three bytes (the top one signed): off by 2^-23 of the row's largest
+//       e4m3: t0 = e4m3(q), t1 = e4m3(16 (q - t0)), t2 = e4m3(256 (q - t0 - t1 / 16))
+//       with the row scaled to [2^7, 2^8): all bits of bf16 and fp16 down to 2^-25 of the row's largest
+//   w   relative to the largest of its 32 tokens (so that a long flat tail
+//       behind one large weight keeps its bits); int8: 16-bit integers, two unsigned bytes: off
+//       by 2^-17 of that largest; e4m3: three terms of four bits, 2^-13 of the weight or 2^-18 of that largest
+// K comes by ldmatrix (lane (r, q) holds codes 4q.. of token r), V by the
+// byte-transposing ldmatrix (codes of four tokens of dim r), whose row order makes
+// a lane's four tokens {2q, 2q + 1, 8 + 2q, 9 + 2q}: those a movmatrix of the weights delivers.
 // ---------------------------------------------------------------------------
-// Power-of-two factors that take a row with this largest magnitude to [2^13,
-// 2^14) and back; zero and non-finite rows stay.
+// Power-of-two factors that take a row with this largest magnitude to [2^X,
+// 2^(X + 1)) and back; zero and non-finite rows stay.
+template <int X>
 __device__ __forceinline__ void pow2_scale(float amax, float& up, float& down) {
   int e = (int)(__float_as_uint(amax) >> 23) - 127;
-  e = (amax == 0.f || e > 127) ? 13 : (e < -100 ? -100 : e);
-  up = __uint_as_float((uint32_t)(13 - e + 127) << 23);
-  down = __uint_as_float((uint32_t)(e - 13 + 127) << 23);
+  e = (amax == 0.f || e > 127) ? X : (e < -100 ? -100 : e);
+  up = __uint_as_float((uint32_t)(X - e + 127) << 23);
+  down = __uint_as_float((uint32_t)(e - X + 127) << 23);
 }
 
-template <typename T, int G>
-__device__ __forceinline__ void load_q_frags8(const T* __restrict__ qrow0, int lane, float qscale,
-                                              uint32_t (&qb)[8][2], float& slA, float& slB) {
+// Four values as bytes of an e4m3 word.
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+  return lo | (hi << 16);
+}
+
+// The terms of this warp's query rows as B fragments: qt[t][2j + h] holds
+// dims 32j + 16h + 4q + {0..3} of head r (zero for r >= G); slA, slB: logit factors of heads 2q, 2q + 1.
+constexpr int kQTerms = 3;
+template <typename T, typename KV, int G>
+__device__ __forceinline__ void load_q_terms(const T* __restrict__ qrow0, int lane, float qscale,
+                                             uint32_t (&qt)[kQTerms][8], float& slA, float& slB) {
   const int qh = lane >> 2, qc = (lane & 3) * 4;
   const T* qr = qrow0 + (qh < G ? qh : 0) * kD;
   float f[8][4];
@@ -239,13 +254,46 @@ __device__ __forceinline__ void load_q_frags8(const T* __restrict__ qrow0, int l
   amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
   amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
   float up, down;
-  pow2_scale(amax, up, down);
+  if constexpr (std::is_same<KV, int8_t>::value) {
+    pow2_scale<22>(amax, up, down);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    qb[j][0] = pack_pair<__half>(f[j][0] * up, f[j][2] * up);
-    qb[j][1] = pack_pair<__half>(f[j][1] * up, f[j][3] * up);
+    for (int j = 0; j < 8; ++j) {
+      uint32_t v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = (uint32_t)__float2int_rn(f[j][i] * up);
+#pragma unroll
+      for (int t = 0; t < kQTerms; ++t) {  // t = 0: the top (signed) byte
+        const int sel = 2 - t;
+        const uint32_t lo = __byte_perm(v[0], v[1], sel | ((4 + sel) << 4));
+        const uint32_t hi = __byte_perm(v[2], v[3], sel | ((4 + sel) << 4));
+        qt[t][j] = __byte_perm(lo, hi, 0x5410);
+      }
+    }
+  } else {
+    pow2_scale<7>(amax, up, down);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float r[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r[i] = f[j][i] * up;
+#pragma unroll
+      for (int t = 0; t < kQTerms; ++t) {
+        qt[t][j] = e4m3x4(r[0], r[1], r[2], r[3]);
+        float b[4];
+        kv8_to_f32x4<e4m3_t>(qt[t][j], b);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = (r[i] - b[i]) * 16.0f;
+      }
+    }
   }
-  const float sl = qscale * down;
+  // a row with an infinity or a NaN has no such terms: its logits are NaN
+  bool bad = false;
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bad |= !(fabsf(f[j][i]) < INFINITY);
+  const unsigned any = __ballot_sync(0xffffffffu, bad);
+  const float sl = any & (0xfu << (lane & ~3)) ? __uint_as_float(0x7fc00000u) : qscale * down;
   slA = __shfl_sync(0xffffffffu, sl, (lane & 3) * 8);
   slB = __shfl_sync(0xffffffffu, sl, (lane & 3) * 8 + 4);
 }
@@ -282,90 +330,165 @@ __device__ __forceinline__ void raise_max_lazy(const float (&top)[2], float (&mu
 
 // Two chunks of sixteen tokens (nt[c] of them live) of one kv head: codes as
 // [head][token][128] rows, 128-byte swizzled, scales as [head][token], chunk c
-// at at + c * chunk_bytes.  Two at once, so that one's chain of ldmatrix,
-// products, exp2 and products runs under the other's.
-// row_at: the lane's ldmatrix row with its first 16 bytes (16 bytes 2j + k of the
-// row are 32 j on, in the swizzle an exclusive or); scale_at: its token's key scale.
+// at at + c * chunk_bytes.  k_at: the lane's ldmatrix row of K with its first
+// 16 bytes (16 bytes 2j + k of the row are 32 j on, in the swizzle an exclusive
+// or); v_at: its row of V, from at; scale_at: its token's key scale.
 template <typename KV>
-__device__ __forceinline__ void mma_chunks8(uint32_t at, uint32_t chunk_bytes, uint32_t box, uint32_t row_at,
-                                            uint32_t scale_at, const int (&nt)[2], int lane, float slA, float slB,
-                                            const uint32_t (&qb)[8][2], float (&o)[8][4], float (&mu)[2],
-                                            float (&lp)[2]) {
-  const int tr = lane >> 2, tq = (lane & 3) * 2;
+__device__ __forceinline__ void mma_chunks8(uint32_t at, uint32_t chunk_bytes, uint32_t k_at, uint32_t v_at,
+                                            uint32_t scale_at, uint32_t v_rows, const int (&nt)[2], int lane,
+                                            float slA, float slB, const uint32_t (&qt)[kQTerms][8], float (&o)[8][4],
+                                            float (&mu)[2], float (&lp)[2]) {
+  constexpr bool kInt = std::is_same<KV, int8_t>::value;
+  constexpr float kBase = kInt ? 256.0f : 1.0f / 16.0f;  // a term's weight against the next (int8) or the last (e4m3)
+  const int tr = lane >> 2;
   float y[2][4], iv[2][2];
-  uint32_t vr[2][4][4];
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
-    const uint32_t ka = at + c * chunk_bytes + row_at, sa = at + c * chunk_bytes + scale_at;
-    float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
-    uint32_t kr[4][4];
+    const uint32_t ka = at + c * chunk_bytes + k_at, sa = at + c * chunk_bytes + scale_at;
+    typename Acc8<KV>::word s[kQTerms][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) ldsm_x4(ka ^ (j << 5), kr[j][0], kr[j][1], kr[j][2], kr[j][3]);
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      ldsm_x4_t((ka + box) ^ (j << 5), vr[c][j][0], vr[c][j][1], vr[c][j][2], vr[c][j][3]);
+    for (int j = 0; j < 4; ++j) {
+      uint32_t kr[4];
+      ldsm_x4(ka ^ (j << 5), kr[0], kr[1], kr[2], kr[3]);
+      if (j == 0) {
+        mma8_start<false>(s[0], kr, qt[0][0], qt[0][1], Acc8<KV>::start());
+        mma8_start<true>(s[1], kr, qt[1][0], qt[1][1], Acc8<KV>::start());
+        mma8_start<true>(s[2], kr, qt[2][0], qt[2][1], Acc8<KV>::start());
+      } else {
+        mma8_add<false>(s[0], kr, qt[0][2 * j], qt[0][2 * j + 1]);
+        mma8_add<true>(s[1], kr, qt[1][2 * j], qt[1][2 * j + 1]);
+        mma8_add<true>(s[2], kr, qt[2][2 * j], qt[2][2 * j + 1]);
+      }
+    }
     const float k0 = lds_f32(sa), k1 = lds_f32(sa + 32);
     float lv0, lv1;
     kv8_value_scale(lds_f32(sa + 512), lv0, iv[c][0]);
     kv8_value_scale(lds_f32(sa + 544), lv1, iv[c][1]);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint32_t a[4], b[4];
-      kv8_pairs<KV>(kr[j][0], a[0], a[2]);
-      kv8_pairs<KV>(kr[j][1], a[1], a[3]);
-      kv8_pairs<KV>(kr[j][2], b[0], b[2]);
-      kv8_pairs<KV>(kr[j][3], b[1], b[3]);
-      mma16816<__half>(s0, a[0], a[1], a[2], a[3], qb[2 * j][0], qb[2 * j][1]);
-      mma16816<__half>(s1, b[0], b[1], b[2], b[3], qb[2 * j + 1][0], qb[2 * j + 1][1]);
-    }
     // y[0]/y[1]: token tr of heads 2(lane%4), +1; y[2]/y[3]: token tr + 8
-    y[c][0] = fmaf(s0[0] + s1[0], k0 * slA, lv0);
-    y[c][1] = fmaf(s0[1] + s1[1], k0 * slB, lv0);
-    y[c][2] = fmaf(s0[2] + s1[2], k1 * slA, lv1);
-    y[c][3] = fmaf(s0[3] + s1[3], k1 * slB, lv1);
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+      float a0, a1, m0, m1, b0, b1;
+      Acc8<KV>::values(s[0][i], s[0][i + 1], a0, a1);
+      Acc8<KV>::values(s[1][i], s[1][i + 1], m0, m1);
+      Acc8<KV>::values(s[2][i], s[2][i + 1], b0, b1);
+      if constexpr (kInt) {
+        sm100::ffma2(m0, m1, a0, a1, kBase, kBase, m0, m1);
+        sm100::ffma2(a0, a1, m0, m1, kBase, kBase, b0, b1);
+      } else {
+        sm100::ffma2(m0, m1, b0, b1, kBase, kBase, m0, m1);
+        sm100::ffma2(a0, a1, m0, m1, kBase, kBase, a0, a1);
+      }
+      const float kt = i ? k1 : k0, lv = i ? lv1 : lv0;
+      sm100::ffma2(y[c][i], y[c][i + 1], a0, a1, kt * slA, kt * slB, lv, lv);
+    }
     if (nt[c] < 16) {
-      // tokens past the end may hold any code (e4m3 has a NaN) and any scale: no
-      // weight, and V zero.  A V register holds two codes of token tq and two of tq + 1.
+      // tokens past the end may hold any code and any scale: no weight, and no V
+      // (an e4m3 NaN times a weight of 0 is NaN: their rows are zeroed)
       if (tr >= nt[c]) y[c][0] = y[c][1] = -INFINITY, iv[c][0] = 0.f;
       if (tr + 8 >= nt[c]) y[c][2] = y[c][3] = -INFINITY, iv[c][1] = 0.f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        vr[c][j][0] = mask_pair(vr[c][j][0], tq, nt[c]);
-        vr[c][j][1] = mask_pair(vr[c][j][1], 8 + tq, nt[c]);
-        vr[c][j][2] = mask_pair(vr[c][j][2], tq, nt[c]);
-        vr[c][j][3] = mask_pair(vr[c][j][3], 8 + tq, nt[c]);
+      if (!kInt) {
+        for (int i = nt[c] * 8 + lane; i < 128; i += 32)
+          sts128(at + c * chunk_bytes + v_rows + i * 16, make_uint4(0, 0, 0, 0));
+        sm100::fence_proxy_async_smem();  // (before the entry's next filling)
+        __syncwarp();
       }
     }
   }
-  const float top[2] = {fmaxf(sm100::fmax3(y[0][0], y[0][2], y[1][0]), y[1][2]),
-                        fmaxf(sm100::fmax3(y[0][1], y[0][3], y[1][1]), y[1][3])};
-  raise_max_lazy(top, mu, lp, o);
-  uint32_t pb[2][2];
+  // the pair's largest y of the two heads, over the eight lanes that hold its tokens
+  float m[2] = {fmaxf(sm100::fmax3(y[0][0], y[0][2], y[1][0]), y[1][2]),
+                fmaxf(sm100::fmax3(y[0][1], y[0][3], y[1][1]), y[1][3])};
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    const float p0 = ex2(y[c][0] - mu[0]), p2 = ex2(y[c][2] - mu[0]);
-    const float p1 = ex2(y[c][1] - mu[1]), p3 = ex2(y[c][3] - mu[1]);
-    lp[0] = fmaf(p0, iv[c][0], fmaf(p2, iv[c][1], lp[0]));
-    lp[1] = fmaf(p1, iv[c][0], fmaf(p3, iv[c][1], lp[1]));
-    pb[c][0] = movm_t(pack_pair<__half>(p0, p1));
-    pb[c][1] = movm_t(pack_pair<__half>(p2, p3));
+  for (int off = 4; off <= 16; off <<= 1) {
+    m[0] = fmaxf(m[0], __shfl_xor_sync(0xffffffffu, m[0], off));
+    m[1] = fmaxf(m[1], __shfl_xor_sync(0xffffffffu, m[1], off));
   }
+  m[0] = fmaxf(m[0], kNoMax), m[1] = fmaxf(m[1], kNoMax);
+  // running maxima: raised when exceeded by more than 2^8 (exact: O and l share the offset)
+  if (__any_sync(0xffffffffu, m[0] - mu[0] > 8.0f || m[1] - mu[1] > 8.0f)) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      if (!(m[c] > mu[c])) continue;
+      const float alpha = ex2(mu[c] - m[c]);
+      mu[c] = m[c];
+      lp[c] *= alpha;
+#pragma unroll
+      for (int mt = 0; mt < 8; ++mt) {
+        o[mt][c] *= alpha;
+        o[mt][c + 2] *= alpha;
+      }
+    }
+  }
+  const float f[2] = {ex2(m[0] - mu[0]), ex2(m[1] - mu[1])};
+  // weights relative to the pair's largest, as B fragments: pb[t][c]
+  constexpr int kPTerms = kInt ? 2 : 3;
+  uint32_t pb[kPTerms][2];
+  float sum[2] = {0.f, 0.f};
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
+    float w[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int i = 0; i < 4; ++i) {
+      w[i] = ex2(y[c][i] - m[i & 1]);
+      sum[i & 1] = fmaf(w[i], iv[c][i >> 1], sum[i & 1]);
+    }
+    if constexpr (kInt) {
+      // 16-bit integers by 2^23 + 65535 w; a 16-bit cell of the transposed matrix is one weight
+      uint32_t u[4];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        uint32_t a[4];
-        kv8_pairs<KV>(vr[c][j][2 * u], a[0], a[1]);
-        kv8_pairs<KV>(vr[c][j][2 * u + 1], a[2], a[3]);
-        mma16816<__half>(o[2 * j + u], a[0], a[1], a[2], a[3], pb[c][0], pb[c][1]);
+      for (int i = 0; i < 4; ++i) u[i] = __float_as_uint(fmaf(w[i], 65535.0f, 8388608.0f));
+      const uint32_t t0 = movm_t(__byte_perm(u[0], u[1], 0x5410)), t1 = movm_t(__byte_perm(u[2], u[3], 0x5410));
+      pb[0][c] = __byte_perm(t0, t1, 0x7531);
+      pb[1][c] = __byte_perm(t0, t1, 0x6420);
+    } else {
+      // terms of four bits by truncation, the last one rounded; a cell is a term
+      // of tokens tr and tr + 8
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] *= 256.0f;
+#pragma unroll
+      for (int t = 0; t < kPTerms; ++t) {
+        float e[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          e[i] = t + 1 < kPTerms ? __uint_as_float(__float_as_uint(w[i]) & 0xfff00000u) : w[i];
+          w[i] -= e[i];
+        }
+        const uint32_t cell = movm_t(e4m3x4(e[0], e[2], e[1], e[3]));
+        pb[t][c] = __byte_perm(cell, 0, 0x3120);
       }
+    }
+  }
+  lp[0] = fmaf(f[0], sum[0], lp[0]);
+  lp[1] = fmaf(f[1], sum[1], lp[1]);
+  constexpr float kUnit = kInt ? 1.0f / 65535.0f : 1.0f / 256.0f;
+  const float fo[2] = {f[0] * kUnit, f[1] * kUnit};
+  const uint32_t va = at + v_at;
+#pragma unroll
+  for (int mt = 0; mt < 8; ++mt) {
+    uint32_t a[4];
+    typename Acc8<KV>::word d[4], e[4];
+    ldsm_x2_t8(va ^ (mt << 4), a);
+    mma8_start<true>(d, a, pb[0][0], pb[0][1], Acc8<KV>::start());
+    if constexpr (kInt) {
+      mma8_start<true>(e, a, pb[1][0], pb[1][1], Acc8<KV>::start());
+    } else {
+      mma8_add<true>(d, a, pb[1][0], pb[1][1]);
+      mma8_add<true>(d, a, pb[2][0], pb[2][1]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+      float x0, x1;
+      Acc8<KV>::values(d[i], d[i + 1], x0, x1);
+      if constexpr (kInt) {
+        float z0, z1;
+        Acc8<KV>::values(e[i], e[i + 1], z0, z1);
+        sm100::ffma2(x0, x1, x0, x1, 256.0f, 256.0f, z0, z1);
+      }
+      sm100::ffma2(o[mt][i], o[mt][i + 1], x0, x1, fo[0], fo[1], o[mt][i], o[mt][i + 1]);
     }
   }
 }
 
-// The same for 16-bit caches: K and V as two boxes of 64 dims each, `box` bytes apart.
+// One chunk of a 16-bit cache: K and V as two boxes of 64 dims each, `box` bytes apart.
 template <typename T>
 __device__ __forceinline__ void mma_chunk16(uint32_t kb, uint32_t vb, uint32_t box, int ntok, int row0,
                                             int lane, float sl, const uint32_t (&qb)[8][2], float (&o)[8][4],
@@ -419,36 +542,21 @@ __device__ __forceinline__ void mma_chunk16(uint32_t kb, uint32_t vb, uint32_t b
   for (int mt = 0; mt < 8; ++mt) mma16816<T>(o[mt], va[mt][0], va[mt][1], va[mt][2], va[mt][3], b0, b1);
 }
 
-// Rows of the 8-bit accumulator (dims 16mt + 2r of o[mt][0..1], 16mt + 2r + 1
-// of o[mt][2..3]), normalised, as 8-byte stores of four dims.
+// store_rows with a NaN sum reaching the output (it has no value for l > 0 to fail).
 template <typename T, int G>
-__device__ __forceinline__ void store_rows8(T* __restrict__ orow0, const float (&o)[8][4], float lA, float lB,
-                                            int lane) {
+__device__ __forceinline__ void store_rows_nan(T* __restrict__ orow0, const float (&o)[8][4], float lA, float lB,
+                                               int lane) {
   const float iA = lA == 0.f ? 0.f : 1.f / lA, iB = lB == 0.f ? 0.f : 1.f / lB;
-  const int h = lane >> 2, c = (lane & 3) * 4;
+  const int h = lane >> 2, tq = (lane & 3) * 2;
   T* orow = orow0 + (h < G ? h : 0) * kD;
 #pragma unroll
   for (int mt = 0; mt < 8; ++mt) {
     const uint32_t r0 = movm_t(pack_pair<T>(o[mt][0] * iA, o[mt][1] * iB));
     const uint32_t r1 = movm_t(pack_pair<T>(o[mt][2] * iA, o[mt][3] * iB));
-    if (h < G)
-      *reinterpret_cast<uint2*>(orow + 16 * mt + c) =
-          make_uint2(__byte_perm(r0, r1, 0x5410), __byte_perm(r0, r1, 0x7632));
-  }
-}
-
-template <int G>
-__device__ __forceinline__ void store_piece8(float* __restrict__ row0, const float (&o)[8][4], const float (&mu)[2],
-                                             float lA, float lB, int lane) {
-  const int hA = (lane & 3) * 2, hB = hA + 1, r = lane >> 2;
-#pragma unroll
-  for (int mt = 0; mt < 8; ++mt) {
-    if (hA < G) *reinterpret_cast<float2*>(row0 + hA * kPiecePitch + 16 * mt + 2 * r) = make_float2(o[mt][0], o[mt][2]);
-    if (hB < G) *reinterpret_cast<float2*>(row0 + hB * kPiecePitch + 16 * mt + 2 * r) = make_float2(o[mt][1], o[mt][3]);
-  }
-  if (r == 0) {
-    if (hA < G) *reinterpret_cast<float2*>(row0 + hA * kPiecePitch + kD) = make_float2(mu[0], lA);
-    if (hB < G) *reinterpret_cast<float2*>(row0 + hB * kPiecePitch + kD) = make_float2(mu[1], lB);
+    if (h < G) {
+      *reinterpret_cast<uint32_t*>(orow + 16 * mt + tq) = r0;
+      *reinterpret_cast<uint32_t*>(orow + 16 * mt + 8 + tq) = r1;
+    }
   }
 }
 
@@ -459,10 +567,7 @@ __device__ __forceinline__ void store_piece8(float* __restrict__ row0, const flo
 // one chunk of sixteen tokens of a page (16-bit caches) or two (8-bit): K and V boxes of
 // HG heads, and for 8-bit caches the tokens' scales.  sub consumer warps share
 // a kv head: entry i goes to the HG warps of slot i % sub, so that eight
-// warps have work whatever Hkv is.  A chunk's chain from ldmatrix over exp2 to the
-// second product is long: 8-bit chunks go through it in pairs (64 sequences,
-// int8: 164 us with one chunk at a time and eight warps, 118 us with sixteen
-// warps of 96 registers, which spill).  End
+// warps have work whatever Hkv is.  End
 // markers, one for each slot, close a segment: the warps of a head add up their (m,
 // l, o) in shared memory, and the first writes the normalised row when the
 // range holds the whole segment, else the range's piece at row segment +
@@ -755,10 +860,15 @@ __global__ void __launch_bounds__((kConsumers + 1) * 32, 1)
     const uint32_t base = sm100::smem_u32(smem), meta_at = sm100::smem_u32(meta);
     const uint32_t xch_at = sm100::smem_u32(xch) + (uint32_t)(w * kXchPitch + lane) * 4;
     const uint32_t box = (uint32_t)(HG * kChunk * 128);
+    const uint32_t chunk_bytes = 2 * box + 1024;
     const int mat = lane >> 3, lrow = w * kChunk + (mat & 1) * 8 + (lane & 7);
-    const uint32_t row_at = lrow * 128 + (((mat >> 1) ^ (lrow & 7)) << 4);
+    const uint32_t k_at = lrow * 128 + (((mat >> 1) ^ (lrow & 7)) << 4);
+    // V: lanes 0-15 the first chunk's tokens in the order 0, 1, 8, 9, 2, 3, 10, 11, ...
+    const int vtok = ((lane >> 2) & 3) * 2 + (lane & 1) + ((lane & 2) << 2), vrow = w * kChunk + vtok;
+    const uint32_t v_rows = box + (uint32_t)(w * kChunk) * 128;
+    const uint32_t v_at = (lane >> 4) * chunk_bytes + box + vrow * 128 + ((vrow & 7) << 4);
     const uint32_t scale_at = 2 * box + (uint32_t)(w * kChunk + (lane >> 2)) * 4;
-    uint32_t qb[8][2];
+    uint32_t qb[8][2], qt[kQTerms][8];
     float o[8][4];
     float mu[2] = {kNoMax, kNoMax}, lp[2] = {0.f, 0.f};
     float slA = p.qscale, slB = p.qscale;
@@ -783,13 +893,13 @@ __global__ void __launch_bounds__((kConsumers + 1) * 32, 1)
           cur = m.seg;
           const int64_t b = m.seg % B, kvh = (int64_t)(m.seg / B) * HG + w;
           const T* qrow = q + (b * p.Hq + kvh * G) * kD;
-          if constexpr (k8) load_q_frags8<T, G>(qrow, lane, p.qscale, qb, slA, slB);
+          if constexpr (k8) load_q_terms<T, KV, G>(qrow, lane, p.qscale, qt, slA, slB);
           else load_q_frags<T, G>(qrow, lane, qb);
         }
         const uint32_t pg = base + st * p.entry_bytes;
         if constexpr (k8) {
           const int nt[2] = {m.ntok, m.piece};
-          mma_chunks8<KV>(pg, 2 * box + 1024, box, row_at, scale_at, nt, lane, slA, slB, qb, o, mu, lp);
+          mma_chunks8<KV>(pg, chunk_bytes, k_at, v_at, scale_at, v_rows, nt, lane, slA, slB, qt, o, mu, lp);
         } else {
           mma_chunk16<T>(pg, pg + 2 * box, box, m.ntok, w * kChunk, lane, p.qscale, qb, o, mu, lp);
         }
@@ -852,12 +962,10 @@ __global__ void __launch_bounds__((kConsumers + 1) * 32, 1)
           const int64_t b = m.seg % B, hg = m.seg / B;
           if (m.piece < 0) {
             T* orow = out + (b * p.Hq + hg * heads_cta + w * G) * kD;
-            if constexpr (k8) store_rows8<T, G>(orow, o, lA, lB, lane);
-            else store_rows<T, G>(orow, o, lA, lB, lane);
+            store_rows_nan<T, G>(orow, o, lA, lB, lane);
           } else {
             float* row0 = ws_rows + ((int64_t)m.piece * heads_cta + w * G) * kPiecePitch;
-            if constexpr (k8) store_piece8<G>(row0, o, mu, lA, lB, lane);
-            else store_partial<G>(row0, kPiecePitch, row0 + kD, kPiecePitch, o, mu, lA, lB, lane);
+            store_partial<G>(row0, kPiecePitch, row0 + kD, kPiecePitch, o, mu, lA, lB, lane);
           }
         }
         mu[0] = mu[1] = kNoMax;

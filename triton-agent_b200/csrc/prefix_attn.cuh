@@ -88,7 +88,7 @@ __device__ __forceinline__ float stage_q_rows(const T* __restrict__ q, int r0, i
       for (int k = 0; k < 8; ++k) amax = fmaxf(amax, fabsf(f[k]));
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-      pow2_scale(amax, up, down);
+      pow2_scale<13>(amax, up, down);
 #pragma unroll
       for (int k = 0; k < 8; ++k) f[k] *= up;
       raw[i] = pack16<__half>(f);
