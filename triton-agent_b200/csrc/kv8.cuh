@@ -35,38 +35,19 @@ __device__ __forceinline__ void kv8_to_f32x4(uint32_t w, float* f) {
   }
 }
 
-// The codes of w as f16 pairs, exactly: bytes 0 and 2, bytes 1 and 3.  int8: a
+// The codes of w as f16 pairs, exactly: bytes 0 and 1, bytes 2 and 3.  int8: a
 // byte with its sign bit flipped, below the exponent of 2^10, is 1024 + 128 +
-// code; one packed subtraction takes the rest off.  (The shift of the odd bytes
-// as a high multiplication, to relieve the integer pipe, was slower: decode of 64
-// sequences 126 -> 144 us.)  e4m3: the hardware conversion, NaN codes included.
-template <typename KV>
-__device__ __forceinline__ void kv8_pairs(uint32_t w, uint32_t& even, uint32_t& odd) {
-  if constexpr (std::is_same<KV, int8_t>::value) {
-    const uint32_t e = (w & 0x00ff00ffu) ^ 0x64806480u;
-    const uint32_t o = __byte_perm(w ^ 0x80808080u, 0x64646464u, 0x4341);
-    const uint32_t off = 0x64806480u;
-    const __half2 de = __hsub2(*reinterpret_cast<const __half2*>(&e), *reinterpret_cast<const __half2*>(&off));
-    const __half2 d1 = __hsub2(*reinterpret_cast<const __half2*>(&o), *reinterpret_cast<const __half2*>(&off));
-    even = *reinterpret_cast<const uint32_t*>(&de);
-    odd = *reinterpret_cast<const uint32_t*>(&d1);
-  } else {
-    const uint32_t p = __byte_perm(w, 0, 0x3120);
-    const __half2_raw e = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(p & 0xffffu), __NV_E4M3);
-    const __half2_raw o = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(p >> 16), __NV_E4M3);
-    even = *reinterpret_cast<const uint32_t*>(&e);
-    odd = *reinterpret_cast<const uint32_t*>(&o);
-  }
-}
-
-// The codes of w in order: bytes 0 and 1, bytes 2 and 3.
+// code; one packed subtraction takes the rest off.  e4m3: the hardware
+// conversion, NaN codes included.
 template <typename KV>
 __device__ __forceinline__ void kv8_in_order(uint32_t w, uint32_t& lo, uint32_t& hi) {
   if constexpr (std::is_same<KV, int8_t>::value) {
-    uint32_t e, o;
-    kv8_pairs<KV>(w, e, o);
-    lo = __byte_perm(e, o, 0x5410);
-    hi = __byte_perm(e, o, 0x7632);
+    const uint32_t u = w ^ 0x80808080u, off = 0x64806480u;
+    const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+    const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&off));
+    const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&b), *reinterpret_cast<const __half2*>(&off));
+    lo = *reinterpret_cast<const uint32_t*>(&x);
+    hi = *reinterpret_cast<const uint32_t*>(&y);
   } else {
     const __half2_raw a = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3);
     const __half2_raw b = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3);
@@ -75,58 +56,32 @@ __device__ __forceinline__ void kv8_in_order(uint32_t w, uint32_t& lo, uint32_t&
   }
 }
 
-// D = A B + C on 16 x 8 x 32 tiles of 8-bit operands: A codes, B a term of the
-// other operand (e4m3; int8 as signed bytes, or unsigned ones).  Accumulators are
-// 32-bit words: fp32 for e4m3, int32 for int8.  The first form starts all of D at
-// one word (no register has to be set first).
-#define B200_MMA8(SHAPE, TYPES, CT, CLIST, ...)                                                               \
-  asm volatile("mma.sync.aligned." SHAPE ".row.col." TYPES " {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, " CLIST ";" \
-               : "=" CT(d[0]), "=" CT(d[1]), "=" CT(d[2]), "=" CT(d[3])                                       \
+// D = A B + C on 16 x 8 x 32 tiles of bytes: A signed codes, B signed or unsigned.
+// The first form starts all of D at one word (no register has to be set first).
+#define B200_MMA8(TYPES, CLIST, ...)                                                                          \
+  asm volatile("mma.sync.aligned.m16n8k32.row.col." TYPES " {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, " CLIST ";" \
+               : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])                                               \
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), __VA_ARGS__)
 template <bool UB>
 __device__ __forceinline__ void mma8_start(int32_t (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, int32_t c) {
-  if constexpr (UB) B200_MMA8("m16n8k32", "s32.s8.u8.s32", "r", "{%10,%10,%10,%10}", "r"(c));
-  else B200_MMA8("m16n8k32", "s32.s8.s8.s32", "r", "{%10,%10,%10,%10}", "r"(c));
+  if constexpr (UB) B200_MMA8("s32.s8.u8.s32", "{%10,%10,%10,%10}", "r"(c));
+  else B200_MMA8("s32.s8.s8.s32", "{%10,%10,%10,%10}", "r"(c));
 }
 template <bool UB>
 __device__ __forceinline__ void mma8_add(int32_t (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   const int32_t c0 = d[0], c1 = d[1], c2 = d[2], c3 = d[3];
-  if constexpr (UB)
-    B200_MMA8("m16n8k32", "s32.s8.u8.s32", "r", "{%10,%11,%12,%13}", "r"(c0), "r"(c1), "r"(c2), "r"(c3));
-  else
-    B200_MMA8("m16n8k32", "s32.s8.s8.s32", "r", "{%10,%11,%12,%13}", "r"(c0), "r"(c1), "r"(c2), "r"(c3));
-}
-template <bool UB>
-__device__ __forceinline__ void mma8_start(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c) {
-  B200_MMA8("m16n8k32", "f32.e4m3.e4m3.f32", "f", "{%10,%10,%10,%10}", "f"(c));
-}
-template <bool UB>
-__device__ __forceinline__ void mma8_add(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  const float c0 = d[0], c1 = d[1], c2 = d[2], c3 = d[3];
-  B200_MMA8("m16n8k32", "f32.e4m3.e4m3.f32", "f", "{%10,%11,%12,%13}", "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+  if constexpr (UB) B200_MMA8("s32.s8.u8.s32", "{%10,%11,%12,%13}", "r"(c0), "r"(c1), "r"(c2), "r"(c3));
+  else B200_MMA8("s32.s8.s8.s32", "{%10,%11,%12,%13}", "r"(c0), "r"(c1), "r"(c2), "r"(c3));
 }
 #undef B200_MMA8
 
-// Accumulators of the codes' products.  int32 sums below 2^22 start at the bit
-// pattern of 1.5 * 2^23, whose low bits they then count: a value is one exact
-// subtraction, without the conversion pipe.
-template <typename KV>
-struct Acc8 {
-  using word = typename std::conditional<std::is_same<KV, int8_t>::value, int32_t, float>::type;
-  static __device__ __forceinline__ word start() {
-    if constexpr (std::is_same<KV, int8_t>::value) return 0x4B400000;
-    else return 0.0f;
-  }
-  // Values of two accumulators.
-  static __device__ __forceinline__ void values(word a, word b, float& x, float& y) {
-    if constexpr (std::is_same<KV, int8_t>::value) {
-      x = -12582912.0f, y = -12582912.0f;
-      sm100::fadd2_acc(x, y, __int_as_float(a), __int_as_float(b));
-    } else {
-      x = a, y = b;
-    }
-  }
-};
+// Sums below 2^22 start at the bit pattern of 1.5 * 2^23, whose low bits they
+// then count: a value is one exact subtraction, without the conversion pipe.
+constexpr int32_t kAccStart = 0x4B400000;
+__device__ __forceinline__ void acc_values(int32_t a, int32_t b, float& x, float& y) {
+  x = -12582912.0f, y = -12582912.0f;
+  sm100::fadd2_acc(x, y, __int_as_float(a), __int_as_float(b));
+}
 
 // Two 16 x 16 byte matrices, transposed: lane (r, q) gets rows 4q..4q+3 of
 // columns r and r + 8 of the first (lanes 0-15 give its row addresses) and of the second.

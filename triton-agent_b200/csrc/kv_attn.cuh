@@ -15,10 +15,10 @@
 // feed weights w_t = 2^(y_t - m) to the second product with the bare codes, and sum
 // l = sum_t w_t / vs_t in fp32.  Taking maxima over y rather than x keeps the largest
 // weight at 1 however the value scales of the tokens differ.
-// The streaming kernel multiplies 8-bit by 8-bit: q and the weights are sums
-// of 8-bit terms, each its own product, added in fp32 (below).  The prefix kernel
-// widens the codes to f16 (exact), q to f16 after an exact power-of-two scaling of
-// each row, and rounds the weights to f16 (half a step 2^-12).
+// The streaming kernel multiplies int8 codes by bytes of the queries and weights.
+// e4m3 codes there, and all codes in the prefix kernel, are widened to f16 (exact),
+// with q in f16 after an exact power-of-two scaling of each row, and the weights
+// rounded to f16 (half a step 2^-12).
 #pragma once
 
 #include <math.h>
@@ -199,20 +199,20 @@ __global__ void __launch_bounds__(128)
 
 // ---------------------------------------------------------------------------
 // 8-bit pages on the tensor cores.  As in the 16-bit tiles tokens (S^T = K Q^T)
-// and head dims (O^T = V^T P^T) are the M side and the G query heads the N side,
-// but the tiles are m16n8k32 of 8-bit operands, so that codes need no widening
-// (which was two thirds of the instructions: 64 sequences int8 121 us with codes
-// widened to f16).  The other operand is split into 8-bit terms:
-//   q   int8: the row scaled by a power of two to [2^22, 2^23), rounded to an
-//       integer, its three bytes (the top one signed): off by 2^-23 of the row's largest
-//       e4m3: t0 = e4m3(q), t1 = e4m3(16 (q - t0)), t2 = e4m3(256 (q - t0 - t1 / 16))
-//       with the row scaled to [2^7, 2^8): all bits of bf16 and fp16 down to 2^-25 of the row's largest
-//   w   relative to the largest of its 32 tokens (so that a long flat tail
-//       behind one large weight keeps its bits); int8: 16-bit integers, two unsigned bytes: off
-//       by 2^-17 of that largest; e4m3: three terms of four bits, 2^-13 of the weight or 2^-18 of that largest
+// and head dims (O^T = V^T P^T) are the M side and the G query heads the N side.
 // K comes by ldmatrix (lane (r, q) holds codes 4q.. of token r), V by the
 // byte-transposing ldmatrix (codes of four tokens of dim r), whose row order makes
 // a lane's four tokens {2q, 2q + 1, 8 + 2q, 9 + 2q}: those a movmatrix of the weights delivers.
+// int8: m16n8k32 tiles of bytes, so that codes need no widening (which was half
+// of the instructions: 64 sequences 121 us with codes widened to f16, 114 us
+// so).  The other operand is a sum of byte terms, a product each:
+//   q   the row scaled by a power of two to [2^22, 2^23) and rounded to an integer,
+//       its three bytes (the top one signed): off by 2^-23 of the row's largest
+//   w   relative to the largest of its 32 tokens (so that a long flat tail behind
+//       one large weight keeps its bits), as a 16-bit integer, two unsigned bytes:
+//       off by 2^-17 of that largest
+// e4m3: widened to f16, m16n8k16 tiles (the m16n8k32 tiles of e4m3 are no
+// hardware form here: ten instructions each); w in f16.
 // ---------------------------------------------------------------------------
 // Power-of-two factors that take a row with this largest magnitude to [2^X,
 // 2^(X + 1)) and back; zero and non-finite rows stay.
@@ -224,31 +224,28 @@ __device__ __forceinline__ void pow2_scale(float amax, float& up, float& down) {
   down = __uint_as_float((uint32_t)(e - X + 127) << 23);
 }
 
-// Four values as bytes of an e4m3 word.
-__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
-  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
-  return lo | (hi << 16);
-}
-
-// The terms of this warp's query rows as B fragments: qt[t][2j + h] holds
-// dims 32j + 16h + 4q + {0..3} of head r (zero for r >= G); slA, slB: logit factors of heads 2q, 2q + 1.
-constexpr int kQTerms = 3;
+// This warp's query rows as B fragments; slA, slB: logit factors of heads 2q, 2q + 1.
+// int8: qf[8t + i], t = 0 the top byte, holds dims 16i + 4q + {0..3} of head r
+// (zero for r >= G).  e4m3: qf[2i + {0, 1}] those dims in f16.
+template <typename KV>
+constexpr int q_words() { return std::is_same<KV, int8_t>::value ? 24 : 16; }
 template <typename T, typename KV, int G>
-__device__ __forceinline__ void load_q_terms(const T* __restrict__ qrow0, int lane, float qscale,
-                                             uint32_t (&qt)[kQTerms][8], float& slA, float& slB) {
+__device__ __forceinline__ void load_q_frags8(const T* __restrict__ qrow0, int lane, float qscale,
+                                              uint32_t (&qf)[q_words<KV>()], float& slA, float& slB) {
   const int qh = lane >> 2, qc = (lane & 3) * 4;
   const T* qr = qrow0 + (qh < G ? qh : 0) * kD;
   float f[8][4];
   float amax = 0.f;
+  bool bad = false;  // an infinity or a NaN: the row's logits are NaN
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint2 raw = *reinterpret_cast<const uint2*>(qr + 16 * j + qc);
+  for (int i = 0; i < 8; ++i) {
+    const uint2 raw = *reinterpret_cast<const uint2*>(qr + 16 * i + qc);
     const T* e = reinterpret_cast<const T*>(&raw);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f[j][i] = qh < G ? to_f32(e[i]) : 0.f;
-      amax = fmaxf(amax, fabsf(f[j][i]));
+    for (int u = 0; u < 4; ++u) {
+      f[i][u] = qh < G ? to_f32(e[u]) : 0.f;
+      amax = fmaxf(amax, fabsf(f[i][u]));
+      bad |= !(fabsf(f[i][u]) < INFINITY);
     }
   }
   amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
@@ -257,41 +254,26 @@ __device__ __forceinline__ void load_q_terms(const T* __restrict__ qrow0, int la
   if constexpr (std::is_same<KV, int8_t>::value) {
     pow2_scale<22>(amax, up, down);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int i = 0; i < 8; ++i) {
       uint32_t v[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = (uint32_t)__float2int_rn(f[j][i] * up);
+      for (int u = 0; u < 4; ++u) v[u] = (uint32_t)__float2int_rn(f[i][u] * up);
 #pragma unroll
-      for (int t = 0; t < kQTerms; ++t) {  // t = 0: the top (signed) byte
+      for (int t = 0; t < 3; ++t) {
         const int sel = 2 - t;
         const uint32_t lo = __byte_perm(v[0], v[1], sel | ((4 + sel) << 4));
         const uint32_t hi = __byte_perm(v[2], v[3], sel | ((4 + sel) << 4));
-        qt[t][j] = __byte_perm(lo, hi, 0x5410);
+        qf[8 * t + i] = __byte_perm(lo, hi, 0x5410);
       }
     }
   } else {
-    pow2_scale<7>(amax, up, down);
+    pow2_scale<13>(amax, up, down);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      float r[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) r[i] = f[j][i] * up;
-#pragma unroll
-      for (int t = 0; t < kQTerms; ++t) {
-        qt[t][j] = e4m3x4(r[0], r[1], r[2], r[3]);
-        float b[4];
-        kv8_to_f32x4<e4m3_t>(qt[t][j], b);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) r[i] = (r[i] - b[i]) * 16.0f;
-      }
+    for (int i = 0; i < 8; ++i) {
+      qf[2 * i] = pack_pair<__half>(f[i][0] * up, f[i][1] * up);
+      qf[2 * i + 1] = pack_pair<__half>(f[i][2] * up, f[i][3] * up);
     }
   }
-  // a row with an infinity or a NaN has no such terms: its logits are NaN
-  bool bad = false;
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) bad |= !(fabsf(f[j][i]) < INFINITY);
   const unsigned any = __ballot_sync(0xffffffffu, bad);
   const float sl = any & (0xfu << (lane & ~3)) ? __uint_as_float(0x7fc00000u) : qscale * down;
   slA = __shfl_sync(0xffffffffu, sl, (lane & 3) * 8);
@@ -302,18 +284,8 @@ __device__ __forceinline__ void load_q_terms(const T* __restrict__ qrow0, int la
 // and nothing scaled by it survives, and finite, so that differences are.
 constexpr float kNoMax = -1e30f;
 
-// Raises the running maxima of this thread's two heads to the largest logits
-// in the warp (of this thread: top), when one exceeds its maximum by more than
-// 2^8 (exact: O and l share the offset).  Most entries need one vote here and no exchange.
-__device__ __forceinline__ void raise_max_lazy(const float (&top)[2], float (&mu)[2], float (&lp)[2],
-                                               float (&o)[8][4]) {
-  float m[2] = {top[0], top[1]};
-  if (!__any_sync(0xffffffffu, m[0] - mu[0] > 8.0f || m[1] - mu[1] > 8.0f)) return;
-#pragma unroll
-  for (int off = 4; off <= 16; off <<= 1) {
-    m[0] = fmaxf(m[0], __shfl_xor_sync(0xffffffffu, m[0], off));
-    m[1] = fmaxf(m[1], __shfl_xor_sync(0xffffffffu, m[1], off));
-  }
+// Raises the running maxima of this thread's two heads to m where that is larger.
+__device__ __forceinline__ void raise_to(const float (&m)[2], float (&mu)[2], float (&lp)[2], float (&o)[8][4]) {
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     if (!(m[c] > mu[c])) continue;
@@ -328,59 +300,99 @@ __device__ __forceinline__ void raise_max_lazy(const float (&top)[2], float (&mu
   }
 }
 
-// Two chunks of sixteen tokens (nt[c] of them live) of one kv head: codes as
-// [head][token][128] rows, 128-byte swizzled, scales as [head][token], chunk c
-// at at + c * chunk_bytes.  k_at: the lane's ldmatrix row of K with its first
+// The same to the largest logits in the warp (of this thread: top), when one
+// exceeds its maximum by more than 2^8 (exact: O and l share the offset).  Most
+// entries need one vote here and no exchange.
+__device__ __forceinline__ void raise_max_lazy(const float (&top)[2], float (&mu)[2], float (&lp)[2],
+                                               float (&o)[8][4]) {
+  float m[2] = {top[0], top[1]};
+  if (!__any_sync(0xffffffffu, m[0] - mu[0] > 8.0f || m[1] - mu[1] > 8.0f)) return;
+#pragma unroll
+  for (int off = 4; off <= 16; off <<= 1) {
+    m[0] = fmaxf(m[0], __shfl_xor_sync(0xffffffffu, m[0], off));
+    m[1] = fmaxf(m[1], __shfl_xor_sync(0xffffffffu, m[1], off));
+  }
+  raise_to(m, mu, lp, o);
+}
+
+// Where a lane reads an entry's two chunks: its ldmatrix row of K with its first
 // 16 bytes (16 bytes 2j + k of the row are 32 j on, in the swizzle an exclusive
-// or); v_at: its row of V, from at; scale_at: its token's key scale.
+// or), its row of V, its token's key scale, the head's rows of V; bytes of a chunk.
+struct Lane8 {
+  uint32_t k_at, v_at, scale_at, v_rows, chunk;
+  __device__ __forceinline__ Lane8(int w, uint32_t box, int lane) {
+    chunk = 2 * box + 1024;
+    const int mat = lane >> 3, krow = w * 16 + (mat & 1) * 8 + (lane & 7);
+    k_at = krow * 128 + (((mat >> 1) ^ (krow & 7)) << 4);
+    // V: lanes 0-15 the first chunk's tokens in the order 0, 1, 8, 9, 2, 3, 10, 11, ...
+    const int vrow = w * 16 + ((lane >> 2) & 3) * 2 + (lane & 1) + ((lane & 2) << 2);
+    v_at = (lane >> 4) * chunk + box + vrow * 128 + ((vrow & 7) << 4);
+    v_rows = box + (uint32_t)(w * 16) * 128;
+    scale_at = 2 * box + (uint32_t)(w * 16 + (lane >> 2)) * 4;
+  }
+};
+
+// Two chunks of sixteen tokens (nt[c] of them live) of one kv head, folded into
+// the running (o, mu, lp): codes as [head][token][128] rows, 128-byte
+// swizzled, scales as [head][token], the entry at `at`.
 template <typename KV>
-__device__ __forceinline__ void mma_chunks8(uint32_t at, uint32_t chunk_bytes, uint32_t k_at, uint32_t v_at,
-                                            uint32_t scale_at, uint32_t v_rows, const int (&nt)[2], int lane,
-                                            float slA, float slB, const uint32_t (&qt)[kQTerms][8], float (&o)[8][4],
-                                            float (&mu)[2], float (&lp)[2]) {
+__device__ __forceinline__ void mma_pair8(uint32_t at, const Lane8& x, const int (&nt)[2], int lane, float slA,
+                                          float slB, const uint32_t (&qf)[q_words<KV>()], float (&o)[8][4],
+                                          float (&mu)[2], float (&lp)[2]) {
   constexpr bool kInt = std::is_same<KV, int8_t>::value;
-  constexpr float kBase = kInt ? 256.0f : 1.0f / 16.0f;  // a term's weight against the next (int8) or the last (e4m3)
   const int tr = lane >> 2;
   float y[2][4], iv[2][2];
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
-    const uint32_t ka = at + c * chunk_bytes + k_at, sa = at + c * chunk_bytes + scale_at;
-    typename Acc8<KV>::word s[kQTerms][4];
+    const uint32_t ka = at + c * x.chunk + x.k_at, sa = at + c * x.chunk + x.scale_at;
+    // products of tokens tr and tr + 8 with heads 2(lane%4), +1
+    float s[4];
+    if constexpr (kInt) {
+      int32_t d[3][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint32_t kr[4];
-      ldsm_x4(ka ^ (j << 5), kr[0], kr[1], kr[2], kr[3]);
-      if (j == 0) {
-        mma8_start<false>(s[0], kr, qt[0][0], qt[0][1], Acc8<KV>::start());
-        mma8_start<true>(s[1], kr, qt[1][0], qt[1][1], Acc8<KV>::start());
-        mma8_start<true>(s[2], kr, qt[2][0], qt[2][1], Acc8<KV>::start());
-      } else {
-        mma8_add<false>(s[0], kr, qt[0][2 * j], qt[0][2 * j + 1]);
-        mma8_add<true>(s[1], kr, qt[1][2 * j], qt[1][2 * j + 1]);
-        mma8_add<true>(s[2], kr, qt[2][2 * j], qt[2][2 * j + 1]);
+      for (int j = 0; j < 4; ++j) {
+        uint32_t kr[4];
+        ldsm_x4(ka ^ (j << 5), kr[0], kr[1], kr[2], kr[3]);
+        if (j == 0) {
+          mma8_start<false>(d[0], kr, qf[0], qf[1], kAccStart);
+          mma8_start<true>(d[1], kr, qf[8], qf[9], kAccStart);
+          mma8_start<true>(d[2], kr, qf[16], qf[17], kAccStart);
+        } else {
+          mma8_add<false>(d[0], kr, qf[2 * j], qf[2 * j + 1]);
+          mma8_add<true>(d[1], kr, qf[8 + 2 * j], qf[9 + 2 * j]);
+          mma8_add<true>(d[2], kr, qf[16 + 2 * j], qf[17 + 2 * j]);
+        }
       }
+#pragma unroll
+      for (int i = 0; i < 4; i += 2) {
+        float m0, m1, b0, b1;
+        acc_values(d[0][i], d[0][i + 1], s[i], s[i + 1]);
+        acc_values(d[1][i], d[1][i + 1], m0, m1);
+        acc_values(d[2][i], d[2][i + 1], b0, b1);
+        sm100::ffma2(m0, m1, s[i], s[i + 1], 256.0f, 256.0f, m0, m1);
+        sm100::ffma2(s[i], s[i + 1], m0, m1, 256.0f, 256.0f, b0, b1);
+      }
+    } else {
+      float s1[4] = {0.f, 0.f, 0.f, 0.f};
+      s[0] = s[1] = s[2] = s[3] = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t kr[4], a[4][2];
+        ldsm_x4(ka ^ (j << 5), kr[0], kr[1], kr[2], kr[3]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) kv8_in_order<KV>(kr[i], a[i][0], a[i][1]);
+        mma16816<__half>(s, a[0][0], a[1][0], a[0][1], a[1][1], qf[4 * j], qf[4 * j + 1]);
+        mma16816<__half>(s1, a[2][0], a[3][0], a[2][1], a[3][1], qf[4 * j + 2], qf[4 * j + 3]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[i] += s1[i];
     }
     const float k0 = lds_f32(sa), k1 = lds_f32(sa + 32);
     float lv0, lv1;
     kv8_value_scale(lds_f32(sa + 512), lv0, iv[c][0]);
     kv8_value_scale(lds_f32(sa + 544), lv1, iv[c][1]);
-    // y[0]/y[1]: token tr of heads 2(lane%4), +1; y[2]/y[3]: token tr + 8
-#pragma unroll
-    for (int i = 0; i < 4; i += 2) {
-      float a0, a1, m0, m1, b0, b1;
-      Acc8<KV>::values(s[0][i], s[0][i + 1], a0, a1);
-      Acc8<KV>::values(s[1][i], s[1][i + 1], m0, m1);
-      Acc8<KV>::values(s[2][i], s[2][i + 1], b0, b1);
-      if constexpr (kInt) {
-        sm100::ffma2(m0, m1, a0, a1, kBase, kBase, m0, m1);
-        sm100::ffma2(a0, a1, m0, m1, kBase, kBase, b0, b1);
-      } else {
-        sm100::ffma2(m0, m1, b0, b1, kBase, kBase, m0, m1);
-        sm100::ffma2(a0, a1, m0, m1, kBase, kBase, a0, a1);
-      }
-      const float kt = i ? k1 : k0, lv = i ? lv1 : lv0;
-      sm100::ffma2(y[c][i], y[c][i + 1], a0, a1, kt * slA, kt * slB, lv, lv);
-    }
+    sm100::ffma2(y[c][0], y[c][1], s[0], s[1], k0 * slA, k0 * slB, lv0, lv0);
+    sm100::ffma2(y[c][2], y[c][3], s[2], s[3], k1 * slA, k1 * slB, lv1, lv1);
     if (nt[c] < 16) {
       // tokens past the end may hold any code and any scale: no weight, and no V
       // (an e4m3 NaN times a weight of 0 is NaN: their rows are zeroed)
@@ -388,102 +400,81 @@ __device__ __forceinline__ void mma_chunks8(uint32_t at, uint32_t chunk_bytes, u
       if (tr + 8 >= nt[c]) y[c][2] = y[c][3] = -INFINITY, iv[c][1] = 0.f;
       if (!kInt) {
         for (int i = nt[c] * 8 + lane; i < 128; i += 32)
-          sts128(at + c * chunk_bytes + v_rows + i * 16, make_uint4(0, 0, 0, 0));
+          sts128(at + c * x.chunk + x.v_rows + i * 16, make_uint4(0, 0, 0, 0));
         sm100::fence_proxy_async_smem();  // (before the entry's next filling)
         __syncwarp();
       }
     }
   }
-  // the pair's largest y of the two heads, over the eight lanes that hold its tokens
   float m[2] = {fmaxf(sm100::fmax3(y[0][0], y[0][2], y[1][0]), y[1][2]),
                 fmaxf(sm100::fmax3(y[0][1], y[0][3], y[1][1]), y[1][3])};
+  const uint32_t va = at + x.v_at;
+  if constexpr (kInt) {
+    // the pair's largest y of the two heads, over the eight lanes that hold its tokens
 #pragma unroll
-  for (int off = 4; off <= 16; off <<= 1) {
-    m[0] = fmaxf(m[0], __shfl_xor_sync(0xffffffffu, m[0], off));
-    m[1] = fmaxf(m[1], __shfl_xor_sync(0xffffffffu, m[1], off));
-  }
-  m[0] = fmaxf(m[0], kNoMax), m[1] = fmaxf(m[1], kNoMax);
-  // running maxima: raised when exceeded by more than 2^8 (exact: O and l share the offset)
-  if (__any_sync(0xffffffffu, m[0] - mu[0] > 8.0f || m[1] - mu[1] > 8.0f)) {
+    for (int off = 4; off <= 16; off <<= 1) {
+      m[0] = fmaxf(m[0], __shfl_xor_sync(0xffffffffu, m[0], off));
+      m[1] = fmaxf(m[1], __shfl_xor_sync(0xffffffffu, m[1], off));
+    }
+    m[0] = fmaxf(m[0], kNoMax), m[1] = fmaxf(m[1], kNoMax);
+    if (__any_sync(0xffffffffu, m[0] - mu[0] > 8.0f || m[1] - mu[1] > 8.0f)) raise_to(m, mu, lp, o);
+    const float f[2] = {ex2(m[0] - mu[0]), ex2(m[1] - mu[1])};
+    // weights relative to the pair's largest, as B fragments: pb[t][c], t = 0 the high byte
+    uint32_t pb[2][2];
+    float sum[2] = {0.f, 0.f};
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      if (!(m[c] > mu[c])) continue;
-      const float alpha = ex2(mu[c] - m[c]);
-      mu[c] = m[c];
-      lp[c] *= alpha;
-#pragma unroll
-      for (int mt = 0; mt < 8; ++mt) {
-        o[mt][c] *= alpha;
-        o[mt][c + 2] *= alpha;
-      }
-    }
-  }
-  const float f[2] = {ex2(m[0] - mu[0]), ex2(m[1] - mu[1])};
-  // weights relative to the pair's largest, as B fragments: pb[t][c]
-  constexpr int kPTerms = kInt ? 2 : 3;
-  uint32_t pb[kPTerms][2];
-  float sum[2] = {0.f, 0.f};
-#pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    float w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      w[i] = ex2(y[c][i] - m[i & 1]);
-      sum[i & 1] = fmaf(w[i], iv[c][i >> 1], sum[i & 1]);
-    }
-    if constexpr (kInt) {
       // 16-bit integers by 2^23 + 65535 w; a 16-bit cell of the transposed matrix is one weight
       uint32_t u[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) u[i] = __float_as_uint(fmaf(w[i], 65535.0f, 8388608.0f));
+      for (int i = 0; i < 4; ++i) {
+        const float w = ex2(y[c][i] - m[i & 1]);
+        sum[i & 1] = fmaf(w, iv[c][i >> 1], sum[i & 1]);
+        u[i] = __float_as_uint(fmaf(w, 65535.0f, 8388608.0f));
+      }
       const uint32_t t0 = movm_t(__byte_perm(u[0], u[1], 0x5410)), t1 = movm_t(__byte_perm(u[2], u[3], 0x5410));
       pb[0][c] = __byte_perm(t0, t1, 0x7531);
       pb[1][c] = __byte_perm(t0, t1, 0x6420);
-    } else {
-      // terms of four bits by truncation, the last one rounded; a cell is a term
-      // of tokens tr and tr + 8
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] *= 256.0f;
-#pragma unroll
-      for (int t = 0; t < kPTerms; ++t) {
-        float e[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          e[i] = t + 1 < kPTerms ? __uint_as_float(__float_as_uint(w[i]) & 0xfff00000u) : w[i];
-          w[i] -= e[i];
-        }
-        const uint32_t cell = movm_t(e4m3x4(e[0], e[2], e[1], e[3]));
-        pb[t][c] = __byte_perm(cell, 0, 0x3120);
-      }
     }
-  }
-  lp[0] = fmaf(f[0], sum[0], lp[0]);
-  lp[1] = fmaf(f[1], sum[1], lp[1]);
-  constexpr float kUnit = kInt ? 1.0f / 65535.0f : 1.0f / 256.0f;
-  const float fo[2] = {f[0] * kUnit, f[1] * kUnit};
-  const uint32_t va = at + v_at;
+    lp[0] = fmaf(f[0], sum[0], lp[0]);
+    lp[1] = fmaf(f[1], sum[1], lp[1]);
+    const float fo[2] = {f[0] * (1.0f / 65535.0f), f[1] * (1.0f / 65535.0f)};
 #pragma unroll
-  for (int mt = 0; mt < 8; ++mt) {
-    uint32_t a[4];
-    typename Acc8<KV>::word d[4], e[4];
-    ldsm_x2_t8(va ^ (mt << 4), a);
-    mma8_start<true>(d, a, pb[0][0], pb[0][1], Acc8<KV>::start());
-    if constexpr (kInt) {
-      mma8_start<true>(e, a, pb[1][0], pb[1][1], Acc8<KV>::start());
-    } else {
-      mma8_add<true>(d, a, pb[1][0], pb[1][1]);
-      mma8_add<true>(d, a, pb[2][0], pb[2][1]);
-    }
+    for (int mt = 0; mt < 8; ++mt) {
+      uint32_t a[4];
+      int32_t d[4], e[4];
+      ldsm_x2_t8(va ^ (mt << 4), a);
+      mma8_start<true>(d, a, pb[0][0], pb[0][1], kAccStart);
+      mma8_start<true>(e, a, pb[1][0], pb[1][1], kAccStart);
 #pragma unroll
-    for (int i = 0; i < 4; i += 2) {
-      float x0, x1;
-      Acc8<KV>::values(d[i], d[i + 1], x0, x1);
-      if constexpr (kInt) {
-        float z0, z1;
-        Acc8<KV>::values(e[i], e[i + 1], z0, z1);
+      for (int i = 0; i < 4; i += 2) {
+        float x0, x1, z0, z1;
+        acc_values(d[i], d[i + 1], x0, x1);
+        acc_values(e[i], e[i + 1], z0, z1);
         sm100::ffma2(x0, x1, x0, x1, 256.0f, 256.0f, z0, z1);
+        sm100::ffma2(o[mt][i], o[mt][i + 1], x0, x1, fo[0], fo[1], o[mt][i], o[mt][i + 1]);
       }
-      sm100::ffma2(o[mt][i], o[mt][i + 1], x0, x1, fo[0], fo[1], o[mt][i], o[mt][i + 1]);
+    }
+  } else {
+    raise_max_lazy(m, mu, lp, o);
+    uint32_t pb[2][2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const float p0 = ex2(y[c][0] - mu[0]), p2 = ex2(y[c][2] - mu[0]);
+      const float p1 = ex2(y[c][1] - mu[1]), p3 = ex2(y[c][3] - mu[1]);
+      lp[0] = fmaf(p0, iv[c][0], fmaf(p2, iv[c][1], lp[0]));
+      lp[1] = fmaf(p1, iv[c][0], fmaf(p3, iv[c][1], lp[1]));
+      pb[c][0] = movm_t(pack_pair<__half>(p0, p1));
+      pb[c][1] = movm_t(pack_pair<__half>(p2, p3));
+    }
+#pragma unroll
+    for (int mt = 0; mt < 8; ++mt) {
+      uint32_t v[4], a[4][2];
+      ldsm_x2_t8(va ^ (mt << 4), v);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) kv8_in_order<KV>(v[i], a[i][0], a[i][1]);
+      mma16816<__half>(o[mt], a[0][0], a[1][0], a[0][1], a[1][1], pb[0][0], pb[0][1]);
+      mma16816<__half>(o[mt], a[2][0], a[3][0], a[2][1], a[3][1], pb[1][0], pb[1][1]);
     }
   }
 }
@@ -860,15 +851,8 @@ __global__ void __launch_bounds__((kConsumers + 1) * 32, 1)
     const uint32_t base = sm100::smem_u32(smem), meta_at = sm100::smem_u32(meta);
     const uint32_t xch_at = sm100::smem_u32(xch) + (uint32_t)(w * kXchPitch + lane) * 4;
     const uint32_t box = (uint32_t)(HG * kChunk * 128);
-    const uint32_t chunk_bytes = 2 * box + 1024;
-    const int mat = lane >> 3, lrow = w * kChunk + (mat & 1) * 8 + (lane & 7);
-    const uint32_t k_at = lrow * 128 + (((mat >> 1) ^ (lrow & 7)) << 4);
-    // V: lanes 0-15 the first chunk's tokens in the order 0, 1, 8, 9, 2, 3, 10, 11, ...
-    const int vtok = ((lane >> 2) & 3) * 2 + (lane & 1) + ((lane & 2) << 2), vrow = w * kChunk + vtok;
-    const uint32_t v_rows = box + (uint32_t)(w * kChunk) * 128;
-    const uint32_t v_at = (lane >> 4) * chunk_bytes + box + vrow * 128 + ((vrow & 7) << 4);
-    const uint32_t scale_at = 2 * box + (uint32_t)(w * kChunk + (lane >> 2)) * 4;
-    uint32_t qb[8][2], qt[kQTerms][8];
+    const Lane8 lane8(w, box, lane);
+    uint32_t qb[8][2], qf[q_words<KV>()];
     float o[8][4];
     float mu[2] = {kNoMax, kNoMax}, lp[2] = {0.f, 0.f};
     float slA = p.qscale, slB = p.qscale;
@@ -893,13 +877,13 @@ __global__ void __launch_bounds__((kConsumers + 1) * 32, 1)
           cur = m.seg;
           const int64_t b = m.seg % B, kvh = (int64_t)(m.seg / B) * HG + w;
           const T* qrow = q + (b * p.Hq + kvh * G) * kD;
-          if constexpr (k8) load_q_terms<T, KV, G>(qrow, lane, p.qscale, qt, slA, slB);
+          if constexpr (k8) load_q_frags8<T, KV, G>(qrow, lane, p.qscale, qf, slA, slB);
           else load_q_frags<T, G>(qrow, lane, qb);
         }
         const uint32_t pg = base + st * p.entry_bytes;
         if constexpr (k8) {
           const int nt[2] = {m.ntok, m.piece};
-          mma_chunks8<KV>(pg, chunk_bytes, k_at, v_at, scale_at, v_rows, nt, lane, slA, slB, qt, o, mu, lp);
+          mma_pair8<KV>(pg, lane8, nt, lane, slA, slB, qf, o, mu, lp);
         } else {
           mma_chunk16<T>(pg, pg + 2 * box, box, m.ntok, w * kChunk, lane, p.qscale, qb, o, mu, lp);
         }
