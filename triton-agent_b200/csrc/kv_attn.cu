@@ -156,18 +156,35 @@ PieceGeom piece_geometry(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t 
   return g;
 }
 
-// Splits of the prefix.  A CTA of the prefix kernel is one (split, pair of
-// 128-row tiles, kv head) and holds its SM alone, so the time is about
-// waves * (key tiles a split + the CTA's start and end, about three tiles' time); the
-// fewest splits within the minimum, since each leaves a piece a row to join.
-// The length lives on the device; the table's size bounds it.
-int prefix_splits(const PieceGeom& g, int64_t B, int64_t Hkv, int64_t bs, int64_t max_prefix_blocks) {
+// Splits of the prefix, and the SMs that stream the own pages beside it (g.grid).
+// A CTA of either kernel holds its SM alone.  In units of a prefix key tile's time
+// (2.8 us), a prefix CTA -- (split, pair of 128-row tiles, kv head) -- takes its
+// key tiles + 3 for its start and end; the own pages of 128 tokens of a kv head
+// take 0.27 of an SM, a segment 0.7 more, and the kernel 3 to start and end.
+// Both kernels mostly wait at their starts and ends, so side by side on an SM each
+// is best where it fits (64 sequences, prefix 8192: one after the other on
+// all SMs 56 us, 11 splits beside 60 SMs 44 us, 6 beside 100 59 us, 16 beside 20 70 us).
+// One after the other remains where the prefix alone fills the GPU, or the own
+// pages outweigh it.  Lengths live on the device: the prefix counts with its table's
+// size, the own tokens with half of theirs, and the streaming kernel keeps a
+// sixteenth of the SMs.  Fewest splits within the minimum: each leaves a piece a row to join.
+int share_sms(PieceGeom& g, int64_t Hkv, int64_t bs, int64_t max_prefix_blocks, int64_t max_blocks) {
   const int64_t ppt = 128 / bs, tiles = (max_prefix_blocks + ppt - 1) / ppt;
-  const int64_t units = (B * g.G + 255) / 256 * Hkv;
-  int64_t best = 1, best_cost = INT64_MAX;
-  for (int64_t s = 1; s <= tiles && s <= g.grid; ++s) {
-    const int64_t cost = (units * s + g.grid - 1) / g.grid * ((tiles + s - 1) / s + 3);
-    if (cost < best_cost) best = s, best_cost = cost;
+  const int64_t units = (g.seqs * g.G + 255) / 256 * Hkv;
+  const int sms = g.grid;
+  const double own = 0.27 / 256 * (double)(g.seqs * max_blocks * bs) * (double)Hkv + 0.7 * (double)(g.seqs * g.n_hg);
+  int64_t best = 1;
+  double best_cost = 1e300;
+  for (int64_t s = 1; s <= tiles && s <= sms; ++s) {
+    const double prefix = (double)((units * s + sms - 1) / sms * ((tiles + s - 1) / s + 3));
+    const int64_t left = sms - units * s;
+    const double after = prefix + own / sms + 3;
+    const double beside = left * 16 >= sms ? fmax(prefix, own / (double)left + 3) : 1e300;
+    const double cost = fmin(after, beside);
+    if (cost < best_cost) {
+      best = s, best_cost = cost;
+      g.grid = beside < after ? (int)left : sms;
+    }
   }
   return (int)best;
 }
@@ -193,7 +210,7 @@ int launch_join(const AttnCall& a, const PieceGeom& g, const PieceSpace& w, cuda
   // pieces a row, about: the grid's ranges over the segments, and the splits;
   // two or three a warp while the rows alone would not fill the SMs
   const int64_t rows = a.B * a.Hq, pieces = g.grid / p.nseg + 1 + w.prefix_splits;
-  while (p.W < 8 && p.W * 3 <= pieces && rows * p.W < 16 * (int64_t)g.grid) p.W *= 2;
+  while (p.W < 8 && p.W * 3 <= pieces && rows * p.W < 16 * (int64_t)device_sm_count()) p.W *= 2;
   cudaLaunchConfig_t lc = {};
   lc.gridDim = dim3((unsigned)((rows * p.W + 7) / 8));
   lc.blockDim = dim3(256);
@@ -227,7 +244,7 @@ bool prefix_fits(const PieceGeom& g, int64_t Hkv, int64_t bs, int64_t max_prefix
 }
 
 int attend(const AttnCall& a, const b200_launch_cfg* cfg, void* workspace, size_t workspace_bytes, cudaStream_t s) {
-  const PieceGeom g = piece_geometry(a.B, a.Hq, a.Hkv, a.D, a.block_size, a.num_blocks, a.max_blocks, elem_of(a), cfg);
+  PieceGeom g = piece_geometry(a.B, a.Hq, a.Hkv, a.D, a.block_size, a.num_blocks, a.max_blocks, elem_of(a), cfg);
   const bool aligned = aligned16(a.q) && aligned16(a.out) && aligned16(a.k_cache) && aligned16(a.v_cache) &&
                        aligned16(a.k_scale) && aligned16(a.v_scale);
   const bool prefix = a.prefix_table != nullptr;
@@ -239,7 +256,7 @@ int attend(const AttnCall& a, const b200_launch_cfg* cfg, void* workspace, size_
     if (a.cache_dtype == B200_F8E4M3) return launch_attn_generic_e4m3(a, s);
     return launch_attn_generic_16(a, s);
   }
-  const int splits = prefix ? prefix_splits(g, g.seqs, a.Hkv, a.block_size, a.max_prefix_blocks) : 0;
+  const int splits = prefix ? share_sms(g, a.Hkv, a.block_size, a.max_prefix_blocks, a.max_blocks) : 0;
   const SpaceBytes sb = space_bytes(g, a.Hq, splits);
   if (workspace == nullptr || workspace_bytes < sb.cum + sb.rows + sb.prefix) return B200_ERR_WORKSPACE;
   if (!aligned16(workspace)) return B200_ERR_ALIGNMENT;
@@ -331,9 +348,10 @@ extern "C" size_t b200_paged_attention_prefix_workspace_size(int64_t B, int64_t 
       max_blocks < 0 || Hq % Hkv)
     return 0;
   const int elem = cache_dtype == B200_I8 || cache_dtype == B200_F8E4M3 ? 1 : 2;
-  const PieceGeom g = piece_geometry(B, Hq, Hkv, D, block_size, num_blocks, max_blocks, elem, cfg);
+  PieceGeom g = piece_geometry(B, Hq, Hkv, D, block_size, num_blocks, max_blocks, elem, cfg);
   if (!prefix_fits(g, Hkv, block_size, max_prefix_blocks)) return 0;
-  const SpaceBytes sb = space_bytes(g, Hq, prefix_splits(g, g.seqs, Hkv, block_size, max_prefix_blocks));
+  const int splits = share_sms(g, Hkv, block_size, max_prefix_blocks, max_blocks);
+  const SpaceBytes sb = space_bytes(g, Hq, splits);
   return sb.cum + sb.rows + sb.prefix;
 }
 
