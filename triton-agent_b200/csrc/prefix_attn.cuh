@@ -22,8 +22,8 @@
 // in the K/V ring as the MMA reads them; warp 2 zeroes V rows behind the last
 // token (a weight of 0 times a NaN left in the cache is NaN).  8-bit caches:
 // pages land in a ring of code tiles, and warps 12-15 widen them to f16 tiles
-// (codes are exact in f16; the scales go beside them in fp32 and meet
-// the logits and weights as in the streaming kernel).
+// (codes are exact in f16) and load the scales, a tile ahead; the scales meet the
+// logits and weights in fp32 as in the streaming kernel.
 #pragma once
 
 #include "kv_attn.cuh"
@@ -41,13 +41,14 @@ constexpr uint32_t kPHalf = kPM * 128;     // 64 dims (16-bit) of 128 rows
 constexpr uint32_t kPTile = 2 * kPHalf;    // a Q, K or V tile
 constexpr uint32_t kPCodes = kPHalf;       // an 8-bit K or V tile
 constexpr int kPRing16 = 5, kPRing8 = 3;   // K/V tiles in shared memory
-constexpr int kPMaxCodes = 6;              // code tiles, at most
+constexpr int kPCodeRing = 3;              // code tiles (8-bit); with one row tile
+constexpr int kPMoreCodes = 2;             // two more, in the second Q tile's place
+constexpr int kPScaleRing = 4;             // key tiles whose scales wait for the softmax (8-bit), and page ids
 constexpr int kPMaxPages = 8;              // pages of a tile (block size 16)
 
 struct PrefixParams {
   int64_t B, Hq, Hkv, num_blocks, max_prefix;
   int lgG, bs, ppt;  // log2 of the query heads a kv head, block size, pages a key tile
-  int codes;       // ring depth of the code tiles (8-bit)
   int splits;
   float qscale;  // scale * log2(e)
 };
@@ -57,46 +58,52 @@ struct PrefixSmem {
   static constexpr uint32_t oQ = 0;  // two Q tiles
   static constexpr uint32_t oRing = 2 * kPTile;
   static constexpr uint32_t oCodes = oRing + (k8 ? kPRing8 : kPRing16) * kPTile;
+  static constexpr uint32_t oScales = oCodes + (k8 ? kPCodeRing * kPCodes : 0);  // [tile][ks, log2 vs, 1 / vs][128]
+  static constexpr uint32_t oBars = oScales + (k8 ? kPScaleRing * 3 * kPM * 4 : 0);
 };
 
 // A warp's 32 rows of Q (row r of the batch's matrix: sequence r / G, head h G +
 // r % G) into the swizzled tile at `tile`: 16-byte chunk c of row r sits at
 // chunk c ^ (r & 7) of its 128-byte row, dims 64.. in the second half.  Sixteen
 // lanes a row, so that the loads are whole rows.  8-bit caches: f16, each row scaled
-// to [2^13, 2^14) by a power of two.  Returns the logit factor of row `lane`.
+// to [2^13, 2^14) by a power of two.  Returns the logit factor of row `lane`; a
+// tile of 0 stages nothing else.
 template <typename T, bool k8>
 __device__ __forceinline__ float stage_q_rows(const T* __restrict__ q, int r0, int R, int64_t Hq, int h, int lgG,
                                               uint32_t tile, int r_tile, int lane, float qscale) {
   const int c = lane & 15, odd = lane >> 4;
-  uint4 raw[16];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int r = r0 + 2 * i + odd;
-    raw[i] = make_uint4(0, 0, 0, 0);
-    if (r < R) {
-      const int64_t row = (int64_t)(r >> lgG) * Hq + (h << lgG) + (r & ((1 << lgG) - 1));
-      raw[i] = __ldg(reinterpret_cast<const uint4*>(q + row * kPieceDim) + c);
-    }
-  }
   float factor = qscale;
+#pragma unroll 1
+  for (int i0 = 0; i0 < 16; i0 += 8) {
+    uint4 raw[8];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    if constexpr (k8) {
-      float f[8], amax = 0.f, up, down;
-      unpack16<T>(raw[i], f);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) amax = fmaxf(amax, fabsf(f[k]));
-#pragma unroll
-      for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-      pow2_scale<13>(amax, up, down);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) f[k] *= up;
-      raw[i] = pack16<__half>(f);
-      const float d = __shfl_sync(0xffffffffu, down, (lane & 1) * 16);
-      if (i == lane >> 1) factor = qscale * d;
+    for (int i = 0; i < 8; ++i) {
+      const int r = r0 + 2 * (i0 + i) + odd;
+      raw[i] = make_uint4(0, 0, 0, 0);
+      if (r < R) {
+        const int64_t row = (int64_t)(r >> lgG) * Hq + (h << lgG) + (r & ((1 << lgG) - 1));
+        raw[i] = __ldg(reinterpret_cast<const uint4*>(q + row * kPieceDim) + c);
+      }
     }
-    const int r = r_tile + 2 * i + odd;
-    sts128(tile + (c >> 3) * kPHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4), raw[i]);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (k8) {
+        float f[8], amax = 0.f, up, down;
+        unpack16<T>(raw[i], f);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) amax = fmaxf(amax, fabsf(f[k]));
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        pow2_scale<13>(amax, up, down);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) f[k] *= up;
+        raw[i] = pack16<__half>(f);
+        const float d = __shfl_sync(0xffffffffu, down, (lane & 1) * 16);
+        if (i0 + i == lane >> 1) factor = qscale * d;
+      }
+      const int r = r_tile + 2 * (i0 + i) + odd;
+      if (tile != 0) sts128(tile + (c >> 3) * kPHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4), raw[i]);
+    }
   }
   return factor;
 }
@@ -132,22 +139,27 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
   const int both = tiles == 2;  // else: streams 0 and 1 are the even and odd key tiles of one row tile
   const int bs = p.bs, tile_tok = p.ppt * bs;
 
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::oCodes + (k8 ? p.codes * kPCodes : 0));
-  uint64_t* ring_full = bars;                   // [kRing]
+  // code tile i; with one row tile the second Q tile's place holds two more
+  const int codes = kPCodeRing + (both ? 0 : kPMoreCodes);
+  auto code_at = [&](int i) {
+    return sbase + (i < kPCodeRing ? L::oCodes + i * kPCodes : L::oQ + kPTile + (i - kPCodeRing) * kPCodes);
+  };
+
+  uint64_t* ring_full = reinterpret_cast<uint64_t*>(smem + L::oBars);  // [kRing]
   uint64_t* ring_empty = ring_full + kPRing16;  // [kRing]
   uint64_t* s_full = ring_empty + kPRing16;     // [2]
   uint64_t* p_full = s_full + 2;                // [2]
   uint64_t* o_done = p_full + 2;                // [2]
   uint64_t* v_fixed = o_done + 2;
-  uint64_t* sc_full = v_fixed + 1;              // [2]
-  uint64_t* sc_empty = sc_full + 2;             // [2]
-  uint64_t* code_full = sc_empty + 2;           // [kPMaxCodes]
-  uint64_t* code_empty = code_full + kPMaxCodes;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(code_empty + kPMaxCodes);
+  uint64_t* sc_full = v_fixed + 1;               // [kPScaleRing]
+  uint64_t* sc_empty = sc_full + kPScaleRing;    // [kPScaleRing]
+  uint64_t* ids_full = sc_empty + kPScaleRing;   // [kPScaleRing]
+  uint64_t* code_full = ids_full + kPScaleRing;  // [codes]
+  uint64_t* code_empty = code_full + kPCodeRing + kPMoreCodes;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(code_empty + kPCodeRing + kPMoreCodes);
   int* s_abort = reinterpret_cast<int*>(tmem_slot + 1);
-  int* s_count = s_abort + 5;  // (16-byte aligned from here) [2][4] valid entries before the split and in it, by warp
-  int* s_ids = s_count + 8;    // [kPMaxCodes][kPMaxPages] page ids of a code tile
-  float* s_sc = reinterpret_cast<float*>(s_ids + kPMaxCodes * kPMaxPages);  // [2][3][kPM]: ks, log2 vs, 1 / vs
+  int* s_count = s_abort + 1;  // [2][4] valid entries before the split and in it, by warp
+  int* s_ids = s_count + 8;    // [kPScaleRing][kPMaxPages] page ids of a key tile
 
   // the own-token kernel may run beside this one
   asm volatile("griddepcontrol.launch_dependents;");
@@ -192,11 +204,14 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
       sm100::mbar_init(sm100::smem_u32(&s_full[i]), 1);
       sm100::mbar_init(sm100::smem_u32(&p_full[i]), 4);
       sm100::mbar_init(sm100::smem_u32(&o_done[i]), 1);
-      sm100::mbar_init(sm100::smem_u32(&sc_full[i]), 4);
-      sm100::mbar_init(sm100::smem_u32(&sc_empty[i]), 4 * tiles);  // one stream's warps, or both's
     }
     sm100::mbar_init(sm100::smem_u32(v_fixed), 1);
-    for (int i = 0; i < kPMaxCodes; ++i) {
+    for (int i = 0; i < kPScaleRing; ++i) {
+      sm100::mbar_init(sm100::smem_u32(&sc_full[i]), 4);
+      sm100::mbar_init(sm100::smem_u32(&ids_full[i]), 1);
+      sm100::mbar_init(sm100::smem_u32(&sc_empty[i]), 4 * tiles);  // one stream's warps, or both's
+    }
+    for (int i = 0; i < codes; ++i) {
       sm100::mbar_init(sm100::smem_u32(&code_full[i]), kPProducers);
       sm100::mbar_init(sm100::smem_u32(&code_empty[i]), 4);
     }
@@ -214,13 +229,14 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
     sm100::tmem_alloc(sm100::smem_u32(tmem_slot), 512);
     sm100::tmem_relinquish();
   }
-  // the softmax warps stage Q meanwhile (with one row tile the second stream
-  // stages it too, into the unused tile, for its rows' factors)
+  // the softmax warps stage Q meanwhile (with one row tile the second warpgroup
+  // only takes its rows' factors)
   float sl = p.qscale;
   if (warp >= 4 && warp < 12) {
     const int t = (warp >> 2) - 1, rw = (warp & 3) * 32;
-    sl = stage_q_rows<T, k8>(q, row0 + both * t * kPM + rw, R, p.Hq, h, p.lgG, sbase + L::oQ + t * kPTile, rw, lane,
-                             p.qscale);
+    const uint32_t tile = t == 0 || both ? sbase + L::oQ + t * kPTile : 0;
+    if (k8 || tile != 0)
+      sl = stage_q_rows<T, k8>(q, row0 + both * t * kPM + rw, R, p.Hq, h, p.lgG, tile, rw, lane, p.qscale);
     sm100::fence_proxy_async_smem();
   }
   sm100::tc_fence_before();
@@ -247,27 +263,30 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
       sm100::tma_prefetch_desc(&tm_v);
     }
     constexpr int kHalves = k8 ? 1 : 2;  // boxes of a page
-    const int depth = k8 ? p.codes : kRing;
+    const int depth = k8 ? codes : kRing;
     uint64_t* fulls = k8 ? code_full : ring_full;
     uint64_t* empties = k8 ? code_empty : ring_empty;
     int left = (ntok + bs - 1) / bs;  // pages still to copy
     int issued = 0, np = 0;           // tiles issued, pages of the open tile
+    int slot = 0;
+    uint32_t ph = 1;  // parity of the empty barriers in this round
     int ids[kPMaxPages];
     bool ok = true;
     // lane 0: this warp's boxes of a tile (box x = page and half)
     auto copy_tile = [&](int which) -> bool {
-      const int slot = issued % depth;
       if (*(volatile int*)s_abort) return false;
-      if (!sm100::mbar_wait(sm100::smem_u32(&empties[slot]), ((issued / depth) & 1) ^ 1)) return false;
+      if (!sm100::mbar_wait(sm100::smem_u32(&empties[slot]), ph)) return false;
       const uint32_t fb = sm100::smem_u32(&fulls[slot]);
       const CUtensorMap* map = which ? &tm_v : &tm_k;
-      const uint32_t dst = sbase + (k8 ? L::oCodes + slot * kPCodes : L::oRing + slot * kPTile);
-      if (k8 && mine == 0) {
+      const uint32_t dst = k8 ? code_at(slot) : sbase + L::oRing + slot * kPTile;
+      const int n = np * kHalves;
+      if (k8 && which == 0 && mine == 0) {
+        const int at = (issued >> 1) % kPScaleRing;
 #pragma unroll
         for (int i = 0; i < kPMaxPages; ++i)
-          if (i < np) s_ids[slot * kPMaxPages + i] = ids[i];
+          if (i < np) s_ids[at * kPMaxPages + i] = ids[i];
+        sm100::mbar_arrive(sm100::smem_u32(&ids_full[at]));
       }
-      const int n = np * kHalves;
       sm100::mbar_arrive_expect_tx(fb, (uint32_t)((n - mine + kPProducers - 1) / kPProducers * bs * 128));
 #pragma unroll
       for (int x = 0; x < kPMaxPages * kHalves; ++x) {
@@ -276,6 +295,10 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
                              ids[x / kHalves] * bs, h);
       }
       ++issued;
+      if (++slot == depth) {
+        slot = 0;
+        ph ^= 1u;
+      }
       return true;
     };
     for (int j0 = e0; j0 < e1 && left > 0 && ok; j0 += 32) {
@@ -309,11 +332,11 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
     __syncwarp();
     if (warp == 2 && fix_v) {
       // V rows behind the last token are zero
-      const int it = 2 * nkt - 1, slot = it % kRing;
-      if (sm100::mbar_wait_warp(sm100::smem_u32(&ring_full[slot]), (it / kRing) & 1)) {
+      const int it = 2 * nkt - 1, vslot = it % kRing;
+      if (sm100::mbar_wait_warp(sm100::smem_u32(&ring_full[vslot]), (it / kRing) & 1)) {
         for (int i = lane; i < 2 * (tile_tok - last_valid) * 8; i += 32) {
           const int c = i & 7, r = (i >> 3) % (tile_tok - last_valid), half = (i >> 3) / (tile_tok - last_valid);
-          sts128(sbase + L::oRing + slot * kPTile + half * kPHalf + (last_valid + r) * 128 + c * 16,
+          sts128(sbase + L::oRing + vslot * kPTile + half * kPHalf + (last_valid + r) * 128 + c * 16,
                  make_uint4(0, 0, 0, 0));
         }
         sm100::fence_proxy_async_smem();
@@ -406,20 +429,30 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
       const int r = threadIdx.x - 384;  // this thread's key of every tile
       const int page = r / bs, off = r - page * bs;
       bool ok = true;
-      for (int it = 0; it < 2 * nkt && ok; ++it) {
-        const int cs = it % p.codes, slot = it % kRing, j = it >> 1, which = it & 1;
-        const int valid = j == nkt - 1 ? last_valid : tile_tok;
-        const bool live = r < valid;
-        ok = sm100::mbar_wait_warp(sm100::smem_u32(&code_full[cs]), (it / p.codes) & 1);
-        float ks = 0.f, vs = 1.f;
-        if (ok && which == 0 && live) {
-          const int64_t at = ((int64_t)lds_s32(sm100::smem_u32(s_ids + cs * kPMaxPages + page)) * p.Hkv + h) * bs + off;
+      int cs = 0;
+      uint32_t cph = 0;
+      // scales of this thread's key of tile j, when that is live (its page ids are
+      // there: a code ring of three tiles or more holds K of the next tile)
+      float ks = 0.f, vs = 1.f;
+      auto load_scales = [&](int j) {
+        if (!sm100::mbar_wait_warp(sm100::smem_u32(&ids_full[j % kPScaleRing]), (j / kPScaleRing) & 1)) return false;
+        if (r < (j == nkt - 1 ? last_valid : tile_tok)) {
+          const int id = lds_s32(sm100::smem_u32(s_ids + (j % kPScaleRing) * kPMaxPages + page));
+          const int64_t at = ((int64_t)id * p.Hkv + h) * bs + off;
           ks = __ldg(&k_scale[at]);
           vs = __ldg(&v_scale[at]);
         }
+        return true;
+      };
+      if (nkt > 0) ok = load_scales(0);
+      for (int it = 0; it < 2 * nkt && ok; ++it) {
+        const int slot = it % kRing, j = it >> 1, which = it & 1;
+        const int valid = j == nkt - 1 ? last_valid : tile_tok;
+        const bool live = r < valid;
+        ok = sm100::mbar_wait_warp(sm100::smem_u32(&code_full[cs]), cph);
         ok = ok && sm100::mbar_wait_warp(sm100::smem_u32(&ring_empty[slot]), ((it / kRing) & 1) ^ 1);
         if (!ok) break;
-        const uint32_t src = sbase + L::oCodes + cs * kPCodes + r * 128;
+        const uint32_t src = code_at(cs) + r * 128;
         const uint32_t dst = sbase + L::oRing + slot * kPTile + r * 128;
 #pragma unroll
         for (int c0 = 0; c0 < 8; c0 += 4) {
@@ -442,19 +475,25 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
         sm100::fence_proxy_async_smem();
         if (which == 0) {
           // scales of the tile; a key behind the last token has log2 weight -inf
-          ok = sm100::mbar_wait_warp(sm100::smem_u32(&sc_empty[j & 1]), ((j >> 1) & 1) ^ 1);
+          const int ss = j % kPScaleRing;
+          ok = sm100::mbar_wait_warp(sm100::smem_u32(&sc_empty[ss]), ((j / kPScaleRing) & 1) ^ 1);
           float lv = -INFINITY, iv = 0.f;
           if (live) kv8_value_scale(vs, lv, iv);
-          const uint32_t sc = sm100::smem_u32(s_sc) + (uint32_t)((j & 1) * 3 * kPM + r) * 4;
-          sts_f32(sc, ks);
+          const uint32_t sc = sbase + L::oScales + (uint32_t)(ss * 3 * kPM + r) * 4;
+          sts_f32(sc, live ? ks : 0.f);
           sts_f32(sc + kPM * 4, lv);
           sts_f32(sc + 2 * kPM * 4, iv);
+          if (ok && j + 1 < nkt) ok = load_scales(j + 1);
         }
         __syncwarp();
         if (lane == 0) {
           sm100::mbar_arrive(sm100::smem_u32(&ring_full[slot]));
           sm100::mbar_arrive(sm100::smem_u32(&code_empty[cs]));
-          if (which == 0) sm100::mbar_arrive(sm100::smem_u32(&sc_full[j & 1]));
+          if (which == 0) sm100::mbar_arrive(sm100::smem_u32(&sc_full[j % kPScaleRing]));
+        }
+        if (++cs == codes) {
+          cs = 0;
+          cph ^= 1u;
         }
       }
       if (!ok && lane == 0) {
@@ -476,9 +515,9 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
     bool ok = true;
     const int n_tiles = both ? nkt : (nkt - t + 1) / 2;  // key tiles of this stream
     for (int n = 0; n < n_tiles; ++n) {
-      const int j = both ? n : 2 * n + t;
+      const int j = both ? n : 2 * n + t, ss = j % kPScaleRing;
       ok = sm100::mbar_wait_warp(sm100::smem_u32(&s_full[t]), n & 1);
-      if (k8 && ok) ok = sm100::mbar_wait_warp(sm100::smem_u32(&sc_full[j & 1]), (j >> 1) & 1);
+      if (k8 && ok) ok = sm100::mbar_wait_warp(sm100::smem_u32(&sc_full[ss]), (j / kPScaleRing) & 1);
       if (!ok) break;
       sm100::tc_fence_after();
       uint32_t v[kPM];
@@ -488,7 +527,7 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
       sm100::tmem_wait_ld_regs(v + 32);
       sm100::tmem_wait_ld_regs(v + 64);
       sm100::tmem_wait_ld_regs(v + 96);
-      const uint32_t sc = sm100::smem_u32(s_sc) + (uint32_t)((j & 1) * 3 * kPM) * 4;
+      const uint32_t sc = sbase + L::oScales + (uint32_t)(ss * 3 * kPM) * 4;
       float f = sl;  // logits in log2 units: f times v (16-bit), or v itself
       if constexpr (k8) {
         // y = (S sl) ks + log2 vs; a key behind the last token has log2 vs = -inf
@@ -570,7 +609,7 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
       __syncwarp();
       if (lane == 0) {
         sm100::mbar_arrive(sm100::smem_u32(&p_full[t]));
-        if (k8) sm100::mbar_arrive(sm100::smem_u32(&sc_empty[j & 1]));
+        if (k8) sm100::mbar_arrive(sm100::smem_u32(&sc_empty[ss]));
       }
     }
     // ---- the row's piece
@@ -660,12 +699,11 @@ int launch_prefix(const AttnCall& a, const PieceGeom& g, const PieceSpace& w, cu
   p.B = a.B, p.Hq = a.Hq, p.Hkv = a.Hkv, p.num_blocks = a.num_blocks, p.max_prefix = a.max_prefix_blocks;
   while ((1 << p.lgG) < g.G) ++p.lgG;
   p.bs = (int)a.block_size, p.ppt = kPM / (int)a.block_size;
-  p.codes = 3;
   p.splits = w.prefix_splits;
   p.qscale = a.scale * 1.4426950408889634f;
-  const size_t smem = 1024 + PrefixSmem<k8>::oCodes + (k8 ? p.codes * kPCodes : 0) +
-                      8 * (2 * kPRing16 + 6 + 1 + 4 + 2 * kPMaxCodes) + 24 + 32 + 4 * kPMaxCodes * kPMaxPages +
-                      (k8 ? 2 * 3 * kPM * 4 : 0);
+  const size_t smem = 1024 + PrefixSmem<k8>::oBars +
+                      8 * (2 * kPRing16 + 6 + 1 + 3 * kPScaleRing + 2 * (kPCodeRing + kPMoreCodes)) + 8 + 32 + 4 * kPScaleRing * kPMaxPages;
+  static_assert(PrefixSmem<k8>::oBars + 1024 + 512 <= 227 * 1024, "shared memory of a CTA");
   auto kern = prefix_attn_kernel<T, KV>;
   if (k8) {
     // the register split (setmaxnreg) needs what it hands out at launch
