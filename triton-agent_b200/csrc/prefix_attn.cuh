@@ -16,8 +16,8 @@
 // Reading the prefix costs its bytes once a CTA column instead of once a
 // sequence: at 64 sequences of an 8192-token prefix 33.5 MB instead of 2.1 GB.
 //
-// Roles: warps 0, 2 and 3 walk the block table and copy pages (TMA boxes of bs
-// tokens; a tile is as many pages as fit 128 tokens), warp 1 issues the MMAs,
+// Roles: warps 0 and 2 walk the block table and copy the pages of K and V (one TMA
+// box a page; a tile is as many pages as fit 128 tokens), warp 1 issues the MMAs,
 // warps 4-11 are the two streams' softmax warpgroups.  16-bit caches: pages land
 // in the K/V ring as the MMA reads them; warp 2 zeroes V rows behind the last
 // token (a weight of 0 times a NaN left in the cache is NaN).  8-bit caches:
@@ -45,6 +45,7 @@ constexpr int kPCodeRing = 3;              // code tiles (8-bit); with one row t
 constexpr int kPMoreCodes = 2;             // two more, in the second Q tile's place
 constexpr int kPScaleRing = 4;             // key tiles whose scales wait for the softmax (8-bit), and page ids
 constexpr int kPMaxPages = 8;              // pages of a tile (block size 16)
+constexpr int kPList = 32 + kPMaxPages;    // pages a producer holds
 
 struct PrefixParams {
   int64_t B, Hq, Hkv, num_blocks, max_prefix;
@@ -59,7 +60,8 @@ struct PrefixSmem {
   static constexpr uint32_t oRing = 2 * kPTile;
   static constexpr uint32_t oCodes = oRing + (k8 ? kPRing8 : kPRing16) * kPTile;
   static constexpr uint32_t oScales = oCodes + (k8 ? kPCodeRing * kPCodes : 0);  // [tile][ks, log2 vs, 1 / vs][128]
-  static constexpr uint32_t oBars = oScales + (k8 ? kPScaleRing * 3 * kPM * 4 : 0);
+  static constexpr uint32_t oRaw = oScales + (k8 ? kPScaleRing * 3 * kPM * 4 : 0);  // [ks, vs][128] of the next tile
+  static constexpr uint32_t oBars = oRaw + (k8 ? 2 * kPM * 4 : 0);
 };
 
 // A warp's 32 rows of Q (row r of the batch's matrix: sequence r / G, head h G +
@@ -115,9 +117,13 @@ __device__ __forceinline__ void stg256(float* dst, const uint32_t* v) {
                : "memory");
 }
 
-// Producer warps share a tile's boxes: issuing one costs a thread about a
-// hundred cycles, and a tile of 16-token pages is 16 or 32 of them.
-constexpr int kPProducers = 3;
+// A K or V tile: groups of eight tokens, each with dims 0..63 and then 64..127
+// as an atom of eight swizzled 128-byte rows, so that a page is one contiguous
+// box whatever its size.  Where 16-byte chunk c of token r sits:
+__device__ __forceinline__ uint32_t kv_at(int r, int c) {
+  return (uint32_t)((r >> 3) * 2048 + (c >> 3) * 1024 + (r & 7) * 128 + (((c & 7) ^ (r & 7)) << 4));
+}
+
 constexpr int kPRegsLow = 72, kPRegsHigh = 184;  // 8-bit kernel: 8 warps each way, 128 a thread at launch
 
 template <typename T, typename KV>
@@ -160,6 +166,7 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
   int* s_abort = reinterpret_cast<int*>(tmem_slot + 1);
   int* s_count = s_abort + 1;  // [2][4] valid entries before the split and in it, by warp
   int* s_ids = s_count + 8;    // [kPScaleRing][kPMaxPages] page ids of a key tile
+  int* s_list = s_ids + kPScaleRing * kPMaxPages;  // [K, V][kPList] pages to copy
 
   // the own-token kernel may run beside this one
   asm volatile("griddepcontrol.launch_dependents;");
@@ -197,7 +204,7 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
   if (threadIdx.x == 32) {
     *s_abort = 0;
     for (int i = 0; i < kRing; ++i) {
-      sm100::mbar_init(sm100::smem_u32(&ring_full[i]), k8 ? 4 : kPProducers);
+      sm100::mbar_init(sm100::smem_u32(&ring_full[i]), k8 ? 4 : 1);
       sm100::mbar_init(sm100::smem_u32(&ring_empty[i]), 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -212,16 +219,17 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
       sm100::mbar_init(sm100::smem_u32(&sc_empty[i]), 4 * tiles);  // one stream's warps, or both's
     }
     for (int i = 0; i < codes; ++i) {
-      sm100::mbar_init(sm100::smem_u32(&code_full[i]), kPProducers);
+      sm100::mbar_init(sm100::smem_u32(&code_full[i]), 1);
       sm100::mbar_init(sm100::smem_u32(&code_empty[i]), 4);
     }
     sm100::fence_barrier_init();
   }
   if (!k8 && tile_tok < kPM) {
     // rows no page reaches stay zero in every ring tile (both operands)
-    for (int i = threadIdx.x; i < kRing * 2 * (kPM - tile_tok) * 8; i += blockDim.x) {
-      const int c = i & 7, r = (i >> 3) % (kPM - tile_tok), half = (i >> 3) / (kPM - tile_tok);
-      *reinterpret_cast<uint4*>(smem + L::oRing + half * kPHalf + (tile_tok + r) * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+    const int dead = kPM - tile_tok;
+    for (int i = threadIdx.x; i < kRing * dead * 16; i += blockDim.x) {
+      const int c = i & 15, r = (i >> 4) % dead, slot = (i >> 4) / dead;
+      sts128(sbase + L::oRing + slot * kPTile + kv_at(tile_tok + r, c), make_uint4(0, 0, 0, 0));
     }
     sm100::fence_proxy_async_smem();
   }
@@ -255,70 +263,62 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
   const bool fix_v = !k8 && nkt > 0 && last_valid < tile_tok;
 
   if (k8 && warp < 4) sm100::setmaxnreg_dec<kPRegsLow>();
-  if (warp == 0 || warp == 2 || warp == 3) {
-    // ------------------------------------------------------------- producers
-    const int mine = warp == 0 ? 0 : warp - 1;  // of kPProducers
-    if (lane == 0) {
-      sm100::tma_prefetch_desc(&tm_k);
-      sm100::tma_prefetch_desc(&tm_v);
-    }
-    constexpr int kHalves = k8 ? 1 : 2;  // boxes of a page
+  if (warp == 0 || warp == 2) {
+    // ------------------------------------- producers: K tiles and V tiles, in turn in one ring
+    const int which = warp >> 1;
+    const CUtensorMap* map = which ? &tm_v : &tm_k;
+    if (lane == 0) sm100::tma_prefetch_desc(map);
     const int depth = k8 ? codes : kRing;
     uint64_t* fulls = k8 ? code_full : ring_full;
     uint64_t* empties = k8 ? code_empty : ring_empty;
+    const uint32_t page_bytes = (uint32_t)(bs * kPieceDim * (int)sizeof(KV));
+    int* list = s_list + which * kPList;
     int left = (ntok + bs - 1) / bs;  // pages still to copy
-    int issued = 0, np = 0;           // tiles issued, pages of the open tile
-    int slot = 0;
+    int have = 0, issued = 0;         // pages in the list, tiles copied
+    int slot = which;
     uint32_t ph = 1;  // parity of the empty barriers in this round
-    int ids[kPMaxPages];
     bool ok = true;
-    // lane 0: this warp's boxes of a tile (box x = page and half)
-    auto copy_tile = [&](int which) -> bool {
-      if (*(volatile int*)s_abort) return false;
-      if (!sm100::mbar_wait(sm100::smem_u32(&empties[slot]), ph)) return false;
-      const uint32_t fb = sm100::smem_u32(&fulls[slot]);
-      const CUtensorMap* map = which ? &tm_v : &tm_k;
-      const uint32_t dst = k8 ? code_at(slot) : sbase + L::oRing + slot * kPTile;
-      const int n = np * kHalves;
-      if (k8 && which == 0 && mine == 0) {
-        const int at = (issued >> 1) % kPScaleRing;
-#pragma unroll
-        for (int i = 0; i < kPMaxPages; ++i)
-          if (i < np) s_ids[at * kPMaxPages + i] = ids[i];
-        sm100::mbar_arrive(sm100::smem_u32(&ids_full[at]));
-      }
-      sm100::mbar_arrive_expect_tx(fb, (uint32_t)((n - mine + kPProducers - 1) / kPProducers * bs * 128));
-#pragma unroll
-      for (int x = 0; x < kPMaxPages * kHalves; ++x) {
-        if (x % kPProducers == mine && x < n)
-          sm100::tma_load_3d(dst + (x % kHalves) * kPHalf + (x / kHalves) * bs * 128, map, fb, (x % kHalves) * 64,
-                             ids[x / kHalves] * bs, h);
-      }
-      ++issued;
-      if (++slot == depth) {
-        slot = 0;
-        ph ^= 1u;
-      }
-      return true;
-    };
+    int64_t next = e0 + lane < e1 ? ptab.at(e0 + lane) : -1;
     for (int j0 = e0; j0 < e1 && left > 0 && ok; j0 += 32) {
-      const int64_t id = j0 + lane < e1 ? ptab.at(j0 + lane) : -1;
-      unsigned use = __ballot_sync(0xffffffffu, id >= 0 && id < p.num_blocks);
-      while (use != 0 && left > 0 && ok) {
-        const int src = __ffs(use) - 1;
-        use &= use - 1;
-        const int page = (int)__shfl_sync(0xffffffffu, (int)id, src);
-        --left;
-#pragma unroll
-        for (int i = 0; i < kPMaxPages; ++i)
-          if (i == np) ids[i] = page;
-        ++np;
-        if (np == p.ppt || left == 0) {
-          if (lane == 0) ok = copy_tile(0) && copy_tile(1);
-          ok = __shfl_sync(0xffffffffu, ok, 0);
-          np = 0;
+      const int64_t id = next;
+      next = j0 + 32 + lane < e1 ? ptab.at(j0 + 32 + lane) : -1;
+      const bool valid = id >= 0 && id < p.num_blocks;
+      const unsigned use = __ballot_sync(0xffffffffu, valid);
+      if (valid) list[have + __popc(use & ((1u << lane) - 1u))] = (int)id;
+      have += __popc(use);
+      __syncwarp();
+      int at = 0;
+      while (left > 0 && (have - at >= p.ppt || have - at >= left)) {
+        const int np = left < p.ppt ? left : p.ppt;
+        ok = !*(volatile int*)s_abort && sm100::mbar_wait(sm100::smem_u32(&empties[slot]), ph);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const uint32_t fb = sm100::smem_u32(&fulls[slot]);
+        const int page = lane < np ? list[at + lane] : 0;
+        if (lane == 0) sm100::mbar_arrive_expect_tx(fb, np * page_bytes);
+        if (k8 && which == 0 && lane < np) s_ids[issued % kPScaleRing * kPMaxPages + lane] = page;
+        __syncwarp();
+        if (lane < np) {
+          if constexpr (k8)
+            sm100::tma_load_3d(code_at(slot) + lane * page_bytes, map, fb, 0, page * bs, h);
+          else
+            sm100::tma_load_4d(sbase + L::oRing + slot * kPTile + lane * page_bytes, map, fb, 0, 0, 2 * h,
+                               page * (bs >> 3));
+        }
+        if (k8 && which == 0 && lane == 0) sm100::mbar_arrive(sm100::smem_u32(&ids_full[issued % kPScaleRing]));
+        at += np;
+        left -= np;
+        ++issued;
+        slot += 2;
+        if (slot >= depth) {
+          slot -= depth;
+          ph ^= 1u;
         }
       }
+      have -= at;  // (fewer than a tile's pages are left)
+      const int rest = lane < have ? list[at + lane] : 0;
+      __syncwarp();
+      if (lane < have) list[lane] = rest;
     }
     if (lane == 0) {
       if (!ok) {
@@ -326,7 +326,7 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
         atomicExch(s_abort, 1);
       }
       // no copy may still be writing shared memory when the CTA exits
-      for (int i = issued - 1; i >= 0 && i >= issued - depth; --i)
+      for (int i = 2 * issued - 2 + which; i >= 0 && i >= 2 * issued - depth; i -= 2)
         if (!sm100::mbar_wait(sm100::smem_u32(&fulls[i % depth]), (i / depth) & 1)) b200_dev_error(kDevErrTimeoutFull);
     }
     __syncwarp();
@@ -334,11 +334,8 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
       // V rows behind the last token are zero
       const int it = 2 * nkt - 1, vslot = it % kRing;
       if (sm100::mbar_wait_warp(sm100::smem_u32(&ring_full[vslot]), (it / kRing) & 1)) {
-        for (int i = lane; i < 2 * (tile_tok - last_valid) * 8; i += 32) {
-          const int c = i & 7, r = (i >> 3) % (tile_tok - last_valid), half = (i >> 3) / (tile_tok - last_valid);
-          sts128(sbase + L::oRing + vslot * kPTile + half * kPHalf + (last_valid + r) * 128 + c * 16,
-                 make_uint4(0, 0, 0, 0));
-        }
+        for (int i = lane; i < (tile_tok - last_valid) * 16; i += 32)
+          sts128(sbase + L::oRing + vslot * kPTile + kv_at(last_valid + (i >> 4), i & 15), make_uint4(0, 0, 0, 0));
         sm100::fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) sm100::mbar_arrive(sm100::smem_u32(v_fixed));
@@ -354,8 +351,8 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
     constexpr uint32_t idesc_o = sm100::make_idesc(1, fmt, fmt, 0, 1, kPM, kPieceDim);
     const uint32_t leader = sm100::elect_one();
     const uint64_t dq = sm100::make_smem_desc(sbase + L::oQ, 16, 1024, sm100::kSwizzle128B);
-    const uint64_t dk = sm100::make_smem_desc(sbase + L::oRing, 16, 1024, sm100::kSwizzle128B);
-    const uint64_t dv = sm100::make_smem_desc(sbase + L::oRing, kPHalf, 1024, sm100::kSwizzle128B);
+    const uint64_t dk = sm100::make_smem_desc(sbase + L::oRing, 16, 2048, sm100::kSwizzle128B);
+    const uint64_t dv = sm100::make_smem_desc(sbase + L::oRing, 1024, 2048, sm100::kSwizzle128B);
     bool ok = nkt > 0;
     auto full = [&](int it) -> bool {
       return sm100::mbar_wait_warp(sm100::smem_u32(&ring_full[it % kRing]), (it / kRing) & 1);
@@ -369,8 +366,9 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
       const uint64_t bd = dk + (uint64_t)((((2 * j) % kRing) * kPTile) >> 4);
 #pragma unroll
       for (int kk = 0; kk < kPieceDim / 16; ++kk) {
-        const uint32_t off = ((kk >> 2) * kPHalf + (kk & 3) * 32) >> 4;
-        sm100::mma_f16_ss(tmem + t * 128, ad + off, bd + off, idesc_s, kk > 0 ? 1u : 0u, leader);
+        const uint32_t offa = ((kk >> 2) * kPHalf + (kk & 3) * 32) >> 4;
+        const uint32_t offb = ((kk >> 2) * 1024 + (kk & 3) * 32) >> 4;
+        sm100::mma_f16_ss(tmem + t * 128, ad + offa, bd + offb, idesc_s, kk > 0 ? 1u : 0u, leader);
       }
       sm100::tc_commit(sm100::smem_u32(&s_full[t]), leader);
       return true;
@@ -382,7 +380,7 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
       const uint64_t bd = dv + (uint64_t)((((2 * j + 1) % kRing) * kPTile) >> 4);
 #pragma unroll
       for (int kk = 0; kk < kPM / 16; ++kk)
-        sm100::mma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, bd + (uint64_t)((kk * 2048) >> 4), idesc_o,
+        sm100::mma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, bd + (uint64_t)((kk * 4096) >> 4), idesc_o,
                           (n > 0 || kk > 0) ? 1u : 0u, leader);
       return true;
     };
@@ -431,16 +429,17 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
       bool ok = true;
       int cs = 0;
       uint32_t cph = 0;
-      // scales of this thread's key of tile j, when that is live (its page ids are
-      // there: a code ring of three tiles or more holds K of the next tile)
-      float ks = 0.f, vs = 1.f;
+      // scales of this thread's key of tile j on their way to its own places in
+      // shared memory (its page ids are there: a code ring of three tiles or more
+      // holds K of the next tile)
+      const uint32_t raw = sbase + L::oRaw + r * 4;
       auto load_scales = [&](int j) {
         if (!sm100::mbar_wait_warp(sm100::smem_u32(&ids_full[j % kPScaleRing]), (j / kPScaleRing) & 1)) return false;
         if (r < (j == nkt - 1 ? last_valid : tile_tok)) {
           const int id = lds_s32(sm100::smem_u32(s_ids + (j % kPScaleRing) * kPMaxPages + page));
           const int64_t at = ((int64_t)id * p.Hkv + h) * bs + off;
-          ks = __ldg(&k_scale[at]);
-          vs = __ldg(&v_scale[at]);
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(raw), "l"(k_scale + at) : "memory");
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(raw + kPM * 4), "l"(v_scale + at) : "memory");
         }
         return true;
       };
@@ -453,7 +452,7 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
         ok = ok && sm100::mbar_wait_warp(sm100::smem_u32(&ring_empty[slot]), ((it / kRing) & 1) ^ 1);
         if (!ok) break;
         const uint32_t src = code_at(cs) + r * 128;
-        const uint32_t dst = sbase + L::oRing + slot * kPTile + r * 128;
+        const uint32_t dst = sbase + L::oRing + slot * kPTile;
 #pragma unroll
         for (int c0 = 0; c0 < 8; c0 += 4) {
           uint4 w[4];
@@ -467,9 +466,8 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
             kv8_in_order<KV>(w[c].z, b.x, b.y);
             kv8_in_order<KV>(w[c].w, b.z, b.w);
             if (!live) a = b = make_uint4(0, 0, 0, 0);
-            const uint32_t d = dst + (c0 >> 2) * kPHalf;
-            sts128(d + (((2 * c) ^ (r & 7)) << 4), a);
-            sts128(d + (((2 * c + 1) ^ (r & 7)) << 4), b);
+            sts128(dst + kv_at(r, 2 * (c0 + c)), a);
+            sts128(dst + kv_at(r, 2 * (c0 + c) + 1), b);
           }
         }
         sm100::fence_proxy_async_smem();
@@ -477,10 +475,14 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
           // scales of the tile; a key behind the last token has log2 weight -inf
           const int ss = j % kPScaleRing;
           ok = sm100::mbar_wait_warp(sm100::smem_u32(&sc_empty[ss]), ((j / kPScaleRing) & 1) ^ 1);
-          float lv = -INFINITY, iv = 0.f;
-          if (live) kv8_value_scale(vs, lv, iv);
+          float ks = 0.f, lv = -INFINITY, iv = 0.f;
+          asm volatile("cp.async.wait_all;" ::: "memory");
+          if (live) {
+            ks = lds_f32(raw);
+            kv8_value_scale(lds_f32(raw + kPM * 4), lv, iv);
+          }
           const uint32_t sc = sbase + L::oScales + (uint32_t)(ss * 3 * kPM + r) * 4;
-          sts_f32(sc, live ? ks : 0.f);
+          sts_f32(sc, ks);
           sts_f32(sc + kPM * 4, lv);
           sts_f32(sc + 2 * kPM * 4, iv);
           if (ok && j + 1 < nkt) ok = load_scales(j + 1);
@@ -496,6 +498,7 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
           cph ^= 1u;
         }
       }
+      asm volatile("cp.async.wait_all;" ::: "memory");
       if (!ok && lane == 0) {
         b200_dev_error(kDevErrTimeoutFull);
         atomicExch(s_abort, 1);
@@ -686,14 +689,23 @@ int launch_prefix(const AttnCall& a, const PieceGeom& g, const PieceSpace& w, cu
   const CUtensorMapDataType dt = k8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                     : (std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                                       : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16);
-  // a box: 128 bytes of dims x one page's tokens x one head, as 128-byte rows swizzled in 8-row atoms
+  // a box is a page of one head.  8-bit: its tokens' rows of 128 bytes, swizzled in
+  // 8-row atoms; 16-bit: (64 dims, 8 tokens, 2 halves of the dims, groups of 8 tokens)
   CUtensorMap tk, tv;
-  const uint64_t dims[3] = {(uint64_t)kPieceDim, (uint64_t)(a.num_blocks * a.block_size), (uint64_t)a.Hkv};
-  const uint64_t strides[2] = {(uint64_t)a.Hkv * kPieceDim * el, (uint64_t)kPieceDim * el};
-  const uint32_t box[3] = {(uint32_t)(128 / el), (uint32_t)a.block_size, 1};
-  int st = encode_tensor_map(&tk, dt, 3, a.k_cache, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  const uint64_t tokens = (uint64_t)(a.num_blocks * a.block_size), row = (uint64_t)a.Hkv * kPieceDim * el;
+  const uint64_t dims8[3] = {(uint64_t)kPieceDim, tokens, (uint64_t)a.Hkv};
+  const uint64_t strides8[2] = {row, (uint64_t)kPieceDim};
+  const uint32_t box8[3] = {(uint32_t)kPieceDim, (uint32_t)a.block_size, 1};
+  const uint64_t dims16[4] = {64, 8, (uint64_t)(2 * a.Hkv), tokens / 8};
+  const uint64_t strides16[3] = {row, 128, 8 * row};
+  const uint32_t box16[4] = {64, 8, 2, (uint32_t)(a.block_size / 8)};
+  auto encode = [&](CUtensorMap* m, const void* base) {
+    return encode_tensor_map(m, dt, k8 ? 3 : 4, base, k8 ? dims8 : dims16, k8 ? strides8 : strides16,
+                             k8 ? box8 : box16, CU_TENSOR_MAP_SWIZZLE_128B);
+  };
+  int st = encode(&tk, a.k_cache);
   if (st) return st;
-  st = encode_tensor_map(&tv, dt, 3, a.v_cache, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  st = encode(&tv, a.v_cache);
   if (st) return st;
   PrefixParams p{};
   p.B = a.B, p.Hq = a.Hq, p.Hkv = a.Hkv, p.num_blocks = a.num_blocks, p.max_prefix = a.max_prefix_blocks;
@@ -702,8 +714,8 @@ int launch_prefix(const AttnCall& a, const PieceGeom& g, const PieceSpace& w, cu
   p.splits = w.prefix_splits;
   p.qscale = a.scale * 1.4426950408889634f;
   const size_t smem = 1024 + PrefixSmem<k8>::oBars +
-                      8 * (2 * kPRing16 + 6 + 1 + 3 * kPScaleRing + 2 * (kPCodeRing + kPMoreCodes)) + 8 + 32 + 4 * kPScaleRing * kPMaxPages;
-  static_assert(PrefixSmem<k8>::oBars + 1024 + 512 <= 227 * 1024, "shared memory of a CTA");
+                      8 * (2 * kPRing16 + 6 + 1 + 3 * kPScaleRing + 2 * (kPCodeRing + kPMoreCodes)) + 8 + 32 + 4 * (kPScaleRing * kPMaxPages + 2 * kPList);
+  static_assert(PrefixSmem<k8>::oBars + 1024 + 1024 <= 227 * 1024, "shared memory of a CTA");
   auto kern = prefix_attn_kernel<T, KV>;
   if (k8) {
     // the register split (setmaxnreg) needs what it hands out at launch
