@@ -157,10 +157,10 @@ PieceGeom piece_geometry(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t 
 }
 
 // Splits of the prefix, and the SMs that stream the own pages beside it (g.grid).
-// A CTA of either kernel holds its SM alone.  In units of a prefix key tile's time
-// (2.8 us), a prefix CTA -- (split, pair of 128-row tiles, kv head) -- takes its
-// key tiles + 3 for its start and end; the own pages of 128 tokens of a kv head
-// take 0.27 of an SM, a segment 0.7 more, and the kernel 3 to start and end.
+// A CTA of either kernel holds its SM alone.  Measured, in us: a prefix CTA --
+// (split, pair of 128-row tiles, kv head) -- takes 2.5 for a key tile (2.0 with one row
+// tile) and 13 to start and end; the own pages 1.1 (8-bit: 0.8) for 128 tokens of a
+// kv head and 2 a segment, over their SMs, and 10 to start and end.
 // Both kernels mostly wait at their starts and ends, so side by side on an SM each
 // is best where it fits (64 sequences, prefix 8192: one after the other on
 // all SMs 56 us, 11 splits beside 60 SMs 44 us, 6 beside 100 59 us, 16 beside 20 70 us).
@@ -168,18 +168,20 @@ PieceGeom piece_geometry(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t 
 // pages outweigh it.  Lengths live on the device: the prefix counts with its table's
 // size, the own tokens with half of theirs, and the streaming kernel keeps a
 // sixteenth of the SMs.  Fewest splits within the minimum: each leaves a piece a row to join.
-int share_sms(PieceGeom& g, int64_t Hkv, int64_t bs, int64_t max_prefix_blocks, int64_t max_blocks) {
+int share_sms(PieceGeom& g, int64_t Hkv, int64_t bs, int64_t max_prefix_blocks, int64_t max_blocks,
+              int elem) {
   const int64_t ppt = 128 / bs, tiles = (max_prefix_blocks + ppt - 1) / ppt;
   const int64_t units = (g.seqs * g.G + 255) / 256 * Hkv;
   const int sms = g.grid;
-  const double own = 0.27 / 256 * (double)(g.seqs * max_blocks * bs) * (double)Hkv + 0.7 * (double)(g.seqs * g.n_hg);
+  const double unit = elem == 1 ? 0.8 : 1.1, tile = g.seqs * g.G > 128 ? 2.5 : 2.0;
+  const double own = unit / 256 * (double)(g.seqs * max_blocks * bs) * (double)Hkv + 2.0 * (double)(g.seqs * g.n_hg);
   int64_t best = 1;
   double best_cost = 1e300;
   for (int64_t s = 1; s <= tiles && s <= sms; ++s) {
-    const double prefix = (double)((units * s + sms - 1) / sms * ((tiles + s - 1) / s + 3));
+    const double prefix = (double)((units * s + sms - 1) / sms) * ((double)((tiles + s - 1) / s) * tile + 13);
     const int64_t left = sms - units * s;
-    const double after = prefix + own / sms + 3;
-    const double beside = left * 16 >= sms ? fmax(prefix, own / (double)left + 3) : 1e300;
+    const double after = prefix + own / sms + 10;
+    const double beside = left * 16 >= sms ? fmax(prefix, own / (double)left + 10) : 1e300;
     const double cost = fmin(after, beside);
     if (cost < best_cost) {
       best = s, best_cost = cost;
@@ -256,7 +258,7 @@ int attend(const AttnCall& a, const b200_launch_cfg* cfg, void* workspace, size_
     if (a.cache_dtype == B200_F8E4M3) return launch_attn_generic_e4m3(a, s);
     return launch_attn_generic_16(a, s);
   }
-  const int splits = prefix ? share_sms(g, a.Hkv, a.block_size, a.max_prefix_blocks, a.max_blocks) : 0;
+  const int splits = prefix ? share_sms(g, a.Hkv, a.block_size, a.max_prefix_blocks, a.max_blocks, elem_of(a)) : 0;
   const SpaceBytes sb = space_bytes(g, a.Hq, splits);
   if (workspace == nullptr || workspace_bytes < sb.cum + sb.rows + sb.prefix) return B200_ERR_WORKSPACE;
   if (!aligned16(workspace)) return B200_ERR_ALIGNMENT;
@@ -350,7 +352,7 @@ extern "C" size_t b200_paged_attention_prefix_workspace_size(int64_t B, int64_t 
   const int elem = cache_dtype == B200_I8 || cache_dtype == B200_F8E4M3 ? 1 : 2;
   PieceGeom g = piece_geometry(B, Hq, Hkv, D, block_size, num_blocks, max_blocks, elem, cfg);
   if (!prefix_fits(g, Hkv, block_size, max_prefix_blocks)) return 0;
-  const int splits = share_sms(g, Hkv, block_size, max_prefix_blocks, max_blocks);
+  const int splits = share_sms(g, Hkv, block_size, max_prefix_blocks, max_blocks, elem);
   const SpaceBytes sb = space_bytes(g, Hq, splits);
   return sb.cum + sb.rows + sb.prefix;
 }

@@ -75,37 +75,34 @@ __device__ __forceinline__ float stage_q_rows(const T* __restrict__ q, int r0, i
                                               uint32_t tile, int r_tile, int lane, float qscale) {
   const int c = lane & 15, odd = lane >> 4;
   float factor = qscale;
-#pragma unroll 1
-  for (int i0 = 0; i0 < 16; i0 += 8) {
-    uint4 raw[8];
+  uint4 raw[16];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = r0 + 2 * (i0 + i) + odd;
-      raw[i] = make_uint4(0, 0, 0, 0);
-      if (r < R) {
-        const int64_t row = (int64_t)(r >> lgG) * Hq + (h << lgG) + (r & ((1 << lgG) - 1));
-        raw[i] = __ldg(reinterpret_cast<const uint4*>(q + row * kPieceDim) + c);
-      }
+  for (int i = 0; i < 16; ++i) {
+    const int r = r0 + 2 * i + odd;
+    raw[i] = make_uint4(0, 0, 0, 0);
+    if (r < R) {
+      const int64_t row = (int64_t)(r >> lgG) * Hq + (h << lgG) + (r & ((1 << lgG) - 1));
+      raw[i] = __ldg(reinterpret_cast<const uint4*>(q + row * kPieceDim) + c);
     }
+  }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if constexpr (k8) {
-        float f[8], amax = 0.f, up, down;
-        unpack16<T>(raw[i], f);
+  for (int i = 0; i < 16; ++i) {
+    if constexpr (k8) {
+      float f[8], amax = 0.f, up, down;
+      unpack16<T>(raw[i], f);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) amax = fmaxf(amax, fabsf(f[k]));
+      for (int k = 0; k < 8; ++k) amax = fmaxf(amax, fabsf(f[k]));
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        pow2_scale<13>(amax, up, down);
+      for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      pow2_scale<13>(amax, up, down);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) f[k] *= up;
-        raw[i] = pack16<__half>(f);
-        const float d = __shfl_sync(0xffffffffu, down, (lane & 1) * 16);
-        if (i0 + i == lane >> 1) factor = qscale * d;
-      }
-      const int r = r_tile + 2 * (i0 + i) + odd;
-      if (tile != 0) sts128(tile + (c >> 3) * kPHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4), raw[i]);
+      for (int k = 0; k < 8; ++k) f[k] *= up;
+      raw[i] = pack16<__half>(f);
+      const float d = __shfl_sync(0xffffffffu, down, (lane & 1) * 16);
+      if (i == lane >> 1) factor = qscale * d;
     }
+    const int r = r_tile + 2 * i + odd;
+    if (tile != 0) sts128(tile + (c >> 3) * kPHalf + r * 128 + (((c & 7) ^ (r & 7)) << 4), raw[i]);
   }
   return factor;
 }
@@ -157,15 +154,16 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
   uint64_t* p_full = s_full + 2;                // [2]
   uint64_t* o_done = p_full + 2;                // [2]
   uint64_t* v_fixed = o_done + 2;
-  uint64_t* sc_full = v_fixed + 1;               // [kPScaleRing]
+  uint64_t* q_full = v_fixed + 1;
+  uint64_t* sc_full = q_full + 1;                // [kPScaleRing]
   uint64_t* sc_empty = sc_full + kPScaleRing;    // [kPScaleRing]
   uint64_t* ids_full = sc_empty + kPScaleRing;   // [kPScaleRing]
   uint64_t* code_full = ids_full + kPScaleRing;  // [codes]
   uint64_t* code_empty = code_full + kPCodeRing + kPMoreCodes;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(code_empty + kPCodeRing + kPMoreCodes);
   int* s_abort = reinterpret_cast<int*>(tmem_slot + 1);
-  int* s_count = s_abort + 1;  // [2][4] valid entries before the split and in it, by warp
-  int* s_ids = s_count + 8;    // [kPScaleRing][kPMaxPages] page ids of a key tile
+  int* s_count = s_abort + 1;  // [2][16] valid entries before the split and in it, by warp
+  int* s_ids = s_count + 32;   // [kPScaleRing][kPMaxPages] page ids of a key tile
   int* s_list = s_ids + kPScaleRing * kPMaxPages;  // [K, V][kPList] pages to copy
 
   // the own-token kernel may run beside this one
@@ -183,22 +181,20 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
     const int64_t a = (int64_t)split * per, b = a + per;
     e0 = (int)(a < E ? a : E);
     e1 = (int)(b < E ? b : E);
-    if (warp < 4) {
-      // valid entries before the split and in it, counted by the first four warps
-      int before = 0, in = 0;
-#pragma unroll 4
-      for (int j = threadIdx.x; j < e1; j += 128) {
-        const int64_t id = ptab.at(j);
-        const int ok = id >= 0 && id < p.num_blocks;
-        if (j < e0) before += ok;
-        else in += ok;
-      }
-      before = __reduce_add_sync(0xffffffffu, before);
-      in = __reduce_add_sync(0xffffffffu, in);
-      if (lane == 0) {
-        s_count[warp] = before;
-        s_count[4 + warp] = in;
-      }
+    // valid entries before the split and in it
+    int before = 0, in = 0;
+#pragma unroll 8
+    for (int j = threadIdx.x; j < e1; j += blockDim.x) {
+      const int64_t id = ptab.at(j);
+      const int ok = id >= 0 && id < p.num_blocks;
+      if (j < e0) before += ok;
+      else in += ok;
+    }
+    before = __reduce_add_sync(0xffffffffu, before);
+    in = __reduce_add_sync(0xffffffffu, in);
+    if (lane == 0) {
+      s_count[warp] = before;
+      s_count[16 + warp] = in;
     }
   }
   if (threadIdx.x == 32) {
@@ -213,6 +209,7 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
       sm100::mbar_init(sm100::smem_u32(&o_done[i]), 1);
     }
     sm100::mbar_init(sm100::smem_u32(v_fixed), 1);
+    sm100::mbar_init(sm100::smem_u32(q_full), 8);
     for (int i = 0; i < kPScaleRing; ++i) {
       sm100::mbar_init(sm100::smem_u32(&sc_full[i]), 4);
       sm100::mbar_init(sm100::smem_u32(&ids_full[i]), 1);
@@ -237,24 +234,17 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
     sm100::tmem_alloc(sm100::smem_u32(tmem_slot), 512);
     sm100::tmem_relinquish();
   }
-  // the softmax warps stage Q meanwhile (with one row tile the second warpgroup
-  // only takes its rows' factors)
-  float sl = p.qscale;
-  if (warp >= 4 && warp < 12) {
-    const int t = (warp >> 2) - 1, rw = (warp & 3) * 32;
-    const uint32_t tile = t == 0 || both ? sbase + L::oQ + t * kPTile : 0;
-    if (k8 || tile != 0)
-      sl = stage_q_rows<T, k8>(q, row0 + both * t * kPM + rw, R, p.Hq, h, p.lgG, tile, rw, lane, p.qscale);
-    sm100::fence_proxy_async_smem();
-  }
   sm100::tc_fence_before();
   __syncthreads();
   sm100::tc_fence_after();
   const uint32_t tmem = *tmem_slot;  // columns: S_t at 128 t, O_t at 256 + 128 t
   int ntok;
   {
-    const int before = s_count[0] + s_count[1] + s_count[2] + s_count[3];
-    const int in = s_count[4] + s_count[5] + s_count[6] + s_count[7];
+    int before = 0, in = 0;
+    for (int w = 0; w < (int)(blockDim.x >> 5); ++w) {
+      before += s_count[w];
+      in += s_count[16 + w];
+    }
     const int64_t left = plen_tokens - (int64_t)before * bs, have = (int64_t)in * bs;
     ntok = (int)(left < 0 ? 0 : (left < have ? left : have));
   }
@@ -353,7 +343,7 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
     const uint64_t dq = sm100::make_smem_desc(sbase + L::oQ, 16, 1024, sm100::kSwizzle128B);
     const uint64_t dk = sm100::make_smem_desc(sbase + L::oRing, 16, 2048, sm100::kSwizzle128B);
     const uint64_t dv = sm100::make_smem_desc(sbase + L::oRing, 1024, 2048, sm100::kSwizzle128B);
-    bool ok = nkt > 0;
+    bool ok = nkt > 0 && sm100::mbar_wait_warp(sm100::smem_u32(q_full), 0);
     auto full = [&](int it) -> bool {
       return sm100::mbar_wait_warp(sm100::smem_u32(&ring_full[it % kRing]), (it / kRing) & 1);
     };
@@ -514,6 +504,16 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
     const int64_t qrow = live ? (int64_t)(qr >> p.lgG) * p.Hq + (h << p.lgG) + (qr & ((1 << p.lgG) - 1)) : 0;
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
     const uint32_t tS = tmem + t * 128 + lane_off, tO = tmem + 256 + t * 128 + lane_off;
+    // Q, while the first pages are on their way (with one row tile the second
+    // warpgroup only takes its rows' factors)
+    const uint32_t q_tile = t == 0 || both ? sbase + L::oQ + t * kPTile : 0;
+    float sl = p.qscale;
+    if (k8 || q_tile != 0)
+      sl = stage_q_rows<T, k8>(q, row0 + both * t * kPM + quarter * 32, R, p.Hq, h, p.lgG, q_tile, quarter * 32, lane,
+                               p.qscale);
+    sm100::fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) sm100::mbar_arrive(sm100::smem_u32(q_full));
     float m_used = -INFINITY, l = 0.f;
     bool ok = true;
     const int n_tiles = both ? nkt : (nkt - t + 1) / 2;  // key tiles of this stream
@@ -714,7 +714,7 @@ int launch_prefix(const AttnCall& a, const PieceGeom& g, const PieceSpace& w, cu
   p.splits = w.prefix_splits;
   p.qscale = a.scale * 1.4426950408889634f;
   const size_t smem = 1024 + PrefixSmem<k8>::oBars +
-                      8 * (2 * kPRing16 + 6 + 1 + 3 * kPScaleRing + 2 * (kPCodeRing + kPMoreCodes)) + 8 + 32 + 4 * (kPScaleRing * kPMaxPages + 2 * kPList);
+                      8 * (2 * kPRing16 + 6 + 2 + 3 * kPScaleRing + 2 * (kPCodeRing + kPMoreCodes)) + 8 + 128 + 4 * (kPScaleRing * kPMaxPages + 2 * kPList);
   static_assert(PrefixSmem<k8>::oBars + 1024 + 1024 <= 227 * 1024, "shared memory of a CTA");
   auto kern = prefix_attn_kernel<T, KV>;
   if (k8) {
