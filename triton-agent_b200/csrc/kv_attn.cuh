@@ -31,6 +31,7 @@
 namespace b200 {
 
 constexpr int kPieceDim = 128;
+constexpr int kChunk = 16;  // tokens of a chunk
 constexpr int kPiecePitch = kPieceDim + 8;  // floats of a piece row: o[128], m, l, pad to whole 32-byte sectors
 constexpr int kMaxSeg = 2048;               // (sequence, head group) segments a launch takes
 
@@ -479,33 +480,33 @@ __device__ __forceinline__ void mma_pair8(uint32_t at, const Lane8& x, const int
   }
 }
 
-// One chunk of a 16-bit cache: K and V as two boxes of 64 dims each, `box` bytes apart.
+// One chunk of a 16-bit cache: K and V as [half of the dims][token][64] rows.
 template <typename T>
-__device__ __forceinline__ void mma_chunk16(uint32_t kb, uint32_t vb, uint32_t box, int ntok, int row0,
-                                            int lane, float sl, const uint32_t (&qb)[8][2], float (&o)[8][4],
+__device__ __forceinline__ void mma_chunk16(uint32_t kb, uint32_t vb, int ntok, int lane, float sl, const uint32_t (&qb)[8][2], float (&o)[8][4],
                                             float (&mu)[2], float (&lp)[2]) {
+  constexpr uint32_t kHalf = kChunk * 128;
   const int mat = lane >> 3, mrow = lane & 7;
   const int tr = lane >> 2, tq = (lane & 3) * 2;
   float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
   {
     // A = K rows: matrix `mat` = (token half mat&1, dim-chunk parity mat>>1)
-    const int row = row0 + (mat & 1) * 8 + mrow;
+    const int row = (mat & 1) * 8 + mrow;
     const uint32_t at = kb + row * 128, sw = ((mat >> 1) ^ (row & 7)) << 4;
 #pragma unroll
     for (int ks = 0; ks < 8; ++ks) {
       uint32_t a0, a1, a2, a3;
-      ldsm_x4(at + (ks >> 2) * box + (sw ^ ((ks & 3) << 5)), a0, a1, a2, a3);
+      ldsm_x4(at + (ks >> 2) * kHalf + (sw ^ ((ks & 3) << 5)), a0, a1, a2, a3);
       mma16816<T>((ks & 1) ? s1 : s0, a0, a1, a2, a3, qb[ks][0], qb[ks][1]);
     }
   }
   // A = V^T by ldmatrix.trans: matrix `mat` = (token half mat>>1, dim-chunk parity mat&1)
   uint32_t va[8][4];
   {
-    const int row = row0 + (mat >> 1) * 8 + mrow;
+    const int row = (mat >> 1) * 8 + mrow;
     const uint32_t at = vb + row * 128, sw = ((mat & 1) ^ (row & 7)) << 4;
 #pragma unroll
     for (int mt = 0; mt < 8; ++mt)
-      ldsm_x4_t(at + (mt >> 2) * box + (sw ^ ((mt & 3) << 5)), va[mt][0], va[mt][1], va[mt][2], va[mt][3]);
+      ldsm_x4_t(at + (mt >> 2) * kHalf + (sw ^ ((mt & 3) << 5)), va[mt][0], va[mt][1], va[mt][2], va[mt][3]);
   }
   float y[4];
 #pragma unroll
@@ -575,7 +576,6 @@ struct PiecesParams {
   float qscale;  // scale * log2(e)
 };
 
-constexpr int kChunk = 16;     // tokens of a chunk
 constexpr int kConsumers = 8;  // consumer warps, at most
 struct EntryMeta {
   int kind;  // 0 tokens, 1 end of segment, 2 end of stream
@@ -626,13 +626,15 @@ __global__ void __launch_bounds__((kConsumers + 1) * 32, 1)
   // the join kernel may be scheduled; it waits for this grid
   asm volatile("griddepcontrol.launch_dependents;");
   // ---- prologue: contexts, entries before each segment, barriers
-  if (warp == consumers) {
+  {
     const int64_t most = p.max_blocks * bs;
-    for (int64_t b = lane; b < B; b += 32) {
+    for (int64_t b = threadIdx.x; b < B; b += blockDim.x) {
       const int64_t c = clen.at(b);
       s_ctx[b] = (int)(c < 0 ? 0 : (c < most ? c : most));
     }
-    __syncwarp();
+    __syncthreads();
+  }
+  if (warp == consumers) {
     int run = 0;
     for (int s0 = 0; s0 < p.nseg; s0 += 32) {
       const int s = s0 + lane;
@@ -712,15 +714,14 @@ __global__ void __launch_bounds__((kConsumers + 1) * 32, 1)
     const uint32_t sbox = (uint32_t)(HG * kChunk * 4);
     const uint32_t chunk_tx = k8 ? 2 * box + 2 * sbox : 4 * box;
     const uint32_t chunk_bytes = k8 ? 2 * box + 1024 : 4 * box;
-    int fill = 0;  // (lane 0) chunks in the open entry
     const unsigned lt_mask = (1u << lane) - 1u;
     int it = 0, st = 0;
     uint32_t ph = 1;  // parity of the empty barriers in this round
     bool ok = true, waited = p.overlap != 0;
-    // lane 0: the next ring entry, free to fill; false when the wait gave up
+    // the next ring entry, free to fill; false when the wait gave up
     auto acquire = [&]() -> bool {
-      if (*(volatile int*)s_abort) return false;
-      return sm100::mbar_wait(sm100::smem_u32(&empty_bar[st]), ph);
+      const bool got = !*(volatile int*)s_abort && sm100::mbar_wait(sm100::smem_u32(&empty_bar[st]), ph);
+      return __all_sync(0xffffffffu, got);
     };
     auto advance = [&]() {
       ++it;
@@ -732,10 +733,50 @@ __global__ void __launch_bounds__((kConsumers + 1) * 32, 1)
     auto markers = [&](int kind, int seg, int piece) -> bool {  // one for each slot
       for (int i = 0; i < sub; ++i) {
         if (!acquire()) return false;
-        meta[st] = EntryMeta{kind, seg, 0, piece};
-        sm100::mbar_arrive(sm100::smem_u32(&full_bar[st]));
+        if (lane == 0) {
+          meta[st] = EntryMeta{kind, seg, 0, piece};
+          sm100::mbar_arrive(sm100::smem_u32(&full_bar[st]));
+        }
         advance();
       }
+      return true;
+    };
+    // The open entry's chunks: page, first token, live tokens.  Its copies are
+    // issued by a lane each: as one lane's instructions in turn they took about 350
+    // cycles each and bounded small boxes (48 sequences of 4 kv heads: 61 us).
+    int fill = 0, c_id[2] = {0, 0}, c_t0[2] = {0, 0}, c_live[2] = {0, 0};
+    auto issue_entry = [&](int seg, int h0) -> bool {
+      if (!acquire()) return false;
+      if (!waited) {  // programmatic launch: the first copy waits for the previous kernel
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        waited = true;
+      }
+      const uint32_t fb = sm100::smem_u32(&full_bar[st]), dst = base + st * p.entry_bytes;
+      if (lane == 0) {
+        meta[st] = EntryMeta{0, seg, c_live[0], fill > 1 ? c_live[1] : 0};
+        sm100::mbar_arrive_expect_tx(fb, fill * chunk_tx);
+      }
+      __syncwarp();
+      const int odd = lane & 1;
+      if constexpr (k8) {
+        const int ch = lane >> 2;  // lanes of a chunk: K, V, and their scales
+        if (ch < fill) {
+          const uint32_t cd = dst + ch * chunk_bytes;
+          const int id = ch ? c_id[1] : c_id[0], t0 = ch ? c_t0[1] : c_t0[0];
+          if ((lane & 2) == 0) {
+            sm100::tma_load_3d(cd + odd * box, odd ? &tm_v : &tm_k, fb, 0, id * bs + t0, h0);
+          } else if (p.scale_maps) {
+            sm100::tma_load_2d(cd + 2 * box + odd * 512, odd ? &tm_vs : &tm_ks, fb, t0, id * (int32_t)p.Hkv + h0);
+          } else {
+            const int64_t sat = ((int64_t)id * p.Hkv + h0) * kChunk;
+            bulk_load(cd + 2 * box + odd * 512, (odd ? v_scale : k_scale) + sat, sbox, fb);
+          }
+        }
+      } else {
+        if (lane < 2) sm100::tma_load_3d(dst + odd * 2 * box, odd ? &tm_v : &tm_k, fb, 0, c_id[0] * bs + c_t0[0], 2 * h0);
+      }
+      fill = 0;
+      advance();
       return true;
     };
     int s = seg0;
@@ -767,75 +808,29 @@ __global__ void __launch_bounds__((kConsumers + 1) * 32, 1)
         }
         inval += __popc(ib);
         __syncwarp();
-        if (lane == 0) {
-          const int n = __popc(ub);
-          for (int u = 0; u < n && ok; ++u) {
-            const int32_t id = chunk_id[u], h0 = hg * HG;
-            const int nt_page = chunk_ntok[u];
-            for (int t0 = 0; t0 < nt_page; t0 += kChunk) {
-              if (fill == 0) {
-                ok = acquire();
-                if (!ok) break;
-                if (!waited) {  // programmatic launch: the first copy waits for the previous kernel
-                  asm volatile("griddepcontrol.wait;" ::: "memory");
-                  waited = true;
-                }
-              }
-              const int live = nt_page - t0 < kChunk ? nt_page - t0 : kChunk;
-              const uint32_t fb = sm100::smem_u32(&full_bar[st]);
-              const uint32_t dst = base + st * p.entry_bytes + fill * chunk_bytes;
-              const int32_t tok0 = id * bs + t0;
-              if (fill == 0) meta[st] = EntryMeta{0, s, live, 0};
-              else meta[st].piece = live;
-              ++fill;
-              const bool full = !k8 || fill == 2;
-              // an entry's one arrival comes with its last chunk; the first only adds bytes
-              if (full) sm100::mbar_arrive_expect_tx(fb, chunk_tx);
-              else
-                asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(fb), "r"(chunk_tx)
-                             : "memory");
-              if constexpr (k8) {
-                sm100::tma_load_3d(dst, &tm_k, fb, 0, tok0, h0);
-                sm100::tma_load_3d(dst + box, &tm_v, fb, 0, tok0, h0);
-                if (p.scale_maps) {
-                  sm100::tma_load_2d(dst + 2 * box, &tm_ks, fb, t0, id * (int32_t)p.Hkv + h0);
-                  sm100::tma_load_2d(dst + 2 * box + 512, &tm_vs, fb, t0, id * (int32_t)p.Hkv + h0);
-                } else {
-                  const int64_t sat = ((int64_t)id * p.Hkv + h0) * kChunk;
-                  bulk_load(dst + 2 * box, k_scale + sat, sbox, fb);
-                  bulk_load(dst + 2 * box + 512, v_scale + sat, sbox, fb);
-                }
-              } else {
-                sm100::tma_load_3d(dst, &tm_k, fb, 0, tok0, h0);
-                sm100::tma_load_3d(dst + box, &tm_k, fb, 64, tok0, h0);
-                sm100::tma_load_3d(dst + 2 * box, &tm_v, fb, 0, tok0, h0);
-                sm100::tma_load_3d(dst + 3 * box, &tm_v, fb, 64, tok0, h0);
-              }
-              if (full) {
-                advance();
-                fill = 0;
-              }
-            }
+        const int n = __popc(ub);
+        for (int u = 0; u < n && ok; ++u) {
+          const int page = chunk_id[u], nt_page = chunk_ntok[u];
+          for (int t0 = 0; t0 < nt_page && ok; t0 += kChunk) {
+            const int live = nt_page - t0 < kChunk ? nt_page - t0 : kChunk;
+            if (fill == 0) c_id[0] = page, c_t0[0] = t0, c_live[0] = live;
+            else c_id[1] = page, c_t0[1] = t0, c_live[1] = live;
+            ++fill;
+            if (!k8 || fill == 2) ok = issue_entry(s, hg * HG);
           }
         }
-        ok = __shfl_sync(0xffffffffu, ok, 0);
         __syncwarp();
       }
-      if (lane == 0 && ok) {
-        if (fill > 0) {  // the segment ends in the first chunk of an entry
-          sm100::mbar_arrive(sm100::smem_u32(&full_bar[st]));
-          advance();
-          fill = 0;
-        }
+      if (ok && fill > 0) ok = issue_entry(s, hg * HG);  // the segment ends in the first chunk of an entry
+      if (ok) {
         const bool one = range_of(segs, E, R) == range_of(sege - 1, E, R);
         ok = markers(1, s, one && !p.always ? -1 : s + c);
       }
-      ok = __shfl_sync(0xffffffffu, ok, 0);
       e = segs + j1;
       if (e == sege) ++s;
     }
+    if (ok) ok = markers(2, 0, 0);
     if (lane == 0) {
-      if (ok) ok = markers(2, 0, 0);
       if (!ok) {
         b200_dev_error(kDevErrTimeoutEmpty);
         atomicExch(s_abort, 1);
@@ -885,7 +880,7 @@ __global__ void __launch_bounds__((kConsumers + 1) * 32, 1)
           const int nt[2] = {m.ntok, m.piece};
           mma_pair8<KV>(pg, lane8, nt, lane, slA, slB, qf, o, mu, lp);
         } else {
-          mma_chunk16<T>(pg, pg + 2 * box, box, m.ntok, w * kChunk, lane, p.qscale, qb, o, mu, lp);
+          mma_chunk16<T>(pg + w * kChunk * 256, pg + 2 * box + w * kChunk * 256, m.ntok, lane, p.qscale, qb, o, mu, lp);
         }
       } else if (m.kind == 1) {
         bool write = true;
@@ -984,11 +979,11 @@ int launch_pieces(const AttnCall& a, const PieceGeom& g, const PieceSpace& w, bo
   const CUtensorMapDataType dt = k8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                     : (std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                                       : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16);
-  // dims (d, token slot, head): a box of 128 bytes of dims x 16 tokens x HG heads
-  // lands as rows ordered (head, token) of 128 bytes, swizzled in 8-row atoms
-  const uint64_t dims[3] = {(uint64_t)kD, (uint64_t)(a.num_blocks * a.block_size), (uint64_t)a.Hkv};
-  const uint64_t strides[2] = {(uint64_t)a.Hkv * kD * el, (uint64_t)kD * el};
-  const uint32_t box[3] = {(uint32_t)(128 / el), (uint32_t)kChunk, (uint32_t)g.HG};
+  // dims (128 bytes of dims, token slot, head or half of its dims): a box of 16
+  // tokens x HG heads lands as [head][half][token] rows of 128 bytes, swizzled in 8-row atoms
+  const uint64_t dims[3] = {128 / el, (uint64_t)(a.num_blocks * a.block_size), (uint64_t)a.Hkv * el};
+  const uint64_t strides[2] = {(uint64_t)a.Hkv * kD * el, 128};
+  const uint32_t box[3] = {(uint32_t)(128 / el), (uint32_t)kChunk, (uint32_t)(g.HG * el)};
   int st = encode_tensor_map(&tk, dt, 3, a.k_cache, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
   if (st) return st;
   st = encode_tensor_map(&tv, dt, 3, a.v_cache, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
