@@ -25,6 +25,13 @@ struct JoinParams {
   int heads_cta, nseg, grid, always, splits, W;
 };
 
+// Two entries in two ranges, and a piece with a sum but no values.
+struct JoinNothing {
+  int32_t cum[4];
+  float piece[kPiecePitch];
+};
+__device__ const JoinNothing g_join_nothing = {{0, 1, 2, 0}, {}};
+
 template <typename T>
 __global__ void __launch_bounds__(256)
     paged_attn_join_kernel(const int32_t* __restrict__ cum, const float* __restrict__ rows,
@@ -37,63 +44,77 @@ __global__ void __launch_bounds__(256)
   const int64_t b = live ? row / p.Hq : 0;
   const int h = (int)(row - b * p.Hq), hg = h / p.heads_cta, hh = h - hg * p.heads_cta;
   const int seg = (int)(hg * p.B + b);
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  int c1 = 0, own = 0;
-  bool done = !live;
-  if (live) {
-    const int64_t E = __ldcg(&cum[p.nseg]), s0 = __ldcg(&cum[seg]), s1 = __ldcg(&cum[seg + 1]);
-    const int64_t R = E < p.grid ? E : p.grid;
-    if (s1 > s0) {
-      c1 = range_of(s0, E, R);
-      const int c2 = range_of(s1 - 1, E, R);
-      done = c1 == c2 && !p.always;
-      own = c2 - c1 + 1;
-    }
-  }
-  const int n = done ? 0 : own + p.splits;
-  auto piece = [&](int i) -> const float* {
-    return i < own ? rows + (((int64_t)seg + c1 + i) * p.heads_cta + hh) * kPiecePitch
-                   : prefix + ((int64_t)(i - own) * p.B * p.Hq + row) * kPiecePitch;
-  };
-  // weight of a piece: none without tokens (l = 0); NaN logits only leave m
-  // without a value and l = NaN
-  auto weight = [](float m, float l, float M) { return l == 0.f ? 0.f : (m > -1e29f ? ex2(m - M) : l); };
-  float M = -INFINITY;
-  for (int i = lane; i < n; i += 32) M = fmaxf(M, __ldcg(piece(i) + kD));
-  M = warp_max(M);
   float L = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  // this warp's share: pieces share, share + W, ...; 32 of them at a time
-  const int mine = n > share ? (n - share + W - 1) / W : 0;
-  for (int i0 = 0; i0 < mine; i0 += 32) {
-    float w = 0.f;
-    if (i0 + lane < mine) {
-      const float2 ml = __ldcg(reinterpret_cast<const float2*>(piece(share + (i0 + lane) * W) + kD));
-      w = weight(ml.x, ml.y, M);
-      if (w != 0.f) L += w * ml.y;
-    }
-    const int nb = mine - i0 < 32 ? mine - i0 : 32;
-    for (int u0 = 0; u0 < nb; u0 += 4) {
-      float4 v[4];
-      float wu[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        wu[u] = __shfl_sync(0xffffffffu, w, (u0 + u) & 31);
-        if (u0 + u >= nb) wu[u] = 0.f;
-        v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (wu[u] != 0.f)
-          v[u] = __ldcg(reinterpret_cast<const float4*>(piece(share + (i0 + u0 + u) * W) + 4 * lane));
-      }
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        acc.x = fmaf(wu[u], v[u].x, acc.x);
-        acc.y = fmaf(wu[u], v[u].y, acc.y);
-        acc.z = fmaf(wu[u], v[u].z, acc.z);
-        acc.w = fmaf(wu[u], v[u].w, acc.w);
+  bool done = true;
+  // Twice: first over two pieces of nothing, while the streaming kernel still runs, so that
+  // the second pass finds its instructions near (pages streamed through the L2
+  // have driven them out of it, and fetching them costs more than the reads).
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
+    const bool real = pass == 1;
+    if (real) asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int32_t* at = real ? cum : g_join_nothing.cum;
+    int c1 = 0, own = 0;
+    done = real && !live;
+    if (!done) {
+      const int64_t E = __ldcg(&at[real ? p.nseg : 2]), s0 = __ldcg(&at[real ? seg : 0]);
+      const int64_t s1 = __ldcg(&at[real ? seg + 1 : 2]);
+      const int64_t R = E < p.grid ? E : p.grid;
+      if (s1 > s0) {
+        c1 = range_of(s0, E, R);
+        const int c2 = range_of(s1 - 1, E, R);
+        done = real && c1 == c2 && !p.always;
+        own = c2 - c1 + 1;
       }
     }
+    const int n = done ? 0 : own + (real ? p.splits : 0);
+    const float* const own0 =
+        real ? rows + (((int64_t)seg + c1) * p.heads_cta + hh) * kPiecePitch : g_join_nothing.piece;
+    const float* const pre0 = prefix + (row - (int64_t)own * p.B * p.Hq) * kPiecePitch;
+    const int64_t own_step = real ? (int64_t)p.heads_cta * kPiecePitch : 0, pre_step = p.B * p.Hq * kPiecePitch;
+    auto piece = [&](int i) -> const float* { return i < own ? own0 + i * own_step : pre0 + i * pre_step; };
+    // weight of a piece: none without tokens (l = 0); NaN logits only leave m
+    // without a value and l = NaN
+    auto weight = [](float m, float l, float M) { return l == 0.f ? 0.f : (m > -1e29f ? ex2(m - M) : l); };
+    float M = -INFINITY;
+    for (int i = lane; i < n; i += 32) M = fmaxf(M, __ldcg(piece(i) + kD));
+    M = warp_max(M);
+    L = 0.f;
+    acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    // this warp's share: pieces share, share + W, ...; 32 of them at a time
+    const int first = real ? share : 0, step = real ? W : 1;
+    const int mine = n > first ? (n - first + step - 1) / step : 0;
+    for (int i0 = 0; i0 < mine; i0 += 32) {
+      float w = 0.f;
+      if (i0 + lane < mine) {
+        const float2 ml = __ldcg(reinterpret_cast<const float2*>(piece(first + (i0 + lane) * step) + kD));
+        w = weight(ml.x, ml.y, M);
+        if (w != 0.f) L += w * ml.y;
+      }
+      const int nb = mine - i0 < 32 ? mine - i0 : 32;
+      for (int u0 = 0; u0 < nb; u0 += 4) {
+        float4 v[4];
+        float wu[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          wu[u] = __shfl_sync(0xffffffffu, w, (u0 + u) & 31);
+          if (u0 + u >= nb) wu[u] = 0.f;
+          v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (wu[u] != 0.f)
+            v[u] = __ldcg(reinterpret_cast<const float4*>(piece(first + (i0 + u0 + u) * step) + 4 * lane));
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          acc.x = fmaf(wu[u], v[u].x, acc.x);
+          acc.y = fmaf(wu[u], v[u].y, acc.y);
+          acc.z = fmaf(wu[u], v[u].z, acc.z);
+          acc.w = fmaf(wu[u], v[u].w, acc.w);
+        }
+      }
+    }
+    L = warp_sum(L);
   }
-  L = warp_sum(L);
   if (W > 1) {
     *reinterpret_cast<float4*>(&s_part[warp][4 * lane]) = acc;
     if (lane == 0) s_part[warp][kD] = L;
