@@ -311,14 +311,18 @@ int b200_paged_kv_dequant(const void* k_cache, const void* v_cache, const float*
                           const b200_launch_cfg* cfg, void* stream);
 
 /* Paged decode attention over an 8-bit cache: b200_paged_attention of the
- * cache's values code * scale, without writing them out.  Softmax, sums and
- * accumulation in fp32; the softmax weights enter the second product as f16.  A sequence without
- * tokens gives a zero row.  workspace: 16-byte aligned, of
- * b200_paged_attention_quant_workspace_size() bytes (may be 0: NULL); nothing
- * in it is kept between calls, it needs no clearing.  Streaming kernel for D = 128, block sizes
- * of 16, 32, ..., 256, 1, 2, 4 or 8 query heads a kv head and 16-byte aligned
- * tensors; a general kernel for the rest (D <= 256).  cfg: stages (ring depth in entries of 32 tokens, default about 204
- * KB), rows_per_cta (kv heads per CTA, at most 8), flags bit 0: general kernel; bit 3: programmatic
+ * cache's values code * scale, without writing them out.  Softmax statistics,
+ * sums and accumulation in fp32.  int8: the queries enter as 24-bit integers
+ * (off by 2^-23 of a row's largest), the softmax weights as 16-bit integers
+ * relative to the largest of their 32 tokens (off by 2^-17 of that); e4m3:
+ * both as f16.  A sequence without tokens gives a zero row.  workspace:
+ * 16-byte aligned, of b200_paged_attention_quant_workspace_size() bytes (may
+ * be 0: NULL); nothing in it is kept between calls, it needs no clearing.
+ * Streaming kernel for D = 128, block sizes of 16, 32, ..., 256, 1, 2, 4 or 8
+ * query heads a kv head and 16-byte aligned tensors; a general kernel for the
+ * rest (D <= 256).  cfg: stages (ring depth in entries of 32 tokens, of 16
+ * over 16-bit caches; default about 204 KB), rows_per_cta (kv heads per CTA,
+ * at most 8), flags bit 0: general kernel; bit 3: programmatic
  * dependent launch (the kernel's prologue overlaps the previous kernel on
  * the stream; the caller guarantees that kernel writes neither context_len
  * nor block_table, as the append does not). */
@@ -341,8 +345,10 @@ int b200_paged_attention_quant(const void* q, const void* k_cache, const void* v
  * of a kv head.  Caches of `cache_dtype`: dtype itself (scales NULL), or
  * B200_I8 / B200_F8E4M3 with scales as above.  prefix_len, context_len and
  * the tables are of `index_dtype` and on the device.  A sequence without any
- * token gives a zero row.  workspace, cfg and limits as
- * b200_paged_attention_quant. */
+ * token gives a zero row.  Softmax weights enter the second product in the
+ * cache's 16-bit type, over 8-bit prefixes as f16.  workspace, cfg and limits
+ * as b200_paged_attention_quant (the prefix's product takes block sizes up to
+ * 128; larger ones go to the general kernel). */
 size_t b200_paged_attention_prefix_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t num_blocks,
                                                   int64_t block_size, int64_t max_prefix_blocks,
                                                   int64_t max_blocks, int32_t cache_dtype,

@@ -371,8 +371,8 @@ def rope_kv_append_paged_quant(q, k, v, positions, cos, sin, slot_mapping, k_cac
     dev = _on_one_device(op, k, q, v, positions, cos, sin, slot_mapping, k_cache, v_cache, k_scale, v_scale, q_out)
     if _elsewhere(dev):
         with torch.cuda.device(dev):
-            return rope_kv_append_paged_quant(q, k, v, positions, cos, sin, slot_mapping, k_cache, v_cache, k_scale, v_scale,
-                                              q_out, cfg)
+            return rope_kv_append_paged_quant(q, k, v, positions, cos, sin, slot_mapping, k_cache, v_cache, k_scale,
+                                              v_scale, q_out, cfg)
     nb, bs, Hkv, D = _check_cache(op, k_cache, v_cache, k_scale, v_scale)
     if not (k.is_contiguous() and v.is_contiguous() and cos.is_contiguous() and sin.is_contiguous() and
             (q is None or q.is_contiguous())):
@@ -461,7 +461,8 @@ def paged_attention_quant(q, k_cache, v_cache, k_scale, v_scale, block_table, co
     dev = _on_one_device(op, q, k_cache, v_cache, k_scale, v_scale, block_table, context_len, out)
     if _elsewhere(dev):
         with torch.cuda.device(dev):
-            return paged_attention_quant(q, k_cache, v_cache, k_scale, v_scale, block_table, context_len, scale, out, cfg)
+            return paged_attention_quant(q, k_cache, v_cache, k_scale, v_scale, block_table, context_len, scale, out,
+                                         cfg)
     nb, bs, Hkv, D = _check_cache(op, k_cache, v_cache, k_scale, v_scale)
     if q.dim() != 3 or q.shape[2] != D or block_table.dim() != 2:
         raise L.B200OpsError(L.ERR_BAD_ARG, op, "q must be [B, Hq, D] and block_table [B, max_blocks]")

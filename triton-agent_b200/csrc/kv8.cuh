@@ -63,7 +63,8 @@ __device__ __forceinline__ void kv8_in_order(uint32_t w, uint32_t& lo, uint32_t&
                : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])                                               \
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), __VA_ARGS__)
 template <bool UB>
-__device__ __forceinline__ void mma8_start(int32_t (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, int32_t c) {
+__device__ __forceinline__ void mma8_start(int32_t (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
+                                           int32_t c) {
   if constexpr (UB) B200_MMA8("s32.s8.u8.s32", "{%10,%10,%10,%10}", "r"(c));
   else B200_MMA8("s32.s8.s8.s32", "{%10,%10,%10,%10}", "r"(c));
 }

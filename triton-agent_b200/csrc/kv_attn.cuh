@@ -97,7 +97,10 @@ __device__ __forceinline__ float lds_f32(uint32_t a) {
 }
 __device__ __forceinline__ float4 lds_f32x4(uint32_t a) {
   float4 v;
-  asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
+  asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(a)
+               : "memory");
   return v;
 }
 __device__ __forceinline__ int lds_s32(uint32_t a) {
@@ -482,8 +485,8 @@ __device__ __forceinline__ void mma_pair8(uint32_t at, const Lane8& x, const int
 
 // One chunk of a 16-bit cache: K and V as [half of the dims][token][64] rows.
 template <typename T>
-__device__ __forceinline__ void mma_chunk16(uint32_t kb, uint32_t vb, int ntok, int lane, float sl, const uint32_t (&qb)[8][2], float (&o)[8][4],
-                                            float (&mu)[2], float (&lp)[2]) {
+__device__ __forceinline__ void mma_chunk16(uint32_t kb, uint32_t vb, int ntok, int lane, float sl,
+                                            const uint32_t (&qb)[8][2], float (&o)[8][4], float (&mu)[2], float (&lp)[2]) {
   constexpr uint32_t kHalf = kChunk * 128;
   const int mat = lane >> 3, mrow = lane & 7;
   const int tr = lane >> 2, tq = (lane & 3) * 2;
@@ -586,7 +589,9 @@ struct EntryMeta {
 constexpr int kXchPitch = 36 * 32;  // floats a warp hands over: 32 o, 2 m, 2 l a lane
 
 __device__ __forceinline__ int64_t range_lo(int64_t c, int64_t E, int64_t R) { return c * E / R; }
-__device__ __forceinline__ int range_of(int64_t e, int64_t E, int64_t R) { return (int)(((e + 1) * R + E - 1) / E - 1); }
+__device__ __forceinline__ int range_of(int64_t e, int64_t E, int64_t R) {
+  return (int)(((e + 1) * R + E - 1) / E - 1);
+}
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile(
@@ -773,7 +778,8 @@ __global__ void __launch_bounds__((kConsumers + 1) * 32, 1)
           }
         }
       } else {
-        if (lane < 2) sm100::tma_load_3d(dst + odd * 2 * box, odd ? &tm_v : &tm_k, fb, 0, c_id[0] * bs + c_t0[0], 2 * h0);
+        if (lane < 2)
+          sm100::tma_load_3d(dst + odd * 2 * box, odd ? &tm_v : &tm_k, fb, 0, c_id[0] * bs + c_t0[0], 2 * h0);
       }
       fill = 0;
       advance();

@@ -700,7 +700,8 @@ extern "C" int b200_rope_kv_append_paged_quant(const void* q, const void* k, con
   if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return B200_ERR_WORKSPACE;
   if (need > 0 && !aligned16(workspace)) return B200_ERR_ALIGNMENT;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  AppendParams p{T, D, num_blocks * block_size, cs_rows, block_size, q ? (int)Hq : 0, (int)Hkv, -1, {nullptr, nullptr, nullptr, 0}};
+  AppendParams p{T,         D, num_blocks * block_size, cs_rows, block_size, q ? (int)Hq : 0,
+                 (int)Hkv, -1, {nullptr, nullptr, nullptr, 0}};
   for (int i = 0; i < 17; ++i)
     if (block_size == (1ll << i)) p.lg_bs = i;
   return B200_DISPATCH_HALF(dtype, [&]() -> int {

@@ -714,7 +714,8 @@ int launch_prefix(const AttnCall& a, const PieceGeom& g, const PieceSpace& w, cu
   p.splits = w.prefix_splits;
   p.qscale = a.scale * 1.4426950408889634f;
   const size_t smem = 1024 + PrefixSmem<k8>::oBars +
-                      8 * (2 * kPRing16 + 6 + 2 + 3 * kPScaleRing + 2 * (kPCodeRing + kPMoreCodes)) + 8 + 128 + 4 * (kPScaleRing * kPMaxPages + 2 * kPList);
+                      8 * (2 * kPRing16 + 6 + 2 + 3 * kPScaleRing + 2 * (kPCodeRing + kPMoreCodes)) + 8 + 128 +
+                      4 * (kPScaleRing * kPMaxPages + 2 * kPList);
   static_assert(PrefixSmem<k8>::oBars + 1024 + 1024 <= 227 * 1024, "shared memory of a CTA");
   auto kern = prefix_attn_kernel<T, KV>;
   if (k8) {
