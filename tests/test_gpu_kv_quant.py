@@ -251,6 +251,24 @@ def test_context_longer_than_the_table(cuda_device):
 
 
 @pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("B,Hkv,bs,pages", [(1, 8, 16, 10), (1, 8, 16, 11), (9, 2, 32, 3), (40, 16, 16, 24),
+                                            (75, 16, 16, 8), (148, 4, 16, 1)])
+def test_short_tables(B, Hkv, bs, pages, code, cuda_device):
+    """Tables of few entries, with sequences of every length down to none, some
+    without a valid block; and the same batch in a table of many columns."""
+    ctx = [pages * bs - (7 * b) % (pages * bs + 1) for b in range(B)]
+    q, cache, bt, cl = attention_case(cuda_device, B, 2 * Hkv, Hkv, 128, bs, torch.bfloat16, code, ctx)
+    bt = bt[:, :pages].contiguous()
+    cl[B // 2] = -3
+    bt[B // 3] = -1
+    out = K.paged_attention_quant(q, *cache, bt, cl)
+    check_rows(out, q, *cache, bt, cl)
+    wide = torch.full((B, 60), -1, dtype=bt.dtype, device=cuda_device)
+    wide[:, :pages] = bt
+    check_rows(K.paged_attention_quant(q, *cache, wide, cl), q, *cache, wide, cl)
+
+
+@pytest.mark.parametrize("code", CODES)
 @pytest.mark.parametrize("Hkv", [8, 2, 3])
 def test_value_scales_of_every_size(Hkv, code, cuda_device):
     """Value scales from 2^-90 to 2^60 side by side, unwritten (zero) scales and

@@ -293,7 +293,7 @@ if hasattr(torch._C, "_cuda_getCurrentRawStream"):
 
 def _elsewhere(dev: int) -> bool:
     """Whether another device than the tensors' is current."""
-    return torch.cuda.current_device() != dev
+    return torch._C._cuda_getDevice() != dev
 
 
 def _p(t: torch.Tensor | None):

@@ -158,6 +158,11 @@ PieceGeom piece_geometry(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t 
   if (g.seqs < 1 || g.n_hg * g.seqs * max_blocks >= (1ll << 31)) return g;
   g.grid = device_sm_count();
   g.pdl = cfg && (cfg->flags & 8);
+  // A CTA a segment while the table bounds it to a few entries: no pieces, no join,
+  // one launch less (1 sequence: of 64 tokens 8.2 us instead of 10.7, of 128 10.3 / 11.0, of 256
+  // 14.3 / 11.8; 64 sequences: 64 tokens 8.7 / 17.2, 384 19.0 / 21.8, 512 23.2 / 24.4).
+  const int64_t nseg = g.n_hg * B, most = 160 + 8 * nseg;
+  g.whole = nseg <= g.grid && max_blocks * bs <= (most < 384 ? most : 384);
   const size_t per = g.entry_bytes + 16 + sizeof(EntryMeta);
   const size_t fixed = 1024 + 16 * 8 + (size_t)(g.n_hg * g.seqs + 1) * 4 + (size_t)g.seqs * 4 + 66 * 4 +
                        (size_t)(g.sub - 1) * g.HG * kXchPitch * 4;
@@ -279,9 +284,10 @@ int attend(const AttnCall& a, const b200_launch_cfg* cfg, void* workspace, size_
     if (a.cache_dtype == B200_F8E4M3) return launch_attn_generic_e4m3(a, s);
     return launch_attn_generic_16(a, s);
   }
+  if (prefix) g.whole = false;
   const int splits = prefix ? share_sms(g, a.Hkv, a.block_size, a.max_prefix_blocks, a.max_blocks, elem_of(a)) : 0;
   const SpaceBytes sb = space_bytes(g, a.Hq, splits);
-  if (workspace == nullptr || workspace_bytes < sb.cum + sb.rows + sb.prefix) return B200_ERR_WORKSPACE;
+  if (!g.whole && (workspace == nullptr || workspace_bytes < sb.cum + sb.rows + sb.prefix)) return B200_ERR_WORKSPACE;
   if (!aligned16(workspace)) return B200_ERR_ALIGNMENT;
   PieceSpace w{};
   w.cum = static_cast<int32_t*>(workspace);
@@ -302,7 +308,7 @@ int attend(const AttnCall& a, const b200_launch_cfg* cfg, void* workspace, size_
     st = a.cache_dtype == B200_I8       ? launch_pieces_i8(c, gs, w, prefix, s)
              : a.cache_dtype == B200_F8E4M3 ? launch_pieces_e4m3(c, gs, w, prefix, s)
                                             : launch_pieces_16(c, gs, w, prefix, s);
-    if (st) return st;
+    if (st || g.whole) return st;
     st = B200_DISPATCH_HALF(a.dtype, [&] { return launch_join<scalar_t>(c, gs, w, s); });
     if (st) return st;
   }
@@ -339,7 +345,7 @@ extern "C" size_t b200_paged_attention_quant_workspace_size(int64_t B, int64_t H
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || num_blocks <= 0 || block_size <= 0 || max_blocks <= 0 || Hq % Hkv)
     return 0;
   const PieceGeom g = piece_geometry(B, Hq, Hkv, D, block_size, num_blocks, max_blocks, 1, cfg);
-  if (!g.fast) return 0;
+  if (!g.fast || g.whole) return 0;
   const SpaceBytes sb = space_bytes(g, Hq, 0);
   return sb.cum + sb.rows + sb.prefix;
 }

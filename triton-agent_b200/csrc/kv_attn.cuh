@@ -50,6 +50,7 @@ struct AttnCall {
 // Launch geometry of the fast path.
 struct PieceGeom {
   bool fast;
+  bool whole;             // short tables: a CTA a segment, and nothing to join
   int G, HG, n_hg, sub;   // query heads a kv head, kv heads a CTA, head groups, warps a kv head
   int stages, grid;
   int64_t seqs;           // sequences a launch takes (the batch runs in slices of this many)
@@ -568,12 +569,15 @@ __device__ __forceinline__ void store_rows_nan(T* __restrict__ orow0, const floa
 // range holds the whole segment, else the range's piece at row segment +
 // range -- the (segment, range) pairs of a call, taken in order, have distinct sums, so
 // a piece's place needs no counters.  No state is kept between calls.
+// Where the table bounds every segment to a few entries, a CTA takes a segment
+// whole and there are no pieces.
 // ---------------------------------------------------------------------------
 struct PiecesParams {
   int64_t B, Hq, Hkv, num_blocks, max_blocks;
   int bs, HG, n_hg, sub, stages, nseg;
   int scale_maps;  // scales by tensor maps (pages of more than 16 tokens), else one copy a page
   int always;   // write every segment as pieces (a prefix joins them)
+  int whole;    // range c is segment c
   int overlap;  // launched beside the previous grid of the call: wait for it at the end
   uint32_t entry_bytes;
   float qscale;  // scale * log2(e)
@@ -671,11 +675,14 @@ __global__ void __launch_bounds__((kConsumers + 1) * 32, 1)
   }
   __syncthreads();
   const int64_t E = s_cum[p.nseg];
-  const int64_t R = E < (int64_t)gridDim.x ? E : (int64_t)gridDim.x;  // ranges
+  const int64_t R = p.whole || E > (int64_t)gridDim.x ? (int64_t)gridDim.x : E;  // ranges
   const int c = blockIdx.x;
-  const int64_t lo = c < R ? range_lo(c, E, R) : 0, hi = c < R ? range_lo(c + 1, E, R) : 0;
+  int64_t lo = c < R ? range_lo(c, E, R) : 0, hi = c < R ? range_lo(c + 1, E, R) : 0;
   int seg0 = 0;  // segment of the range's first entry
-  if (c < R) {
+  if (p.whole) {
+    seg0 = c;
+    lo = s_cum[c], hi = s_cum[c + 1];
+  } else if (c < R) {
     int r = p.nseg;  // cum[seg0] <= lo < cum[r]
     while (r - seg0 > 1) {
       const int mid = (seg0 + r) >> 1;
@@ -705,7 +712,7 @@ __global__ void __launch_bounds__((kConsumers + 1) * 32, 1)
   // ordinary launch.  `overlap`: the previous kernel is the same call's prefix
   // grid, which shares nothing with this one; the wait comes at the end.
   if (warp < consumers && !p.overlap) asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (c == 0 && warp < consumers)
+  if (c == 0 && warp < consumers && !p.whole)
     for (int s = threadIdx.x; s <= p.nseg; s += consumers * 32) ws_cum[s] = s_cum[s];
 
   if (c < R && warp == consumers) {
@@ -787,6 +794,7 @@ __global__ void __launch_bounds__((kConsumers + 1) * 32, 1)
     };
     int s = seg0;
     int64_t e = lo;
+    if (lo == hi) ok = markers(1, s, -1);  // (whole: a sequence without tokens)
     while (e < hi && ok) {
       while (s_cum[s + 1] == s_cum[s]) ++s;
       const int64_t b = s % B;
@@ -829,7 +837,7 @@ __global__ void __launch_bounds__((kConsumers + 1) * 32, 1)
       }
       if (ok && fill > 0) ok = issue_entry(s, hg * HG);  // the segment ends in the first chunk of an entry
       if (ok) {
-        const bool one = range_of(segs, E, R) == range_of(sege - 1, E, R);
+        const bool one = p.whole || range_of(segs, E, R) == range_of(sege - 1, E, R);
         ok = markers(1, s, one && !p.always ? -1 : s + c);
       }
       e = segs + j1;
@@ -1013,6 +1021,7 @@ int launch_pieces(const AttnCall& a, const PieceGeom& g, const PieceSpace& w, bo
   p.bs = (int)a.block_size, p.HG = g.HG, p.n_hg = g.n_hg, p.sub = g.sub, p.stages = g.stages;
   p.nseg = (int)(g.n_hg * a.B);
   p.always = a.prefix_table != nullptr;
+  p.whole = g.whole;
   p.overlap = overlap;
   p.entry_bytes = g.entry_bytes;
   p.qscale = a.scale * 1.4426950408889634f;
@@ -1021,7 +1030,7 @@ int launch_pieces(const AttnCall& a, const PieceGeom& g, const PieceSpace& w, bo
   cudaError_t e = grant(kern, g.smem);
   if (e != cudaSuccess) return launch_status(e);
   cudaLaunchConfig_t lc = {};
-  lc.gridDim = dim3((unsigned)g.grid);
+  lc.gridDim = dim3((unsigned)(g.whole ? p.nseg : g.grid));
   lc.blockDim = dim3((unsigned)((g.HG * g.sub + 1) * 32));
   lc.dynamicSmemBytes = g.smem;
   lc.stream = stream;
