@@ -22,117 +22,89 @@ constexpr size_t kSmemMost = 227 * 1024;
 // ---------------------------------------------------------------------------
 struct JoinParams {
   int64_t B, Hq;
-  int heads_cta, nseg, grid, always, splits, W;
+  int heads_cta, splits, W;
 };
 
-// Two entries in two ranges, and a piece with a sum but no values.
-struct JoinNothing {
-  int32_t cum[4];
-  float piece[kPiecePitch];
-};
-__device__ const JoinNothing g_join_nothing = {{0, 1, 2, 0}, {}};
-
+constexpr int kAhead = 4;
 template <typename T>
 __global__ void __launch_bounds__(256)
-    paged_attn_join_kernel(const int32_t* __restrict__ cum, const float* __restrict__ rows,
+    paged_attn_join_kernel(const int2* __restrict__ spans, const float* __restrict__ rows,
                            const float* __restrict__ prefix, T* __restrict__ out, JoinParams p) {
-  __shared__ float s_part[8][kPiecePitch];
+  __shared__ float s_part[8][kD];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int W = p.W, share = warp % W;
-  const int64_t row = (int64_t)blockIdx.x * (8 / W) + warp / W;
-  const bool live = row < p.B * p.Hq;
-  const int64_t b = live ? row / p.Hq : 0;
-  const int h = (int)(row - b * p.Hq), hg = h / p.heads_cta, hh = h - hg * p.heads_cta;
+  const uint32_t row = blockIdx.x * (uint32_t)(8 / W) + warp / W;
+  const bool live = row < (uint32_t)(p.B * p.Hq);
+  const uint32_t b = live ? row / (uint32_t)p.Hq : 0;
+  const int h = live ? (int)(row - b * (uint32_t)p.Hq) : 0, hg = h / p.heads_cta, hh = h - hg * p.heads_cta;
   const int seg = (int)(hg * p.B + b);
+  const float* own = rows + ((int64_t)seg * p.heads_cta + hh) * kPiecePitch;
+  const float* const pre = prefix + row * (int64_t)kPiecePitch;
+  const int64_t own_step = (int64_t)p.heads_cta * kPiecePitch, pre_step = p.B * p.Hq * kPiecePitch;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int2 span = live ? __ldcg(&spans[seg]) : make_int2(0, -1);
+  own += span.x * own_step;
+  const int n = span.y < 0 ? 0 : span.y + p.splits;
+  auto piece = [&](int i) -> const float* {
+    return i < span.y ? own + i * own_step : pre + (i - span.y) * pre_step;
+  };
+  // this warp's share: pieces share, share + W, ...
+  const int mine = n > share ? (n - share + W - 1) / W : 0;
+  float4 v[kAhead];
+  auto fetch = [&](int i0) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (i0 + u < mine) v[u] = __ldcg(reinterpret_cast<const float4*>(piece(share + (i0 + u) * W) + 4 * lane));
+  };
+  auto sums = [&](int i) {
+    return i < n ? __ldcg(reinterpret_cast<const float2*>(piece(i) + kD)) : make_float2(-INFINITY, 0.f);
+  };
+  float2 ml = sums(lane);
+  fetch(0);
+  float M = ml.x;
+  for (int i = lane + 32; i < n; i += 32) M = fmaxf(M, sums(i).x);
+  M = warp_max(M);
   float L = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  bool done = true;
-  // Twice: first over two pieces of nothing, while the streaming kernel still runs, so that
-  // the second pass finds its instructions near (pages streamed through the L2
-  // have driven them out of it, and fetching them costs more than the reads).
-#pragma unroll 1
-  for (int pass = 0; pass < 2; ++pass) {
-    const bool real = pass == 1;
-    if (real) asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int32_t* at = real ? cum : g_join_nothing.cum;
-    int c1 = 0, own = 0;
-    done = real && !live;
-    if (!done) {
-      const int64_t E = __ldcg(&at[real ? p.nseg : 2]), s0 = __ldcg(&at[real ? seg : 0]);
-      const int64_t s1 = __ldcg(&at[real ? seg + 1 : 2]);
-      const int64_t R = E < p.grid ? E : p.grid;
-      if (s1 > s0) {
-        c1 = range_of(s0, E, R);
-        const int c2 = range_of(s1 - 1, E, R);
-        done = real && c1 == c2 && !p.always;
-        own = c2 - c1 + 1;
+  // pieces in runs of 32, a weight a lane
+  for (int i0 = 0; i0 < n; i0 += 32) {
+    if (i0 > 0) ml = sums(i0 + lane);
+    // no weight without tokens (l = 0); NaN logits only leave m without a value and l = NaN
+    const float w = ml.y == 0.f ? 0.f : (ml.x > -1e29f ? ex2(ml.x - M) : ml.y);
+    if (w != 0.f) L = fmaf(w, ml.y, L);
+    const int k1 = i0 + 32 < n ? i0 + 32 : n;
+    const int j0 = (i0 + W - 1 - share) / W, j1 = (k1 + W - 1 - share) / W;  // of this share
+    for (int j = j0; j < j1; j += kAhead) {
+      if (j > 0) fetch(j);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const float wu = __shfl_sync(0xffffffffu, w, (share + (j + u) * W) & 31);
+        if (j + u >= j1 || wu == 0.f) continue;  // (its row may never have been written)
+        acc.x = fmaf(wu, v[u].x, acc.x);
+        acc.y = fmaf(wu, v[u].y, acc.y);
+        acc.z = fmaf(wu, v[u].z, acc.z);
+        acc.w = fmaf(wu, v[u].w, acc.w);
       }
     }
-    const int n = done ? 0 : own + (real ? p.splits : 0);
-    const float* const own0 =
-        real ? rows + (((int64_t)seg + c1) * p.heads_cta + hh) * kPiecePitch : g_join_nothing.piece;
-    const float* const pre0 = prefix + (row - (int64_t)own * p.B * p.Hq) * kPiecePitch;
-    const int64_t own_step = real ? (int64_t)p.heads_cta * kPiecePitch : 0, pre_step = p.B * p.Hq * kPiecePitch;
-    auto piece = [&](int i) -> const float* { return i < own ? own0 + i * own_step : pre0 + i * pre_step; };
-    // weight of a piece: none without tokens (l = 0); NaN logits only leave m
-    // without a value and l = NaN
-    auto weight = [](float m, float l, float M) { return l == 0.f ? 0.f : (m > -1e29f ? ex2(m - M) : l); };
-    float M = -INFINITY;
-    for (int i = lane; i < n; i += 32) M = fmaxf(M, __ldcg(piece(i) + kD));
-    M = warp_max(M);
-    L = 0.f;
-    acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    // this warp's share: pieces share, share + W, ...; 32 of them at a time
-    const int first = real ? share : 0, step = real ? W : 1;
-    const int mine = n > first ? (n - first + step - 1) / step : 0;
-    for (int i0 = 0; i0 < mine; i0 += 32) {
-      float w = 0.f;
-      if (i0 + lane < mine) {
-        const float2 ml = __ldcg(reinterpret_cast<const float2*>(piece(first + (i0 + lane) * step) + kD));
-        w = weight(ml.x, ml.y, M);
-        if (w != 0.f) L += w * ml.y;
-      }
-      const int nb = mine - i0 < 32 ? mine - i0 : 32;
-      for (int u0 = 0; u0 < nb; u0 += 4) {
-        float4 v[4];
-        float wu[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          wu[u] = __shfl_sync(0xffffffffu, w, (u0 + u) & 31);
-          if (u0 + u >= nb) wu[u] = 0.f;
-          v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (wu[u] != 0.f)
-            v[u] = __ldcg(reinterpret_cast<const float4*>(piece(first + (i0 + u0 + u) * step) + 4 * lane));
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          acc.x = fmaf(wu[u], v[u].x, acc.x);
-          acc.y = fmaf(wu[u], v[u].y, acc.y);
-          acc.z = fmaf(wu[u], v[u].z, acc.z);
-          acc.w = fmaf(wu[u], v[u].w, acc.w);
-        }
-      }
-    }
-    L = warp_sum(L);
   }
+  L = warp_sum(L);
   if (W > 1) {
+    // (every warp has the whole sum)
     *reinterpret_cast<float4*>(&s_part[warp][4 * lane]) = acc;
-    if (lane == 0) s_part[warp][kD] = L;
     __syncthreads();
     if (share == 0) {
       for (int u = 1; u < W; ++u) {
-        const float4 v = *reinterpret_cast<const float4*>(&s_part[warp + u][4 * lane]);
-        acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
-        L += s_part[warp + u][kD];
+        const float4 x = *reinterpret_cast<const float4*>(&s_part[warp + u][4 * lane]);
+        acc.x += x.x, acc.y += x.y, acc.z += x.z, acc.w += x.w;
       }
     }
   }
-  if (done || share != 0) return;
+  if (span.y < 0 || share != 0) return;
   const float inv = L == 0.f ? 0.f : 1.f / L;
   uint2 pk;
   pk.x = pack_pair<T>(acc.x * inv, acc.y * inv);
   pk.y = pack_pair<T>(acc.z * inv, acc.w * inv);
-  *reinterpret_cast<uint2*>(out + row * kD + 4 * lane) = pk;
+  *reinterpret_cast<uint2*>(out + row * (int64_t)kD + 4 * lane) = pk;
 }
 
 // ---------------------------------------------------------------------------
@@ -221,12 +193,12 @@ size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 // Bytes of the workspace's parts for one slice.
 struct SpaceBytes {
-  size_t cum, rows, prefix;
+  size_t spans, rows, prefix;
 };
 SpaceBytes space_bytes(const PieceGeom& g, int64_t Hq, int prefix_splits) {
   const int64_t nseg = g.n_hg * g.seqs;
   SpaceBytes s;
-  s.cum = up256((size_t)(nseg + 1) * 4);
+  s.spans = up256((size_t)nseg * sizeof(int2));
   s.rows = up256((size_t)(nseg + g.grid) * g.HG * g.G * kPiecePitch * 4);
   s.prefix = up256((size_t)prefix_splits * g.seqs * Hq * kPiecePitch * 4);
   return s;
@@ -234,10 +206,10 @@ SpaceBytes space_bytes(const PieceGeom& g, int64_t Hq, int prefix_splits) {
 
 template <typename T>
 int launch_join(const AttnCall& a, const PieceGeom& g, const PieceSpace& w, cudaStream_t s) {
-  JoinParams p{a.B, a.Hq, g.HG * g.G, (int)(g.n_hg * a.B), g.grid, a.prefix_table != nullptr, w.prefix_splits, 1};
+  JoinParams p{a.B, a.Hq, g.HG * g.G, w.prefix_splits, 1};
   // pieces a row, about: the grid's ranges over the segments, and the splits;
   // two or three a warp while the rows alone would not fill the SMs
-  const int64_t rows = a.B * a.Hq, pieces = g.grid / p.nseg + 1 + w.prefix_splits;
+  const int64_t rows = a.B * a.Hq, pieces = g.grid / (g.n_hg * a.B) + 1 + w.prefix_splits;
   while (p.W < 8 && p.W * 3 <= pieces && rows * p.W < 16 * (int64_t)device_sm_count()) p.W *= 2;
   cudaLaunchConfig_t lc = {};
   lc.gridDim = dim3((unsigned)((rows * p.W + 7) / 8));
@@ -248,7 +220,7 @@ int launch_join(const AttnCall& a, const PieceGeom& g, const PieceSpace& w, cuda
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   lc.attrs = attr;
   lc.numAttrs = 1;
-  return launch_status(cudaLaunchKernelEx(&lc, paged_attn_join_kernel<T>, (const int32_t*)w.cum, (const float*)w.rows,
+  return launch_status(cudaLaunchKernelEx(&lc, paged_attn_join_kernel<T>, (const int2*)w.spans, (const float*)w.rows,
                                           (const float*)w.prefix, static_cast<T*>(a.out), p));
 }
 
@@ -287,12 +259,12 @@ int attend(const AttnCall& a, const b200_launch_cfg* cfg, void* workspace, size_
   if (prefix) g.whole = false;
   const int splits = prefix ? share_sms(g, a.Hkv, a.block_size, a.max_prefix_blocks, a.max_blocks, elem_of(a)) : 0;
   const SpaceBytes sb = space_bytes(g, a.Hq, splits);
-  if (!g.whole && (workspace == nullptr || workspace_bytes < sb.cum + sb.rows + sb.prefix)) return B200_ERR_WORKSPACE;
+  if (!g.whole && (workspace == nullptr || workspace_bytes < sb.spans + sb.rows + sb.prefix)) return B200_ERR_WORKSPACE;
   if (!aligned16(workspace)) return B200_ERR_ALIGNMENT;
   PieceSpace w{};
-  w.cum = static_cast<int32_t*>(workspace);
-  w.rows = reinterpret_cast<float*>(static_cast<char*>(workspace) + sb.cum);
-  w.prefix = reinterpret_cast<float*>(static_cast<char*>(workspace) + sb.cum + sb.rows);
+  w.spans = static_cast<int2*>(workspace);
+  w.rows = reinterpret_cast<float*>(static_cast<char*>(workspace) + sb.spans);
+  w.prefix = reinterpret_cast<float*>(static_cast<char*>(workspace) + sb.spans + sb.rows);
   for (int64_t b0 = 0; b0 < a.B; b0 += g.seqs) {
     const AttnCall c = slice_of(a, b0, a.B - b0 < g.seqs ? a.B - b0 : g.seqs);
     PieceGeom gs = g;
@@ -347,7 +319,7 @@ extern "C" size_t b200_paged_attention_quant_workspace_size(int64_t B, int64_t H
   const PieceGeom g = piece_geometry(B, Hq, Hkv, D, block_size, num_blocks, max_blocks, 1, cfg);
   if (!g.fast || g.whole) return 0;
   const SpaceBytes sb = space_bytes(g, Hq, 0);
-  return sb.cum + sb.rows + sb.prefix;
+  return sb.spans + sb.rows + sb.prefix;
 }
 
 extern "C" int b200_paged_attention_quant(const void* q, const void* k_cache, const void* v_cache,
@@ -381,7 +353,7 @@ extern "C" size_t b200_paged_attention_prefix_workspace_size(int64_t B, int64_t 
   if (!prefix_fits(g, Hkv, block_size, max_prefix_blocks)) return 0;
   const int splits = share_sms(g, Hkv, block_size, max_prefix_blocks, max_blocks, elem);
   const SpaceBytes sb = space_bytes(g, Hq, splits);
-  return sb.cum + sb.rows + sb.prefix;
+  return sb.spans + sb.rows + sb.prefix;
 }
 
 extern "C" int b200_paged_attention_prefix(const void* q, const void* k_cache, const void* v_cache,

@@ -59,9 +59,10 @@ struct PieceGeom {
   bool pdl;
 };
 
-// Workspace: [segment prefix sums | pieces of the own pages | pieces of the prefix].
+// Workspace: [spans | pieces of the own pages | pieces of the prefix].  A segment's
+// span: its first range, and how many ranges left a piece (-1: the row itself is written).
 struct PieceSpace {
-  int32_t* cum;   // nseg + 1
+  int2* spans;    // nseg
   float* rows;    // piece segment + range, heads_cta rows each
   float* prefix;  // split-major: [splits][seqs * Hq] rows
   int prefix_splits;
@@ -610,7 +611,7 @@ __global__ void __launch_bounds__((kConsumers + 1) * 32, 1)
                              const __grid_constant__ CUtensorMap tm_ks, const __grid_constant__ CUtensorMap tm_vs,
                              const float* __restrict__ k_scale, const float* __restrict__ v_scale,
                              const T* __restrict__ q, IndexPtr btab, IndexPtr clen, T* __restrict__ out,
-                             float* __restrict__ ws_rows, int32_t* __restrict__ ws_cum, PiecesParams p) {
+                             float* __restrict__ ws_rows, int2* __restrict__ ws_spans, PiecesParams p) {
   constexpr bool k8 = sizeof(KV) == 1;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -712,8 +713,17 @@ __global__ void __launch_bounds__((kConsumers + 1) * 32, 1)
   // ordinary launch.  `overlap`: the previous kernel is the same call's prefix
   // grid, which shares nothing with this one; the wait comes at the end.
   if (warp < consumers && !p.overlap) asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (c == 0 && warp < consumers && !p.whole)
-    for (int s = threadIdx.x; s <= p.nseg; s += consumers * 32) ws_cum[s] = s_cum[s];
+  if (c == 0 && warp < consumers && !p.whole) {
+    for (int s = threadIdx.x; s < p.nseg; s += consumers * 32) {
+      const int64_t s0 = s_cum[s], s1 = s_cum[s + 1];
+      int2 span = make_int2(0, 0);
+      if (s1 > s0) {
+        const int c1 = range_of(s0, E, R), c2 = range_of(s1 - 1, E, R);
+        span = make_int2(c1, c1 == c2 && !p.always ? -1 : c2 - c1 + 1);
+      }
+      ws_spans[s] = span;
+    }
+  }
 
   if (c < R && warp == consumers) {
     // ------------------------------------------------------------ producer
@@ -1042,7 +1052,7 @@ int launch_pieces(const AttnCall& a, const PieceGeom& g, const PieceSpace& w, bo
   const int wide = a.index_dtype == B200_I64;
   e = cudaLaunchKernelEx(&lc, kern, tk, tv, tks, tvs, a.k_scale, a.v_scale, static_cast<const T*>(a.q),
                          IndexPtr{a.block_table, wide}, IndexPtr{a.context_len, wide}, static_cast<T*>(a.out), w.rows,
-                         w.cum, p);
+                         w.spans, p);
   return launch_status(e);
 }
 
