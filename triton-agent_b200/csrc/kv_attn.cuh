@@ -75,12 +75,34 @@ int launch_attn_generic_i8(const AttnCall& a, cudaStream_t s);
 int launch_attn_generic_e4m3(const AttnCall& a, cudaStream_t s);
 int launch_attn_generic_16(const AttnCall& a, cudaStream_t s);
 
+// Ids outside [0, num_blocks) among a table's n, this thread's share: sixteen loads in flight.
+template <typename I>
+__device__ __forceinline__ int dropped_ids(const I* __restrict__ ids, int n, int64_t num_blocks) {
+  int drop = 0;
+#pragma unroll 1
+  for (int j = threadIdx.x; j < n; j += 16 * blockDim.x) {
+    I v[16];
+#pragma unroll
+    for (int u = 0; u < 16; ++u) {
+      const int k = j + u * (int)blockDim.x;
+      v[u] = k < n ? __ldg(ids + k) : 0;
+    }
+#pragma unroll
+    for (int u = 0; u < 16; ++u) drop += v[u] < 0 || (int64_t)v[u] >= num_blocks;
+  }
+  return drop;
+}
+
 // Block ids and lengths are int32 or int64 by a flag (uniform; read by one warp).
 struct IndexPtr {
   const void* p;
   int wide;
   __device__ __forceinline__ int64_t at(int64_t i) const {
     return wide ? __ldg(static_cast<const long long*>(p) + i) : (int64_t)__ldg(static_cast<const int*>(p) + i);
+  }
+  __device__ __forceinline__ int dropped(int64_t first, int n, int64_t num_blocks) const {
+    return wide ? dropped_ids(static_cast<const long long*>(p) + first, n, num_blocks)
+                : dropped_ids(static_cast<const int*>(p) + first, n, num_blocks);
   }
 };
 
@@ -691,15 +713,11 @@ __global__ void __launch_bounds__((kConsumers + 1) * 32, 1)
       else r = mid;
     }
     // Dropped entries before the range shift the token ranks of its pages:
-    // counted by the whole CTA (a warp alone takes 20 us over 8192 entries).
+    // counted by the whole CTA (over 8192 entries a warp alone takes 20 us, the
+    // CTA with a load at a time 12; 3 sequences of 90001..131072 tokens: 131 us, so 124).
     const int j0 = (int)(lo - s_cum[seg0]);
     if (j0 > 0) {
-      int drop = 0;
-#pragma unroll 8
-      for (int j = threadIdx.x; j < j0; j += blockDim.x) {
-        const int64_t id = btab.at((seg0 % B) * p.max_blocks + j);
-        drop += id < 0 || id >= p.num_blocks;
-      }
+      int drop = btab.dropped((seg0 % B) * p.max_blocks, j0, p.num_blocks);
       drop = __reduce_add_sync(0xffffffffu, drop);
       if (lane == 0 && drop) atomicAdd(s_drop, drop);
       __syncthreads();

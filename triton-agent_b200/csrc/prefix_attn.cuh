@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
   uint64_t* code_empty = code_full + kPCodeRing + kPMoreCodes;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(code_empty + kPCodeRing + kPMoreCodes);
   int* s_abort = reinterpret_cast<int*>(tmem_slot + 1);
-  int* s_count = s_abort + 1;  // [2][16] valid entries before the split and in it, by warp
+  int* s_count = s_abort + 1;  // [2][16] dropped entries before the split and in it, by warp
   int* s_ids = s_count + 32;   // [kPScaleRing][kPMaxPages] page ids of a key tile
   int* s_list = s_ids + kPScaleRing * kPMaxPages;  // [K, V][kPList] pages to copy
 
@@ -181,17 +181,9 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
     const int64_t a = (int64_t)split * per, b = a + per;
     e0 = (int)(a < E ? a : E);
     e1 = (int)(b < E ? b : E);
-    // valid entries before the split and in it
-    int before = 0, in = 0;
-#pragma unroll 8
-    for (int j = threadIdx.x; j < e1; j += blockDim.x) {
-      const int64_t id = ptab.at(j);
-      const int ok = id >= 0 && id < p.num_blocks;
-      if (j < e0) before += ok;
-      else in += ok;
-    }
-    before = __reduce_add_sync(0xffffffffu, before);
-    in = __reduce_add_sync(0xffffffffu, in);
+    // dropped entries before the split and in it
+    const int before = __reduce_add_sync(0xffffffffu, ptab.dropped(0, e0, p.num_blocks));
+    const int in = __reduce_add_sync(0xffffffffu, ptab.dropped(e0, e1 - e0, p.num_blocks));
     if (lane == 0) {
       s_count[warp] = before;
       s_count[16 + warp] = in;
@@ -240,10 +232,10 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
   const uint32_t tmem = *tmem_slot;  // columns: S_t at 128 t, O_t at 256 + 128 t
   int ntok;
   {
-    int before = 0, in = 0;
+    int before = e0, in = e1 - e0;
     for (int w = 0; w < (int)(blockDim.x >> 5); ++w) {
-      before += s_count[w];
-      in += s_count[16 + w];
+      before -= s_count[w];
+      in -= s_count[16 + w];
     }
     const int64_t left = plen_tokens - (int64_t)before * bs, have = (int64_t)in * bs;
     ntok = (int)(left < 0 ? 0 : (left < have ? left : have));
