@@ -121,10 +121,15 @@ __device__ __forceinline__ uint32_t kv_at(int r, int c) {
   return (uint32_t)((r >> 3) * 2048 + (c >> 3) * 1024 + (r & 7) * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
-constexpr int kPRegsLow = 72, kPRegsHigh = 184;  // 8-bit kernel: 8 warps each way, 128 a thread at launch
+// Registers a thread, softmax warps and the others: 128 at launch with 8-bit caches (8 warps each), 168
+// with 16-bit ones (8 and 4).
+template <bool k8>
+struct PrefixRegs {
+  static constexpr int low = 72, high = k8 ? 184 : 216, threads = k8 ? 512 : 384;
+};
 
 template <typename T, typename KV>
-__global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
+__global__ void __launch_bounds__(PrefixRegs<sizeof(KV) == 1>::threads, 1)
     prefix_attn_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                        const float* __restrict__ k_scale, const float* __restrict__ v_scale, const T* __restrict__ q,
                        IndexPtr ptab, IndexPtr plen, float* __restrict__ pieces, PrefixParams p) {
@@ -244,7 +249,7 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
   const int last_valid = ntok - (nkt - 1) * tile_tok;  // tokens of the last tile
   const bool fix_v = !k8 && nkt > 0 && last_valid < tile_tok;
 
-  if (k8 && warp < 4) sm100::setmaxnreg_dec<kPRegsLow>();
+  if (warp < 4) sm100::setmaxnreg_dec<PrefixRegs<k8>::low>();
   if (warp == 0 || warp == 2) {
     // ------------------------------------- producers: K tiles and V tiles, in turn in one ring
     const int which = warp >> 1;
@@ -405,7 +410,7 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
   } else if (k8 && warp >= 12) {
     // ------------------------------------------------- code tiles to f16 tiles
     if constexpr (k8) {
-      sm100::setmaxnreg_dec<kPRegsLow>();
+      sm100::setmaxnreg_dec<PrefixRegs<k8>::low>();
       const int r = threadIdx.x - 384;  // this thread's key of every tile
       const int page = r / bs, off = r - page * bs;
       bool ok = true;
@@ -488,7 +493,7 @@ __global__ void __launch_bounds__(sizeof(KV) == 1 ? 512 : 384, 1)
     }
   } else if (warp >= 4 && warp < 12) {
     // --------------------------------------------------------------- softmax
-    if constexpr (k8) sm100::setmaxnreg_inc<kPRegsHigh>();
+    sm100::setmaxnreg_inc<PrefixRegs<k8>::high>();
     const int t = (warp >> 2) - 1, quarter = warp & 3;
     const int r = quarter * 32 + lane;
     const int qr = row0 + both * t * kPM + r;  // row of Q_h
@@ -710,22 +715,21 @@ int launch_prefix(const AttnCall& a, const PieceGeom& g, const PieceSpace& w, cu
                       4 * (kPScaleRing * kPMaxPages + 2 * kPList);
   static_assert(PrefixSmem<k8>::oBars + 1024 + 1024 <= 227 * 1024, "shared memory of a CTA");
   auto kern = prefix_attn_kernel<T, KV>;
-  if (k8) {
-    // the register split (setmaxnreg) needs what it hands out at launch
-    static const int regs = [&] {
-      cudaFuncAttributes at{};
-      return cudaFuncGetAttributes(&at, kern) == cudaSuccess ? at.numRegs : 0;
-    }();
-    if (regs * 512 < 256 * (kPRegsLow + kPRegsHigh)) {
-      set_last_error_detail("prefix_attn_kernel: too few registers at launch for its split");
-      return B200_ERR_LAUNCH;
-    }
+  // the register split (setmaxnreg) needs what it hands out at launch
+  using Regs = PrefixRegs<k8>;
+  static const int regs = [&] {
+    cudaFuncAttributes at{};
+    return cudaFuncGetAttributes(&at, kern) == cudaSuccess ? at.numRegs : 0;
+  }();
+  if (regs * Regs::threads < 256 * Regs::high + (Regs::threads - 256) * Regs::low) {
+    set_last_error_detail("prefix_attn_kernel: too few registers at launch for its split");
+    return B200_ERR_LAUNCH;
   }
   static SmemGrant grant;
   cudaError_t e = grant(kern, smem);
   if (e != cudaSuccess) return launch_status(e);
   const int64_t pairs = (a.B * g.G + 2 * kPM - 1) / (2 * kPM);
-  kern<<<dim3((unsigned)p.splits, (unsigned)pairs, (unsigned)a.Hkv), k8 ? 512 : 384, smem, stream>>>(
+  kern<<<dim3((unsigned)p.splits, (unsigned)pairs, (unsigned)a.Hkv), Regs::threads, smem, stream>>>(
       tk, tv, a.k_scale, a.v_scale, static_cast<const T*>(a.q), IndexPtr{a.prefix_table, a.index_dtype == B200_I64},
       IndexPtr{a.prefix_len, a.index_dtype == B200_I64}, w.prefix, p);
   return launch_status(cudaGetLastError());
