@@ -436,26 +436,27 @@ __global__ void __launch_bounds__(PrefixRegs<sizeof(KV) == 1>::threads, 1)
         const int valid = j == nkt - 1 ? last_valid : tile_tok;
         const bool live = r < valid;
         ok = sm100::mbar_wait_warp(sm100::smem_u32(&code_full[cs]), cph);
-        ok = ok && sm100::mbar_wait_warp(sm100::smem_u32(&ring_empty[slot]), ((it / kRing) & 1) ^ 1);
         if (!ok) break;
         const uint32_t src = code_at(cs) + r * 128;
+        uint4 w[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) w[c] = lds128(src + ((c ^ (r & 7)) << 4));
+        ok = sm100::mbar_wait_warp(sm100::smem_u32(&ring_empty[slot]), ((it / kRing) & 1) ^ 1);
+        if (!ok) break;
         const uint32_t dst = sbase + L::oRing + slot * kPTile;
+        if (live) {
 #pragma unroll
-        for (int c0 = 0; c0 < 8; c0 += 4) {
-          uint4 w[4];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) w[c] = lds128(src + (((c0 + c) ^ (r & 7)) << 4));
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
+          for (int c = 0; c < 8; ++c) {
             uint4 a, b;
             kv8_in_order<KV>(w[c].x, a.x, a.y);
             kv8_in_order<KV>(w[c].y, a.z, a.w);
             kv8_in_order<KV>(w[c].z, b.x, b.y);
             kv8_in_order<KV>(w[c].w, b.z, b.w);
-            if (!live) a = b = make_uint4(0, 0, 0, 0);
-            sts128(dst + kv_at(r, 2 * (c0 + c)), a);
-            sts128(dst + kv_at(r, 2 * (c0 + c) + 1), b);
+            sts128(dst + kv_at(r, 2 * c), a);
+            sts128(dst + kv_at(r, 2 * c + 1), b);
           }
+        } else {
+          for (int c = 0; c < 16; ++c) sts128(dst + kv_at(r, c), make_uint4(0, 0, 0, 0));
         }
         sm100::fence_proxy_async_smem();
         if (which == 0) {
