@@ -40,9 +40,8 @@ constexpr int kPM = 128;                   // rows of a query tile, keys of a ke
 constexpr uint32_t kPHalf = kPM * 128;     // 64 dims (16-bit) of 128 rows
 constexpr uint32_t kPTile = 2 * kPHalf;    // a Q, K or V tile
 constexpr uint32_t kPCodes = kPHalf;       // an 8-bit K or V tile
-constexpr int kPRing16 = 5, kPRing8 = 3;   // K/V tiles in shared memory
-constexpr int kPCodeRing = 3;              // code tiles (8-bit); with one row tile
-constexpr int kPMoreCodes = 2;             // two more, in the second Q tile's place
+constexpr int kPRing16 = 5, kPRing8 = 3;   // K/V tiles in shared memory; one more with one row tile
+constexpr int kPCodeRing = 3;              // code tiles (8-bit)
 constexpr int kPScaleRing = 4;             // key tiles whose scales wait for the softmax (8-bit), and page ids
 constexpr int kPMaxPages = 8;              // pages of a tile (block size 16)
 constexpr int kPList = 32 + kPMaxPages;    // pages a producer holds
@@ -136,7 +135,6 @@ __global__ void __launch_bounds__(PrefixRegs<sizeof(KV) == 1>::threads, 1)
   constexpr bool k8 = sizeof(KV) == 1;
   using M = typename std::conditional<k8, __half, T>::type;  // type of the matrix operands
   using L = PrefixSmem<k8>;
-  constexpr int kRing = k8 ? kPRing8 : kPRing16;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = sm100::smem_u32(smem);
@@ -147,15 +145,16 @@ __global__ void __launch_bounds__(PrefixRegs<sizeof(KV) == 1>::threads, 1)
   const int both = tiles == 2;  // else: streams 0 and 1 are the even and odd key tiles of one row tile
   const int bs = p.bs, tile_tok = p.ppt * bs;
 
-  // code tile i; with one row tile the second Q tile's place holds two more
-  const int codes = kPCodeRing + (both ? 0 : kPMoreCodes);
-  auto code_at = [&](int i) {
-    return sbase + (i < kPCodeRing ? L::oCodes + i * kPCodes : L::oQ + kPTile + (i - kPCodeRing) * kPCodes);
-  };
+  // with one row tile the second Q tile's place belongs to the ring
+  const int depth = (k8 ? kPRing8 : kPRing16) + (both ? 0 : 1);
+  const uint32_t ring = sbase + L::oRing - (both ? 0 : kPTile);
+  const uint32_t depth_inv = 0xffffffffu / (uint32_t)depth + 1;  // i / depth for i < 2^29
+  auto round_of = [&](int i) { return (int)__umulhi((uint32_t)i, depth_inv); };
+  auto slot_of = [&](int i) { return i - round_of(i) * depth; };
 
-  uint64_t* ring_full = reinterpret_cast<uint64_t*>(smem + L::oBars);  // [kRing]
-  uint64_t* ring_empty = ring_full + kPRing16;  // [kRing]
-  uint64_t* s_full = ring_empty + kPRing16;     // [2]
+  uint64_t* ring_full = reinterpret_cast<uint64_t*>(smem + L::oBars);  // [depth]
+  uint64_t* ring_empty = ring_full + kPRing16 + 1;  // [depth]
+  uint64_t* s_full = ring_empty + kPRing16 + 1;  // [2]
   uint64_t* p_full = s_full + 2;                // [2]
   uint64_t* o_done = p_full + 2;                // [2]
   uint64_t* v_fixed = o_done + 2;
@@ -163,9 +162,9 @@ __global__ void __launch_bounds__(PrefixRegs<sizeof(KV) == 1>::threads, 1)
   uint64_t* sc_full = q_full + 1;                // [kPScaleRing]
   uint64_t* sc_empty = sc_full + kPScaleRing;    // [kPScaleRing]
   uint64_t* ids_full = sc_empty + kPScaleRing;   // [kPScaleRing]
-  uint64_t* code_full = ids_full + kPScaleRing;  // [codes]
-  uint64_t* code_empty = code_full + kPCodeRing + kPMoreCodes;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(code_empty + kPCodeRing + kPMoreCodes);
+  uint64_t* code_full = ids_full + kPScaleRing;  // [kPCodeRing]
+  uint64_t* code_empty = code_full + kPCodeRing;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(code_empty + kPCodeRing);
   int* s_abort = reinterpret_cast<int*>(tmem_slot + 1);
   int* s_count = s_abort + 1;  // [2][16] dropped entries before the split and in it, by warp
   int* s_ids = s_count + 32;   // [kPScaleRing][kPMaxPages] page ids of a key tile
@@ -196,7 +195,7 @@ __global__ void __launch_bounds__(PrefixRegs<sizeof(KV) == 1>::threads, 1)
   }
   if (threadIdx.x == 32) {
     *s_abort = 0;
-    for (int i = 0; i < kRing; ++i) {
+    for (int i = 0; i < depth; ++i) {
       sm100::mbar_init(sm100::smem_u32(&ring_full[i]), k8 ? 4 : 1);
       sm100::mbar_init(sm100::smem_u32(&ring_empty[i]), 1);
     }
@@ -212,7 +211,7 @@ __global__ void __launch_bounds__(PrefixRegs<sizeof(KV) == 1>::threads, 1)
       sm100::mbar_init(sm100::smem_u32(&ids_full[i]), 1);
       sm100::mbar_init(sm100::smem_u32(&sc_empty[i]), 4 * tiles);  // one stream's warps, or both's
     }
-    for (int i = 0; i < codes; ++i) {
+    for (int i = 0; i < kPCodeRing; ++i) {
       sm100::mbar_init(sm100::smem_u32(&code_full[i]), 1);
       sm100::mbar_init(sm100::smem_u32(&code_empty[i]), 4);
     }
@@ -221,9 +220,9 @@ __global__ void __launch_bounds__(PrefixRegs<sizeof(KV) == 1>::threads, 1)
   if (!k8 && tile_tok < kPM) {
     // rows no page reaches stay zero in every ring tile (both operands)
     const int dead = kPM - tile_tok;
-    for (int i = threadIdx.x; i < kRing * dead * 16; i += blockDim.x) {
+    for (int i = threadIdx.x; i < depth * dead * 16; i += blockDim.x) {
       const int c = i & 15, r = (i >> 4) % dead, slot = (i >> 4) / dead;
-      sts128(sbase + L::oRing + slot * kPTile + kv_at(tile_tok + r, c), make_uint4(0, 0, 0, 0));
+      sts128(ring + slot * kPTile + kv_at(tile_tok + r, c), make_uint4(0, 0, 0, 0));
     }
     sm100::fence_proxy_async_smem();
   }
@@ -255,7 +254,7 @@ __global__ void __launch_bounds__(PrefixRegs<sizeof(KV) == 1>::threads, 1)
     const int which = warp >> 1;
     const CUtensorMap* map = which ? &tm_v : &tm_k;
     if (lane == 0) sm100::tma_prefetch_desc(map);
-    const int depth = k8 ? codes : kRing;
+    const int slots = k8 ? kPCodeRing : depth;
     uint64_t* fulls = k8 ? code_full : ring_full;
     uint64_t* empties = k8 ? code_empty : ring_empty;
     const uint32_t page_bytes = (uint32_t)(bs * kPieceDim * (int)sizeof(KV));
@@ -287,9 +286,9 @@ __global__ void __launch_bounds__(PrefixRegs<sizeof(KV) == 1>::threads, 1)
         __syncwarp();
         if (lane < np) {
           if constexpr (k8)
-            sm100::tma_load_3d(code_at(slot) + lane * page_bytes, map, fb, 0, page * bs, h);
+            sm100::tma_load_3d(sbase + L::oCodes + slot * kPCodes + lane * page_bytes, map, fb, 0, page * bs, h);
           else
-            sm100::tma_load_4d(sbase + L::oRing + slot * kPTile + lane * page_bytes, map, fb, 0, 0, 2 * h,
+            sm100::tma_load_4d(ring + slot * kPTile + lane * page_bytes, map, fb, 0, 0, 2 * h,
                                page * (bs >> 3));
         }
         if (k8 && which == 0 && lane == 0) sm100::mbar_arrive(sm100::smem_u32(&ids_full[issued % kPScaleRing]));
@@ -297,8 +296,8 @@ __global__ void __launch_bounds__(PrefixRegs<sizeof(KV) == 1>::threads, 1)
         left -= np;
         ++issued;
         slot += 2;
-        if (slot >= depth) {
-          slot -= depth;
+        if (slot >= slots) {
+          slot -= slots;
           ph ^= 1u;
         }
       }
@@ -313,16 +312,16 @@ __global__ void __launch_bounds__(PrefixRegs<sizeof(KV) == 1>::threads, 1)
         atomicExch(s_abort, 1);
       }
       // no copy may still be writing shared memory when the CTA exits
-      for (int i = 2 * issued - 2 + which; i >= 0 && i >= 2 * issued - depth; i -= 2)
-        if (!sm100::mbar_wait(sm100::smem_u32(&fulls[i % depth]), (i / depth) & 1)) b200_dev_error(kDevErrTimeoutFull);
+      for (int i = 2 * issued - 2 + which; i >= 0 && i >= 2 * issued - slots; i -= 2)
+        if (!sm100::mbar_wait(sm100::smem_u32(&fulls[i % slots]), (i / slots) & 1)) b200_dev_error(kDevErrTimeoutFull);
     }
     __syncwarp();
     if (warp == 2 && fix_v) {
       // V rows behind the last token are zero
-      const int it = 2 * nkt - 1, vslot = it % kRing;
-      if (sm100::mbar_wait_warp(sm100::smem_u32(&ring_full[vslot]), (it / kRing) & 1)) {
+      const int it = 2 * nkt - 1, vslot = slot_of(it);
+      if (sm100::mbar_wait_warp(sm100::smem_u32(&ring_full[vslot]), round_of(it) & 1)) {
         for (int i = lane; i < (tile_tok - last_valid) * 16; i += 32)
-          sts128(sbase + L::oRing + vslot * kPTile + kv_at(last_valid + (i >> 4), i & 15), make_uint4(0, 0, 0, 0));
+          sts128(ring + vslot * kPTile + kv_at(last_valid + (i >> 4), i & 15), make_uint4(0, 0, 0, 0));
         sm100::fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) sm100::mbar_arrive(sm100::smem_u32(v_fixed));
@@ -338,19 +337,19 @@ __global__ void __launch_bounds__(PrefixRegs<sizeof(KV) == 1>::threads, 1)
     constexpr uint32_t idesc_o = sm100::make_idesc(1, fmt, fmt, 0, 1, kPM, kPieceDim);
     const uint32_t leader = sm100::elect_one();
     const uint64_t dq = sm100::make_smem_desc(sbase + L::oQ, 16, 1024, sm100::kSwizzle128B);
-    const uint64_t dk = sm100::make_smem_desc(sbase + L::oRing, 16, 2048, sm100::kSwizzle128B);
-    const uint64_t dv = sm100::make_smem_desc(sbase + L::oRing, 1024, 2048, sm100::kSwizzle128B);
+    const uint64_t dk = sm100::make_smem_desc(ring, 16, 2048, sm100::kSwizzle128B);
+    const uint64_t dv = sm100::make_smem_desc(ring, 1024, 2048, sm100::kSwizzle128B);
     bool ok = nkt > 0 && sm100::mbar_wait_warp(sm100::smem_u32(q_full), 0);
     auto full = [&](int it) -> bool {
-      return sm100::mbar_wait_warp(sm100::smem_u32(&ring_full[it % kRing]), (it / kRing) & 1);
+      return sm100::mbar_wait_warp(sm100::smem_u32(&ring_full[slot_of(it)]), round_of(it) & 1);
     };
-    auto release = [&](int it) { sm100::tc_commit(sm100::smem_u32(&ring_empty[it % kRing]), leader); };
+    auto release = [&](int it) { sm100::tc_commit(sm100::smem_u32(&ring_empty[slot_of(it)]), leader); };
     // stream t's n-th key tile: j = n with two row tiles, 2n + t with one
     auto issue_s = [&](int t, int j) -> bool {
       if (!full(2 * j)) return false;
       sm100::tc_fence_after();
       const uint64_t ad = dq + (uint64_t)((both * t * kPTile) >> 4);
-      const uint64_t bd = dk + (uint64_t)((((2 * j) % kRing) * kPTile) >> 4);
+      const uint64_t bd = dk + (uint64_t)((slot_of(2 * j) * kPTile) >> 4);
 #pragma unroll
       for (int kk = 0; kk < kPieceDim / 16; ++kk) {
         const uint32_t offa = ((kk >> 2) * kPHalf + (kk & 3) * 32) >> 4;
@@ -364,7 +363,7 @@ __global__ void __launch_bounds__(PrefixRegs<sizeof(KV) == 1>::threads, 1)
       if (!sm100::mbar_wait_warp(sm100::smem_u32(&p_full[t]), n & 1) || !full(2 * j + 1)) return false;
       if (fix_v && j == nkt - 1 && !sm100::mbar_wait_warp(sm100::smem_u32(v_fixed), 0)) return false;
       sm100::tc_fence_after();
-      const uint64_t bd = dv + (uint64_t)((((2 * j + 1) % kRing) * kPTile) >> 4);
+      const uint64_t bd = dv + (uint64_t)((slot_of(2 * j + 1) * kPTile) >> 4);
 #pragma unroll
       for (int kk = 0; kk < kPM / 16; ++kk)
         sm100::mma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, bd + (uint64_t)((kk * 4096) >> 4), idesc_o,
@@ -432,18 +431,18 @@ __global__ void __launch_bounds__(PrefixRegs<sizeof(KV) == 1>::threads, 1)
       };
       if (nkt > 0) ok = load_scales(0);
       for (int it = 0; it < 2 * nkt && ok; ++it) {
-        const int slot = it % kRing, j = it >> 1, which = it & 1;
+        const int slot = slot_of(it), j = it >> 1, which = it & 1;
         const int valid = j == nkt - 1 ? last_valid : tile_tok;
         const bool live = r < valid;
         ok = sm100::mbar_wait_warp(sm100::smem_u32(&code_full[cs]), cph);
         if (!ok) break;
-        const uint32_t src = code_at(cs) + r * 128;
+        const uint32_t src = sbase + L::oCodes + cs * kPCodes + r * 128;
         uint4 w[8];
 #pragma unroll
         for (int c = 0; c < 8; ++c) w[c] = lds128(src + ((c ^ (r & 7)) << 4));
-        ok = sm100::mbar_wait_warp(sm100::smem_u32(&ring_empty[slot]), ((it / kRing) & 1) ^ 1);
+        ok = sm100::mbar_wait_warp(sm100::smem_u32(&ring_empty[slot]), (round_of(it) & 1) ^ 1);
         if (!ok) break;
-        const uint32_t dst = sbase + L::oRing + slot * kPTile;
+        const uint32_t dst = ring + slot * kPTile;
         if (live) {
 #pragma unroll
           for (int c = 0; c < 8; ++c) {
@@ -481,7 +480,7 @@ __global__ void __launch_bounds__(PrefixRegs<sizeof(KV) == 1>::threads, 1)
           sm100::mbar_arrive(sm100::smem_u32(&code_empty[cs]));
           if (which == 0) sm100::mbar_arrive(sm100::smem_u32(&sc_full[j % kPScaleRing]));
         }
-        if (++cs == codes) {
+        if (++cs == kPCodeRing) {
           cs = 0;
           cph ^= 1u;
         }
@@ -623,7 +622,7 @@ __global__ void __launch_bounds__(PrefixRegs<sizeof(KV) == 1>::threads, 1)
     // With one row tile stream 1 hands its state to stream 0 through the K/V
     // ring, which nothing reads any more once both streams' products are done.
     // (Every path leads both warpgroups to the barrier.)
-    const uint32_t hand = sbase + L::oRing + r * 4;  // [130][128] floats
+    const uint32_t hand = ring + r * 4;  // [130][128] floats
     const bool join = !both && nkt > 1;
     float f0 = 1.f, f1 = 0.f;
     if (join) {
@@ -712,7 +711,7 @@ int launch_prefix(const AttnCall& a, const PieceGeom& g, const PieceSpace& w, cu
   p.splits = w.prefix_splits;
   p.qscale = a.scale * 1.4426950408889634f;
   const size_t smem = 1024 + PrefixSmem<k8>::oBars +
-                      8 * (2 * kPRing16 + 6 + 2 + 3 * kPScaleRing + 2 * (kPCodeRing + kPMoreCodes)) + 8 + 128 +
+                      8 * (2 * (kPRing16 + 1) + 6 + 2 + 3 * kPScaleRing + 2 * kPCodeRing) + 8 + 128 +
                       4 * (kPScaleRing * kPMaxPages + 2 * kPList);
   static_assert(PrefixSmem<k8>::oBars + 1024 + 1024 <= 227 * 1024, "shared memory of a CTA");
   auto kern = prefix_attn_kernel<T, KV>;
