@@ -40,10 +40,11 @@ def test_kv8_bad_arguments_rejected_on_host():
     assert attend(Hq=9) == L.ERR_BAD_ARG and attend(maxb=0) == L.ERR_BAD_ARG and attend(ks=None) == L.ERR_BAD_ARG
     assert attend(code=L.BF16) == L.ERR_UNSUPPORTED and attend(dt=L.F32) == L.ERR_UNSUPPORTED
     assert attend(ix=L.I8) == L.ERR_UNSUPPORTED and attend(D=257 * 2) == L.ERR_UNSUPPORTED
-    assert attend() == L.ERR_WORKSPACE
-    need = lib.b200_paged_attention_quant_workspace_size(2, 8, 2, 128, 16, 16, 4, None)
-    assert attend(ws=p, n=need - 1) == L.ERR_WORKSPACE
-    assert attend(ws=ctypes.c_void_p((1 << 20) + 8), n=need) == L.ERR_ALIGNMENT
+    assert attend(maxb=40) == L.ERR_WORKSPACE
+    need = lib.b200_paged_attention_quant_workspace_size(2, 8, 2, 128, 16, 16, 40, None)
+    assert need > 0 and lib.b200_paged_attention_quant_workspace_size(2, 8, 2, 128, 16, 16, 4, None) == 0  # short tables
+    assert attend(maxb=40, ws=p, n=need - 1) == L.ERR_WORKSPACE
+    assert attend(maxb=40, ws=ctypes.c_void_p((1 << 20) + 8), n=need) == L.ERR_ALIGNMENT
     assert attend(B=0) == L.OK
 
     def prefix(B=2, P=4, maxb=4, dt=L.BF16, code=L.BF16, table=p):
