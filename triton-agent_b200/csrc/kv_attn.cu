@@ -18,7 +18,10 @@ constexpr size_t kSmemMost = 227 * 1024;
 // of its segment's ranges and those of the prefix's splits; every warp folds the (m) of
 // all of them, then adds the weighted rows of its share, four dims a lane,
 // and the first warp adds up the shares.  A row that the streaming kernel
-// wrote itself is skipped; a row without any token is zero.
+// wrote itself is skipped; a row without any token is zero.  What bounds it is the chain of
+// loads behind the wait -- span, sums, rows -- so spans come ready from the streaming kernel
+// and the first kAhead rows are fetched beside the sums (with divisions
+// for the spans and rows after the weights: 250 sequences behind a prefix 65 us, so 58).
 // ---------------------------------------------------------------------------
 struct JoinParams {
   int64_t B, Hq;
@@ -161,7 +164,7 @@ PieceGeom piece_geometry(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t 
 // kv head and 2 a segment, over their SMs, and 10 to start and end.
 // Both kernels mostly wait at their starts and ends, so side by side on an SM each
 // is best where it fits (64 sequences, prefix 8192: one after the other on
-// all SMs 56 us, 11 splits beside 60 SMs 44 us, 6 beside 100 59 us, 16 beside 20 70 us).
+// all SMs 53 us, 10 splits beside 68 SMs 40 us, 6 beside 100 48 us, 16 beside 20 67 us).
 // One after the other remains where the prefix alone fills the GPU, or the own
 // pages outweigh it.  Lengths live on the device: the prefix counts with its table's
 // size, the own tokens with half of theirs, and the streaming kernel keeps a
