@@ -372,6 +372,25 @@ def test_prefix_attention(Hq, Hkv, D, bs, B, dtype, code, cuda_device):
 
 
 @pytest.mark.parametrize("code", [None, *CODES])
+@pytest.mark.parametrize("B,Hq,prefix_pages,pages", [(40, 32, 600, 24), (6, 32, 600, 200), (150, 16, 9, 60),
+                                                     (20, 64, 2500, 2)])
+def test_prefix_lengths_far_from_the_tables(B, Hq, prefix_pages, pages, code, cuda_device):
+    """The SMs are shared out by the tables' sizes; the lengths follow later."""
+    q, cache, bt, cl = attention_case(cuda_device, B, Hq, 8, 128, 16, torch.bfloat16, code, [pages * 16] * B, seed=B,
+                                      nb=B * pages + 100)
+    g = torch.Generator().manual_seed(B)
+    pt = torch.randint(0, cache[0].shape[0], (prefix_pages,), generator=g).to(cuda_device, torch.int32)
+    some = torch.randint(0, pages * 16 + 1, (B,), generator=g).to(cuda_device, torch.int32)
+    for n, ctx in ((0, some), (37, torch.zeros_like(cl)), (prefix_pages * 16 - 3, torch.zeros_like(cl)), (1, cl),
+                   (prefix_pages * 16 + 99, torch.ones_like(cl))):
+        pl = torch.tensor([n], dtype=torch.int32, device=cuda_device)
+        out = K.paged_attention_prefix(q, cache[0], cache[1], pt, pl, bt, ctx, cache[2], cache[3])
+        torch.cuda.synchronize()
+        assert K.read_device_error() == 0
+        check_rows(out, q, *cache, bt, ctx, pt, min(n, prefix_pages * 16))
+
+
+@pytest.mark.parametrize("code", [None, *CODES])
 @pytest.mark.parametrize("bs", [16, 8])
 def test_prefix_dropped_ids_garbage_and_no_own_tokens(bs, code, cuda_device):
     B, n = 20, 515
