@@ -346,9 +346,11 @@ int b200_paged_attention_quant(const void* q, const void* k_cache, const void* v
  * B200_I8 / B200_F8E4M3 with scales as above.  prefix_len, context_len and
  * the tables are of `index_dtype` and on the device.  A sequence without any
  * token gives a zero row.  Softmax weights enter the second product in the
- * cache's 16-bit type, over 8-bit prefixes as f16.  workspace, cfg and limits
- * as b200_paged_attention_quant (the prefix's product takes block sizes up to
- * 128; larger ones go to the general kernel). */
+ * cache's 16-bit type, over 8-bit prefixes as f16.  workspace: 32-byte aligned
+ * (B200_ERR_ALIGNMENT otherwise), of
+ * b200_paged_attention_prefix_workspace_size() bytes (may be 0: NULL); cfg and
+ * limits as b200_paged_attention_quant (the prefix's product takes block sizes
+ * up to 128; larger ones go to the general kernel). */
 size_t b200_paged_attention_prefix_workspace_size(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t num_blocks,
                                                   int64_t block_size, int64_t max_prefix_blocks,
                                                   int64_t max_blocks, int32_t cache_dtype,

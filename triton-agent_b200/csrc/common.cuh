@@ -42,6 +42,7 @@ inline int dtype_size(int32_t dt) {
 }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+inline bool aligned32(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31u) == 0; }
 
 inline int device_sm_count() {
   int dev = 0, n = 0;

@@ -263,7 +263,8 @@ int attend(const AttnCall& a, const b200_launch_cfg* cfg, void* workspace, size_
   const int splits = prefix ? share_sms(g, a.Hkv, a.block_size, a.max_prefix_blocks, a.max_blocks, elem_of(a)) : 0;
   const SpaceBytes sb = space_bytes(g, a.Hq, splits);
   if (!g.whole && (workspace == nullptr || workspace_bytes < sb.spans + sb.rows + sb.prefix)) return B200_ERR_WORKSPACE;
-  if (!aligned16(workspace)) return B200_ERR_ALIGNMENT;
+  // (the prefix kernel stores 32 bytes of a piece row at a time; its parts and rows keep the base's alignment)
+  if (prefix ? !aligned32(workspace) : !aligned16(workspace)) return B200_ERR_ALIGNMENT;
   PieceSpace w{};
   w.spans = static_cast<int2*>(workspace);
   w.rows = reinterpret_cast<float*>(static_cast<char*>(workspace) + sb.spans);

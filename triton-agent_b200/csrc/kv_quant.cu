@@ -748,7 +748,6 @@ extern "C" int b200_paged_kv_dequant(const void* k_cache, const void* v_cache, c
   while (pages < kPages && B * out_pages > (int64_t)pages * 8 * device_sm_count()) pages *= 2;
   const int64_t chunks = (out_pages + pages - 1) / pages;
   if (chunks * B > 0x7fffffffLL || block_size * Hkv * D > (1 << 28)) return B200_ERR_UNSUPPORTED;
-  auto aligned32 = [](const void* q) { return (reinterpret_cast<uintptr_t>(q) & 31u) == 0; };
   const bool vec = D % 16 == 0 && aligned16(k_cache) && aligned16(v_cache) && aligned32(k_out) && aligned32(v_out);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   DequantParams p{B, Hkv, D, num_blocks, block_size, max_blocks, max_len, pages};
