@@ -3,7 +3,51 @@ what their documentation allows."""
 
 import ctypes
 
+import pytest
+import torch
+
 from b200ops.runtime import lib as L
+from b200ops.runtime import ops as K
+
+
+class Recorder:
+    """Stands in for the loaded library: keeps the arguments of each entry and answers
+    workspace queries with `size` (a number, or a function of the arguments)."""
+
+    def __init__(self, size=0):
+        self.size, self.calls = size, {}
+
+    def __getattr__(self, name):
+        def entry(*a):
+            self.calls.setdefault(name, []).append(a)
+            if name.endswith("_workspace_size"):
+                return self.size(*a) if callable(self.size) else self.size
+            return L.OK
+
+        return entry
+
+
+@pytest.fixture
+def recorder(monkeypatch):
+    """CPU tensors taken as if they were on device 0, entries recorded instead of run."""
+    r = Recorder()
+    monkeypatch.setattr(L, "load", lambda: r)
+    monkeypatch.setattr(K, "_on_one_device", lambda op, *t: 0)
+    monkeypatch.setattr(K, "_need_cuda", lambda op, *t: torch.device("cuda", 0))
+    monkeypatch.setattr(K, "_elsewhere", lambda dev: False)
+    monkeypatch.setattr(K, "_raw_stream", lambda dev: 0)
+    monkeypatch.setattr(K, "_stream", lambda dev: None)
+    monkeypatch.setattr(K.WORKSPACES, "get", lambda dev, n, tag: torch.empty(max(n, 1), dtype=torch.uint8))
+    K._scratch_bytes.cache_clear()
+    yield r
+    K._scratch_bytes.cache_clear()
+
+
+def decode_args(B=2, pages=4, index=torch.int32, D=128, Hkv=2, code=torch.int8, nb=16, bs=16):
+    cache = [torch.zeros(nb, bs, Hkv, D, dtype=code) for _ in range(2)]
+    scale = [torch.zeros(nb, Hkv, bs) for _ in range(2)] if code.itemsize == 1 else []
+    return (torch.zeros(B, 8, D).bfloat16(), *cache, *scale, torch.zeros(B, pages, dtype=index),
+            torch.ones(B, dtype=index))
 
 
 def test_prefix_workspace_alignment():
@@ -19,3 +63,36 @@ def test_prefix_workspace_alignment():
             assert lib.b200_paged_attention_prefix(
                 p, p, p, scale, scale, p, p, p, p, p, 2, 8, 2, 128, 16, 16, 8, 4, 0.0, L.BF16, code, L.I32,
                 ctypes.c_void_p((1 << 20) + off), need, None, None) == L.ERR_ALIGNMENT
+
+
+def launch_flags(arg):
+    return arg._obj.flags if arg is not None else 0
+
+
+@pytest.mark.parametrize("as_struct", [False, True])
+@pytest.mark.parametrize("entry", ["b200_paged_attention_quant", "b200_paged_attention"])
+def test_rewritten_lengths_and_tables_are_waited_for(entry, as_struct, recorder):
+    """Launch flag 8 reads table and lengths before the previous kernel is over.
+    Where the wrapper converts or compacts one of them, its own kernel is the
+    previous one: the flag is taken off; the other parameters and the caller's stay."""
+    quant = entry.endswith("quant")
+    op, pos = (K.paged_attention_quant, -2) if quant else (K.paged_attention, -2)
+    *front, bt, cl = decode_args(code=torch.int8 if quant else torch.bfloat16)
+    cfg = {"flags": 9, "stages": 6}
+    if as_struct:
+        cfg = L.LaunchCfg.from_dict(cfg)
+
+    def flags(table, lengths):
+        op(*front, table, lengths, cfg=cfg)
+        got = recorder.calls[entry][-1][pos]
+        assert got._obj.stages == 6
+        return launch_flags(got)
+
+    assert flags(bt, cl) == 9
+    assert flags(bt, cl.long()) == 1
+    assert flags(bt, torch.ones(4, dtype=torch.int32)[::2]) == 1
+    if quant:
+        assert flags(torch.zeros(2, 9, dtype=torch.int32)[:, :4], cl) == 1
+    assert flags(bt, cl) == 9
+    op(*front, bt, cl.long())
+    assert recorder.calls[entry][-1][pos] is None

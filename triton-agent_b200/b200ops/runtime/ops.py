@@ -48,6 +48,24 @@ def _cfg(cfg):
     return ctypes.byref(c) if c is not None else None
 
 
+_OVERLAP = 8  # launch flag: the kernel's prologue runs beside the previous kernel
+
+
+def _ordered(cfg):
+    """cfg without the overlap flag: for a call whose tables or lengths this
+    module has just rewritten with a kernel of its own, which an overlapping
+    prologue would not wait for."""
+    if cfg is None:
+        return None
+    c = L.LaunchCfg()
+    given = cfg if isinstance(cfg, L.LaunchCfg) else L.LaunchCfg.from_dict(cfg)
+    if given is None:
+        return None
+    ctypes.pointer(c)[0] = given
+    c.flags &= ~_OVERLAP
+    return c
+
+
 def _need_cuda(op: str, *ts: torch.Tensor | None) -> torch.device:
     dev = None
     for t in ts:
@@ -248,9 +266,9 @@ def paged_attention(q, k_cache, v_cache, block_table, context_len, scale: float 
     nb, bs, Hkv, D2 = k_cache.shape
     if D2 != D or tuple(v_cache.shape) != tuple(k_cache.shape):
         raise L.B200OpsError(L.ERR_BAD_ARG, "paged_attention", "cache shape mismatch")
-    if block_table.dtype != context_len.dtype:
-        context_len = context_len.to(block_table.dtype)
-    cl = context_len.contiguous()
+    cl = context_len.to(block_table.dtype).contiguous()
+    if cl is not context_len:
+        cfg = _ordered(cfg)
     max_blocks = block_table.shape[1]
     o = torch.empty_like(q) if out is None else out
     ws_bytes = paged_attention_workspace_size(B, Hq, max_blocks, bs, D, cfg)
@@ -477,6 +495,8 @@ def paged_attention_quant(q, k_cache, v_cache, k_scale, v_scale, block_table, co
     else:
         _check_out(op, "out", out, q.shape, q.dtype)
     sc = float(scale) if scale is not None else 1.0 / math.sqrt(D)
+    if bt is not block_table or cl is not context_len:
+        cfg = _ordered(cfg)
     c = _cfg(cfg)
     ws = _scratch(q, _scratch_size("b200_paged_attention_quant_workspace_size", c, B, Hq, Hkv, D, nb, bs,
                                    max_blocks))
