@@ -2,6 +2,9 @@
 what their documentation allows."""
 
 import ctypes
+import shutil
+import subprocess
+from pathlib import Path
 
 import pytest
 import torch
@@ -96,3 +99,50 @@ def test_rewritten_lengths_and_tables_are_waited_for(entry, as_struct, recorder)
     assert flags(bt, cl) == 9
     op(*front, bt, cl.long())
     assert recorder.calls[entry][-1][pos] is None
+
+
+GRANT_RACE = r"""
+#include <cuda_runtime.h>
+#include <atomic>
+#include <cstdio>
+#include <thread>
+static std::atomic<int> attribute{49152}, asked{0};
+static cudaError_t fake_device(int* d) { *d = 0; return cudaSuccess; }
+// the first two requests meet here, the larger one takes effect first
+template <typename K>
+static cudaError_t fake_set(K, cudaFuncAttribute, int bytes) {
+  const int n = asked.fetch_add(1);
+  if (n < 2) for (int i = 0; i < 500 && asked.load() < 2; ++i) std::this_thread::sleep_for(std::chrono::milliseconds(1));
+  if (n < 2 && bytes < 200000) std::this_thread::sleep_for(std::chrono::milliseconds(200));
+  attribute.store(bytes);
+  return cudaSuccess;
+}
+#define cudaGetDevice fake_device
+#define cudaFuncSetAttribute fake_set
+#include "common.cuh"
+static void kernel() {}
+int main() {
+  static b200::SmemGrant grant;
+  std::thread a([] { grant(kernel, 100000); }), b([] { grant(kernel, 200000); });
+  a.join(), b.join();
+  const int first = attribute.load();
+  if (grant(kernel, 200000) != cudaSuccess) return 3;
+  std::printf("%d %d\n", first, attribute.load());
+  return attribute.load() >= 200000 ? 0 : 1;
+}
+"""
+
+
+def test_shared_memory_grants_of_two_threads(tmp_path):
+    """Two threads' first calls of one kernel ask for different sizes at once: the
+    kernel's limit ends at or above both (against a fake of the CUDA calls)."""
+    nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
+    if not Path(nvcc).exists():
+        pytest.skip("no nvcc")
+    csrc = Path(K.__file__).resolve().parents[2] / "csrc"
+    src, exe = tmp_path / "grant.cu", tmp_path / "grant"
+    src.write_text(GRANT_RACE)
+    subprocess.run([nvcc, "-std=c++17", "-gencode", "arch=compute_100a,code=sm_100a", "-I", str(csrc), "-o", str(exe),
+                    str(src)], check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, r.stdout

@@ -52,23 +52,23 @@ inline int device_sm_count() {
 }
 
 // Shared memory beyond the default for a kernel, requested once for each device
-// and size (a request costs about a microsecond a launch otherwise).  One
-// SmemGrant per kernel, static at its launch site.
+// (a request costs about a microsecond a launch otherwise).  Always the most a
+// CTA may have: a request lowers the limit as well as it raises it, so that
+// requests of different sizes from two threads could leave the smaller one.
+// One SmemGrant per kernel without static shared memory, static at its launch site.
+constexpr size_t kSmemMost = 227 * 1024;
 struct SmemGrant {
-  std::atomic<int> most[64] = {};
+  std::atomic<bool> done[64] = {};
   template <typename K>
   cudaError_t operator()(K kern, size_t bytes) {
+    if (bytes > kSmemMost) return cudaErrorInvalidValue;
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     const bool known = dev >= 0 && dev < 64;
-    if (known && most[dev].load(std::memory_order_relaxed) >= (int)bytes) return cudaSuccess;
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-    if (e == cudaSuccess && known) {
-      int old = most[dev].load(std::memory_order_relaxed);
-      while (old < (int)bytes && !most[dev].compare_exchange_weak(old, (int)bytes)) {
-      }
-    }
+    if (known && done[dev].load(std::memory_order_acquire)) return cudaSuccess;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemMost);
+    if (e == cudaSuccess && known) done[dev].store(true, std::memory_order_release);
     return e;
   }
 };

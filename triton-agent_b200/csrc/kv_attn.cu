@@ -10,8 +10,6 @@ B200_DEVICE_ERROR_WORD()
 namespace b200 {
 namespace {
 
-constexpr size_t kSmemMost = 227 * 1024;
-
 // ---------------------------------------------------------------------------
 // Join: W warps a query row (1, 2, 4 or 8: as many as keep a GPU's worth of
 // warps busy when rows are few and their pieces many).  The row's pieces are those
