@@ -101,6 +101,21 @@ def test_rewritten_lengths_and_tables_are_waited_for(entry, as_struct, recorder)
     assert recorder.calls[entry][-1][pos] is None
 
 
+def test_workspace_of_each_device(monkeypatch, recorder):
+    """Workspace sizes follow the current device's SM count: the size of one device is
+    not given to a call on another (here: 1000 bytes on device 0, 2000 on 1)."""
+    at = [0]
+    monkeypatch.setattr(K, "_on_one_device", lambda op, *t: at[0])
+    recorder.size = lambda *a: 1000 * (at[0] + 1)
+    args = decode_args()
+    q, kc, vc, ks, vs, bt, cl = args
+    for at[0] in (0, 1, 0):
+        K.paged_attention_quant(*args)
+        K.paged_attention_prefix(q, kc, vc, bt[0], cl[:1], bt, cl, ks, vs)
+        for entry in ("b200_paged_attention_quant", "b200_paged_attention_prefix"):
+            assert recorder.calls[entry][-1][-3] == 1000 * (at[0] + 1)
+
+
 GRANT_RACE = r"""
 #include <cuda_runtime.h>
 #include <atomic>

@@ -327,14 +327,15 @@ def _scratch(like: torch.Tensor, nbytes: int) -> torch.Tensor | None:
 
 
 @functools.lru_cache(maxsize=256)
-def _scratch_bytes(fn: str, *sizes) -> int:
-    """A workspace size query of the library at the default launch parameters."""
+def _scratch_bytes(fn: str, dev: int, *sizes) -> int:
+    """A workspace size query of the library at the default launch parameters,
+    asked with `dev` current (the sizes follow its number of SMs)."""
     return int(getattr(L.load(), fn)(*sizes))
 
 
-def _scratch_size(fn: str, cfg, *sizes) -> int:
+def _scratch_size(fn: str, dev: int, cfg, *sizes) -> int:
     if cfg is None:
-        return _scratch_bytes(fn, *sizes, None)
+        return _scratch_bytes(fn, dev, *sizes, None)
     return int(getattr(L.load(), fn)(*sizes, cfg))
 
 
@@ -417,7 +418,7 @@ def rope_kv_append_paged_quant(q, k, v, positions, cos, sin, slot_mapping, k_cac
     else:
         _check_out(op, "q_out", q_out, q.shape, dt)
     pos, sm, c = positions.contiguous(), slot_mapping.contiguous(), _cfg(cfg)
-    ws = _scratch(k, _scratch_bytes("b200_rope_kv_append_paged_quant_workspace_size", T)) if T > 512 else None
+    ws = _scratch(k, _scratch_bytes("b200_rope_kv_append_paged_quant_workspace_size", dev, T)) if T > 512 else None
     st = L.load().b200_rope_kv_append_paged_quant(
         _p(q), k.data_ptr(), v.data_ptr(), pos.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0],
         sm.data_ptr(), _p(q_out), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
@@ -498,7 +499,7 @@ def paged_attention_quant(q, k_cache, v_cache, k_scale, v_scale, block_table, co
     if bt is not block_table or cl is not context_len:
         cfg = _ordered(cfg)
     c = _cfg(cfg)
-    ws = _scratch(q, _scratch_size("b200_paged_attention_quant_workspace_size", c, B, Hq, Hkv, D, nb, bs,
+    ws = _scratch(q, _scratch_size("b200_paged_attention_quant_workspace_size", dev, c, B, Hq, Hkv, D, nb, bs,
                                    max_blocks))
     st = L.load().b200_paged_attention_quant(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
                                              k_scale.data_ptr(), v_scale.data_ptr(), bt.data_ptr(), cl.data_ptr(),
@@ -555,7 +556,7 @@ def paged_attention_prefix(q, k_cache, v_cache, prefix_table, prefix_len, block_
         _check_out(op, "out", out, q.shape, q.dtype)
     sc = float(scale) if scale is not None else 1.0 / math.sqrt(D)
     c, code = _cfg(cfg), dtype_code(k_cache.dtype)
-    ws = _scratch(q, _scratch_size("b200_paged_attention_prefix_workspace_size", c, B, Hq, Hkv, D, nb, bs,
+    ws = _scratch(q, _scratch_size("b200_paged_attention_prefix_workspace_size", dev, c, B, Hq, Hkv, D, nb, bs,
                                    max_prefix, max_blocks, code))
     st = L.load().b200_paged_attention_prefix(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _p(k_scale),
                                               _p(v_scale), pt.data_ptr(), pl.data_ptr(), bt.data_ptr(),
