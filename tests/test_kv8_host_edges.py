@@ -116,6 +116,18 @@ def test_workspace_of_each_device(monkeypatch, recorder):
             assert recorder.calls[entry][-1][-3] == 1000 * (at[0] + 1)
 
 
+def test_64_bit_lengths_and_ids_beside_a_32_bit_table():
+    """Lengths and ids beyond 32 bits stay beyond every table and pool when they
+    are brought to the table's type (2^32 + 3 is no length of 3, nor block 3)."""
+    far = torch.tensor([5, 0, -7, 2 ** 31 - 1, 2 ** 31, 2 ** 32 + 3, -(2 ** 32) + 3, 2 ** 63 - 1, -(2 ** 63)])
+    got = K._index("op", "x", far, torch.int32, far.shape)
+    top = 2 ** 31 - 1
+    assert got.dtype == torch.int32 and got.tolist() == [5, 0, -1, top, top, top, -1, top, -1]
+    near = torch.tensor([3, -9], dtype=torch.int32)
+    assert K._index("op", "x", near, torch.int64, near.shape).tolist() == [3, -9]
+    assert K._index("op", "x", near, torch.int32, near.shape) is near
+
+
 GRANT_RACE = r"""
 #include <cuda_runtime.h>
 #include <atomic>

@@ -369,7 +369,8 @@ def _index(op: str, name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple
     if t.dtype not in (torch.int32, torch.int64):
         raise L.B200OpsError(L.ERR_UNSUPPORTED, op, f"{name} must be int32 or int64")
     if t.dtype != dtype:
-        t = t.to(dtype)
+        # saturated, not wrapped: a length beyond the table stays one, an id outside the pool outside
+        t = (t.clamp(-1, 2 ** 31 - 1) if dtype == torch.int32 else t).to(dtype)
     return t if t.is_contiguous() else t.contiguous()
 
 
