@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(128)
     const IndexPtr tab = part ? btab : ptab;
     const int64_t at0 = part ? b * max_blocks : 0;
     const int64_t ctx = part ? clen.at(b) : plen.at(0);
-    const int64_t nvb = ctx > 0 ? min((ctx + bs - 1) / bs, part ? max_blocks : max_prefix) : 0;
+    const int64_t nvb = ctx > 0 ? min((ctx - 1) / bs + 1, part ? max_blocks : max_prefix) : 0;
     int64_t rank = 0;
     for (int64_t j = 0; j < nvb; ++j) {
       const int64_t id = tab.at(at0 + j);

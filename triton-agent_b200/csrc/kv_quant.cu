@@ -600,7 +600,7 @@ __global__ void __launch_bounds__(256, 4)
   const int64_t b = blockIdx.x / chunks, first = (blockIdx.x - b * chunks) * p.pages;
   const int64_t bs = p.block_size;
   int64_t ctx = (int64_t)context_len[b];
-  const int64_t nvb = ctx > 0 ? min((ctx + bs - 1) / bs, p.max_blocks) : 0;
+  const int64_t nvb = ctx > 0 ? min((ctx - 1) / bs + 1, p.max_blocks) : 0;
   ctx = ctx < 0 ? 0 : (ctx < p.max_len ? ctx : p.max_len);
   cta_find_blocks(block_table + b * p.max_blocks, nvb, p.num_blocks, first, p.pages, s_id);
   constexpr int W = VEC ? 16 : 1;  // codes a thread takes at a time
