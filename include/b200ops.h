@@ -299,11 +299,13 @@ int b200_rope_kv_append_paged_quant(const void* q, const void* k, const void* v,
                                     const b200_launch_cfg* cfg, void* stream);
 
 /* Reads the contexts of an 8-bit cache back into dense k_out, v_out
- * [B, Hkv, max_len, D] of `dtype` (F16/BF16), as b200_flash_attn takes K and
- * V: row s < min(context_len[b], max_len) is code * scale of the sequence's
- * token s (blocks as in b200_paged_attention: ids outside [0, num_blocks)
- * are dropped and later blocks move up), rounded once; every other row is
- * zero.  cfg: none. */
+ * [B, Hkv, max_len, D] of `dtype` (F16/BF16): row s < min(context_len[b],
+ * max_len) is code * scale of the sequence's token s (blocks as in
+ * b200_paged_attention: ids outside [0, num_blocks) are dropped and later
+ * blocks move up), rounded once; every other row is zero.  b200_flash_attn
+ * takes the result where Hkv is its head count and every context fills
+ * max_len (it knows neither grouped heads nor lengths: a zero row is a key
+ * like any other).  cfg: none. */
 int b200_paged_kv_dequant(const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
                           const void* block_table, const void* context_len, void* k_out, void* v_out, int64_t B,
                           int64_t Hkv, int64_t D, int64_t num_blocks, int64_t block_size, int64_t max_blocks,
@@ -464,9 +466,9 @@ int b200_quantize_int8(const void* x, int8_t* q, float* scale, int64_t rows,
 
 /* ---- causal / full flash attention prefill -----------------------------------
  * Replaces triton_agent/ops/flash_attn_like/reference.py:7-31
- * q: [B, H, T, D]; k, v: [B, H, S, D]; o: [B, H, T, D]; dtype F16/BF16;
- * D = 128 on the tensor-core path.  causal: mask key s > query t
- * (reference.py:25-28, which assumes T == S).  lse (nullable): [B, H, T] f32
+ * q: [B, H, T, D]; k, v: [B, H, S, D] (as many heads as q, every key
+ * counts); o: [B, H, T, D]; dtype F16/BF16; D = 128 on the tensor-core path.
+ * causal: mask key s > query t (reference.py:25-28, which assumes T == S).  lse (nullable): [B, H, T] f32
  * natural-log softmax normaliser.  scale <= 0 means 1/sqrt(D).
  * cfg: split (heads per scheduling group, default 8), tile_k (exponential
  * pairs of every 8 computed by a polynomial on the FMA pipe: 1-3, default 2,

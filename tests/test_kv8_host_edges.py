@@ -128,6 +128,20 @@ def test_64_bit_lengths_and_ids_beside_a_32_bit_table():
     assert K._index("op", "x", near, torch.int32, near.shape) is near
 
 
+def test_flash_attn_refuses_keys_of_other_heads(recorder):
+    """K and V with fewer heads (as a grouped cache is read back), other sizes or
+    another type would be read out of range: refused before the launch."""
+    q = torch.zeros(2, 8, 4, 128).bfloat16()
+    good = torch.zeros(2, 8, 6, 128).bfloat16()
+    K.flash_attn(q, good, good)
+    bad = [good[:, :2].contiguous(), good[:1], good[..., :64].contiguous(), good.half(), good[:, :, :5].contiguous()]
+    for k, v in [(b, good) for b in bad] + [(good, b) for b in bad]:
+        with pytest.raises(L.B200OpsError) as e:
+            K.flash_attn(q, k, v)
+        assert e.value.code == L.ERR_BAD_ARG
+    assert len(recorder.calls["b200_flash_attn"]) == 1
+
+
 GRANT_RACE = r"""
 #include <cuda_runtime.h>
 #include <atomic>

@@ -434,7 +434,9 @@ def paged_kv_dequant(k_cache, v_cache, k_scale, v_scale, block_table, context_le
                      dtype: torch.dtype = torch.bfloat16, k_out: torch.Tensor | None = None,
                      v_out: torch.Tensor | None = None, cfg=None):
     """Contexts of an 8-bit paged cache read back as dense K and V
-    [B, Hkv, max_len, D] of `dtype`, as flash_attn takes them.  Row s <
+    [B, Hkv, max_len, D] of `dtype`.  (flash_attn takes them where Hkv is the
+    query's head count and every context is max_len; grouped heads and shorter
+    contexts need an attention that knows them.)  Row s <
     min(context_len[b], max_len) is code * scale of the sequence's token s
     (block rules of paged_attention), rounded once; all other rows are zero."""
     op = "paged_kv_dequant"
@@ -634,11 +636,15 @@ def quantize_int8(x: torch.Tensor, by_column: bool = False, cfg=None):
 # ------------------------------------------------------------ flash attention
 def flash_attn(q, k, v, causal: bool = False, scale: float | None = None, out=None, lse=None, cfg=None):
     """softmax(q k^T * scale [+ causal mask]) v (flash_attn_like/reference.py:22-31).
-    q [B,H,T,D], k/v [B,H,S,D]; returns [B,H,T,D] in q's dtype."""
+    q [B,H,T,D], k/v [B,H,S,D] of q's dtype and head count (no grouped heads,
+    no lengths: every key counts); returns [B,H,T,D] in q's dtype."""
     dev = _need_cuda("flash_attn", q, k, v, out, lse)
     _contig("flash_attn", q=q, k=k, v=v)
     B, H, T, D = q.shape
     S = k.shape[2]
+    for name, t in (("k", k), ("v", v)):
+        if t.shape != (B, H, S, D) or t.dtype != q.dtype:
+            raise L.B200OpsError(L.ERR_BAD_ARG, "flash_attn", f"{name} must be {q.dtype} {[B, H, S, D]}, as q's heads")
     if causal and T != S:
         raise L.B200OpsError(L.ERR_BAD_ARG, "flash_attn", "causal requires T == S (reference.py:25-28)")
     o = torch.empty_like(q) if out is None else out
