@@ -30,3 +30,57 @@ def test_lengths_at_the_ends_of_64_bits(D, flags, cuda_device):
         want = torch.zeros(2, 70, D, dtype=torch.float64, device=cuda_device)
         want[:, : n[b]] = rows64(cache[0], cache[2], bt[b], n[b]).transpose(0, 1)
         assert torch.equal(kd[b], want.to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("T,Hq,Hkv,D,bs,code", [(900, 3, 2, 64, 16, torch.int8), (900, 0, 3, 80, 5, torch.float8_e4m3fn),
+                                                (600, 240, 12, 128, 16, torch.int8), (700, 4, 140, 128, 32, torch.int8),
+                                                (2600, 8, 2, 128, 16, torch.float8_e4m3fn)])
+def test_colliding_slots_of_many_tokens(T, Hq, Hkv, D, bs, code, cuda_device):
+    """More than 512 tokens with shared slots: other head dims (general kernel), more
+    rows a token than a CTA holds (264 and 284), and many shared slots: the last token
+    that writes a slot is found in it, tokens out of range hide nothing."""
+    nb = (T + bs - 1) // bs + 10
+    x = list(append_inputs(T, Hq, Hkv, D, torch.bfloat16, nb, bs, code, seed=T))
+    g = torch.Generator().manual_seed(T)
+    slots, pos = x[6].clone(), x[3].clone()
+    slots[torch.randperm(T, generator=g)[: T // 4]] = int(slots[0])  # a quarter of the tokens, one slot
+    half = torch.randperm(T, generator=g)[: T // 2]
+    slots[half] = slots[half.flip(0)]  # pairs
+    slots[5], slots[T // 3] = -1, nb * bs
+    slots[T - 2] = slots[T - 1] = slots[3]
+    pos[T - 1], pos[T // 2] = 600, -3
+    x[6], x[3] = slots, pos
+    same(run_append(x, cuda_device), expect_append(x))
+
+
+def test_unaligned_append_of_many_tokens(cuda_device):
+    """K at 2 bytes past an aligned address: the general kernel, with shared slots."""
+    x = list(append_inputs(700, 2, 2, 128, torch.float16, 60, 16, torch.int8, seed=3))
+    x[6][100:140] = x[6][600:640].clone()
+    flat = torch.empty(x[1].numel() + 1, dtype=torch.float16, device=cuda_device)
+    k = flat[1:].view_as(x[1]).copy_(x[1])
+    assert k.data_ptr() % 16 == 2
+    q, _, v, pos, cos, sin, slots, c = x
+    d = [t.to(cuda_device) for t in (q, k, v, pos, cos, sin, slots)]
+    d[1] = k
+    cache = [t.to(cuda_device).clone() for t in (c.k_cache, c.v_cache, c.k_scale, c.v_scale)]
+    same((K.rope_kv_append_paged_quant(*d, *cache), cache), expect_append(x))
+
+
+@pytest.mark.parametrize("code", [None, torch.int8])
+def test_prefix_batch_of_more_segments_than_a_launch_takes(code, cuda_device):
+    """Eight head groups a sequence, 2400 segments: the call runs in slices of 256
+    sequences that share a workspace, prefix, own pages and join in turn."""
+    B, Hkv, n = 300, 64, 200
+    g = torch.Generator().manual_seed(2)
+    ctx = [int(c) for c in torch.randint(0, 40, (B,), generator=g)]
+    q, cache, bt, cl = attention_case(cuda_device, B, Hkv, Hkv, 128, 16, torch.float16, code, ctx, nb=1000)
+    pt = torch.randint(0, 1000, (13,), generator=g).to(cuda_device, torch.int32)
+    pl = torch.tensor([n], dtype=torch.int32, device=cuda_device)
+    run = lambda: K.paged_attention_prefix(q, cache[0], cache[1], pt, pl, bt, cl, cache[2], cache[3])  # noqa: E731
+    out = run()
+    torch.cuda.synchronize()
+    assert K.read_device_error() == 0
+    for b in (0, 1, 100, 255, 256, 257, 299):
+        check_rows(out[b:b + 1], q[b:b + 1], *cache, bt[b:b + 1], cl[b:b + 1], pt, n)
+    assert torch.equal(out, run())
