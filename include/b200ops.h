@@ -317,7 +317,8 @@ int b200_paged_kv_dequant(const void* k_cache, const void* v_cache, const float*
  * sums and accumulation in fp32.  int8: the queries enter as 24-bit integers
  * (off by 2^-23 of a row's largest), the softmax weights as 16-bit integers
  * relative to the largest of their 32 tokens (off by 2^-17 of that); e4m3:
- * both as f16.  A sequence without tokens gives a zero row.  workspace:
+ * both as f16 (weights off by 2^-11 of themselves, or 2^-32 of the largest
+ * where that is more).  A sequence without tokens gives a zero row.  workspace:
  * 16-byte aligned, of b200_paged_attention_quant_workspace_size() bytes (may
  * be 0: NULL); nothing in it is kept between calls, it needs no clearing.
  * Streaming kernel for D = 128, block sizes of 16, 32, ..., 256, 1, 2, 4 or 8
@@ -348,7 +349,7 @@ int b200_paged_attention_quant(const void* q, const void* k_cache, const void* v
  * B200_I8 / B200_F8E4M3 with scales as above.  prefix_len, context_len and
  * the tables are of `index_dtype` and on the device.  A sequence without any
  * token gives a zero row.  Softmax weights enter the second product in the
- * cache's 16-bit type, over 8-bit prefixes as f16.  workspace: 32-byte aligned
+ * cache's 16-bit type, over 8-bit prefixes as f16 (f16 with the same bounds).  workspace: 32-byte aligned
  * (B200_ERR_ALIGNMENT otherwise), of
  * b200_paged_attention_prefix_workspace_size() bytes (may be 0: NULL); cfg and
  * limits as b200_paged_attention_quant (the prefix's product takes block sizes

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from b200ops import workloads as WL
+from b200ops.ops.rope_kv_append_paged_quant import reference as RA
 from b200ops.runtime import ops as K
 from kv8_ref import check_rows, rows64
 from test_gpu_kv_quant import CODES, append_inputs, attention_case, expect_append, run_append, same
@@ -84,3 +85,80 @@ def test_prefix_batch_of_more_segments_than_a_launch_takes(code, cuda_device):
     for b in (0, 1, 100, 255, 256, 257, 299):
         check_rows(out[b:b + 1], q[b:b + 1], *cache, bt[b:b + 1], cl[b:b + 1], pt, n)
     assert torch.equal(out, run())
+
+
+def loud_key_case(dev, code, dtype, B, n, at, Hkv=8, G=4, bs=16):
+    """n tokens of which one (at) has a logit that leaves the others weights of 2^-20 to
+    2^-31 of its own, by head, and a value only in dim 0 (16-bit caches: none): dims 1..
+    of the output are the flat tail alone.  Tail keys are zero (their logits are exactly
+    0), tail values' largest element is the loud one's.  The same pages for every sequence."""
+    D, Hq = 128, Hkv * G
+    g = torch.Generator().manual_seed(n)
+    k, v = torch.zeros(n, Hkv, D), 100 * torch.rand(n, Hkv, D, generator=g) - 30
+    v[:, :, 0], v[:, :, 1] = 0, 100
+    k[at, :, 0], v[at] = 8, 0
+    if code is not None:
+        v[at, :, 0] = 100
+    want_bits = torch.linspace(20.3, 31.3, Hq)  # log2 of loud over tail
+    q = torch.zeros(B, Hq, D)
+    q[:, :, 0] = want_bits * (D ** 0.5 / 1.4426950408889634 / 8)
+    nb = (n + bs - 1) // bs
+    pad = lambda t: torch.cat((t, torch.zeros(nb * bs - n, *t.shape[1:]))).reshape(nb, bs, Hkv, D)  # noqa: E731
+    if code is None:
+        cache = (pad(k).to(dtype).to(dev), pad(v).to(dtype).to(dev), None, None)
+    else:
+        (kc, ks), (vc, vs) = (RA.quantise_rows(pad(t), code) for t in (k, v))
+        cache = tuple(t.to(dev).contiguous() for t in (kc, vc, ks.transpose(1, 2), vs.transpose(1, 2)))
+    table = torch.arange(nb, dtype=torch.int32, device=dev)
+    return q.to(dtype).to(dev), cache, table
+
+
+def check_tail(out, q, cache, table, n):
+    """Dims 1.. of every row against 64 bits.  A weight w_t (the largest is in [2^7, 2^15]
+    where it is held) rounds to f16: 2^-11 of itself, or 2^-25 where it is subnormal, which is
+    2^-32 of the largest; times at most 100 and n of them over a sum of that largest or more.
+    The logits are one product each (fp32, up to 31 in log2 units: 31 * 4 roundings of 2^-24),
+    exponentials and scale factors 2^-18 relative, sums n 2^-23; the output rounds once more (fp16:
+    at least 2^-25 absolute)."""
+    K64, V64 = rows64(cache[0], cache[2], table, n), rows64(cache[1], cache[3], table, n)
+    G = q.shape[1] // K64.shape[1]
+    u = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}[q.dtype]
+    x = torch.einsum("hd,nhd->hn", q[0].double(), K64.repeat_interleave(G, 1)) / 128 ** 0.5
+    want = torch.einsum("hn,nhd->hd", torch.softmax(x, -1), V64.repeat_interleave(G, 1))[:, 1:]
+    mean = torch.einsum("hn,nhd->hd", torch.softmax(x, -1), V64.abs().repeat_interleave(G, 1))[:, 1:]
+    bound = mean * (2.0 ** -11 + 2.0 ** -17 + 2.0 ** -18 + n * 2.0 ** -23) + 100 * n * 2.0 ** -32
+    bound = bound * (1 + 2.0 ** -7) + u * (want.abs() + bound) + 2.0 ** -25
+    off = (out[:, :, 1:].double() - want).abs()
+    assert (off <= bound).all(), float((off / bound).max())
+
+
+TAIL = [(None, torch.float16), (torch.float8_e4m3fn, torch.float16), (torch.float8_e4m3fn, torch.bfloat16)]
+
+
+@pytest.mark.parametrize("at", [0, 150, 299])
+@pytest.mark.parametrize("code,dtype", [*TAIL, (torch.int8, torch.float16)])
+def test_flat_tail_behind_a_loud_key_in_the_prefix(code, dtype, at, cuda_device):
+    """Weights that the second product takes as f16: a tail far below the largest keeps
+    its bits (16-bit prefix in fp16, 8-bit prefixes)."""
+    n = 300
+    for B in (20, 70):  # one row tile of query rows, and three
+        q, cache, pt = loud_key_case(cuda_device, code, dtype, B, n, at)
+        pl = torch.tensor([n], dtype=torch.int32, device=cuda_device)
+        none = torch.zeros(B, dtype=torch.int32, device=cuda_device)
+        bt = torch.zeros(B, 1, dtype=torch.int32, device=cuda_device)
+        check_tail(K.paged_attention_prefix(q, cache[0], cache[1], pt, pl, bt, none, cache[2], cache[3]), q, cache, pt, n)
+
+
+@pytest.mark.parametrize("at", [0, 150, 299])
+@pytest.mark.parametrize("code,dtype", TAIL)
+def test_flat_tail_behind_a_loud_key_in_own_pages(code, dtype, at, cuda_device):
+    """The same in the streaming kernel: own pages beside an empty prefix, and (8-bit) a decode."""
+    n, B = 300, 150
+    q, cache, table = loud_key_case(cuda_device, code, dtype, B, n, at)
+    bt = table.expand(B, -1).contiguous()
+    cl = torch.full((B,), n, dtype=torch.int32, device=cuda_device)
+    zero = torch.zeros(1, dtype=torch.int32, device=cuda_device)
+    check_tail(K.paged_attention_prefix(q, cache[0], cache[1], table, zero, bt, cl, cache[2], cache[3]), q, cache, table, n)
+    if code is not None:
+        for b in (20, B):  # a CTA a segment, and ranges
+            check_tail(K.paged_attention_quant(q[:b], *cache, bt[:b], cl[:b]), q, cache, table, n)

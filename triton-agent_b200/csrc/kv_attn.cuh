@@ -18,7 +18,8 @@
 // The streaming kernel multiplies int8 codes by bytes of the queries and weights.
 // e4m3 codes there, and all codes in the prefix kernel, are widened to f16 (exact),
 // with q in f16 after an exact power-of-two scaling of each row, and the weights
-// rounded to f16 (half a step 2^-12).
+// rounded to f16: off by 2^-11 of themselves, or by 2^-32 of the largest where
+// that is more (m sits 2^7 below the largest weight, see ref_below).
 #pragma once
 
 #include <math.h>
@@ -312,13 +313,23 @@ __device__ __forceinline__ void load_q_frags8(const T* __restrict__ qrow0, int l
 // and nothing scaled by it survives, and finite, so that differences are.
 constexpr float kNoMax = -1e30f;
 
-// Raises the running maxima of this thread's two heads to m where that is larger.
-__device__ __forceinline__ void raise_to(const float (&m)[2], float (&mu)[2], float (&lp)[2], float (&o)[8][4]) {
+// How far below the largest logit the reference mu is set.  Weights that go to f16 are
+// 2^7 where it is set and, as it may lag by 2^8, 2^15 at most: the range of f16 then
+// holds weights down to 2^-21 of the largest in full, and to 2^-32 as
+// subnormals (set at the largest itself 2^-14 and 2^-25: a long flat tail
+// behind one loud key lost its bits).  bf16 has the range of fp32.
+template <typename M>
+constexpr float ref_below() { return std::is_same<M, __half>::value ? 7.0f : 0.0f; }
+
+// Sets the references of this thread's two heads `below` m where that raises them.
+__device__ __forceinline__ void raise_to(const float (&m)[2], float below, float (&mu)[2], float (&lp)[2],
+                                         float (&o)[8][4]) {
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
-    if (!(m[c] > mu[c])) continue;
-    const float alpha = ex2(mu[c] - m[c]);
-    mu[c] = m[c];
+    const float ref = m[c] - below;
+    if (!(ref > mu[c])) continue;
+    const float alpha = ex2(mu[c] - ref);
+    mu[c] = ref;
     lp[c] *= alpha;
 #pragma unroll
     for (int mt = 0; mt < 8; ++mt) {
@@ -329,18 +340,20 @@ __device__ __forceinline__ void raise_to(const float (&m)[2], float (&mu)[2], fl
 }
 
 // The same to the largest logits in the warp (of this thread: top), when one
-// exceeds its maximum by more than 2^8 (exact: O and l share the offset).  Most
+// exceeds that place by more than 2^8 (exact: O and l share the reference).  Most
 // entries need one vote here and no exchange.
+template <typename M>
 __device__ __forceinline__ void raise_max_lazy(const float (&top)[2], float (&mu)[2], float (&lp)[2],
                                                float (&o)[8][4]) {
+  constexpr float kBelow = ref_below<M>();
   float m[2] = {top[0], top[1]};
-  if (!__any_sync(0xffffffffu, m[0] - mu[0] > 8.0f || m[1] - mu[1] > 8.0f)) return;
+  if (!__any_sync(0xffffffffu, m[0] - mu[0] > 8.0f + kBelow || m[1] - mu[1] > 8.0f + kBelow)) return;
 #pragma unroll
   for (int off = 4; off <= 16; off <<= 1) {
     m[0] = fmaxf(m[0], __shfl_xor_sync(0xffffffffu, m[0], off));
     m[1] = fmaxf(m[1], __shfl_xor_sync(0xffffffffu, m[1], off));
   }
-  raise_to(m, mu, lp, o);
+  raise_to(m, kBelow, mu, lp, o);
 }
 
 // Where a lane reads an entry's two chunks: its ldmatrix row of K with its first
@@ -445,7 +458,7 @@ __device__ __forceinline__ void mma_pair8(uint32_t at, const Lane8& x, const int
       m[1] = fmaxf(m[1], __shfl_xor_sync(0xffffffffu, m[1], off));
     }
     m[0] = fmaxf(m[0], kNoMax), m[1] = fmaxf(m[1], kNoMax);
-    if (__any_sync(0xffffffffu, m[0] - mu[0] > 8.0f || m[1] - mu[1] > 8.0f)) raise_to(m, mu, lp, o);
+    if (__any_sync(0xffffffffu, m[0] - mu[0] > 8.0f || m[1] - mu[1] > 8.0f)) raise_to(m, 0.f, mu, lp, o);
     const float f[2] = {ex2(m[0] - mu[0]), ex2(m[1] - mu[1])};
     // weights relative to the pair's largest, as B fragments: pb[t][c], t = 0 the high byte
     uint32_t pb[2][2];
@@ -484,7 +497,7 @@ __device__ __forceinline__ void mma_pair8(uint32_t at, const Lane8& x, const int
       }
     }
   } else {
-    raise_max_lazy(m, mu, lp, o);
+    raise_max_lazy<__half>(m, mu, lp, o);
     uint32_t pb[2][2];
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
@@ -550,7 +563,7 @@ __device__ __forceinline__ void mma_chunk16(uint32_t kb, uint32_t vb, int ntok, 
     }
   }
   const float top[2] = {fmaxf(y[0], y[2]), fmaxf(y[1], y[3])};
-  raise_max_lazy(top, mu, lp, o);
+  raise_max_lazy<T>(top, mu, lp, o);
   const float p0 = ex2(y[0] - mu[0]), p2 = ex2(y[2] - mu[0]);
   const float p1 = ex2(y[1] - mu[1]), p3 = ex2(y[3] - mu[1]);
   lp[0] += p0 + p2;

@@ -561,11 +561,12 @@ __global__ void __launch_bounds__(PrefixRegs<sizeof(KV) == 1>::threads, 1)
       const float mx = sm100::fmax3(mx4[0], mx4[1], fmaxf(mx4[2], mx4[3])) * f;
       float alpha = 1.f;
       bool rescale = false;
+      constexpr float kBelow = ref_below<M>();  // (f16 weights: the largest between 2^7 and 2^15)
       if (m_used == -INFINITY) {
-        m_used = mx;
-      } else if (mx > m_used + 8.0f) {
-        alpha = ex2(m_used - mx);
-        m_used = mx;
+        m_used = mx - kBelow;
+      } else if (mx > m_used + (8.0f + kBelow)) {
+        alpha = ex2(m_used - (mx - kBelow));
+        m_used = mx - kBelow;
         rescale = true;
       }
       const float neg = m_used == -INFINITY ? 0.f : -m_used;
