@@ -314,8 +314,8 @@ int b200_paged_kv_dequant(const void* k_cache, const void* v_cache, const float*
 
 /* Paged decode attention over an 8-bit cache: b200_paged_attention of the
  * cache's values code * scale, without writing them out.  Softmax statistics,
- * sums and accumulation in fp32.  int8: the queries enter as 24-bit integers
- * (off by 2^-23 of a row's largest), the softmax weights as 16-bit integers
+ * sums and accumulation in fp32.  int8: the queries enter as 32-bit integers
+ * (off by 2^-31 of a row's largest), the softmax weights as 16-bit integers
  * relative to the largest of their 32 tokens (off by 2^-17 of that); e4m3:
  * both as f16 (weights off by 2^-11 of themselves, or 2^-32 of the largest
  * where that is more).  A sequence without tokens gives a zero row.  workspace:

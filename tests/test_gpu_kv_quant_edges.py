@@ -162,3 +162,34 @@ def test_flat_tail_behind_a_loud_key_in_own_pages(code, dtype, at, cuda_device):
     if code is not None:
         for b in (20, B):  # a CTA a segment, and ranges
             check_tail(K.paged_attention_quant(q[:b], *cache, bt[:b], cl[:b]), q, cache, table, n)
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("dtype,loud", [(torch.float16, 3e4), (torch.bfloat16, 1e5), (torch.bfloat16, 1e6)])
+@pytest.mark.parametrize("Hkv,G,rows", [(8, 4, "one"), (2, 8, "all"), (1, 1, "all")])
+def test_loud_query_element_over_silent_key_channels(Hkv, G, rows, dtype, loud, code, cuda_device):
+    """Query rows with one element far above the others, over key channels that hold
+    zeros: the logits are those of the other elements, which keep their bits.  Few
+    tokens, so that a logit's error is the output's (bounds of kv8_ref, which count no
+    term of the row's largest element); other rows of the batch without such an element."""
+    B, D = 6, 128
+    ctx = [2, 3, 2, 5, 2, 40]
+    g = torch.Generator().manual_seed(int(loud))
+    k, v = (torch.randn(60, 16, Hkv, D, generator=g) for _ in range(2))
+    k[..., 17] = 0
+    (kc, ks), (vc, vs) = (RA.quantise_rows(t, code) for t in (k, v))
+    cache = [t.to(cuda_device).contiguous() for t in (kc, vc, ks.transpose(1, 2), vs.transpose(1, 2))]
+    q = torch.randn(B, Hkv * G, D, generator=g).to(dtype)
+    if rows == "one":
+        q[0, 2, 17], q[3, Hkv * G - 1, 17] = loud, -loud
+    else:
+        q[..., 17] = loud
+    q = q.to(cuda_device)
+    bt = torch.randperm(60, generator=g)[: B * 3].reshape(B, 3).to(cuda_device, torch.int32)
+    cl = torch.tensor(ctx, dtype=torch.int32, device=cuda_device)
+    check_rows(K.paged_attention_quant(q, *cache, bt, cl), q, *cache, bt, cl)
+    wide = torch.cat((bt, torch.full((B, 60), -1, dtype=torch.int32, device=cuda_device)), 1)  # (ranges and a join)
+    check_rows(K.paged_attention_quant(q, *cache, wide, cl), q, *cache, wide, cl)
+    pt, pl = bt[5].clone(), cl[5:].clone()
+    check_rows(K.paged_attention_prefix(q, cache[0], cache[1], pt, pl, bt, cl, cache[2], cache[3]), q, *cache, bt, cl, pt,
+               40)

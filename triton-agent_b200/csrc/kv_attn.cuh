@@ -235,8 +235,11 @@ __global__ void __launch_bounds__(128)
 // int8: m16n8k32 tiles of bytes, so that codes need no widening (which was half
 // of the instructions: 64 sequences 121 us with codes widened to f16, 114 us
 // so).  The other operand is a sum of byte terms, a product each:
-//   q   the row scaled by a power of two to [2^22, 2^23) and rounded to an integer,
-//       its three bytes (the top one signed): off by 2^-23 of the row's largest
+//   q   the row scaled by a power of two to [2^30, 2^31) and rounded to an integer,
+//       its four bytes (the top one signed): off by 2^-31 of the row's largest.  The
+//       last byte is zero but for elements below 2^-15 of the largest (fp16: 2^-12);
+//       its products run where a warp's rows have such elements (without it one
+//       element 2^18 above the others, over a key channel of zeros, left them 6 bits)
 //   w   relative to the largest of its 32 tokens (so that a long flat tail behind
 //       one large weight keeps its bits), as a 16-bit integer, two unsigned bytes:
 //       off by 2^-17 of that largest
@@ -255,17 +258,19 @@ __device__ __forceinline__ void pow2_scale(float amax, float& up, float& down) {
 
 // This warp's query rows as B fragments; slA, slB: logit factors of heads 2q, 2q + 1.
 // int8: qf[8t + i], t = 0 the top byte, holds dims 16i + 4q + {0..3} of head r
-// (zero for r >= G).  e4m3: qf[2i + {0, 1}] those dims in f16.
+// (zero for r >= G); true where a last byte (t = 3) of the warp is not zero.
+// e4m3: qf[2i + {0, 1}] those dims in f16; false.
 template <typename KV>
-constexpr int q_words() { return std::is_same<KV, int8_t>::value ? 24 : 16; }
+constexpr int q_words() { return std::is_same<KV, int8_t>::value ? 32 : 16; }
 template <typename T, typename KV, int G>
-__device__ __forceinline__ void load_q_frags8(const T* __restrict__ qrow0, int lane, float qscale,
+__device__ __forceinline__ bool load_q_frags8(const T* __restrict__ qrow0, int lane, float qscale,
                                               uint32_t (&qf)[q_words<KV>()], float& slA, float& slB) {
   const int qh = lane >> 2, qc = (lane & 3) * 4;
   const T* qr = qrow0 + (qh < G ? qh : 0) * kD;
   float f[8][4];
   float amax = 0.f;
   bool bad = false;  // an infinity or a NaN: the row's logits are NaN
+  uint32_t low = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const uint2 raw = *reinterpret_cast<const uint2*>(qr + 16 * i + qc);
@@ -281,15 +286,18 @@ __device__ __forceinline__ void load_q_frags8(const T* __restrict__ qrow0, int l
   amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
   float up, down;
   if constexpr (std::is_same<KV, int8_t>::value) {
-    pow2_scale<22>(amax, up, down);
+    pow2_scale<22>(amax, up, down);  // (units of the third byte)
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       uint32_t v[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) v[u] = (uint32_t)__float2int_rn(f[i][u] * up);
+      for (int u = 0; u < 4; ++u) {
+        v[u] = (uint32_t)__float2int_rn(f[i][u] * up * 256.0f);
+        low |= v[u];
+      }
 #pragma unroll
-      for (int t = 0; t < 3; ++t) {
-        const int sel = 2 - t;
+      for (int t = 0; t < 4; ++t) {
+        const int sel = 3 - t;
         const uint32_t lo = __byte_perm(v[0], v[1], sel | ((4 + sel) << 4));
         const uint32_t hi = __byte_perm(v[2], v[3], sel | ((4 + sel) << 4));
         qf[8 * t + i] = __byte_perm(lo, hi, 0x5410);
@@ -307,6 +315,7 @@ __device__ __forceinline__ void load_q_frags8(const T* __restrict__ qrow0, int l
   const float sl = any & (0xfu << (lane & ~3)) ? __uint_as_float(0x7fc00000u) : qscale * down;
   slA = __shfl_sync(0xffffffffu, sl, (lane & 3) * 8);
   slB = __shfl_sync(0xffffffffu, sl, (lane & 3) * 8 + 4);
+  return std::is_same<KV, int8_t>::value && __any_sync(0xffffffffu, (low & 0xffu) != 0);
 }
 
 // Running maximum of a head without tokens: so low that any logit raises it
@@ -378,8 +387,8 @@ struct Lane8 {
 // swizzled, scales as [head][token], the entry at `at`.
 template <typename KV>
 __device__ __forceinline__ void mma_pair8(uint32_t at, const Lane8& x, const int (&nt)[2], int lane, float slA,
-                                          float slB, const uint32_t (&qf)[q_words<KV>()], float (&o)[8][4],
-                                          float (&mu)[2], float (&lp)[2]) {
+                                          float slB, const uint32_t (&qf)[q_words<KV>()], bool last_byte,
+                                          float (&o)[8][4], float (&mu)[2], float (&lp)[2]) {
   constexpr bool kInt = std::is_same<KV, int8_t>::value;
   const int tr = lane >> 2;
   float y[2][4], iv[2][2];
@@ -412,6 +421,22 @@ __device__ __forceinline__ void mma_pair8(uint32_t at, const Lane8& x, const int
         acc_values(d[2][i], d[2][i + 1], b0, b1);
         sm100::ffma2(m0, m1, s[i], s[i + 1], 256.0f, 256.0f, m0, m1);
         sm100::ffma2(s[i], s[i + 1], m0, m1, 256.0f, 256.0f, b0, b1);
+      }
+      if (last_byte) {  // (uniform; the rows of K once more rather than held)
+        int32_t e[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t kr[4];
+          ldsm_x4(ka ^ (j << 5), kr[0], kr[1], kr[2], kr[3]);
+          if (j == 0) mma8_start<true>(e, kr, qf[24], qf[25], kAccStart);
+          else mma8_add<true>(e, kr, qf[24 + 2 * j], qf[25 + 2 * j]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+          float e0, e1;
+          acc_values(e[i], e[i + 1], e0, e1);
+          sm100::ffma2(s[i], s[i + 1], e0, e1, 1.0f / 256.0f, 1.0f / 256.0f, s[i], s[i + 1]);
+        }
       }
     } else {
       float s1[4] = {0.f, 0.f, 0.f, 0.f};
@@ -908,6 +933,7 @@ __global__ void __launch_bounds__((kConsumers + 1) * 32, 1)
     float slA = p.qscale, slB = p.qscale;
 #pragma unroll
     for (int i = 0; i < 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    bool last_byte = false;
     int cur = -1;
     uint32_t xph = 0;
     int st = slot % p.stages;
@@ -927,13 +953,13 @@ __global__ void __launch_bounds__((kConsumers + 1) * 32, 1)
           cur = m.seg;
           const int64_t b = m.seg % B, kvh = (int64_t)(m.seg / B) * HG + w;
           const T* qrow = q + (b * p.Hq + kvh * G) * kD;
-          if constexpr (k8) load_q_frags8<T, KV, G>(qrow, lane, p.qscale, qf, slA, slB);
+          if constexpr (k8) last_byte = load_q_frags8<T, KV, G>(qrow, lane, p.qscale, qf, slA, slB);
           else load_q_frags<T, G>(qrow, lane, qb);
         }
         const uint32_t pg = base + st * p.entry_bytes;
         if constexpr (k8) {
           const int nt[2] = {m.ntok, m.piece};
-          mma_pair8<KV>(pg, lane8, nt, lane, slA, slB, qf, o, mu, lp);
+          mma_pair8<KV>(pg, lane8, nt, lane, slA, slB, qf, last_byte, o, mu, lp);
         } else {
           mma_chunk16<T>(pg + w * kChunk * 256, pg + 2 * box + w * kChunk * 256, m.ntok, lane, p.qscale, qb, o, mu, lp);
         }
