@@ -2,6 +2,7 @@
 what their documentation allows."""
 
 import ctypes
+import importlib.util
 import shutil
 import subprocess
 from pathlib import Path
@@ -140,6 +141,25 @@ def test_flash_attn_refuses_keys_of_other_heads(recorder):
             K.flash_attn(q, k, v)
         assert e.value.code == L.ERR_BAD_ARG
     assert len(recorder.calls["b200_flash_attn"]) == 1
+
+
+def test_build_refuses_too_few_registers_for_the_split():
+    """The prefix kernel's register split waits for good with fewer registers at
+    launch than it hands out: the build reads ptxas's report and stops."""
+    spec = importlib.util.spec_from_file_location("lib_build", Path(K.__file__).resolve().parents[2] / "build.py")
+    b = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(b)
+    entry = ("ptxas info    : Compiling entry function '_ZN4b20018prefix_attn_kernelI{0}EEv' for 'sm_100a'\n"
+             "ptxas info    : Function properties for _ZN4b20018prefix_attn_kernelI{0}EEv\n"
+             "    0 bytes stack frame, 0 bytes spill stores, 0 bytes spill loads\n"
+             "ptxas info    : Used {1} registers, used 2 barriers\n")
+    other = entry.replace("18prefix_attn_kernel", "24paged_attn_pieces_kernel").format("x", 90)
+    for src, need in (("kv_attn_16.cu", 168), ("kv_attn_i8.cu", 128), ("kv_attn_e4m3.cu", 128)):
+        b.check_registers(src, other + entry.format("6__half", need) + other + entry.format("13__nv_bfloat16", need + 8))
+        with pytest.raises(RuntimeError, match="registers"):
+            b.check_registers(src, entry.format("6__half", need) + other + entry.format("13__nv_bfloat16", need - 8))
+        with pytest.raises(RuntimeError, match="no register report"):
+            b.check_registers(src, other)
 
 
 GRANT_RACE = r"""

@@ -15,6 +15,7 @@ from __future__ import annotations
 import argparse
 import concurrent.futures as cf
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -40,6 +41,27 @@ NVCC_FLAGS = [
 ]
 
 
+# Registers a thread that kernels with a register split (setmaxnreg) need at
+# launch, by source file; with fewer the split would wait for good.
+LAUNCH_REGISTERS = {
+    "kv_attn_16.cu": ("prefix_attn_kernel", 168),
+    "kv_attn_i8.cu": ("prefix_attn_kernel", 128),
+    "kv_attn_e4m3.cu": ("prefix_attn_kernel", 128),
+}
+
+
+def check_registers(src_name: str, log: str) -> None:
+    """Raises if ptxas (its -v report: log) gave a kernel fewer registers than its split hands out."""
+    kernel, need = LAUNCH_REGISTERS[src_name]
+    used = re.findall(r"Compiling entry function '(\w*" + kernel + r"\w*)'(?:(?!Compiling entry).)*?Used (\d+) registers",
+                      log, re.S)
+    if not used:
+        raise RuntimeError(f"{src_name}: no register report of {kernel}")
+    for name, n in used:
+        if int(n) < need:
+            raise RuntimeError(f"{src_name}: {name} has {n} registers at launch, its split hands out {need}")
+
+
 def nvcc() -> str:
     cand = os.environ.get("NVCC") or shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
     return cand
@@ -53,11 +75,14 @@ def _deps_mtime() -> float:
 def _compile(src: Path, verbose: bool, extra: list[str]) -> tuple[Path, str]:
     obj = BUILD / (src.stem + ".o")
     cmd = [nvcc(), *ARCH_FLAGS, *NVCC_FLAGS, *extra, "-I", str(INCLUDE), "-c", str(src), "-o", str(obj)]
-    if verbose:
+    report = src.name in LAUNCH_REGISTERS
+    if verbose or report:
         cmd.insert(1, "-Xptxas=-v")
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
         raise RuntimeError(f"nvcc failed for {src.name}:\n{' '.join(cmd)}\n{proc.stdout}\n{proc.stderr}")
+    if report:
+        check_registers(src.name, proc.stderr)
     return obj, proc.stderr
 
 

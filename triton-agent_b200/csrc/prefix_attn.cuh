@@ -121,10 +121,12 @@ __device__ __forceinline__ uint32_t kv_at(int r, int c) {
 }
 
 // Registers a thread, softmax warps and the others: 128 at launch with 8-bit caches (8 warps each), 168
-// with 16-bit ones (8 and 4).
+// with 16-bit ones (8 and 4).  The split hands out what the kernel has at launch; build.py holds the
+// compiler's choice against `launch`.
 template <bool k8>
 struct PrefixRegs {
-  static constexpr int low = 72, high = k8 ? 184 : 216, threads = k8 ? 512 : 384;
+  static constexpr int low = 72, high = k8 ? 184 : 216, threads = k8 ? 512 : 384, launch = k8 ? 128 : 168;
+  static_assert(launch * threads >= 256 * high + (threads - 256) * low, "more registers than at launch");
 };
 
 template <typename T, typename KV>
@@ -716,15 +718,19 @@ int launch_prefix(const AttnCall& a, const PieceGeom& g, const PieceSpace& w, cu
                       4 * (kPScaleRing * kPMaxPages + 2 * kPList);
   static_assert(PrefixSmem<k8>::oBars + 1024 + 1024 <= 227 * 1024, "shared memory of a CTA");
   auto kern = prefix_attn_kernel<T, KV>;
-  // the register split (setmaxnreg) needs what it hands out at launch
   using Regs = PrefixRegs<k8>;
-  static const int regs = [&] {
+  // (without the registers the split hands out its warps would wait for good; a
+  // failed query is asked again by the next call)
+  static std::atomic<bool> checked{false};
+  if (!checked.load(std::memory_order_relaxed)) {
     cudaFuncAttributes at{};
-    return cudaFuncGetAttributes(&at, kern) == cudaSuccess ? at.numRegs : 0;
-  }();
-  if (regs * Regs::threads < 256 * Regs::high + (Regs::threads - 256) * Regs::low) {
-    set_last_error_detail("prefix_attn_kernel: too few registers at launch for its split");
-    return B200_ERR_LAUNCH;
+    const cudaError_t qe = cudaFuncGetAttributes(&at, kern);
+    if (qe != cudaSuccess) return launch_status(qe);
+    if (at.numRegs < Regs::launch) {
+      set_last_error_detail("prefix_attn_kernel: too few registers at launch for its split");
+      return B200_ERR_LAUNCH;
+    }
+    checked.store(true, std::memory_order_relaxed);
   }
   static SmemGrant grant;
   cudaError_t e = grant(kern, smem);
