@@ -419,7 +419,7 @@ def rope_kv_append_paged_quant(q, k, v, positions, cos, sin, slot_mapping, k_cac
     else:
         _check_out(op, "q_out", q_out, q.shape, dt)
     pos, sm, c = positions.contiguous(), slot_mapping.contiguous(), _cfg(cfg)
-    ws = _scratch(k, _scratch_bytes("b200_rope_kv_append_paged_quant_workspace_size", dev, T)) if T > 512 else None
+    ws = _scratch(k, _scratch_bytes("b200_rope_kv_append_paged_quant_workspace_size", dev, T))
     st = L.load().b200_rope_kv_append_paged_quant(
         _p(q), k.data_ptr(), v.data_ptr(), pos.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0],
         sm.data_ptr(), _p(q_out), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),

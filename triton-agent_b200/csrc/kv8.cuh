@@ -10,6 +10,13 @@ namespace b200 {
 
 using e4m3_t = __nv_fp8_e4m3;
 
+// 32 bytes of one lane as one store (whole sectors; dst 32-byte aligned).
+__device__ __forceinline__ void stg256(void* dst, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
 // Largest code magnitude.
 template <typename KV>
 __host__ __device__ constexpr float kv8_max() {

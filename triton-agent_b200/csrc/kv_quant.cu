@@ -540,13 +540,6 @@ struct DequantParams {
   int pages;
 };
 
-// 32 bytes of one lane as one store (whole sectors).
-__device__ __forceinline__ void stg256(void* dst, const uint32_t* v) {
-  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]),
-               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-               : "memory");
-}
-
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   T e[2] = {from_f32<T>(lo), from_f32<T>(hi)};

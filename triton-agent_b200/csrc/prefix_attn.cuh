@@ -106,13 +106,6 @@ __device__ __forceinline__ float stage_q_rows(const T* __restrict__ q, int r0, i
   return factor;
 }
 
-// 32 bytes of one lane as one store (whole sectors).
-__device__ __forceinline__ void stg256(float* dst, const uint32_t* v) {
-  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst), "r"(v[0]), "r"(v[1]), "r"(v[2]),
-               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-               : "memory");
-}
-
 // A K or V tile: groups of eight tokens, each with dims 0..63 and then 64..127
 // as an atom of eight swizzled 128-byte rows, so that a page is one contiguous
 // box whatever its size.  Where 16-byte chunk c of token r sits:
