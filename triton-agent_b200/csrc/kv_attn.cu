@@ -166,7 +166,8 @@ PieceGeom piece_geometry(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t 
 // One after the other remains where the prefix alone fills the GPU, or the own
 // pages outweigh it.  Lengths live on the device: the prefix counts with its table's
 // size, the own tokens with half of theirs (an own table eight times as wide as the contexts:
-// 65 us instead of 38), and the streaming kernel keeps a sixteenth of the SMs.  Fewest splits within the minimum: each leaves a piece a row to join.
+// 65 us instead of 38), and the streaming kernel keeps a sixteenth of the SMs.  Fewest
+// splits within the minimum: each leaves a piece a row to join.
 int share_sms(PieceGeom& g, int64_t Hkv, int64_t bs, int64_t max_prefix_blocks, int64_t max_blocks,
               int elem) {
   const int64_t ppt = 128 / bs, tiles = (max_prefix_blocks + ppt - 1) / ppt;
